@@ -26,6 +26,26 @@ class CmRowopsDesc(ctypes.Structure):
                 ("aux", _U32), ("bq_sh", _U32), ("win_lo", _U32), ("win_hi", _U32)]
 
 
+class CmPagedCache(ctypes.Structure):
+    """cm_paged_cache: one layer's pool of pages."""
+    _fields_ = [("data", _P), ("pages", _U32), ("page", _U32), ("kv_heads", _U32), ("head_dim", _U32), ("int8", _U32)]
+
+
+class CmPagedBatch(ctypes.Structure):
+    """cm_paged_batch: a step's packed tokens and their sequences' pages."""
+    _fields_ = [("q_start", _P), ("kv_len", _P), ("table", _P), ("batch", _U32), ("tokens", _U32), ("max_pages", _U32),
+                ("table_ld", ctypes.c_uint64)]
+
+
+class CmPagedPrepArgs(ctypes.Structure):
+    """cm_paged_prep_args: the operands, the rotation and the norms of cm_paged_prep."""
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("qr", _P), ("q_ld", ctypes.c_uint64), ("k_ld", ctypes.c_uint64),
+                ("v_ld", ctypes.c_uint64), ("qr_ld", ctypes.c_uint64), ("heads", _U32), ("rope", _P),
+                ("rope_rows", _U32), ("rotary", _U32), ("interleaved", _U32), ("rope_q", _P), ("rope_k", _P),
+                ("rope_q_cols", _U32), ("rope_k_cols", _U32), ("norm_q", _P), ("norm_k", _P),
+                ("eps_q", ctypes.c_int64), ("eps_k", ctypes.c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/cormorant_hip.h declares
 SIGNATURES = {
     "cm_abi_version": (_I32, []),
@@ -70,6 +90,10 @@ SIGNATURES = {
     "cm_matmul_skinny_planes_sat": (_I32, [_P, _U32, _U32, _U32, _P, _P, _P, _P]),
     "cm_matmul_skinny_planes_addx": (_I32, [_P, _U32, _U32, _P, _P, _U32, _P, _P, _U32, _U32, _P, _P]),
     "cm_matmul_skinny_planes_mulact": (_I32, [_P, _U32, _U32, _P, _P, _P, _P, _U32, _P, _U32, _P, _P]),
+    "cm_paged_block_bytes": (ctypes.c_size_t, [_U32] * 3),
+    "cm_paged_prep": (_I32, [_P] * 4),
+    "cm_paged_attention": (_I32, [_P] * 4 + [ctypes.c_uint64] * 2 + [_U32] * 4 + [_P]),
+    "cm_paged_read": (_I32, [_P] * 4 + [ctypes.c_uint64] * 2 + [_P]),
     "cm_timing_enable": (_I32, [_I32]),
     "cm_timing_read": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                               ctypes.POINTER(ctypes.c_uint64)]),

@@ -1,0 +1,178 @@
+"""The paged K / V cache as calls on device tensors: a batch of new tokens (whole prompts, chunks of
+prompts, single decode tokens, packed) normalised, rotated and written into pages (``paged_prep``),
+their attention over the pages (``paged_attention``) and cache rows back out (``paged_read``).
+
+Beside the contiguous caches of ``units.decode_prep`` / ``units.decode_attention`` /
+``units.attention_strided`` (one slab a sequence, one position for the batch): sequences of any
+lengths, rows in pages of one pool, int16 or int8.  The reference has no counterpart; the arithmetic
+is its units' (rowops_spec.py's NORM and ROPE, the pow2 contraction, the softmax unit's exponential).
+
+A ``PagedCache`` (one layer's pool), a ``PagedBatch`` (the step's packing, shared by every layer) and a
+``PagedPrep`` (a layer's rotation and norms) check their tensors once; the calls then check what
+they are given and enqueue on the current torch stream of the cache's device.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .units import _require
+
+
+def block_bytes(page: int, head_dim: int, int8: bool = False) -> int:
+    """Bytes of one KV head of a page (cm_paged_block_bytes)."""
+    return page * (2 * head_dim + 6 if int8 else 4 * head_dim + 4)
+
+
+class PagedCache:
+    """One layer's pool: ``pages`` pages of ``page`` rows (a power of two, 16 .. 4096) for ``kv_heads``
+    heads of ``head_dim`` (64 or 128), held as int16 (two byte planes) or, with ``int8``, as int8 rows
+    with a power-of-two scale a row.  ``data``: the pool's bytes (uint8, cm_paged_cache's layout), by
+    default zeroed memory on ``device``."""
+
+    def __init__(self, pages: int, page: int, kv_heads: int, head_dim: int, int8: bool = False,
+                 data: Optional[torch.Tensor] = None, device="cuda"):
+        if page < 16 or page > 4096 or page & (page - 1):
+            raise ValueError(f"PagedCache: pages of {page} rows (a power of two, 16 .. 4096)")
+        if head_dim not in (64, 128):
+            raise ValueError(f"PagedCache: head_dim {head_dim} (64 or 128)")
+        if pages < 1 or not 1 <= kv_heads <= 1024:
+            raise ValueError(f"PagedCache: {pages} pages of {kv_heads} heads")
+        self.pages, self.page, self.kv_heads, self.head_dim, self.int8 = pages, page, kv_heads, head_dim, bool(int8)
+        nbytes = pages * kv_heads * block_bytes(page, head_dim, self.int8)
+        self.data = torch.zeros(nbytes, dtype=torch.uint8, device=device) if data is None else data
+        _require(self.data, "PagedCache: data", torch.uint8, nbytes)
+        self.width = kv_heads * head_dim
+        self._c = _lib.CmPagedCache(self.data.data_ptr(), pages, page, kv_heads, head_dim, int(self.int8))
+        self._ref = ctypes.byref(self._c)
+
+
+class PagedBatch:
+    """A step's packed tokens: sequence b's are rows q_start[b] .. q_start[b+1] - 1 (int32 [batch + 1]
+    from 0), kv_len[b] (int32 [batch]) its length with them, table[b] (int32 [batch][max_pages], rows
+    any stride apart) its pages in order; ``tokens`` rows in every operand (q_start[batch] or more: the
+    rows behind the last sequence are left alone).  The tensors may change between calls (and replays
+    of a captured call), their sizes not."""
+
+    def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor, tokens: int):
+        batch = kv_len.numel() if kv_len is not None else 0
+        _require(kv_len, "PagedBatch: kv_len", torch.int32, batch)
+        _require(q_start, "PagedBatch: q_start", torch.int32, batch + 1)
+        if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < batch or \
+                table.shape[1] < 1 or table.stride(1) != 1:
+            raise ValueError("PagedBatch: table must be a GPU int32 [batch][max_pages] tensor with contiguous rows")
+        if batch < 1 or tokens < 0:
+            raise ValueError(f"PagedBatch: {batch} sequences, {tokens} tokens")
+        if not (kv_len.device == q_start.device == table.device):
+            raise ValueError("PagedBatch: q_start, kv_len and table on different devices")
+        self.q_start, self.kv_len, self.table, self.tokens, self.batch = q_start, kv_len, table, tokens, batch
+        self._c = _lib.CmPagedBatch(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(), batch, tokens,
+                                    table.shape[1], table.stride(0))
+        self._ref = ctypes.byref(self._c)
+
+
+class PagedPrep:
+    """A layer's rotation and norms: ``table`` int32 [positions][2 rotary] (cos then sin at 2^-23:
+    rowops_nodes.rope_table's rows, or with ``interleaved`` each angle on a pair of neighbouring
+    columns), ``params_q`` / ``params_k`` the ROPE jobs' parameter bytes (one 16-byte entry, or one
+    per column), ``norm_q`` / ``norm_k`` the per-head RMSNorms' entries [head_dim] (None: no norm)
+    with ``eps_q`` / ``eps_k`` (rowops_nodes.norm_params, rms)."""
+
+    def __init__(self, table: torch.Tensor, params_q: torch.Tensor, params_k: torch.Tensor, interleaved: bool = False,
+                 norm_q: Optional[torch.Tensor] = None, norm_k: Optional[torch.Tensor] = None, eps_q: int = 0,
+                 eps_k: int = 0):
+        if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 32 or table.shape[1] % 32:
+            raise ValueError("PagedPrep: a table [positions][2 rotary], rotary a multiple of 16")
+        _require(table, "PagedPrep: table", torch.int32, 2)
+        for name, p in (("params_q", params_q), ("params_k", params_k)):
+            _require(p, f"PagedPrep: {name}", torch.uint8, 16)
+        self.table, self.params_q, self.params_k, self.norm_q, self.norm_k = table, params_q, params_k, norm_q, norm_k
+        self.rotary, self.interleaved = table.shape[1] // 2, bool(interleaved)
+        self.eps_q, self.eps_k = int(eps_q), int(eps_k)
+
+    def _check(self, heads: int, kv_heads: int, head_dim: int) -> None:
+        if self.rotary > head_dim:
+            raise ValueError(f"paged_prep: {self.rotary} rotated columns of a head of {head_dim}")
+        for name, p, n in (("params_q", self.params_q, heads), ("params_k", self.params_k, kv_heads)):
+            if p.numel() != 16 and p.numel() != 16 * n * head_dim:
+                raise ValueError(f"paged_prep: {name} holds {p.numel()} bytes (16, or 16 for each of {n} x {head_dim} columns)")
+        for name, p in (("norm_q", self.norm_q), ("norm_k", self.norm_k)):
+            if p is not None:
+                _require(p, f"paged_prep: {name}", torch.uint8, 16 * head_dim)
+
+
+def _rows(t: torch.Tensor, name: str, tokens: int, width: int) -> int:
+    """The row stride of a [tokens][>= width] int16 operand (rows of contiguous columns)."""
+    if t.dtype != torch.int16 or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU int16 tensor")
+    if t.dim() != 2 or t.shape[0] < tokens or t.shape[1] < width or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be [{tokens}][{width}] rows of contiguous columns, got {list(t.shape)} "
+                         f"at strides {list(t.stride())}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _on(cache: PagedCache, batch: PagedBatch, *ts: torch.Tensor) -> int:
+    """The current stream of the cache's device, which every operand must be on and be current."""
+    dev = cache.data.device
+    for t in (batch.kv_len,) + ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"the cache is on {dev}, an operand on {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def paged_prep(cache: PagedCache, batch: PagedBatch, prep: PagedPrep, q: torch.Tensor, k: torch.Tensor,
+               v: torch.Tensor, qr: torch.Tensor) -> torch.Tensor:
+    """cm_paged_prep: q [tokens][heads hd] normalised per head and rotated into ``qr`` (it may be q), k
+    likewise and v as they are into the cache rows of the tokens' positions.  Rows may be strided
+    (views of a fused projection)."""
+    n, hd = batch.tokens, cache.head_dim
+    heads = qr.shape[-1] // hd
+    if qr.shape[-1] % hd or heads < 1:
+        raise ValueError(f"paged_prep: qr rows of {qr.shape[-1]} columns are no heads of {hd}")
+    lds = [_rows(q, "q", n, heads * hd), _rows(k, "k", n, cache.width), _rows(v, "v", n, cache.width),
+           _rows(qr, "qr", n, heads * hd)]
+    prep._check(heads, cache.kv_heads, hd)
+    if q.data_ptr() == qr.data_ptr() and lds[0] != lds[3]:
+        raise ValueError("paged_prep: qr is q at another stride")
+    stream = _on(cache, batch, q, k, v, qr, prep.table, prep.params_q, prep.params_k, prep.norm_q, prep.norm_k)
+    ptr = lambda t: None if t is None else t.data_ptr()         # noqa: E731
+    args = _lib.CmPagedPrepArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), qr.data_ptr(), *lds, heads,
+                                prep.table.data_ptr(), prep.table.shape[0], prep.rotary, int(prep.interleaved),
+                                prep.params_q.data_ptr(), prep.params_k.data_ptr(), int(prep.params_q.numel() != 16),
+                                int(prep.params_k.numel() != 16), ptr(prep.norm_q), ptr(prep.norm_k), prep.eps_q,
+                                prep.eps_k)
+    _lib.check(_lib.lib().cm_paged_prep(cache._ref, batch._ref, ctypes.byref(args), stream), "cm_paged_prep")
+    return qr
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: torch.Tensor, heads: int, smx_cm: int,
+                    smx_cfg: int, window: int = 0) -> torch.Tensor:
+    """cm_paged_attention: the causal attention of the batch's tokens, q / o [tokens][heads hd], over
+    their sequences' cache rows (the last ``window`` of them, 0: all); smx_cm / smx_cfg as the softmax
+    unit's registers (graph.softmax_regs), o at 2^-(f_p + f_v - 8) as the unit's P . V."""
+    n, hd = batch.tokens, cache.head_dim
+    if heads < 1 or heads % cache.kv_heads or window < 0:
+        raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window}")
+    q_ld, o_ld = _rows(q, "q", n, heads * hd), _rows(o, "o", n, heads * hd)
+    stream = _on(cache, batch, q, o)
+    _lib.check(_lib.lib().cm_paged_attention(cache._ref, batch._ref, q.data_ptr(), o.data_ptr(), q_ld, o_ld, heads,
+                                             window, smx_cm & 0xFFFFFFFF, smx_cfg & 0xFFFFFFFF, stream),
+               "cm_paged_attention")
+    return o
+
+
+def paged_read(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor) -> None:
+    """cm_paged_read: the cache rows of the batch's tokens as int16 rows k / v [tokens][kv_heads hd]."""
+    n = batch.tokens
+    lds = _rows(k, "k", n, cache.width), _rows(v, "v", n, cache.width)
+    stream = _on(cache, batch, k, v)
+    _lib.check(_lib.lib().cm_paged_read(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), *lds, stream),
+               "cm_paged_read")
+
+
+__all__ = ["PagedCache", "PagedBatch", "PagedPrep", "paged_prep", "paged_attention", "paged_read", "block_bytes"]
