@@ -4,6 +4,8 @@
 // A page holds K rows as the byte planes that an MFMA operand lane reads 16 bytes of (d contiguous for
 // q.K^T) and V transposed (keys contiguous for P.V), so the attention neither splits nor transposes
 // what it reads: an int16 x is 256 h + l + 128 (h = x >> 8, l = (x & 255) - 128).
+#include <algorithm>
+
 #include "cm_common.h"
 #include "cm_rowops_math.h"
 
@@ -262,11 +264,45 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Cache c, Batch bt, int1
 }
 
 // ---------------------------------------------------------------- attention
+// The exponential of d = max - s: y = (d Cm) >> Cs, e = TAB[y & 4095] >> (y >> 12).  The kernels take
+// 4 y (a byte offset into TAB) = (min(d, dlim) cm) >> cs from two 24-bit products; at dlim, the least d with
+// y >= 17 * 4096, e is 0, and y there stays below 2^17 (a shift below 32): the host replaces register pairs
+// whose single step passes 15 octaves by one of the same exponentials.
+struct Smx {
+    uint32_t cm, cs, dlim;
+};
+
+Smx smx_of(uint32_t cm24, uint32_t cs) {
+    Smx r{cm24, cs, smx_dlim(cm24, cs)};
+    const uint32_t step = cs < 32 ? cm24 >> cs : 0u;
+    if (step >= 61440u) {                      // d = 1 has y = step, every d >= 2 gives 0
+        r.cs = 0;
+        r.dlim = step > 65536u ? 1u : 2u;      // above 2^16: e(1) = 0
+        r.cm = step > 65536u ? kSmxYZero : (step < 65535u ? step : 65535u);   // e(1) is 1 at 65535 as at 65536
+    }
+    if (r.cs >= 2) r.cs -= 2;
+    else {
+        r.cm <<= 2 - r.cs;                     // below 2^20: step < 61440 * 2^cs, or the pairs above
+        r.cs = 0;
+    }
+    return r;
+}
+
+// w = min(e, 65535), tab = the 4096 words in LDS
+__device__ __forceinline__ uint32_t weight(uint32_t d, const Smx& x, const int32_t* tab) {
+    d = min(d, x.dlim);
+    const uint64_t p = (uint64_t)(d & 0xFFFFFFu) * (x.cm & 0xFFFFFFu);
+    const uint32_t y4 = (uint32_t)(p >> x.cs);
+    const uint32_t t = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(tab) + (y4 & 0x3FFCu));
+    return min(t >> (y4 >> 14), 65535u);
+}
+
 struct Attn {
     const int16_t* q;
     int16_t* o;
     uint64_t q_ld, o_ld;
-    uint32_t G, window, cm, cs, fp, dlim;
+    uint32_t G, window, fp;
+    Smx smx;
 };
 
 // 8 int16 -> their high bytes and low bytes ^ 0x80 (two dwords each)
@@ -292,160 +328,274 @@ __device__ __forceinline__ int finish(int64_t A, int64_t S, uint32_t fp) {
     return (int)(f > 32767 ? 32767 : f < -32768 ? -32768 : f);
 }
 
-// A workgroup takes 16 rows (token, head of the group) of one sequence and KV head; its wavefronts take
-// the 64-key steps of the keys that any row sees, w, w + 4, ..; first the rows' maxima, then weights and
-// P.V with the scores computed again.
-template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256) void paged_attention_kernel(Cache c, Batch bt, Attn a, const int32_t* __restrict__ tab) {
-    constexpr uint32_t KS = HD / 64, DB = HD / 16;
-    typedef Block<HD, I8> B;
-    __shared__ __attribute__((aligned(16))) int32_t stab[4096];
-    __shared__ int32_t redm[4][16];
-    __shared__ int64_t reds[4][16];
-    __shared__ int64_t part[16][HD + 1];
-    const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const uint32_t slot = blockIdx.x, head = blockIdx.y;
-    // sequence b's tiles have the slots from floor(start(b) G / 16) + b on
-    auto first = [&](uint32_t b) { return (uint32_t)((uint64_t)bt.start(b) * a.G / 16) + b; };
-    const uint32_t b = find_le(bt.batch, slot, first);
-    const uint32_t q0 = bt.start(b), n = (uint32_t)max((int)bt.start(b + 1) - (int)q0, 0);
-    const uint32_t tile = slot - first(b), rows = n * a.G;
-    if (tile * 16 >= rows) return;
-    const int base = bt.len(b) - (int)n;                    // position of the sequence's first new token
-    const uint32_t row = tile * 16 + c16;
-    const bool on = row < rows;
-    const uint32_t tok = row / a.G, hh = head * a.G + row % a.G;
-    auto seen = [&](uint32_t tk) { return (uint32_t)min(max(base + (int)tk + 1, 0), (int)bt.cap); };
-    auto begin = [&](uint32_t tk) { return a.window ? (uint32_t)max(base + (int)tk + 1 - (int)a.window, 0) : 0u; };
-    const uint32_t vend = on ? seen(tok) : 0u, vbeg = on ? begin(tok) : 0u;
-    const uint32_t lo = begin(tile * 16 / a.G) & ~63u, hi = seen(min((tile * 16 + 15) / a.G, n - 1));
-    const int32_t* tb = bt.table + b * bt.table_ld;
+// ---- the split of the work.  A tile is R rows (token, head of the group) of one sequence and KV head; sequence b's
+// tiles have the slots from floor(start(b) G / R) + b on (at least as many as it needs, known without a scan).  The
+// 64-key steps that any row of the tile sees are divided over up to `splits` workgroups, kMinSteps each at least.
+constexpr uint32_t kMinSteps = 4;
+
+template <uint32_t R>
+struct Tile {
+    uint32_t b, q0, n, row0, rows;         // sequence, its first token, tokens; the tile's first row, the sequence's rows
+    uint32_t lo, hi, nt;                   // keys [lo, hi) that a row sees, lo a multiple of 64; 64-key steps
+    uint32_t all_lo, all_hi;               // keys that every row sees
+    int base;
+    const int32_t* tb;
+    bool on;
+
+    __device__ __forceinline__ Tile(const Batch& bt, const Attn& a, uint32_t slot) {
+        auto first = [&](uint32_t i) { return (uint32_t)((uint64_t)bt.start(i) * a.G / R) + i; };
+        b = find_le(bt.batch, slot, first);
+        q0 = bt.start(b);
+        n = (uint32_t)max((int)bt.start(b + 1) - (int)q0, 0);
+        row0 = (slot - first(b)) * R;
+        rows = n * a.G;
+        on = row0 < rows;
+        base = bt.len(b) - (int)n;
+        tb = bt.table + b * bt.table_ld;
+        const uint32_t tf = row0 / a.G, tl = on ? min((row0 + R - 1) / a.G, n - 1) : tf;
+        lo = __builtin_amdgcn_readfirstlane(begin(a, tf) & ~63u);
+        hi = __builtin_amdgcn_readfirstlane(seen(bt, tl));
+        all_lo = __builtin_amdgcn_readfirstlane(begin(a, tl));
+        all_hi = __builtin_amdgcn_readfirstlane(seen(bt, tf));
+        nt = hi > lo ? (hi - lo + 63) / 64 : 0u;
+    }
+    __device__ __forceinline__ uint32_t seen(const Batch& bt, uint32_t tk) const {   // keys end
+        return (uint32_t)min(max(base + (int)tk + 1, 0), (int)bt.cap);
+    }
+    __device__ __forceinline__ uint32_t begin(const Attn& a, uint32_t tk) const {
+        return a.window ? (uint32_t)max(base + (int)tk + 1 - (int)a.window, 0) : 0u;
+    }
+    __device__ __forceinline__ uint32_t steps(uint32_t splits) const { return max((nt + splits - 1) / splits, kMinSteps); }
+    __device__ __forceinline__ uint32_t parts(uint32_t splits) const { return nt ? (nt + steps(splits) - 1) / steps(splits) : 1u; }
+};
+
+// The call's workspace: per row (head, token, head of the group: (head T + token) G + i) the maxima of its parts,
+// its scores (few rows), its partial sums of w V and of w.
+struct Work {
+    int32_t* mx;                           // [rows][splits] raw q.K^T sums, kNone: no key
+    int16_t* sc;                           // [rows][cap]
+    int64_t* part;                         // [rows][splits][HD + 1]
+    uint32_t splits;
+};
+constexpr int kNone = (int)0x80000000;
+
+// V's sums and the bytes' offsets put back: the exact sum of w V (int16: hh, mid, ll of w's and V's bytes; int8: the
+// three bytes of w 2^e; every byte was taken less 128)
+template <bool I8>
+__device__ __forceinline__ int64_t whole_sum(int a0, int a1, int a2, int vs0, int vs1, int64_t wsum) {
+    const int64_t x = (int64_t)a0 * 65536 + (int64_t)a1 * 256 + a2;
+    return x + (I8 ? (int64_t)vs0 * (128 * 65793) : ((int64_t)vs0 * 256 + vs1) * 32896 + 128 * wsum);
+}
+
+// four weights (int8: shifted by the bytes of es) -> dword q of the byte operands
+template <bool I8>
+__device__ __forceinline__ void weight_bytes(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t es, v4i (&p)[I8 ? 3 : 2],
+                                             uint32_t q) {
+    if constexpr (I8) {
+        x0 <<= es & 15u;
+        x1 <<= (es >> 8) & 15u;
+        x2 <<= (es >> 16) & 15u;
+        x3 <<= (es >> 24) & 15u;
+    }
+    const uint32_t t01 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), t23 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+    p[0][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x05040100u) ^ 0x80808080u);
+    p[1][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x07060302u) ^ 0x80808080u);
+    if constexpr (I8) {
+        const uint32_t u01 = __builtin_amdgcn_perm(x1, x0, 0x0c0c0602u), u23 = __builtin_amdgcn_perm(x3, x2, 0x0c0c0602u);
+        p[2][q] = (int)(__builtin_amdgcn_perm(u23, u01, 0x05040100u) ^ 0x80808080u);
+    }
+}
+
+// the raw int32 sum of a lane's key r from the limb products (e: the key's shift)
+template <bool I8>
+__device__ __forceinline__ int raw_sum(int hh, int mid, int ll, uint32_t es, uint32_t r, int qterm) {
+    if constexpr (I8) return (int)((((uint32_t)mid << 8) + (uint32_t)ll) << ((es >> (8 * r)) & 31u));
+    return (int)((((((uint32_t)hh << 8) + (uint32_t)mid) << 8) + (uint32_t)ll) + (uint32_t)qterm);
+}
+
+template <bool I8>
+__device__ __forceinline__ void qk(const v4i kh, const v4i kl, const v4i qh, const v4i ql, v4i& hh, v4i& mid, v4i& ll) {
+    if constexpr (I8) {
+        mid = mfma(kh, qh, mid);
+        ll = mfma(kh, ql, ll);
+    } else {
+        hh = mfma(kh, qh, hh);
+        mid = mfma(kh, ql, mid);
+        ll = mfma(kl, ql, ll);
+        mid = mfma(kl, qh, mid);
+    }
+}
+
+__device__ __forceinline__ void stage_tab(int32_t* stab, const int32_t* tab) {
+    const uint32_t t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6);
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) *reinterpret_cast<int4*>(stab + 4 * (t + 256 * i)) = *reinterpret_cast<const int4*>(tab + 4 * (t + 256 * i));
-    for (uint32_t i = t; i < 16 * (HD + 1); i += 256) (&part[0][0])[i] = 0;
+    for (uint32_t i = 0; i < 4; i++)
+        __builtin_amdgcn_global_load_lds(tab + 4 * (t + 256 * i),
+                                         (__attribute__((address_space(3))) void*)(stab + 4 * (64 * w + 256 * i)), 16, 0, 0);
+}
+
+// ---------------------------------------------------------------- attention of few rows
+// Tiles of 16 rows: decode steps, where the cache's bytes are what costs.  A workgroup's four wavefronts take the
+// steps of its part in turn and read K and V straight into the MFMA operands; the first kernel leaves the scores and
+// the part's maxima, the second takes the row's maximum, the weights and P.V.
+template <uint32_t HD, bool I8>
+__global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
+    constexpr uint32_t KS = HD / 64;
+    typedef Block<HD, I8> B;
+    __shared__ int32_t redm[4][16];
+    const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const Tile<16> tl(bt, a, blockIdx.x);
+    const uint32_t per = tl.steps(wk.splits);
+    if (!tl.on || z * per >= max(tl.nt, 1u)) return;
+    const uint32_t row = min(tl.row0 + c16, tl.rows - 1), tok = row / a.G;
+    const bool mine = tl.row0 + c16 < tl.rows;
+    const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
+    const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
 
     v4i qh[KS], ql[KS];
     int qsum = 0;
-    const int16_t* qp = a.q + (uint64_t)(q0 + (on ? tok : 0)) * a.q_ld + (uint64_t)(on ? hh : 0) * HD + 16 * g;
+    const int16_t* qp = a.q + (uint64_t)(tl.q0 + tok) * a.q_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * g;
 #pragma unroll
     for (uint32_t s = 0; s < KS; s++) limbs16(qp + 64 * s, qh[s], ql[s], qsum);
     qsum += __shfl_xor(qsum, 16, 64);
     qsum += __shfl_xor(qsum, 32, 64);
     const int qterm = I8 ? 0 : 128 * qsum;
-    const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-
-    // a key's page: outside the pool its rows are masked (and block 0 read in their place)
-    auto page_of = [&](uint32_t key) { return key < bt.cap ? (uint32_t)tb[key >> c.lg] : 0xFFFFFFFFu; };
-    auto block_of = [&](uint32_t id) { return c.data + ((uint64_t)(id < c.pages ? id : 0) * c.kv + head) * c.block; };
-    // the scores of 64 keys: the lane's are k0 + 16 g + 4 kb + r of query c16 (row i of block kb is key
-    // 16 (i / 4) + 4 kb + i % 4, so that the lane's keys are the 16 consecutive ones of its V operand)
-    auto scores = [&](uint32_t k0, const uint8_t* vb, bool ok, int (&sv)[16]) {
-        const uint32_t kr = k0 + 16 * (c16 >> 2) + (c16 & 3), kg = k0 + 16 * g;
-        const uint8_t* kb0 = block_of(page_of(kr)) + 16 * g;
+    const v4i zero = {0, 0, 0, 0};
+    int mx = kNone;
+    for (uint32_t i = z * per + w; i < min((z + 1) * per, tl.nt); i += 4) {
+        const uint32_t k0 = tl.lo + 64 * i, kr = k0 + 16 * (c16 >> 2) + (c16 & 3), kg = k0 + 16 * g;
+        const uint32_t idr = kr < bt.cap ? (uint32_t)tl.tb[kr >> c.lg] : ~0u, idg = kg < bt.cap ? (uint32_t)tl.tb[kg >> c.lg] : ~0u;
+        const uint8_t* kb0 = c.data + ((uint64_t)(idr < c.pages ? idr : 0) * c.kv + head) * c.block + (kr & (c.page - 1)) * HD + 16 * g;
+        const uint8_t* tb0 = c.data + ((uint64_t)(idg < c.pages ? idg : 0) * c.kv + head) * c.block;
+        const uint32_t in = kg & (c.page - 1);
+        v4i kh[4][KS], kl[4][KS], term[4];
 #pragma unroll
         for (uint32_t kb = 0; kb < 4; kb++) {
-            const uint8_t* kp = kb0 + ((kr + 4 * kb) & (c.page - 1)) * HD;
-            v4i hh4 = zero, mid = zero, ll = *reinterpret_cast<const v4i*>(vb + B::term(c.page) + 4 * ((kg + 4 * kb) & (c.page - 1)));
 #pragma unroll
             for (uint32_t s = 0; s < KS; s++) {
-                const v4i kh = *reinterpret_cast<const v4i*>(kp + 64 * s);
-                if constexpr (I8) {
-                    mid = mfma(kh, qh[s], mid);
-                    ll = mfma(kh, ql[s], ll);
-                } else {
-                    const v4i kl = *reinterpret_cast<const v4i*>(kp + B::k(c.page, 1) + 64 * s);
-                    hh4 = mfma(kh, qh[s], hh4);
-                    mid = mfma(kh, ql[s], mid);
-                    mid = mfma(kl, qh[s], mid);
-                    ll = mfma(kl, ql[s], ll);
-                }
+                kh[kb][s] = *reinterpret_cast<const v4i*>(kb0 + 4 * kb * HD + 64 * s);
+                if constexpr (!I8) kl[kb][s] = *reinterpret_cast<const v4i*>(kb0 + B::k(c.page, 1) + 4 * kb * HD + 64 * s);
             }
-            uint32_t es = 0;
-            if constexpr (I8) es = *reinterpret_cast<const uint32_t*>(vb + B::ke(c.page) + ((kg + 4 * kb) & (c.page - 1)));
+            term[kb] = *reinterpret_cast<const v4i*>(tb0 + B::term(c.page) + 4 * (in + 4 * kb));
+        }
+        v4i es = zero;
+        if constexpr (I8) es = *reinterpret_cast<const v4i*>(tb0 + B::ke(c.page) + in);
+        uint32_t out[8];
+#pragma unroll
+        for (uint32_t kb = 0; kb < 4; kb++) {
+            v4i hh = zero, mid = zero, ll = term[kb];
+#pragma unroll
+            for (uint32_t s = 0; s < KS; s++) qk<I8>(kh[kb][s], kl[kb][s], qh[s], ql[s], hh, mid, ll);
+            int x[4];
 #pragma unroll
             for (uint32_t r = 0; r < 4; r++) {
-                uint32_t acc = ((uint32_t)mid[r] << 8) + (uint32_t)ll[r];
-                if constexpr (I8) acc <<= (es >> (8 * r)) & 31u;
-                else acc += ((uint32_t)hh4[r] << 16) + (uint32_t)qterm;
+                const int acc = raw_sum<I8>(hh[r], mid[r], ll[r], (uint32_t)es[kb], r, qterm);
                 const uint32_t key = kg + 4 * kb + r;
-                sv[4 * kb + r] = ok && key >= vbeg && key < vend ? sat16i((int)acc >> 8) : -0x10000;
+                mx = max(mx, idg < c.pages && key >= vbeg && key < vend ? acc : kNone);
+                x[r] = sat16i(acc >> 8);
+            }
+            out[2 * kb] = (uint32_t)(uint16_t)x[0] | (uint32_t)x[1] << 16;
+            out[2 * kb + 1] = (uint32_t)(uint16_t)x[2] | (uint32_t)x[3] << 16;
+        }
+        if (mine) {
+            int16_t* sp = wk.sc + wrow * bt.cap + kg;                     // kg < cap: cap is a multiple of 16
+            if (kg < bt.cap) {
+                *reinterpret_cast<uint4*>(sp) = make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4*>(sp + 8) = make_uint4(out[4], out[5], out[6], out[7]);
             }
         }
-    };
-
-    int mx = -0x10000;
-    for (uint32_t k0 = lo + 64 * w; k0 < hi; k0 += 256) {
-        const uint32_t id = page_of(k0 + 16 * g);
-        int sv[16];
-        scores(k0, block_of(id), id < c.pages, sv);
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i++) mx = max(mx, sv[i]);
     }
     mx = max(mx, __shfl_xor(mx, 16, 64));
     mx = max(mx, __shfl_xor(mx, 32, 64));
     if (g == 0) redm[w][c16] = mx;
     __syncthreads();
-    mx = max(max(redm[0][c16], redm[1][c16]), max(redm[2][c16], redm[3][c16]));
+    if (t < 16 && mine) wk.mx[wrow * wk.splits + z] = max(max(redm[0][t], redm[1][t]), max(redm[2][t], redm[3][t]));
+}
 
-    constexpr uint32_t NA = 3;             // limb products: int16 hh, mid, ll; int8 the weight's three bytes
-    v4i acc[NA][DB], vs[I8 ? 1 : 2][DB];
+// the maximum score of a row over its parts
+__device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t parts) {
+    int m = kNone;
+    for (uint32_t i = 0; i < parts; i++) m = max(m, wk.mx[wrow * wk.splits + i]);
+    return sat16i(m >> 8);
+}
+
+template <uint32_t HD, bool I8>
+__global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
+    constexpr uint32_t DB = HD / 16, NP = I8 ? 1 : 2;
+    typedef Block<HD, I8> B;
+    __shared__ __attribute__((aligned(16))) int32_t stab[4096];
+    __shared__ int64_t reds[4][16];
+    __shared__ int64_t part[16][HD + 1];
+    const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const Tile<16> tl(bt, a, blockIdx.x);
+    const uint32_t per = tl.steps(wk.splits), parts = tl.parts(wk.splits);
+    if (!tl.on || z >= parts) return;
+    stage_tab(stab, tab);
+    for (uint32_t i = t; i < 16 * (HD + 1); i += 256) (&part[0][0])[i] = 0;
+    const uint32_t row = min(tl.row0 + c16, tl.rows - 1), tok = row / a.G;
+    const bool mine = tl.row0 + c16 < tl.rows;
+    const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
+    const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
+    const int mxs = row_max(wk, wrow, parts);
+    const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __syncthreads();
+
+    v4i acc[3][DB], vs[NP][DB];
 #pragma unroll
     for (uint32_t m = 0; m < DB; m++) {
         acc[0][m] = acc[1][m] = acc[2][m] = zero;
-        vs[0][m] = vs[I8 ? 0 : 1][m] = zero;
+        vs[0][m] = vs[NP - 1][m] = zero;
     }
     int64_t wsum = 0;
-    for (uint32_t k0 = lo + 64 * w; k0 < hi; k0 += 256) {
-        const uint32_t id = page_of(k0 + 16 * g);
-        const uint8_t* vb = block_of(id);
-        int sv[16];
-        scores(k0, vb, id < c.pages, sv);
-        uint32_t part32 = 0;
-        const uint32_t in = (k0 + 16 * g) & (c.page - 1);
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i++) {
-            const bool ok = sv[i] != -0x10000;
-            const uint32_t d = ok ? (uint32_t)(mx - sv[i]) : 0u;
-            const uint32_t y = (uint32_t)(((uint64_t)d * a.cm) >> a.cs);
-            const uint32_t e = ok && d < a.dlim ? min((uint32_t)stab[y & 4095] >> ((y >> 12) & 31), 65535u) : 0u;
-            part32 += e;
-            sv[i] = (int)e;
-        }
-        wsum += part32;
-        v4i p[3];
-#pragma unroll
-        for (uint32_t q = 0; q < 4; q++) {
-            uint32_t e4[4], by[3] = {0, 0, 0};
-#pragma unroll
-            for (uint32_t r = 0; r < 4; r++) {
-                e4[r] = (uint32_t)sv[4 * q + r];
-                if constexpr (I8) e4[r] <<= vb[B::ve(c.page) + in + 4 * q + r] & 15u;
-#pragma unroll
-                for (uint32_t z = 0; z < 3; z++) by[z] |= (((e4[r] >> (8 * z)) & 255u) ^ 128u) << (8 * r);
-            }
-            p[0][q] = (int)by[0];
-            p[1][q] = (int)by[1];
-            p[2][q] = (int)by[2];
-        }
+    for (uint32_t i = z * per + w; i < min((z + 1) * per, tl.nt); i += 4) {
+        const uint32_t k0 = tl.lo + 64 * i, kg = k0 + 16 * g, in = kg & (c.page - 1);
+        const uint32_t id = kg < bt.cap ? (uint32_t)tl.tb[kg >> c.lg] : ~0u;
+        const uint8_t* vb = c.data + ((uint64_t)(id < c.pages ? id : 0) * c.kv + head) * c.block;
+        v4i vh[DB], vl[DB];
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
             const uint8_t* vp = vb + B::v(c.page, 0) + (16 * m + c16) * c.page + in;
-            const v4i vh = *reinterpret_cast<const v4i*>(vp);
+            vh[m] = *reinterpret_cast<const v4i*>(vp);
+            if constexpr (!I8) vl[m] = *reinterpret_cast<const v4i*>(vp + HD * c.page);
+        }
+        uint4 s0 = make_uint4(0, 0, 0, 0), s1 = s0;
+        if (mine && kg < bt.cap) {
+            const int16_t* sp = wk.sc + wrow * bt.cap + kg;
+            s0 = *reinterpret_cast<const uint4*>(sp);
+            s1 = *reinterpret_cast<const uint4*>(sp + 8);
+        }
+        v4i es = zero;
+        if constexpr (I8) es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
+        const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        uint32_t e[16], sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j++) {
+            const int s = j & 1 ? (int)sw[j / 2] >> 16 : (int)(int16_t)sw[j / 2];
+            const bool on = id < c.pages && kg + j >= vbeg && kg + j < vend;
+            e[j] = on ? weight((uint32_t)(mxs - s), a.smx, stab) : 0u;
+            sum += e[j];
+        }
+        wsum += sum;
+        v4i p[I8 ? 3 : 2];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) weight_bytes<I8>(e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3], (uint32_t)es[q], p, q);
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) {
             if constexpr (I8) {
-                acc[0][m] = mfma(vh, p[2], acc[0][m]);
-                acc[1][m] = mfma(vh, p[1], acc[1][m]);
-                acc[2][m] = mfma(vh, p[0], acc[2][m]);
-                vs[0][m] = mfma(vh, ones, vs[0][m]);
+                acc[0][m] = mfma(vh[m], p[2], acc[0][m]);
+                acc[1][m] = mfma(vh[m], p[1], acc[1][m]);
+                acc[2][m] = mfma(vh[m], p[0], acc[2][m]);
             } else {
-                const v4i vl = *reinterpret_cast<const v4i*>(vp + HD * c.page);
-                acc[0][m] = mfma(vh, p[1], acc[0][m]);
-                acc[1][m] = mfma(vh, p[0], acc[1][m]);
-                acc[1][m] = mfma(vl, p[1], acc[1][m]);
-                acc[2][m] = mfma(vl, p[0], acc[2][m]);
-                vs[0][m] = mfma(vh, ones, vs[0][m]);
-                vs[1][m] = mfma(vl, ones, vs[1][m]);
+                acc[0][m] = mfma(vh[m], p[1], acc[0][m]);
+                acc[1][m] = mfma(vh[m], p[0], acc[1][m]);
+                acc[2][m] = mfma(vl[m], p[0], acc[2][m]);
+                acc[1][m] = mfma(vl[m], p[1], acc[1][m]);
+                vs[1][m] = mfma(vl[m], ones, vs[1][m]);
             }
+            vs[0][m] = mfma(vh[m], ones, vs[0][m]);
         }
     }
     wsum += (int64_t)ro::shfl64((uint64_t)wsum, 16);
@@ -454,25 +604,379 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(Cache c, Batch bt,
 #pragma unroll
     for (uint32_t m = 0; m < DB; m++)
 #pragma unroll
-        for (uint32_t r = 0; r < 4; r++) {
-            int64_t x = (int64_t)acc[0][m][r] * 65536 + (int64_t)acc[1][m][r] * 256 + acc[2][m][r];
-            x += I8 ? (int64_t)vs[0][m][r] * (128 * 65793)
-                    : ((int64_t)vs[0][m][r] * 256 + vs[I8 ? 0 : 1][m][r]) * 32896 + 128 * wsum;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&part[c16][16 * m + 4 * g + r]), (unsigned long long)x);
-        }
+        for (uint32_t r = 0; r < 4; r++)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&part[c16][16 * m + 4 * g + r]),
+                      (unsigned long long)whole_sum<I8>(acc[0][m][r], acc[1][m][r], acc[2][m][r], vs[0][m][r], vs[NP - 1][m][r], wsum));
     __syncthreads();
     for (uint32_t i = t; i < 16 * HD / 2; i += 256) {
-        const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2)), rw = tile * 16 + r;
-        if (rw >= rows) break;
+        const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2)), rw = tl.row0 + r;
+        if (rw >= tl.rows) break;
         const int64_t S = reds[0][r] + reds[1][r] + reds[2][r] + reds[3][r];
-        const int o0 = finish(part[r][d], S, a.fp), o1 = finish(part[r][d + 1], S, a.fp);
-        *reinterpret_cast<uint32_t*>(a.o + (uint64_t)(q0 + rw / a.G) * a.o_ld + (uint64_t)(head * a.G + rw % a.G) * HD + d) =
-            (uint32_t)(uint16_t)o0 | ((uint32_t)(uint16_t)o1 << 16);
+        if (parts == 1) {
+            const int o0 = finish(part[r][d], S, a.fp), o1 = finish(part[r][d + 1], S, a.fp);
+            *reinterpret_cast<uint32_t*>(a.o + (uint64_t)(tl.q0 + rw / a.G) * a.o_ld + (uint64_t)(head * a.G + rw % a.G) * HD + d) =
+                (uint32_t)(uint16_t)o0 | ((uint32_t)(uint16_t)o1 << 16);
+        } else {
+            int64_t* pp = wk.part + ((((uint64_t)head * bt.tokens + tl.q0) * a.G + rw) * wk.splits + z) * (HD + 1);
+            pp[d] = part[r][d];
+            pp[d + 1] = part[r][d + 1];
+            if (d == 0) pp[HD] = S;
+        }
+    }
+}
+
+// The parts' sums of a row added and divided: a wavefront per row, two columns a lane at 128 d.  R: the rows of the
+// tiles that made the parts.
+template <uint32_t HD, uint32_t R>
+__global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work wk) {
+    const uint32_t lane = threadIdx.x & 63, head = blockIdx.y;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));   // row of (token, i)
+    const uint32_t tok = at / a.G;
+    if (tok >= bt.start(bt.batch)) return;
+    const uint32_t b = find_le(bt.batch, tok, [&](uint32_t i) { return bt.start(i); });
+    const uint32_t row = at - bt.start(b) * a.G;
+    const Tile<R> tl(bt, a, (uint32_t)((uint64_t)bt.start(b) * a.G / R) + b + row / R);
+    const uint32_t parts = tl.parts(wk.splits);
+    if (!tl.on || parts == 1) return;
+    const int64_t* pp = wk.part + ((uint64_t)head * bt.tokens * a.G + at) * wk.splits * (HD + 1);
+    int64_t x[HD / 64], S = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < HD / 64; k++) x[k] = 0;
+    for (uint32_t i = 0; i < parts; i++, pp += HD + 1) {
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 64; k++) x[k] += pp[lane * (HD / 64) + k];
+        S += pp[HD];
+    }
+    int16_t* op = a.o + (uint64_t)tok * a.o_ld + (uint64_t)(head * a.G + at % a.G) * HD + lane * (HD / 64);
+#pragma unroll
+    for (uint32_t k = 0; k < HD / 64; k++) op[k] = (int16_t)finish(x[k], S, a.fp);
+}
+
+// ---------------------------------------------------------------- attention of many rows
+// Tiles of 64 QB rows, 16 QB a wavefront; the keys go by in steps of 64 through two LDS stages that all four
+// wavefronts read, copied straight into LDS a step ahead.  One kernel for the rows' maxima (q.K^T alone), one for the
+// weights and P.V with the scores computed again: a weight needs the final maximum (its shift drops bits, so a sum
+// over another maximum cannot be rescaled), and the scores of many rows are dearer to keep than to compute twice.
+//
+// LDS layouts.  K: row = key, its 16-byte chunks XORed by the key's place so that the 16 rows of a fragment (keys
+// 16 a + 4 kb + i) fall on 16 bank groups.  V: [plane][16-key group][d][16 bytes], a fragment's lanes consecutive.
+// Wavefront w copies the step's 16-key group w, of one page: a direct copy moves 1 KiB, lane l to 16 l (16 key rows,
+// 8 at 128 d; or 64 d).
+template <uint32_t HD, bool I8, bool V>
+struct Stage {
+    static constexpr uint32_t KBYTES = (I8 ? 1 : 2) * 64 * HD;
+    static constexpr uint32_t TERM = V ? 2 * KBYTES : KBYTES, BYTES = TERM + 256 + (I8 ? 128 : 0);   // K, V, terms, shifts
+};
+
+template <uint32_t HD, bool I8, uint32_t QB, bool V>
+struct Rows {
+    static constexpr uint32_t KS = HD / 64, NP = I8 ? 1 : 2, R = 64 * QB;
+    typedef Block<HD, I8> B;
+    typedef Stage<HD, I8, V> S;
+    const Cache& c;
+    const Batch& bt;
+    const Tile<R>& tl;
+    uint32_t head, lane, c16, g, w;
+    v4i qh[QB][KS], ql[QB][KS];
+    int qterm[QB];
+    uint32_t vend[QB], vbeg[QB];
+
+    __device__ __forceinline__ Rows(const Cache& c_, const Batch& bt_, const Attn& a, const Tile<R>& tl_, uint32_t head_)
+        : c(c_), bt(bt_), tl(tl_), head(head_) {
+        lane = threadIdx.x & 63;
+        c16 = lane & 15;
+        g = lane >> 4;
+        w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            const uint32_t row = row_of(qb), rr = min(row, tl.rows - 1), tok = rr / a.G;
+            vend[qb] = row < tl.rows ? tl.seen(bt, tok) : 0u;
+            vbeg[qb] = tl.begin(a, tok);
+            const int16_t* qp = a.q + (uint64_t)(tl.q0 + tok) * a.q_ld + (uint64_t)(head * a.G + rr % a.G) * HD + 16 * g;
+            int qs = 0;
+#pragma unroll
+            for (uint32_t s = 0; s < KS; s++) limbs16(qp + 64 * s, qh[qb][s], ql[qb][s], qs);
+            qs += __shfl_xor(qs, 16, 64);
+            qs += __shfl_xor(qs, 32, 64);
+            qterm[qb] = I8 ? 0 : 128 * qs;
+        }
+    }
+    __device__ __forceinline__ uint32_t row_of(uint32_t qb) const { return tl.row0 + 16 * QB * w + 16 * qb + c16; }
+    // the page ids of step i's four 16-key groups, one a lane group (~0: no page)
+    __device__ __forceinline__ uint32_t ids(uint32_t i, uint32_t end) const {
+        const uint32_t key = tl.lo + 64 * i + 16 * g;
+        const uint32_t id = i < end && key < bt.cap ? (uint32_t)tl.tb[key >> c.lg] : ~0u;
+        return id < c.pages ? id : ~0u;
+    }
+    static __device__ __forceinline__ void copy(const uint8_t* src, uint8_t* dst) {
+        __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+    }
+    __device__ __forceinline__ void stage(uint8_t* sm, uint32_t i, uint32_t id4) const {
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)id4, 16 * w);
+        const uint8_t* blk = c.data + ((uint64_t)(id == ~0u ? 0u : id) * c.kv + head) * c.block;
+        const uint32_t in = (tl.lo + 64 * i + 16 * w) & (c.page - 1);
+        constexpr uint32_t CH = HD / 16, RPC = 64 / CH;               // chunks a row, rows a copy
+#pragma unroll
+        for (uint32_t pl = 0; pl < NP; pl++)
+#pragma unroll
+            for (uint32_t s = 0; s < KS; s++) {
+                const uint32_t row = RPC * s + lane / CH, f = KS == 1 ? w : ((row >> 1) & 1) | w << 1;
+                copy(blk + B::k(c.page, pl) + in * HD + row * HD + 16 * ((lane % CH) ^ f), sm + pl * 64 * HD + (16 * w + RPC * s) * HD);
+            }
+        if constexpr (V) {
+#pragma unroll
+            for (uint32_t pl = 0; pl < NP; pl++)
+#pragma unroll
+                for (uint32_t s = 0; s < KS; s++)
+                    copy(blk + B::v(c.page, pl) + in + (64 * s + lane) * c.page, sm + S::KBYTES + ((pl * 4 + w) * HD + 64 * s) * 16);
+        }
+        if (lane < 4) copy(blk + B::term(c.page) + 4 * in + 16 * lane, sm + S::TERM + 64 * w);
+        if constexpr (I8) {
+            if (lane == 0) {
+                copy(blk + B::ke(c.page) + in, sm + S::TERM + 256 + 16 * w);
+                if constexpr (V) copy(blk + B::ve(c.page) + in, sm + S::TERM + 320 + 16 * w);
+            }
+        }
+    }
+    // the raw sums of keys 16 g + 4 kb + r, r < 4, for every query block: f(qb, sums)
+    template <class F>
+    __device__ __forceinline__ void dots(const uint8_t* sm, uint32_t kb, F f) const {
+        const v4i zero = {0, 0, 0, 0};
+        const uint32_t row = 16 * (c16 >> 2) + 4 * kb + (c16 & 3);
+        const v4i term = *reinterpret_cast<const v4i*>(sm + S::TERM + 4 * (16 * g + 4 * kb));
+        v4i kh[KS], kl[KS];
+#pragma unroll
+        for (uint32_t s = 0; s < KS; s++) {
+            const uint32_t x = KS == 1 ? c16 >> 2 : ((c16 >> 1) & 1) | (c16 >> 2) << 1;
+            const uint8_t* kp = sm + row * HD + 16 * ((4 * s + g) ^ x);
+            kh[s] = *reinterpret_cast<const v4i*>(kp);
+            if constexpr (!I8) kl[s] = *reinterpret_cast<const v4i*>(kp + 64 * HD);
+            else kl[s] = zero;
+        }
+        uint32_t es = 0;
+        if constexpr (I8) es = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 256 + 16 * g + 4 * kb);
+#pragma unroll
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            v4i hh = zero, mid = zero, ll = term;
+#pragma unroll
+            for (uint32_t s = 0; s < KS; s++) qk<I8>(kh[s], kl[s], qh[qb][s], ql[qb][s], hh, mid, ll);
+            int x[4];
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) x[r] = raw_sum<I8>(hh[r], mid[r], ll[r], es, r, qterm[qb]);
+            f(qb, x);
+        }
+    }
+    // whether every row sees all 64 keys of a step, its pages all there
+    __device__ __forceinline__ bool whole(uint32_t i, uint32_t id4) const {
+        const uint32_t k0 = tl.lo + 64 * i;
+        return k0 >= tl.all_lo && k0 + 64 <= tl.all_hi && __ballot(id4 == ~0u) == 0;
+    }
+    // body(stage, step, ids) for the steps [i, end), two stages deep
+    template <class F>
+    __device__ __forceinline__ void run(uint8_t* sm0, uint8_t* sm1, uint32_t i, uint32_t end, F body) const {
+        if (i >= end) return;
+        uint32_t id0 = ids(i, end), id1 = ids(i + 1, end);
+        stage(sm0, i, id0);
+        for (;; i += 2) {
+            __builtin_amdgcn_s_waitcnt(0x0070);        // this wavefront's copies
+            __syncthreads();                           // every wavefront's; the other stage read
+            const uint32_t id2 = ids(i + 2, end);
+            if (i + 1 < end) stage(sm1, i + 1, id1);
+            body(sm0, i, id0);
+            if (i + 1 >= end) break;
+            __builtin_amdgcn_s_waitcnt(0x0070);
+            __syncthreads();
+            const uint32_t id3 = ids(i + 3, end);
+            if (i + 2 < end) stage(sm0, i + 2, id2);
+            body(sm1, i + 1, id1);
+            if (i + 2 >= end) break;
+            id0 = id2;
+            id1 = id3;
+        }
+    }
+};
+
+template <uint32_t HD, bool I8, uint32_t QB>
+__global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, Attn a, Work wk) {
+    typedef Rows<HD, I8, QB, false> RW;
+    __shared__ __attribute__((aligned(1024))) uint8_t sm0[RW::S::BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t sm1[RW::S::BYTES];
+    const uint32_t head = blockIdx.y, z = blockIdx.z;
+    const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);             // the long tiles first
+    const uint32_t per = tl.steps(wk.splits);
+    if (!tl.on || z >= tl.parts(wk.splits)) return;
+    const RW rw(c, bt, a, tl, head);
+    int mx[QB];
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) mx[qb] = kNone;
+    rw.run(sm0, sm1, z * per, min((z + 1) * per, tl.nt), [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
+        const uint32_t kg = tl.lo + 64 * i + 16 * rw.g;
+        if (rw.whole(i, ids)) {
+#pragma unroll
+            for (uint32_t kb = 0; kb < 4; kb++)
+                rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
+                    mx[qb] = max(max(mx[qb], max(x[0], x[1])), max(x[2], x[3]));
+                });
+        } else {
+#pragma unroll
+            for (uint32_t kb = 0; kb < 4; kb++)
+                rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) {
+                        const uint32_t key = kg + 4 * kb + r;
+                        mx[qb] = max(mx[qb], ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? x[r] : kNone);
+                    }
+                });
+        }
+    });
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) {
+        int m = mx[qb];
+        m = max(m, __shfl_xor(m, 16, 64));
+        m = max(m, __shfl_xor(m, 32, 64));
+        const uint32_t row = rw.row_of(qb);
+        if (rw.g == 0 && row < tl.rows) wk.mx[(((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits + z] = m;
+    }
+}
+
+template <uint32_t HD, bool I8, uint32_t QB>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
+    constexpr uint32_t DB = HD / 16, NP = I8 ? 1 : 2, MW = DB / 4;
+    typedef Rows<HD, I8, QB, true> RW;
+    typedef typename RW::S S;
+    __shared__ __attribute__((aligned(1024))) uint8_t sm0[S::BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t sm1[S::BYTES];
+    __shared__ __attribute__((aligned(16))) int32_t stab[4096];
+    __shared__ int32_t vsum[NP][HD];
+    const uint32_t head = blockIdx.y, z = blockIdx.z;
+    const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);
+    const uint32_t per = tl.steps(wk.splits), parts = tl.parts(wk.splits);
+    if (!tl.on || z >= parts) return;
+    stage_tab(stab, tab);
+    const RW rw(c, bt, a, tl, head);
+    const uint32_t g = rw.g, c16 = rw.c16, w = rw.w, beg = z * per, end = min((z + 1) * per, tl.nt);
+    const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+    int mxs[QB];
+    v4i acc[3][DB][QB], vs[NP][MW];
+    v4i sh[QB], sl[QB];                        // int16: sums of w's bytes, from MFMAs against ones
+    int64_t wsum[QB];
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) {
+        const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
+        mxs[qb] = row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts);
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
+        sh[qb] = sl[qb] = zero;
+        wsum[qb] = 0;
+    }
+#pragma unroll
+    for (uint32_t m = 0; m < MW; m++) vs[0][m] = vs[NP - 1][m] = zero;
+    rw.run(sm0, sm1, beg, end, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
+        const uint32_t kg = tl.lo + 64 * i + 16 * g;
+        const bool full = rw.whole(i, ids);
+        v4i p[QB][I8 ? 3 : 2];
+#pragma unroll
+        for (uint32_t kb = 0; kb < 4; kb++)
+            rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
+                uint32_t e[4];
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) e[r] = weight((uint32_t)(mxs[qb] - sat16i(x[r] >> 8)), a.smx, stab);
+                if (!full) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) {
+                        const uint32_t key = kg + 4 * kb + r;
+                        if (!(ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb])) e[r] = 0;
+                    }
+                }
+                uint32_t es = 0;
+                if constexpr (I8) {
+                    wsum[qb] += e[0] + e[1] + e[2] + e[3];
+                    es = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
+                }
+                weight_bytes<I8>(e[0], e[1], e[2], e[3], es, p[qb], kb);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        if constexpr (!I8) {
+#pragma unroll
+            for (uint32_t qb = 0; qb < QB; qb++) {
+                sh[qb] = mfma(ones, p[qb][1], sh[qb]);
+                sl[qb] = mfma(ones, p[qb][0], sl[qb]);
+            }
+        }
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) {
+            const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * m + c16) * 16;
+            const v4i vh = *reinterpret_cast<const v4i*>(vp);
+            v4i vl = zero;
+            if constexpr (!I8) vl = *reinterpret_cast<const v4i*>(vp + 64 * HD);
+#pragma unroll
+            for (uint32_t qb = 0; qb < QB; qb++) {
+                if constexpr (I8) {
+                    acc[0][m][qb] = mfma(vh, p[qb][I8 ? 2 : 0], acc[0][m][qb]);
+                    acc[1][m][qb] = mfma(vh, p[qb][1], acc[1][m][qb]);
+                    acc[2][m][qb] = mfma(vh, p[qb][0], acc[2][m][qb]);
+                } else {
+                    acc[0][m][qb] = mfma(vh, p[qb][1], acc[0][m][qb]);
+                    acc[1][m][qb] = mfma(vh, p[qb][0], acc[1][m][qb]);
+                    acc[2][m][qb] = mfma(vl, p[qb][0], acc[2][m][qb]);
+                    acc[1][m][qb] = mfma(vl, p[qb][1], acc[1][m][qb]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (m % 4 == w) {                  // V's sums: each wavefront its share of d
+                vs[0][m / 4] = mfma(vh, ones, vs[0][m / 4]);
+                if constexpr (!I8) vs[NP - 1][m / 4] = mfma(vl, ones, vs[NP - 1][m / 4]);
+            }
+        }
+    });
+    if (c16 == 0) {
+#pragma unroll
+        for (uint32_t m = 0; m < MW; m++)
+#pragma unroll
+            for (uint32_t pl = 0; pl < NP; pl++)
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) vsum[pl][16 * (w + 4 * m) + 4 * g + r] = vs[pl][m][r];
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);                // the TAB's copies too, where there were no steps
+    __syncthreads();
+    const int64_t keys = end > beg ? (int64_t)(end - beg) * 64 : 0;
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) {
+        int64_t sum;
+        if constexpr (I8) {
+            sum = wsum[qb];
+            sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
+            sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
+        } else {
+            sum = (int64_t)sh[qb][0] * 256 + sl[qb][0] + 32896 * keys;
+        }
+        const uint32_t row = rw.row_of(qb);
+        if (row >= tl.rows) continue;
+        int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
+        int64_t* pp = wk.part + ((((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits + z) * (HD + 1);
+        if (parts > 1 && g == 0) pp[HD] = sum;
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) {
+            int y[4];
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t d = 16 * m + 4 * g + r;
+                const int64_t x = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
+                if (parts > 1) pp[d] = x;
+                else y[r] = finish(x, sum, a.fp);
+            }
+            if (parts == 1)
+                *reinterpret_cast<uint2*>(op + 16 * m + 4 * g) =
+                    make_uint2((uint32_t)(uint16_t)y[0] | (uint32_t)(uint16_t)y[1] << 16,
+                               (uint32_t)(uint16_t)y[2] | (uint32_t)(uint16_t)y[3] << 16);
+        }
     }
 }
 
 // ---------------------------------------------------------------- the host's checks
 constexpr uint32_t kMaxKeys = 1u << 20;
+constexpr uint32_t kMaxPart = 32768;           // keys of a part of a tile
+constexpr uint64_t kMaxScores = 1ull << 28;    // bytes of scores that a call keeps
 
 int view(const cm_paged_cache* cache, const cm_paged_batch* batch, Cache* c, Batch* b) {
     if (cache == nullptr || batch == nullptr) return fail(CM_EINVAL, "paged: a null cache or batch");
@@ -589,18 +1093,53 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     DeviceState* st;
     if ((rc = state(&st))) return rc;
     const uint32_t cm24 = smx_cm & 0xFFFFFFu, cs = smx_cfg & 63u, G = heads / c.kv;
-    const Attn a{q, o, q_ld, o_ld, G, window, cm24, cs, fp, smx_dlim(cm24, cs)};
-    const uint64_t slots = (uint64_t)b.tokens * G / 16 + b.batch;
+    const Attn a{q, o, q_ld, o_ld, G, window, fp, smx_of(cm24, cs)};
+    // few rows a sequence: tiles of 16 rows that keep their scores; otherwise (or where the scores would take more than
+    // kMaxScores) tiles of 64 or 128 rows that compute them twice
+    const uint64_t rows = (uint64_t)b.tokens * heads;
+    const bool few = (uint64_t)b.tokens * G < 32u * (uint64_t)b.batch && rows * b.cap * 2 <= kMaxScores;
+    const uint32_t R = few ? 16 : cache->head_dim == 64 ? 128 : 64;
+    const uint64_t slots = (uint64_t)b.tokens * G / R + b.batch;
     if (slots > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
-    const dim3 grid((unsigned)slots, c.kv);
-#define CM_ATTN(HD, I8) \
-    CM_LAUNCH("paged_attention_kernel", (paged_attention_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, st->smx_tab)
+    // parts of a tile's keys: enough workgroups to fill the chip, at most kMaxPart keys each (the int32 limb sums: a
+    // product is below 2^14, two a key in the middle limbs)
+    const uint32_t most = (b.cap / 64 + kMinSteps - 1) / kMinSteps;
+    const uint64_t want = (4ull * st->cus + slots * c.kv - 1) / (slots * c.kv);
+    const uint32_t splits = (uint32_t)std::max<uint64_t>({std::min<uint64_t>(want, most), (b.cap + kMaxPart - 1) / kMaxPart, 1});
+    if (splits > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits);
+    const size_t mx_bytes = round_up(rows * splits * 4, 256), sc_bytes = few ? round_up(rows * b.cap * 2, 256) : 0;
+    const size_t part_bytes = splits > 1 ? rows * splits * (cache->head_dim + 1) * 8 : 0;
+    void* ws;
+    if ((rc = workspace(st, mx_bytes + sc_bytes + part_bytes, &ws, s))) return rc;
+    Work wk;
+    wk.mx = static_cast<int32_t*>(ws);
+    wk.sc = reinterpret_cast<int16_t*>(static_cast<uint8_t*>(ws) + mx_bytes);
+    wk.part = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(ws) + mx_bytes + sc_bytes);
+    wk.splits = splits;
+    const dim3 grid((unsigned)slots, c.kv, splits), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
+#define CM_FEW(HD, I8)                                                                                                  \
+    CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk);                \
+    CM_LAUNCH("paged_few_kernel", (paged_few_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);         \
+    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_join_kernel<HD, 16>), jgrid, dim3(256), 0, s, b, a, wk); }
+#define CM_ROWS(HD, I8, QB)                                                                                             \
+    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk);                  \
+    CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);   \
+    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_join_kernel<HD, 64 * QB>), jgrid, dim3(256), 0, s, b, a, wk); }
     if (cache->head_dim == 64) {
-        if (cache->int8) { CM_ATTN(64, true); } else { CM_ATTN(64, false); }
+        if (cache->int8) {
+            if (few) { CM_FEW(64, true) } else { CM_ROWS(64, true, 2) }
+        } else {
+            if (few) { CM_FEW(64, false) } else { CM_ROWS(64, false, 2) }
+        }
     } else {
-        if (cache->int8) { CM_ATTN(128, true); } else { CM_ATTN(128, false); }
+        if (cache->int8) {
+            if (few) { CM_FEW(128, true) } else { CM_ROWS(128, true, 1) }
+        } else {
+            if (few) { CM_FEW(128, false) } else { CM_ROWS(128, false, 1) }
+        }
     }
-#undef CM_ATTN
+#undef CM_FEW
+#undef CM_ROWS
     return CM_OK;
 }
 
