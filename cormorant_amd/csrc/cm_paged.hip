@@ -5,6 +5,7 @@
 // q.K^T) and V transposed (keys contiguous for P.V), so the attention neither splits nor transposes
 // what it reads: an int16 x is 256 h + l + 128 (h = x >> 8, l = (x & 255) - 128).
 #include <algorithm>
+#include <type_traits>
 
 #include "cm_common.h"
 #include "cm_rowops_math.h"
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Cache c, Batch bt, int1
 // y >= 17 * 4096, e is 0, and y there stays below 2^17 (a shift below 32): the host replaces register pairs
 // whose single step passes 15 octaves by one of the same exponentials.
 struct Smx {
-    uint32_t cm, cs, dlim;
+    uint32_t cm, cs, dlim;                     // dlim at most 65535: no d passes it
 };
 
 Smx smx_of(uint32_t cm24, uint32_t cs) {
@@ -280,6 +281,7 @@ Smx smx_of(uint32_t cm24, uint32_t cs) {
         r.dlim = step > 65536u ? 1u : 2u;      // above 2^16: e(1) = 0
         r.cm = step > 65536u ? kSmxYZero : (step < 65535u ? step : 65535u);   // e(1) is 1 at 65535 as at 65536
     }
+    r.dlim = r.dlim < 65535u ? r.dlim : 65535u;
     if (r.cs >= 2) r.cs -= 2;
     else {
         r.cm <<= 2 - r.cs;                     // below 2^20: step < 61440 * 2^cs, or the pairs above
@@ -288,14 +290,33 @@ Smx smx_of(uint32_t cm24, uint32_t cs) {
     return r;
 }
 
-// w = min(e, 65535), tab = the 4096 words in LDS
-__device__ __forceinline__ uint32_t weight(uint32_t d, const Smx& x, const int32_t* tab) {
-    d = min(d, x.dlim);
-    const uint64_t p = (uint64_t)(d & 0xFFFFFFu) * (x.cm & 0xFFFFFFu);
-    const uint32_t y4 = (uint32_t)(p >> x.cs);
-    const uint32_t t = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(tab) + (y4 & 0x3FFCu));
-    return min(t >> (y4 >> 14), 65535u);
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+// The exponentials of two scores s (saturated to int16 as they are packed) under the maximum m: the TAB words and
+// their shifts; w = min(word >> shift, 65535) is taken where two are packed again (v_cvt_pk_u16_u32 saturates).
+// dl = min(dlim, 65535): d <= 65535.
+struct Exp2 {
+    uint32_t t0, t1, k0, k1;
+    __device__ __forceinline__ uint32_t e0() const { return t0 >> k0; }
+    __device__ __forceinline__ uint32_t e1() const { return t1 >> k1; }
+};
+__device__ __forceinline__ Exp2 exps(int s0, int s1, uint32_t m2, uint32_t dl2, const Smx& x, const int32_t* tab) {
+    const u16x2 s = __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pk_i16(s0, s1));
+    const u16x2 d = __builtin_elementwise_min(__builtin_bit_cast(u16x2, m2) - s, __builtin_bit_cast(u16x2, dl2));
+    const uint32_t y0 = (uint32_t)(((uint64_t)d[0] * (x.cm & 0xFFFFFFu)) >> x.cs);
+    const uint32_t y1 = (uint32_t)(((uint64_t)d[1] * (x.cm & 0xFFFFFFu)) >> x.cs);
+    const uint8_t* tb = reinterpret_cast<const uint8_t*>(tab);
+    return Exp2{*reinterpret_cast<const uint32_t*>(tb + (y0 & 0x3FFCu)), *reinterpret_cast<const uint32_t*>(tb + (y1 & 0x3FFCu)),
+                y0 >> 14, y1 >> 14};
 }
+__device__ __forceinline__ uint32_t pair16(uint32_t a, uint32_t b) {      // saturated to 65535
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_u16(a, b));
+}
+__device__ __forceinline__ uint32_t add16(uint32_t p, uint32_t sum) {     // sum + both halves of p
+    return __builtin_amdgcn_udot2(__builtin_bit_cast(u16x2, p), u16x2{1, 1}, sum, false);
+}
+__device__ __forceinline__ uint32_t twice(uint32_t x) { return (x & 0xFFFFu) | x << 16; }
 
 struct Attn {
     const int16_t* q;
@@ -387,22 +408,20 @@ __device__ __forceinline__ int64_t whole_sum(int a0, int a1, int a2, int vs0, in
     return x + (I8 ? (int64_t)vs0 * (128 * 65793) : ((int64_t)vs0 * 256 + vs1) * 32896 + 128 * wsum);
 }
 
-// four weights (int8: shifted by the bytes of es) -> dword q of the byte operands
+// four weights as two pairs (int8: shifted by the bytes of es) -> dword q of the byte operands
 template <bool I8>
-__device__ __forceinline__ void weight_bytes(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t es, v4i (&p)[I8 ? 3 : 2],
-                                             uint32_t q) {
+__device__ __forceinline__ void weight_bytes(uint32_t w01, uint32_t w23, uint32_t es, v4i (&p)[I8 ? 3 : 2], uint32_t q) {
     if constexpr (I8) {
-        x0 <<= es & 15u;
-        x1 <<= (es >> 8) & 15u;
-        x2 <<= (es >> 16) & 15u;
-        x3 <<= (es >> 24) & 15u;
-    }
-    const uint32_t t01 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), t23 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
-    p[0][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x05040100u) ^ 0x80808080u);
-    p[1][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x07060302u) ^ 0x80808080u);
-    if constexpr (I8) {
+        const uint32_t x0 = (w01 & 0xFFFFu) << (es & 15u), x1 = (w01 >> 16) << ((es >> 8) & 15u);
+        const uint32_t x2 = (w23 & 0xFFFFu) << ((es >> 16) & 15u), x3 = (w23 >> 16) << ((es >> 24) & 15u);
+        const uint32_t t01 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), t23 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+        p[0][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x05040100u) ^ 0x80808080u);
+        p[1][q] = (int)(__builtin_amdgcn_perm(t23, t01, 0x07060302u) ^ 0x80808080u);
         const uint32_t u01 = __builtin_amdgcn_perm(x1, x0, 0x0c0c0602u), u23 = __builtin_amdgcn_perm(x3, x2, 0x0c0c0602u);
         p[2][q] = (int)(__builtin_amdgcn_perm(u23, u01, 0x05040100u) ^ 0x80808080u);
+    } else {
+        p[0][q] = (int)(__builtin_amdgcn_perm(w23, w01, 0x06040200u) ^ 0x80808080u);
+        p[1][q] = (int)(__builtin_amdgcn_perm(w23, w01, 0x07050301u) ^ 0x80808080u);
     }
 }
 
@@ -538,7 +557,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
     const bool mine = tl.row0 + c16 < tl.rows;
     const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
     const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
-    const int mxs = row_max(wk, wrow, parts);
+    const uint32_t m2 = twice((uint32_t)row_max(wk, wrow, parts)), dl2 = twice(a.smx.dlim);
     const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
     __builtin_amdgcn_s_waitcnt(0x0070);
     __syncthreads();
@@ -570,18 +589,18 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
         v4i es = zero;
         if constexpr (I8) es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
         const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        uint32_t e[16], sum = 0;
+        v4i p[I8 ? 3 : 2];
+        uint32_t wp[8], sum = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 16; j++) {
-            const int s = j & 1 ? (int)sw[j / 2] >> 16 : (int)(int16_t)sw[j / 2];
-            const bool on = id < c.pages && kg + j >= vbeg && kg + j < vend;
-            e[j] = on ? weight((uint32_t)(mxs - s), a.smx, stab) : 0u;
-            sum += e[j];
+        for (uint32_t j = 0; j < 8; j++) {
+            const Exp2 x = exps((int)(int16_t)sw[j], (int)sw[j] >> 16, m2, dl2, a.smx, stab);
+            auto on = [&](uint32_t key) { return id < c.pages && key >= vbeg && key < vend; };
+            wp[j] = pair16(on(kg + 2 * j) ? x.e0() : 0u, on(kg + 2 * j + 1) ? x.e1() : 0u);
+            sum = add16(wp[j], sum);
         }
         wsum += sum;
-        v4i p[I8 ? 3 : 2];
 #pragma unroll
-        for (uint32_t q = 0; q < 4; q++) weight_bytes<I8>(e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3], (uint32_t)es[q], p, q);
+        for (uint32_t q = 0; q < 4; q++) weight_bytes<I8>(wp[2 * q], wp[2 * q + 1], (uint32_t)es[q], p, q);
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
             if constexpr (I8) {
@@ -738,58 +757,54 @@ struct Rows {
             }
         }
     }
-    // the raw sums of keys 16 g + 4 kb + r, r < 4, for every query block: f(qb, sums)
-    template <class F>
-    __device__ __forceinline__ void dots(const uint8_t* sm, uint32_t kb, F f) const {
-        const v4i zero = {0, 0, 0, 0};
+    // the K operands of keys 16 g + 4 kb + r, r < 4, their terms and shifts
+    struct Frag {
+        v4i kh[KS], kl[KS], term;
+        uint32_t es;
+    };
+    __device__ __forceinline__ void load(const uint8_t* sm, uint32_t kb, Frag& f) const {
         const uint32_t row = 16 * (c16 >> 2) + 4 * kb + (c16 & 3);
-        const v4i term = *reinterpret_cast<const v4i*>(sm + S::TERM + 4 * (16 * g + 4 * kb));
-        v4i kh[KS], kl[KS];
+        f.term = *reinterpret_cast<const v4i*>(sm + S::TERM + 4 * (16 * g + 4 * kb));
 #pragma unroll
         for (uint32_t s = 0; s < KS; s++) {
             const uint32_t x = KS == 1 ? c16 >> 2 : ((c16 >> 1) & 1) | (c16 >> 2) << 1;
             const uint8_t* kp = sm + row * HD + 16 * ((4 * s + g) ^ x);
-            kh[s] = *reinterpret_cast<const v4i*>(kp);
-            if constexpr (!I8) kl[s] = *reinterpret_cast<const v4i*>(kp + 64 * HD);
-            else kl[s] = zero;
+            f.kh[s] = *reinterpret_cast<const v4i*>(kp);
+            if constexpr (!I8) f.kl[s] = *reinterpret_cast<const v4i*>(kp + 64 * HD);
+            else f.kl[s] = v4i{0, 0, 0, 0};
         }
-        uint32_t es = 0;
-        if constexpr (I8) es = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 256 + 16 * g + 4 * kb);
+        if constexpr (I8) f.es = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 256 + 16 * g + 4 * kb);
+        else f.es = 0;
+    }
+    __device__ __forceinline__ void products(const Frag& f, uint32_t qb, v4i& hh, v4i& mid, v4i& ll) const {
+        hh = mid = v4i{0, 0, 0, 0};
+        ll = f.term;
 #pragma unroll
-        for (uint32_t qb = 0; qb < QB; qb++) {
-            v4i hh = zero, mid = zero, ll = term;
-#pragma unroll
-            for (uint32_t s = 0; s < KS; s++) qk<I8>(kh[s], kl[s], qh[qb][s], ql[qb][s], hh, mid, ll);
-            int x[4];
-#pragma unroll
-            for (uint32_t r = 0; r < 4; r++) x[r] = raw_sum<I8>(hh[r], mid[r], ll[r], es, r, qterm[qb]);
-            f(qb, x);
-        }
+        for (uint32_t s = 0; s < KS; s++) qk<I8>(f.kh[s], f.kl[s], qh[qb][s], ql[qb][s], hh, mid, ll);
     }
     // whether every row sees all 64 keys of a step, its pages all there
     __device__ __forceinline__ bool whole(uint32_t i, uint32_t id4) const {
         const uint32_t k0 = tl.lo + 64 * i;
         return k0 >= tl.all_lo && k0 + 64 <= tl.all_hi && __ballot(id4 == ~0u) == 0;
     }
-    // body(stage, step, ids) for the steps [i, end), two stages deep
+    // body(stage, step, ids) for the steps [i, end), two stages deep; an odd count is made even by a step without pages
+    // (a loop that may end between its halves has the accumulators moved from registers to registers)
     template <class F>
     __device__ __forceinline__ void run(uint8_t* sm0, uint8_t* sm1, uint32_t i, uint32_t end, F body) const {
         if (i >= end) return;
         uint32_t id0 = ids(i, end), id1 = ids(i + 1, end);
         stage(sm0, i, id0);
-        for (;; i += 2) {
+        for (; i < end; i += 2) {
             __builtin_amdgcn_s_waitcnt(0x0070);        // this wavefront's copies
             __syncthreads();                           // every wavefront's; the other stage read
             const uint32_t id2 = ids(i + 2, end);
-            if (i + 1 < end) stage(sm1, i + 1, id1);
+            stage(sm1, i + 1, id1);
             body(sm0, i, id0);
-            if (i + 1 >= end) break;
             __builtin_amdgcn_s_waitcnt(0x0070);
             __syncthreads();
             const uint32_t id3 = ids(i + 3, end);
             if (i + 2 < end) stage(sm0, i + 2, id2);
             body(sm1, i + 1, id1);
-            if (i + 2 >= end) break;
             id0 = id2;
             id1 = id3;
         }
@@ -811,23 +826,36 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
     for (uint32_t qb = 0; qb < QB; qb++) mx[qb] = kNone;
     rw.run(sm0, sm1, z * per, min((z + 1) * per, tl.nt), [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
         const uint32_t kg = tl.lo + 64 * i + 16 * rw.g;
-        if (rw.whole(i, ids)) {
+        constexpr uint32_t NB = 4 * QB;
+        auto maxima = [&](auto masked) {
+            typename RW::Frag f;
+            v4i h[2], md[2], l[2];
+            uint32_t es[2];
+            rw.load(sm, 0, f);
 #pragma unroll
-            for (uint32_t kb = 0; kb < 4; kb++)
-                rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
-                    mx[qb] = max(max(mx[qb], max(x[0], x[1])), max(x[2], x[3]));
-                });
-        } else {
-#pragma unroll
-            for (uint32_t kb = 0; kb < 4; kb++)
-                rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
+            for (uint32_t j = 0; j < NB + 1; j++) {
+                if (j < NB) {
+                    rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
+                    es[j & 1] = f.es;
+                    if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
+                }
+                if (j >= 1) {
+                    const uint32_t y = j - 1, qb = y % QB;
 #pragma unroll
                     for (uint32_t r = 0; r < 4; r++) {
-                        const uint32_t key = kg + 4 * kb + r;
-                        mx[qb] = max(mx[qb], ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? x[r] : kNone);
+                        int z = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]);
+                        if constexpr (masked) {
+                            const uint32_t key = kg + 4 * (y / QB) + r;
+                            z = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? z : kNone;
+                        }
+                        mx[qb] = max(mx[qb], z);
                     }
-                });
-        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (rw.whole(i, ids)) maxima(std::false_type{});
+        else maxima(std::true_type{});
     });
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
@@ -856,53 +884,69 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     const RW rw(c, bt, a, tl, head);
     const uint32_t g = rw.g, c16 = rw.c16, w = rw.w, beg = z * per, end = min((z + 1) * per, tl.nt);
     const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-    int mxs[QB];
+    uint32_t m2[QB];
+    const uint32_t dl2 = twice(a.smx.dlim);
     v4i acc[3][DB][QB], vs[NP][MW];
-    v4i sh[QB], sl[QB];                        // int16: sums of w's bytes, from MFMAs against ones
-    int64_t wsum[QB];
+    uint32_t wsum[QB];                         // the lane's keys' weights: below 2^16 * 16 * kMaxPart / 64
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
         const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
-        mxs[qb] = row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts);
+        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts));
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
-        sh[qb] = sl[qb] = zero;
         wsum[qb] = 0;
     }
 #pragma unroll
     for (uint32_t m = 0; m < MW; m++) vs[0][m] = vs[NP - 1][m] = zero;
     rw.run(sm0, sm1, beg, end, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
         const uint32_t kg = tl.lo + 64 * i + 16 * g;
-        const bool full = rw.whole(i, ids);
         v4i p[QB][I8 ? 3 : 2];
+        // the step's blocks (16 keys x 16 rows) in three stages, a block's products under the exponentials of the one
+        // before and the packing of the one before that
+        constexpr uint32_t NB = 4 * QB;
+        auto weights = [&](auto masked) {
+            typename RW::Frag f;
+            v4i h[2], md[2], l[2];
+            uint32_t es[2];
+            Exp2 e[2];
+            rw.load(sm, 0, f);
 #pragma unroll
-        for (uint32_t kb = 0; kb < 4; kb++)
-            rw.dots(sm, kb, [&](uint32_t qb, const int (&x)[4]) {
-                uint32_t e[4];
+            for (uint32_t j = 0; j < NB + 2; j++) {
+                if (j < NB) {
+                    rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
+                    es[j & 1] = f.es;
+                    if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
+                }
+                if (j >= 2) {
+                    const uint32_t y = j - 2, kb = y / QB, qb = y % QB;
+                    uint32_t v[4] = {e[0].e0(), e[0].e1(), e[1].e0(), e[1].e1()};
+                    if constexpr (masked) {
 #pragma unroll
-                for (uint32_t r = 0; r < 4; r++) e[r] = weight((uint32_t)(mxs[qb] - sat16i(x[r] >> 8)), a.smx, stab);
-                if (!full) {
-#pragma unroll
-                    for (uint32_t r = 0; r < 4; r++) {
-                        const uint32_t key = kg + 4 * kb + r;
-                        if (!(ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb])) e[r] = 0;
+                        for (uint32_t r = 0; r < 4; r++) {
+                            const uint32_t key = kg + 4 * kb + r;
+                            v[r] = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? v[r] : 0u;
+                        }
                     }
+                    const uint32_t w01 = pair16(v[0], v[1]), w23 = pair16(v[2], v[3]);
+                    wsum[qb] = add16(w01, add16(w23, wsum[qb]));
+                    uint32_t ve = 0;
+                    if constexpr (I8) ve = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
+                    weight_bytes<I8>(w01, w23, ve, p[qb], kb);
                 }
-                uint32_t es = 0;
-                if constexpr (I8) {
-                    wsum[qb] += e[0] + e[1] + e[2] + e[3];
-                    es = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
-                }
-                weight_bytes<I8>(e[0], e[1], e[2], e[3], es, p[qb], kb);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        if constexpr (!I8) {
+                if (j >= 1 && j <= NB) {
+                    const uint32_t y = j - 1, qb = y % QB;
+                    int z[4];
 #pragma unroll
-            for (uint32_t qb = 0; qb < QB; qb++) {
-                sh[qb] = mfma(ones, p[qb][1], sh[qb]);
-                sl[qb] = mfma(ones, p[qb][0], sl[qb]);
+                    for (uint32_t r = 0; r < 4; r++)
+                        z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
+                    e[0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
+                    e[1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
+        };
+        if (rw.whole(i, ids)) weights(std::false_type{});
+        else weights(std::true_type{});
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
             const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * m + c16) * 16;
@@ -922,11 +966,12 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
                     acc[1][m][qb] = mfma(vl, p[qb][1], acc[1][m][qb]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (m % 4 == w) {                  // V's sums: each wavefront its share of d
-                vs[0][m / 4] = mfma(vh, ones, vs[0][m / 4]);
-                if constexpr (!I8) vs[NP - 1][m / 4] = mfma(vl, ones, vs[NP - 1][m / 4]);
-            }
+        }
+#pragma unroll
+        for (uint32_t m = 0; m < MW; m++) {    // V's sums: each wavefront its share of d
+            const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * (w + 4 * m) + c16) * 16;
+            vs[0][m] = mfma(*reinterpret_cast<const v4i*>(vp), ones, vs[0][m]);
+            if constexpr (!I8) vs[NP - 1][m] = mfma(*reinterpret_cast<const v4i*>(vp + 64 * HD), ones, vs[NP - 1][m]);
         }
     });
     if (c16 == 0) {
@@ -939,17 +984,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     }
     __builtin_amdgcn_s_waitcnt(0x0070);                // the TAB's copies too, where there were no steps
     __syncthreads();
-    const int64_t keys = end > beg ? (int64_t)(end - beg) * 64 : 0;
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
-        int64_t sum;
-        if constexpr (I8) {
-            sum = wsum[qb];
-            sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
-            sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
-        } else {
-            sum = (int64_t)sh[qb][0] * 256 + sl[qb][0] + 32896 * keys;
-        }
+        int64_t sum = wsum[qb];
+        sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
+        sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
         const uint32_t row = rw.row_of(qb);
         if (row >= tl.rows) continue;
         int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
