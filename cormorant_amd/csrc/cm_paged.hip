@@ -337,22 +337,35 @@ __device__ __forceinline__ void limbs16(const int16_t* p, v4i& hi, v4i& lo, int&
     lo = v4i{(int)la.x, (int)la.y, (int)lb.x, (int)lb.y};
 }
 
-// floor(2^(fp - 8) A / S + 1/2) saturated to int16: the quotient estimated in double (2 |A| 2^7 < 2^60, S <
-// 2^37), put right by the int64 remainder
-__device__ __forceinline__ int finish(int64_t A, int64_t S, uint32_t fp) {
-    if (S == 0) return 0;
-    const int64_t num = fp >= 8 ? 2 * (A * ((int64_t)1 << (fp - 8))) + S : 2 * A + (S << (8 - fp));
-    const int64_t den = 2 * (fp >= 8 ? S : S << (8 - fp));
-    int64_t f = (int64_t)floor((double)num / (double)den);
-    const int64_t r = num - f * den;
-    f += r >= den ? 1 : r < 0 ? -1 : 0;
-    return (int)(f > 32767 ? 32767 : f < -32768 ? -32768 : f);
+// floor(2^(fp - 8) A / S + 1/2) saturated to int16, A and S the exact sums of a row.  The quotient is estimated with
+// the row's reciprocal in double (at most 2^23, the estimate off by less than 2^-27) and put right by the remainder
+// in int64: 2 |A| 2^7 < 2^59 and f den < 2^61.
+struct Divide {
+    int64_t S, den;
+    double inv;
+    uint32_t fp;
+    __device__ __forceinline__ Divide(int64_t S_, uint32_t fp_) : S(S_), fp(fp_) {
+        den = fp >= 8 ? 2 * S : S << (9 - fp);
+        inv = S ? 1.0 / (double)den : 0.0;
+    }
+    __device__ __forceinline__ int operator()(int64_t A) const {
+        const int64_t num = (fp >= 8 ? A << (fp - 7) : 2 * A) + (den >> 1);
+        int f = (int)floor((double)num * inv);
+        const int64_t r = num - (int64_t)f * den;
+        f += r >= den ? 1 : r < 0 ? -1 : 0;
+        return S ? sat16i(f) : 0;
+    }
+};
+
+__device__ __forceinline__ void store_out(int16_t* p, const Divide& q, const int64_t (&x)[4]) {
+    const uint32_t y0 = (uint32_t)q(x[0]), y1 = (uint32_t)q(x[1]), y2 = (uint32_t)q(x[2]), y3 = (uint32_t)q(x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2((y0 & 0xFFFFu) | y1 << 16, (y2 & 0xFFFFu) | y3 << 16);
 }
 
 // ---- the split of the work.  A tile is R rows (token, head of the group) of one sequence and KV head; sequence b's
 // tiles have the slots from floor(start(b) G / R) + b on (at least as many as it needs, known without a scan).  The
-// 64-key steps that any row of the tile sees are divided over up to `splits` workgroups, kMinSteps each at least.
-constexpr uint32_t kMinSteps = 4;
+// 64-key steps that any row of the tile sees go to workgroups in parts of `per` steps (the same for every tile: a short
+// sequence has fewer parts, not smaller ones).
 
 template <uint32_t R>
 struct Tile {
@@ -386,8 +399,7 @@ struct Tile {
     __device__ __forceinline__ uint32_t begin(const Attn& a, uint32_t tk) const {
         return a.window ? (uint32_t)max(base + (int)tk + 1 - (int)a.window, 0) : 0u;
     }
-    __device__ __forceinline__ uint32_t steps(uint32_t splits) const { return max((nt + splits - 1) / splits, kMinSteps); }
-    __device__ __forceinline__ uint32_t parts(uint32_t splits) const { return nt ? (nt + steps(splits) - 1) / steps(splits) : 1u; }
+    __device__ __forceinline__ uint32_t parts(uint32_t per) const { return max((nt + per - 1) / per, 1u); }
 };
 
 // The call's workspace: per row (head, token, head of the group: (head T + token) G + i) the maxima of its parts,
@@ -395,8 +407,9 @@ struct Tile {
 struct Work {
     int32_t* mx;                           // [rows][splits] raw q.K^T sums, kNone: no key
     int16_t* sc;                           // [rows][cap]
-    int64_t* part;                         // [rows][splits][HD + 1]
-    uint32_t splits;
+    int64_t* part;                         // few rows: [rows][splits][HD + 1]; many: [tile][splits][R HD + R], each
+                                           // tile in its lanes' order (1 KiB a store)
+    uint32_t splits, per;                  // most parts of a tile, steps of a part
 };
 constexpr int kNone = (int)0x80000000;
 
@@ -465,8 +478,8 @@ __global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, At
     const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
     const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
     const Tile<16> tl(bt, a, blockIdx.x);
-    const uint32_t per = tl.steps(wk.splits);
-    if (!tl.on || z * per >= max(tl.nt, 1u)) return;
+    const uint32_t per = wk.per;
+    if (!tl.on || z >= tl.parts(per)) return;
     const uint32_t row = min(tl.row0 + c16, tl.rows - 1), tok = row / a.G;
     const bool mine = tl.row0 + c16 < tl.rows;
     const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
@@ -532,10 +545,18 @@ __global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, At
     if (t < 16 && mine) wk.mx[wrow * wk.splits + z] = max(max(redm[0][t], redm[1][t]), max(redm[2][t], redm[3][t]));
 }
 
-// the maximum score of a row over its parts
-__device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t parts) {
+// the maximum score of a row over its parts: the four lanes of a row (groups g) take every fourth, loads in fours
+__device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t parts, uint32_t g) {
+    const int32_t* p = wk.mx + wrow * wk.splits;
     int m = kNone;
-    for (uint32_t i = 0; i < parts; i++) m = max(m, wk.mx[wrow * wk.splits + i]);
+    for (uint32_t i = g; i < parts; i += 16) {
+        int x[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) x[k] = p[min(i + 4 * k, parts - 1)];
+        m = max(max(m, max(x[0], x[1])), max(x[2], x[3]));
+    }
+    m = max(m, __shfl_xor(m, 16, 64));
+    m = max(m, __shfl_xor(m, 32, 64));
     return sat16i(m >> 8);
 }
 
@@ -549,7 +570,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
     const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
     const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
     const Tile<16> tl(bt, a, blockIdx.x);
-    const uint32_t per = tl.steps(wk.splits), parts = tl.parts(wk.splits);
+    const uint32_t per = wk.per, parts = tl.parts(per);
     if (!tl.on || z >= parts) return;
     stage_tab(stab, tab);
     for (uint32_t i = t; i < 16 * (HD + 1); i += 256) (&part[0][0])[i] = 0;
@@ -557,7 +578,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
     const bool mine = tl.row0 + c16 < tl.rows;
     const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
     const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
-    const uint32_t m2 = twice((uint32_t)row_max(wk, wrow, parts)), dl2 = twice(a.smx.dlim);
+    const uint32_t m2 = twice((uint32_t)row_max(wk, wrow, parts, g)), dl2 = twice(a.smx.dlim);
     const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
     __builtin_amdgcn_s_waitcnt(0x0070);
     __syncthreads();
@@ -632,7 +653,8 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
         if (rw >= tl.rows) break;
         const int64_t S = reds[0][r] + reds[1][r] + reds[2][r] + reds[3][r];
         if (parts == 1) {
-            const int o0 = finish(part[r][d], S, a.fp), o1 = finish(part[r][d + 1], S, a.fp);
+            const Divide q(S, a.fp);
+            const int o0 = q(part[r][d]), o1 = q(part[r][d + 1]);
             *reinterpret_cast<uint32_t*>(a.o + (uint64_t)(tl.q0 + rw / a.G) * a.o_ld + (uint64_t)(head * a.G + rw % a.G) * HD + d) =
                 (uint32_t)(uint16_t)o0 | ((uint32_t)(uint16_t)o1 << 16);
         } else {
@@ -644,9 +666,8 @@ __global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn 
     }
 }
 
-// The parts' sums of a row added and divided: a wavefront per row, two columns a lane at 128 d.  R: the rows of the
-// tiles that made the parts.
-template <uint32_t HD, uint32_t R>
+// The parts' sums of a row added and divided: a wavefront per row, two columns a lane at 128 d.
+template <uint32_t HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work wk) {
     const uint32_t lane = threadIdx.x & 63, head = blockIdx.y;
     const uint32_t at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));   // row of (token, i)
@@ -654,8 +675,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work 
     if (tok >= bt.start(bt.batch)) return;
     const uint32_t b = find_le(bt.batch, tok, [&](uint32_t i) { return bt.start(i); });
     const uint32_t row = at - bt.start(b) * a.G;
-    const Tile<R> tl(bt, a, (uint32_t)((uint64_t)bt.start(b) * a.G / R) + b + row / R);
-    const uint32_t parts = tl.parts(wk.splits);
+    const Tile<16> tl(bt, a, (uint32_t)((uint64_t)bt.start(b) * a.G / 16) + b + row / 16);
+    const uint32_t parts = tl.parts(wk.per);
     if (!tl.on || parts == 1) return;
     const int64_t* pp = wk.part + ((uint64_t)head * bt.tokens * a.G + at) * wk.splits * (HD + 1);
     int64_t x[HD / 64], S = 0;
@@ -667,8 +688,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work 
         S += pp[HD];
     }
     int16_t* op = a.o + (uint64_t)tok * a.o_ld + (uint64_t)(head * a.G + at % a.G) * HD + lane * (HD / 64);
+    const Divide q(S, a.fp);
 #pragma unroll
-    for (uint32_t k = 0; k < HD / 64; k++) op[k] = (int16_t)finish(x[k], S, a.fp);
+    for (uint32_t k = 0; k < HD / 64; k++) op[k] = (int16_t)q(x[k]);
 }
 
 // ---------------------------------------------------------------- attention of many rows
@@ -818,8 +840,8 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[RW::S::BYTES];
     const uint32_t head = blockIdx.y, z = blockIdx.z;
     const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);             // the long tiles first
-    const uint32_t per = tl.steps(wk.splits);
-    if (!tl.on || z >= tl.parts(wk.splits)) return;
+    const uint32_t per = wk.per;
+    if (!tl.on || z >= tl.parts(per)) return;
     const RW rw(c, bt, a, tl, head);
     int mx[QB];
 #pragma unroll
@@ -878,10 +900,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     __shared__ int32_t vsum[NP][HD];
     const uint32_t head = blockIdx.y, z = blockIdx.z;
     const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);
-    const uint32_t per = tl.steps(wk.splits), parts = tl.parts(wk.splits);
+    const uint32_t per = wk.per, parts = tl.parts(per);
     if (!tl.on || z >= parts) return;
     stage_tab(stab, tab);
     const RW rw(c, bt, a, tl, head);
+    int64_t* part = wk.part + (((uint64_t)(gridDim.x - 1 - blockIdx.x) * c.kv + head) * wk.splits + z) * (RW::R * HD + RW::R);
     const uint32_t g = rw.g, c16 = rw.c16, w = rw.w, beg = z * per, end = min((z + 1) * per, tl.nt);
     const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
     uint32_t m2[QB];
@@ -891,7 +914,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
         const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
-        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts));
+        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts, g));
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
         wsum[qb] = 0;
@@ -990,25 +1013,59 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
         sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
         sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
         const uint32_t row = rw.row_of(qb);
-        if (row >= tl.rows) continue;
+        const bool on = row < tl.rows;
         int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
-        int64_t* pp = wk.part + ((((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits + z) * (HD + 1);
-        if (parts > 1 && g == 0) pp[HD] = sum;
+        const Divide quot(sum, a.fp);
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
-            int y[4];
+            int64_t x[4];
 #pragma unroll
             for (uint32_t r = 0; r < 4; r++) {
                 const uint32_t d = 16 * m + 4 * g + r;
-                const int64_t x = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
-                if (parts > 1) pp[d] = x;
-                else y[r] = finish(x, sum, a.fp);
+                x[r] = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
             }
-            if (parts == 1)
-                *reinterpret_cast<uint2*>(op + 16 * m + 4 * g) =
-                    make_uint2((uint32_t)(uint16_t)y[0] | (uint32_t)(uint16_t)y[1] << 16,
-                               (uint32_t)(uint16_t)y[2] | (uint32_t)(uint16_t)y[3] << 16);
+            if (parts > 1) {
+                longlong2* pp = reinterpret_cast<longlong2*>(part) + (((w * QB + qb) * DB + m) * 2) * 64 + rw.lane;
+                pp[0] = make_longlong2(x[0], x[1]);
+                pp[64] = make_longlong2(x[2], x[3]);
+            } else if (on) {
+                store_out(op + 16 * m + 4 * g, quot, x);
+            }
         }
+        if (parts > 1 && g == 0) part[RW::R * HD + 16 * (w * QB + qb) + c16] = sum;
+    }
+}
+
+// The parts' sums of a tile of many rows added and divided, in the lanes' order of paged_rows_kernel; a workgroup per
+// 16 columns, a wavefront's loads of four parts in flight at once.
+template <uint32_t HD, uint32_t QB>
+__global__ __launch_bounds__(256) void paged_rows_join_kernel(Cache c, Batch bt, Attn a, Work wk) {
+    constexpr uint32_t DB = HD / 16, R = 64 * QB;
+    const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, slot = blockIdx.x;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = blockIdx.z;
+    const Tile<R> tl(bt, a, slot);
+    const uint32_t parts = tl.parts(wk.per);
+    if (!tl.on || parts == 1) return;
+    const int64_t* part = wk.part + ((uint64_t)slot * c.kv + head) * wk.splits * (R * HD + R);
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) {
+        const uint32_t wq = w * QB + qb, row = tl.row0 + 16 * wq + c16;
+        if (tl.row0 + 16 * wq >= tl.rows) break;
+        int64_t x[4] = {0, 0, 0, 0}, S = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < parts; i++) {
+            const int64_t* p = part + (uint64_t)i * (R * HD + R);
+            const longlong2* pp = reinterpret_cast<const longlong2*>(p) + (wq * DB + m) * 128 + lane;
+            const longlong2 u = pp[0], v = pp[64];
+            S += p[R * HD + 16 * wq + c16];
+            x[0] += u.x;
+            x[1] += u.y;
+            x[2] += v.x;
+            x[3] += v.y;
+        }
+        if (row >= tl.rows) continue;
+        const Divide quot(S, a.fp);
+        store_out(a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * m + 4 * g, quot, x);
     }
 }
 
@@ -1142,12 +1199,14 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     if (slots > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
     // parts of a tile's keys: enough workgroups to fill the chip, at most kMaxPart keys each (the int32 limb sums: a
     // product is below 2^14, two a key in the middle limbs)
-    const uint32_t most = (b.cap / 64 + kMinSteps - 1) / kMinSteps;
-    const uint64_t want = (4ull * st->cus + slots * c.kv - 1) / (slots * c.kv);
-    const uint32_t splits = (uint32_t)std::max<uint64_t>({std::min<uint64_t>(want, most), (b.cap + kMaxPart - 1) / kMaxPart, 1});
+    const uint32_t steps = (b.cap + 63) / 64, wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20);
+    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M");
+    const uint32_t target = ev ? atoi(ev) : 1024, mn = em ? atoi(em) : 4;
+    const uint32_t want = std::max(target / wgs, 1u);
+    const uint32_t per = std::min(std::max((steps + want - 1) / want, mn), kMaxPart / 64), splits = (steps + per - 1) / per;
     if (splits > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits);
     const size_t mx_bytes = round_up(rows * splits * 4, 256), sc_bytes = few ? round_up(rows * b.cap * 2, 256) : 0;
-    const size_t part_bytes = splits > 1 ? rows * splits * (cache->head_dim + 1) * 8 : 0;
+    const size_t part_bytes = splits > 1 ? (few ? rows : slots * c.kv * R) * splits * (cache->head_dim + 1) * 8 : 0;
     void* ws;
     if ((rc = workspace(st, mx_bytes + sc_bytes + part_bytes, &ws, s))) return rc;
     Work wk;
@@ -1155,15 +1214,16 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     wk.sc = reinterpret_cast<int16_t*>(static_cast<uint8_t*>(ws) + mx_bytes);
     wk.part = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(ws) + mx_bytes + sc_bytes);
     wk.splits = splits;
+    wk.per = per;
     const dim3 grid((unsigned)slots, c.kv, splits), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
 #define CM_FEW(HD, I8)                                                                                                  \
     CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk);                \
     CM_LAUNCH("paged_few_kernel", (paged_few_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);         \
-    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_join_kernel<HD, 16>), jgrid, dim3(256), 0, s, b, a, wk); }
+    if (splits > 1) { CM_LAUNCH("paged_join_kernel", paged_join_kernel<HD>, jgrid, dim3(256), 0, s, b, a, wk); }
 #define CM_ROWS(HD, I8, QB)                                                                                             \
     CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk);                  \
     CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);   \
-    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_join_kernel<HD, 64 * QB>), jgrid, dim3(256), 0, s, b, a, wk); }
+    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), dim3((unsigned)slots, c.kv, HD / 16), dim3(256), 0, s, c, b, a, wk); }
     if (cache->head_dim == 64) {
         if (cache->int8) {
             if (few) { CM_FEW(64, true) } else { CM_ROWS(64, true, 2) }
