@@ -377,14 +377,30 @@ struct Tile {
     bool on;
 
     __device__ __forceinline__ Tile(const Batch& bt, const Attn& a, uint32_t slot) {
-        auto first = [&](uint32_t i) { return (uint32_t)((uint64_t)bt.start(i) * a.G / R) + i; };
-        b = find_le(bt.batch, slot, first);
-        q0 = bt.start(b);
-        n = (uint32_t)max((int)bt.start(b + 1) - (int)q0, 0);
-        row0 = (slot - first(b)) * R;
+        uint32_t q1, first;
+        int len;
+        if (bt.batch <= 64) {                  // one round of loads: lane i holds sequence i
+            const uint32_t i = min(threadIdx.x & 63, bt.batch - 1);
+            const uint32_t s0 = bt.start(i), s1 = bt.start(i + 1), l = (uint32_t)bt.len(i);
+            const uint32_t f = (uint32_t)((uint64_t)s0 * a.G / R) + i;
+            b = max((uint32_t)__popcll(__ballot((threadIdx.x & 63) < bt.batch && f <= slot)), 1u) - 1;
+            q0 = (uint32_t)__builtin_amdgcn_readlane((int)s0, b);
+            q1 = (uint32_t)__builtin_amdgcn_readlane((int)s1, b);
+            len = __builtin_amdgcn_readlane((int)l, b);
+            first = (uint32_t)__builtin_amdgcn_readlane((int)f, b);
+        } else {
+            auto at = [&](uint32_t i) { return (uint32_t)((uint64_t)bt.start(i) * a.G / R) + i; };
+            b = find_le(bt.batch, slot, at);
+            q0 = bt.start(b);
+            q1 = bt.start(b + 1);
+            len = bt.len(b);
+            first = at(b);
+        }
+        n = (uint32_t)max((int)q1 - (int)q0, 0);
+        row0 = (slot - first) * R;
         rows = n * a.G;
         on = row0 < rows;
-        base = bt.len(b) - (int)n;
+        base = len - (int)n;
         tb = bt.table + b * bt.table_ld;
         const uint32_t tf = row0 / a.G, tl = on ? min((row0 + R - 1) / a.G, n - 1) : tf;
         lo = __builtin_amdgcn_readfirstlane(begin(a, tf) & ~63u);
@@ -407,9 +423,10 @@ struct Tile {
 struct Work {
     int32_t* mx;                           // [rows][splits] raw q.K^T sums, kNone: no key
     int16_t* sc;                           // [rows][cap]
-    int64_t* part;                         // few rows: [rows][splits][HD + 1]; many: [tile][splits][R HD + R], each
+    int64_t* part;                         // few rows: [rows][splits][HD + 2]; many: [tile][splits][R HD + R], each
                                            // tile in its lanes' order (1 KiB a store)
     uint32_t splits, per;                  // most parts of a tile, steps of a part
+    uint32_t splits_s, per_s;              // the same of the maxima's parts
 };
 constexpr int kNone = (int)0x80000000;
 
@@ -467,87 +484,267 @@ __device__ __forceinline__ void stage_tab(int32_t* stab, const int32_t* tab) {
 }
 
 // ---------------------------------------------------------------- attention of few rows
-// Tiles of 16 rows: decode steps, where the cache's bytes are what costs.  A workgroup's four wavefronts take the
-// steps of its part in turn and read K and V straight into the MFMA operands; the first kernel leaves the scores and
-// the part's maxima, the second takes the row's maximum, the weights and P.V.
-template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
-    constexpr uint32_t KS = HD / 64;
-    typedef Block<HD, I8> B;
-    __shared__ int32_t redm[4][16];
-    const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const Tile<16> tl(bt, a, blockIdx.x);
-    const uint32_t per = wk.per;
-    if (!tl.on || z >= tl.parts(per)) return;
-    const uint32_t row = min(tl.row0 + c16, tl.rows - 1), tok = row / a.G;
-    const bool mine = tl.row0 + c16 < tl.rows;
-    const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
-    const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
+// Tiles of 15 rows: decode steps, where the cache's bytes are what costs.  Wavefronts take steps in turn and read K and
+// V straight into the MFMA operands; the MFMA's sixteenth column is all ones, so V's sums (for the offset of the
+// weights' bytes) come with the products.  Short caches: one kernel, every score in its wavefront's registers.
+// Long ones: a kernel that leaves the scores and the maxima, a kernel for the weights and P.V, a join of the parts.
+constexpr uint32_t kFewRows = 15;
 
-    v4i qh[KS], ql[KS];
-    int qsum = 0;
-    const int16_t* qp = a.q + (uint64_t)(tl.q0 + tok) * a.q_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * g;
+template <uint32_t HD, bool I8>
+struct Few {
+    static constexpr uint32_t KS = HD / 64, DB = HD / 16, NP = I8 ? 1 : 2;
+    typedef Block<HD, I8> B;
+    const Cache& c;
+    const Batch& bt;
+    const Tile<kFewRows>& tl;
+    uint32_t head, lane, c16, g, w, row, vend, vbeg;
+    bool mine;
+    uint64_t wrow;                          // the row in the workspace's order
+
+    __device__ __forceinline__ Few(const Cache& c_, const Batch& bt_, const Attn& a, const Tile<kFewRows>& tl_, uint32_t head_)
+        : c(c_), bt(bt_), tl(tl_), head(head_) {
+        lane = threadIdx.x & 63;
+        c16 = lane & 15;
+        g = lane >> 4;
+        w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        mine = c16 < kFewRows && tl.row0 + c16 < tl.rows;
+        row = mine ? tl.row0 + c16 : tl.row0;
+        vend = mine ? tl.seen(bt, row / a.G) : 0u;
+        vbeg = tl.begin(a, row / a.G);
+        wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
+    }
+    struct Query {
+        v4i h[KS], l[KS];
+        int term;
+    };
+    __device__ __forceinline__ Query query(const Attn& a) const {
+        Query q;
+        const int16_t* qp = a.q + (uint64_t)(tl.q0 + row / a.G) * a.q_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * g;
+        int qs = 0;
 #pragma unroll
-    for (uint32_t s = 0; s < KS; s++) limbs16(qp + 64 * s, qh[s], ql[s], qsum);
-    qsum += __shfl_xor(qsum, 16, 64);
-    qsum += __shfl_xor(qsum, 32, 64);
-    const int qterm = I8 ? 0 : 128 * qsum;
-    const v4i zero = {0, 0, 0, 0};
-    int mx = kNone;
-    for (uint32_t i = z * per + w; i < min((z + 1) * per, tl.nt); i += 4) {
-        const uint32_t k0 = tl.lo + 64 * i, kr = k0 + 16 * (c16 >> 2) + (c16 & 3), kg = k0 + 16 * g;
-        const uint32_t idr = kr < bt.cap ? (uint32_t)tl.tb[kr >> c.lg] : ~0u, idg = kg < bt.cap ? (uint32_t)tl.tb[kg >> c.lg] : ~0u;
-        const uint8_t* kb0 = c.data + ((uint64_t)(idr < c.pages ? idr : 0) * c.kv + head) * c.block + (kr & (c.page - 1)) * HD + 16 * g;
-        const uint8_t* tb0 = c.data + ((uint64_t)(idg < c.pages ? idg : 0) * c.kv + head) * c.block;
-        const uint32_t in = kg & (c.page - 1);
-        v4i kh[4][KS], kl[4][KS], term[4];
+        for (uint32_t s = 0; s < KS; s++) limbs16(qp + 64 * s, q.h[s], q.l[s], qs);
+        qs += __shfl_xor(qs, 16, 64);
+        qs += __shfl_xor(qs, 32, 64);
+        q.term = I8 ? 0 : 128 * qs;
+        return q;
+    }
+    // the page ids of the lane's K row and of its own 16 keys in step i (~0: none)
+    __device__ __forceinline__ uint32_t id_at(uint32_t key, bool in) const {
+        const uint32_t id = in && key < bt.cap ? (uint32_t)tl.tb[key >> c.lg] : ~0u;
+        return id < c.pages ? id : ~0u;
+    }
+    __device__ __forceinline__ uint32_t id_row(uint32_t i, uint32_t end) const { return id_at(tl.lo + 64 * i + 16 * (c16 >> 2), i < end); }
+    __device__ __forceinline__ uint32_t id_own(uint32_t i, uint32_t end) const { return id_at(tl.lo + 64 * i + 16 * g, i < end); }
+    __device__ __forceinline__ const uint8_t* block(uint32_t id) const {
+        return c.data + ((uint64_t)(id == ~0u ? 0u : id) * c.kv + head) * c.block;
+    }
+    // the scores of step i's keys 16 g .. 16 g + 15 of query c16, packed, and the maximum of the raw sums
+    __device__ __forceinline__ void scores(uint32_t i, uint32_t idr, uint32_t ido, const Query& q, uint32_t (&out)[8], int& mx) const {
+        const v4i zero = {0, 0, 0, 0};
+        const uint32_t k0 = tl.lo + 64 * i, kr = k0 + 16 * (c16 >> 2) + (c16 & 3), kg = k0 + 16 * g, in = kg & (c.page - 1);
+        const uint8_t *kp = block(idr) + (kr & (c.page - 1)) * HD + 16 * g, *tp = block(ido);
+        v4i kh[4][KS], kl[4][KS], term[4], es = zero;
 #pragma unroll
         for (uint32_t kb = 0; kb < 4; kb++) {
 #pragma unroll
             for (uint32_t s = 0; s < KS; s++) {
-                kh[kb][s] = *reinterpret_cast<const v4i*>(kb0 + 4 * kb * HD + 64 * s);
-                if constexpr (!I8) kl[kb][s] = *reinterpret_cast<const v4i*>(kb0 + B::k(c.page, 1) + 4 * kb * HD + 64 * s);
+                kh[kb][s] = *reinterpret_cast<const v4i*>(kp + 4 * kb * HD + 64 * s);
+                if constexpr (!I8) kl[kb][s] = *reinterpret_cast<const v4i*>(kp + B::k(c.page, 1) + 4 * kb * HD + 64 * s);
             }
-            term[kb] = *reinterpret_cast<const v4i*>(tb0 + B::term(c.page) + 4 * (in + 4 * kb));
+            term[kb] = *reinterpret_cast<const v4i*>(tp + B::term(c.page) + 4 * (in + 4 * kb));
         }
-        v4i es = zero;
-        if constexpr (I8) es = *reinterpret_cast<const v4i*>(tb0 + B::ke(c.page) + in);
-        uint32_t out[8];
+        if constexpr (I8) es = *reinterpret_cast<const v4i*>(tp + B::ke(c.page) + in);
 #pragma unroll
         for (uint32_t kb = 0; kb < 4; kb++) {
             v4i hh = zero, mid = zero, ll = term[kb];
 #pragma unroll
-            for (uint32_t s = 0; s < KS; s++) qk<I8>(kh[kb][s], kl[kb][s], qh[s], ql[s], hh, mid, ll);
+            for (uint32_t s = 0; s < KS; s++) qk<I8>(kh[kb][s], kl[kb][s], q.h[s], q.l[s], hh, mid, ll);
             int x[4];
 #pragma unroll
             for (uint32_t r = 0; r < 4; r++) {
-                const int acc = raw_sum<I8>(hh[r], mid[r], ll[r], (uint32_t)es[kb], r, qterm);
+                x[r] = raw_sum<I8>(hh[r], mid[r], ll[r], (uint32_t)es[kb], r, q.term);
                 const uint32_t key = kg + 4 * kb + r;
-                mx = max(mx, idg < c.pages && key >= vbeg && key < vend ? acc : kNone);
-                x[r] = sat16i(acc >> 8);
+                mx = max(mx, ido != ~0u && key >= vbeg && key < vend ? x[r] : kNone);
             }
-            out[2 * kb] = (uint32_t)(uint16_t)x[0] | (uint32_t)x[1] << 16;
-            out[2 * kb + 1] = (uint32_t)(uint16_t)x[2] | (uint32_t)x[3] << 16;
+            out[2 * kb] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_i16(x[0] >> 8, x[1] >> 8));
+            out[2 * kb + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_i16(x[2] >> 8, x[3] >> 8));
         }
-        if (mine) {
-            int16_t* sp = wk.sc + wrow * bt.cap + kg;                     // kg < cap: cap is a multiple of 16
-            if (kg < bt.cap) {
-                *reinterpret_cast<uint4*>(sp) = make_uint4(out[0], out[1], out[2], out[3]);
-                *reinterpret_cast<uint4*>(sp + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+    }
+    // the weights of those scores and their products with V
+    struct Sums {
+        v4i acc[3][DB];
+        uint32_t w;                         // the lane's weights: below 2^16 * 16 * kMaxPart / 64
+    };
+    __device__ __forceinline__ void values(uint32_t i, uint32_t ido, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2, const Smx& smx,
+                                           const int32_t* stab, Sums& o) const {
+        const uint32_t kg = tl.lo + 64 * i + 16 * g, in = kg & (c.page - 1);
+        const uint8_t *vb = block(ido), *vp = vb + B::v(c.page, 0) + c16 * c.page + in;
+        v4i vh[DB], vl[DB], es = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) {
+            vh[m] = *reinterpret_cast<const v4i*>(vp + 16 * m * c.page);
+            if constexpr (!I8) vl[m] = *reinterpret_cast<const v4i*>(vp + (HD + 16 * m) * c.page);
+        }
+        if constexpr (I8) es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
+        uint32_t wp[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            const Exp2 x = exps((int)(int16_t)sw[j], (int)sw[j] >> 16, m2, dl2, smx, stab);
+            auto on = [&](uint32_t key) { return ido != ~0u && key >= vbeg && key < vend; };
+            wp[j] = pair16(on(kg + 2 * j) ? x.e0() : 0u, on(kg + 2 * j + 1) ? x.e1() : 0u);
+            o.w = add16(wp[j], o.w);
+        }
+        v4i p[I8 ? 3 : 2];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) {
+            weight_bytes<I8>(wp[2 * q], wp[2 * q + 1], (uint32_t)es[q], p, q);
+#pragma unroll
+            for (uint32_t x = 0; x < (I8 ? 3u : 2u); x++) p[x][q] = c16 == kFewRows ? 0x01010101 : p[x][q];
+        }
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) {
+            if constexpr (I8) {
+                o.acc[0][m] = mfma(vh[m], p[I8 ? 2 : 0], o.acc[0][m]);
+                o.acc[1][m] = mfma(vh[m], p[1], o.acc[1][m]);
+                o.acc[2][m] = mfma(vh[m], p[0], o.acc[2][m]);
+            } else {
+                o.acc[0][m] = mfma(vh[m], p[1], o.acc[0][m]);
+                o.acc[1][m] = mfma(vh[m], p[0], o.acc[1][m]);
+                o.acc[2][m] = mfma(vl[m], p[0], o.acc[2][m]);
+                o.acc[1][m] = mfma(vl[m], p[1], o.acc[1][m]);
             }
         }
     }
+};
+
+// The workgroup's sums of a tile: products [row][d] (the bytes' offsets out), weights [row], V's [d].
+template <uint32_t HD>
+struct FewSums {
+    int64_t part[kFewRows][HD], w[kFewRows], v[HD];
+    __device__ __forceinline__ void clear() {
+        for (uint32_t i = threadIdx.x; i < sizeof(FewSums) / 8; i += blockDim.x) reinterpret_cast<int64_t*>(this)[i] = 0;
+    }
+    // a wavefront's sums added (LDS atomics of integers: the order is free)
+    template <bool I8>
+    __device__ __forceinline__ void add(const Few<HD, I8>& f, const typename Few<HD, I8>::Sums& o) {
+        int64_t ws = o.w;
+        ws += (int64_t)ro::shfl64((uint64_t)ws, 16);
+        ws += (int64_t)ro::shfl64((uint64_t)ws, 32);
+        auto put = [](int64_t* p, int64_t x) { atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)x); };
+        if (f.mine && f.g == 0) put(&w[f.c16], ws);
+#pragma unroll
+        for (uint32_t m = 0; m < HD / 16; m++)
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t d = 16 * m + 4 * f.g + r;
+                const int64_t hh = o.acc[0][m][r], mid = o.acc[1][m][r], ll = o.acc[2][m][r];
+                if (f.mine) put(&part[f.c16][d], hh * 65536 + mid * 256 + ll);
+                else if (f.c16 == kFewRows) put(&v[d], I8 ? hh : hh * 256 + ll);
+            }
+    }
+    template <bool I8>
+    __device__ __forceinline__ int64_t sum(uint32_t r, uint32_t d) const {
+        return part[r][d] + (I8 ? v[d] * (128 * 65793) : v[d] * 32896 + 128 * w[r]);
+    }
+    template <bool I8>
+    __device__ __forceinline__ void store(const Attn& a, const Tile<kFewRows>& tl, uint32_t head) const {
+        const uint32_t rows = min(kFewRows, tl.rows - tl.row0);
+        for (uint32_t i = threadIdx.x; i < rows * (HD / 2); i += blockDim.x) {
+            const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2)), rw = tl.row0 + r;
+            const Divide q(w[r], a.fp);
+            const uint32_t y0 = (uint32_t)q(sum<I8>(r, d)), y1 = (uint32_t)q(sum<I8>(r, d + 1));
+            *reinterpret_cast<uint32_t*>(a.o + (uint64_t)(tl.q0 + rw / a.G) * a.o_ld + (uint64_t)(head * a.G + rw % a.G) * HD + d) =
+                (y0 & 0xFFFFu) | y1 << 16;
+        }
+    }
+};
+
+// Caches of at most kShort keys in one launch: a tile's steps over the wavefronts of one workgroup (16, or 8 at 128 d
+// for its registers), at most NS each, their scores kept between the maximum and the weights.
+constexpr uint32_t kShort = 2048;
+
+template <uint32_t HD, bool I8>
+__global__ __launch_bounds__(HD == 64 ? 1024 : 512) void paged_short_kernel(Cache c, Batch bt, Attn a, const int32_t* __restrict__ tab) {
+    constexpr uint32_t NW = HD == 64 ? 16 : 8, NS = kShort / 64 / NW;
+    typedef Few<HD, I8> F;
+    __shared__ __attribute__((aligned(16))) int32_t stab[4096];
+    __shared__ int32_t redm[NW][16];
+    __shared__ FewSums<HD> sums;
+    const Tile<kFewRows> tl(bt, a, blockIdx.x);
+    if (!tl.on) return;
+    const F f(c, bt, a, tl, blockIdx.y);
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / NW; i++)
+        __builtin_amdgcn_global_load_lds(tab + 4 * (threadIdx.x + 64 * NW * i),
+                                         (__attribute__((address_space(3))) void*)(stab + 4 * (64 * f.w + 64 * NW * i)), 16, 0, 0);
+    sums.clear();
+    uint32_t idr[NS], ido[NS], sw[NS][8];
+#pragma unroll
+    for (uint32_t k = 0; k < NS; k++) {
+        idr[k] = f.id_row(f.w + NW * k, tl.nt);
+        ido[k] = f.id_own(f.w + NW * k, tl.nt);
+    }
+    const typename F::Query q = f.query(a);
+    int mx = kNone;
+#pragma unroll
+    for (uint32_t k = 0; k < NS; k++)
+        if (f.w + NW * k < tl.nt) f.scores(f.w + NW * k, idr[k], ido[k], q, sw[k], mx);
     mx = max(mx, __shfl_xor(mx, 16, 64));
     mx = max(mx, __shfl_xor(mx, 32, 64));
-    if (g == 0) redm[w][c16] = mx;
+    if (f.g == 0) redm[f.w][f.c16] = mx;
+    __builtin_amdgcn_s_waitcnt(0x0070);               // the TAB's copies
     __syncthreads();
-    if (t < 16 && mine) wk.mx[wrow * wk.splits + z] = max(max(redm[0][t], redm[1][t]), max(redm[2][t], redm[3][t]));
+#pragma unroll
+    for (uint32_t k = 0; k < NW; k++) mx = max(mx, redm[k][f.c16]);
+    const uint32_t m2 = twice((uint32_t)sat16i(mx >> 8)), dl2 = twice(a.smx.dlim);
+    typename F::Sums o;
+#pragma unroll
+    for (uint32_t m = 0; m < F::DB; m++) o.acc[0][m] = o.acc[1][m] = o.acc[2][m] = v4i{0, 0, 0, 0};
+    o.w = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < NS; k++)
+        if (f.w + NW * k < tl.nt) f.values(f.w + NW * k, ido[k], sw[k], m2, dl2, a.smx, stab, o);
+    if (f.w < tl.nt) sums.template add<I8>(f, o);
+    __syncthreads();
+    sums.template store<I8>(a, tl, blockIdx.y);
+}
+
+// Long caches.  A workgroup takes `per_s` steps, its four wavefronts in turn.
+template <uint32_t HD, bool I8>
+__global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
+    typedef Few<HD, I8> F;
+    __shared__ int32_t redm[4][16];
+    const uint32_t z = blockIdx.z;
+    const Tile<kFewRows> tl(bt, a, blockIdx.x);
+    if (!tl.on || z >= tl.parts(wk.per_s)) return;
+    const F f(c, bt, a, tl, blockIdx.y);
+    const uint32_t beg = z * wk.per_s + f.w, end = min((z + 1) * wk.per_s, tl.nt);
+    uint32_t idr = f.id_row(beg, end), ido = f.id_own(beg, end);
+    const typename F::Query q = f.query(a);
+    int mx = kNone;
+    for (uint32_t i = beg; i < end; i += 4) {
+        const uint32_t nr = f.id_row(i + 4, end), no = f.id_own(i + 4, end), kg = tl.lo + 64 * i + 16 * f.g;
+        uint32_t out[8];
+        f.scores(i, idr, ido, q, out, mx);
+        if (f.mine && kg < bt.cap) {                  // cap is a multiple of 16
+            uint4* sp = reinterpret_cast<uint4*>(wk.sc + f.wrow * bt.cap + kg);
+            sp[0] = make_uint4(out[0], out[1], out[2], out[3]);
+            sp[1] = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+        idr = nr;
+        ido = no;
+    }
+    mx = max(mx, __shfl_xor(mx, 16, 64));
+    mx = max(mx, __shfl_xor(mx, 32, 64));
+    if (f.g == 0) redm[f.w][f.c16] = mx;
+    __syncthreads();
+    if (threadIdx.x < 16 && f.mine)
+        wk.mx[f.wrow * wk.splits_s + z] = max(max(redm[0][f.c16], redm[1][f.c16]), max(redm[2][f.c16], redm[3][f.c16]));
 }
 
 // the maximum score of a row over its parts: the four lanes of a row (groups g) take every fourth, loads in fours
 __device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t parts, uint32_t g) {
-    const int32_t* p = wk.mx + wrow * wk.splits;
+    const int32_t* p = wk.mx + wrow * wk.splits_s;
     int m = kNone;
     for (uint32_t i = g; i < parts; i += 16) {
         int x[4];
@@ -561,112 +758,63 @@ __device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t p
 }
 
 template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
-    constexpr uint32_t DB = HD / 16, NP = I8 ? 1 : 2;
-    typedef Block<HD, I8> B;
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
+    typedef Few<HD, I8> F;
     __shared__ __attribute__((aligned(16))) int32_t stab[4096];
-    __shared__ int64_t reds[4][16];
-    __shared__ int64_t part[16][HD + 1];
-    const uint32_t t = threadIdx.x, lane = t & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, z = blockIdx.z;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const Tile<16> tl(bt, a, blockIdx.x);
-    const uint32_t per = wk.per, parts = tl.parts(per);
+    __shared__ FewSums<HD> sums;
+    const uint32_t z = blockIdx.z;
+    const Tile<kFewRows> tl(bt, a, blockIdx.x);
+    const uint32_t parts = tl.parts(wk.per);
     if (!tl.on || z >= parts) return;
     stage_tab(stab, tab);
-    for (uint32_t i = t; i < 16 * (HD + 1); i += 256) (&part[0][0])[i] = 0;
-    const uint32_t row = min(tl.row0 + c16, tl.rows - 1), tok = row / a.G;
-    const bool mine = tl.row0 + c16 < tl.rows;
-    const uint64_t wrow = ((uint64_t)head * bt.tokens + tl.q0) * a.G + row;
-    const uint32_t vend = mine ? tl.seen(bt, tok) : 0u, vbeg = tl.begin(a, tok);
-    const uint32_t m2 = twice((uint32_t)row_max(wk, wrow, parts, g)), dl2 = twice(a.smx.dlim);
-    const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    __syncthreads();
-
-    v4i acc[3][DB], vs[NP][DB];
-#pragma unroll
-    for (uint32_t m = 0; m < DB; m++) {
-        acc[0][m] = acc[1][m] = acc[2][m] = zero;
-        vs[0][m] = vs[NP - 1][m] = zero;
-    }
-    int64_t wsum = 0;
-    for (uint32_t i = z * per + w; i < min((z + 1) * per, tl.nt); i += 4) {
-        const uint32_t k0 = tl.lo + 64 * i, kg = k0 + 16 * g, in = kg & (c.page - 1);
-        const uint32_t id = kg < bt.cap ? (uint32_t)tl.tb[kg >> c.lg] : ~0u;
-        const uint8_t* vb = c.data + ((uint64_t)(id < c.pages ? id : 0) * c.kv + head) * c.block;
-        v4i vh[DB], vl[DB];
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            const uint8_t* vp = vb + B::v(c.page, 0) + (16 * m + c16) * c.page + in;
-            vh[m] = *reinterpret_cast<const v4i*>(vp);
-            if constexpr (!I8) vl[m] = *reinterpret_cast<const v4i*>(vp + HD * c.page);
-        }
+    sums.clear();
+    const F f(c, bt, a, tl, blockIdx.y);
+    const uint32_t beg = z * wk.per + f.w, end = min((z + 1) * wk.per, tl.nt);
+    auto load = [&](uint32_t i, uint32_t (&x)[8]) {
+        const uint32_t kg = tl.lo + 64 * i + 16 * f.g;
         uint4 s0 = make_uint4(0, 0, 0, 0), s1 = s0;
-        if (mine && kg < bt.cap) {
-            const int16_t* sp = wk.sc + wrow * bt.cap + kg;
-            s0 = *reinterpret_cast<const uint4*>(sp);
-            s1 = *reinterpret_cast<const uint4*>(sp + 8);
+        if (f.mine && i < end && kg < bt.cap) {
+            const uint4* sp = reinterpret_cast<const uint4*>(wk.sc + f.wrow * bt.cap + kg);
+            s0 = sp[0];
+            s1 = sp[1];
         }
-        v4i es = zero;
-        if constexpr (I8) es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
-        const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        v4i p[I8 ? 3 : 2];
-        uint32_t wp[8], sum = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            const Exp2 x = exps((int)(int16_t)sw[j], (int)sw[j] >> 16, m2, dl2, a.smx, stab);
-            auto on = [&](uint32_t key) { return id < c.pages && key >= vbeg && key < vend; };
-            wp[j] = pair16(on(kg + 2 * j) ? x.e0() : 0u, on(kg + 2 * j + 1) ? x.e1() : 0u);
-            sum = add16(wp[j], sum);
-        }
-        wsum += sum;
-#pragma unroll
-        for (uint32_t q = 0; q < 4; q++) weight_bytes<I8>(wp[2 * q], wp[2 * q + 1], (uint32_t)es[q], p, q);
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            if constexpr (I8) {
-                acc[0][m] = mfma(vh[m], p[2], acc[0][m]);
-                acc[1][m] = mfma(vh[m], p[1], acc[1][m]);
-                acc[2][m] = mfma(vh[m], p[0], acc[2][m]);
-            } else {
-                acc[0][m] = mfma(vh[m], p[1], acc[0][m]);
-                acc[1][m] = mfma(vh[m], p[0], acc[1][m]);
-                acc[2][m] = mfma(vl[m], p[0], acc[2][m]);
-                acc[1][m] = mfma(vl[m], p[1], acc[1][m]);
-                vs[1][m] = mfma(vl[m], ones, vs[1][m]);
-            }
-            vs[0][m] = mfma(vh[m], ones, vs[0][m]);
-        }
-    }
-    wsum += (int64_t)ro::shfl64((uint64_t)wsum, 16);
-    wsum += (int64_t)ro::shfl64((uint64_t)wsum, 32);
-    if (g == 0) reds[w][c16] = wsum;
-#pragma unroll
-    for (uint32_t m = 0; m < DB; m++)
-#pragma unroll
-        for (uint32_t r = 0; r < 4; r++)
-            atomicAdd(reinterpret_cast<unsigned long long*>(&part[c16][16 * m + 4 * g + r]),
-                      (unsigned long long)whole_sum<I8>(acc[0][m][r], acc[1][m][r], acc[2][m][r], vs[0][m][r], vs[NP - 1][m][r], wsum));
+        x[0] = s0.x; x[1] = s0.y; x[2] = s0.z; x[3] = s0.w;
+        x[4] = s1.x; x[5] = s1.y; x[6] = s1.z; x[7] = s1.w;
+    };
+    uint32_t ido = f.id_own(beg, end), sw[8];
+    load(beg, sw);
+    const uint32_t m2 = twice((uint32_t)row_max(wk, f.wrow, tl.parts(wk.per_s), f.g)), dl2 = twice(a.smx.dlim);
+    __builtin_amdgcn_s_waitcnt(0x0070);               // the TAB's copies
     __syncthreads();
-    for (uint32_t i = t; i < 16 * HD / 2; i += 256) {
-        const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2)), rw = tl.row0 + r;
-        if (rw >= tl.rows) break;
-        const int64_t S = reds[0][r] + reds[1][r] + reds[2][r] + reds[3][r];
-        if (parts == 1) {
-            const Divide q(S, a.fp);
-            const int o0 = q(part[r][d]), o1 = q(part[r][d + 1]);
-            *reinterpret_cast<uint32_t*>(a.o + (uint64_t)(tl.q0 + rw / a.G) * a.o_ld + (uint64_t)(head * a.G + rw % a.G) * HD + d) =
-                (uint32_t)(uint16_t)o0 | ((uint32_t)(uint16_t)o1 << 16);
-        } else {
-            int64_t* pp = wk.part + ((((uint64_t)head * bt.tokens + tl.q0) * a.G + rw) * wk.splits + z) * (HD + 1);
-            pp[d] = part[r][d];
-            pp[d + 1] = part[r][d + 1];
-            if (d == 0) pp[HD] = S;
-        }
+    typename F::Sums o;
+#pragma unroll
+    for (uint32_t m = 0; m < F::DB; m++) o.acc[0][m] = o.acc[1][m] = o.acc[2][m] = v4i{0, 0, 0, 0};
+    o.w = 0;
+    for (uint32_t i = beg; i < end; i += 4) {
+        const uint32_t no = f.id_own(i + 4, end);
+        uint32_t ns[8];
+        load(i + 4, ns);
+        f.values(i, ido, sw, m2, dl2, a.smx, stab, o);
+        ido = no;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) sw[k] = ns[k];
+    }
+    if (beg < end) sums.template add<I8>(f, o);
+    __syncthreads();
+    if (parts == 1) {
+        sums.template store<I8>(a, tl, blockIdx.y);
+        return;
+    }
+    const uint32_t rows = min(kFewRows, tl.rows - tl.row0);
+    for (uint32_t i = threadIdx.x; i < rows * (HD / 2); i += 256) {
+        const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2));
+        int64_t* pp = wk.part + ((((uint64_t)blockIdx.y * bt.tokens + tl.q0) * a.G + tl.row0 + r) * wk.splits + z) * (HD + 2);
+        *reinterpret_cast<longlong2*>(pp + d) = make_longlong2(sums.template sum<I8>(r, d), sums.template sum<I8>(r, d + 1));
+        if (d == 0) pp[HD] = sums.w[r];
     }
 }
 
-// The parts' sums of a row added and divided: a wavefront per row, two columns a lane at 128 d.
+// The parts' sums of a row added and divided: a wavefront per row, loads of four parts in flight.
 template <uint32_t HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work wk) {
     const uint32_t lane = threadIdx.x & 63, head = blockIdx.y;
@@ -675,17 +823,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work 
     if (tok >= bt.start(bt.batch)) return;
     const uint32_t b = find_le(bt.batch, tok, [&](uint32_t i) { return bt.start(i); });
     const uint32_t row = at - bt.start(b) * a.G;
-    const Tile<16> tl(bt, a, (uint32_t)((uint64_t)bt.start(b) * a.G / 16) + b + row / 16);
+    const Tile<kFewRows> tl(bt, a, (uint32_t)((uint64_t)bt.start(b) * a.G / kFewRows) + b + row / kFewRows);
     const uint32_t parts = tl.parts(wk.per);
     if (!tl.on || parts == 1) return;
-    const int64_t* pp = wk.part + ((uint64_t)head * bt.tokens * a.G + at) * wk.splits * (HD + 1);
+    const int64_t* pp = wk.part + ((uint64_t)head * bt.tokens * a.G + at) * wk.splits * (HD + 2);
     int64_t x[HD / 64], S = 0;
 #pragma unroll
     for (uint32_t k = 0; k < HD / 64; k++) x[k] = 0;
-    for (uint32_t i = 0; i < parts; i++, pp += HD + 1) {
+#pragma unroll 4
+    for (uint32_t i = 0; i < parts; i++) {
+        const int64_t* p = pp + (uint64_t)i * (HD + 2);
 #pragma unroll
-        for (uint32_t k = 0; k < HD / 64; k++) x[k] += pp[lane * (HD / 64) + k];
-        S += pp[HD];
+        for (uint32_t k = 0; k < HD / 64; k++) x[k] += p[lane * (HD / 64) + k];
+        S += p[HD];
     }
     int16_t* op = a.o + (uint64_t)tok * a.o_ld + (uint64_t)(head * a.G + at % a.G) * HD + lane * (HD / 64);
     const Divide q(S, a.fp);
@@ -840,7 +990,7 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[RW::S::BYTES];
     const uint32_t head = blockIdx.y, z = blockIdx.z;
     const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);             // the long tiles first
-    const uint32_t per = wk.per;
+    const uint32_t per = wk.per_s;
     if (!tl.on || z >= tl.parts(per)) return;
     const RW rw(c, bt, a, tl, head);
     int mx[QB];
@@ -885,7 +1035,7 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
         m = max(m, __shfl_xor(m, 16, 64));
         m = max(m, __shfl_xor(m, 32, 64));
         const uint32_t row = rw.row_of(qb);
-        if (rw.g == 0 && row < tl.rows) wk.mx[(((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits + z] = m;
+        if (rw.g == 0 && row < tl.rows) wk.mx[(((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits_s + z] = m;
     }
 }
 
@@ -914,7 +1064,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
         const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
-        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, parts, g));
+        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, tl.parts(wk.per_s), g));
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
         wsum[qb] = 0;
@@ -1190,23 +1340,34 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     if ((rc = state(&st))) return rc;
     const uint32_t cm24 = smx_cm & 0xFFFFFFu, cs = smx_cfg & 63u, G = heads / c.kv;
     const Attn a{q, o, q_ld, o_ld, G, window, fp, smx_of(cm24, cs)};
-    // few rows a sequence: tiles of 16 rows that keep their scores; otherwise (or where the scores would take more than
-    // kMaxScores) tiles of 64 or 128 rows that compute them twice
+    // Few rows a sequence: tiles of 15 rows, in one launch for short caches, with kept scores for long ones (where those
+    // fit kMaxScores); otherwise tiles of 64 or 128 rows that compute the scores twice
     const uint64_t rows = (uint64_t)b.tokens * heads;
-    const bool few = (uint64_t)b.tokens * G < 32u * (uint64_t)b.batch && rows * b.cap * 2 <= kMaxScores;
-    const uint32_t R = few ? 16 : cache->head_dim == 64 ? 128 : 64;
+    const bool few = (uint64_t)b.tokens * G < 32u * (uint64_t)b.batch && (b.cap <= kShort || rows * b.cap * 2 <= kMaxScores);
+    const uint32_t R = few ? kFewRows : cache->head_dim == 64 ? 128 : 64;
     const uint64_t slots = (uint64_t)b.tokens * G / R + b.batch;
     if (slots > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
-    // parts of a tile's keys: enough workgroups to fill the chip, at most kMaxPart keys each (the int32 limb sums: a
-    // product is below 2^14, two a key in the middle limbs)
+    const dim3 tiles((unsigned)slots, c.kv);
+    if (few && b.cap <= kShort) {
+#define CM_SHORT(HD, I8) \
+    CM_LAUNCH("paged_short_kernel", (paged_short_kernel<HD, I8>), tiles, dim3(HD == 64 ? 1024 : 512), 0, s, c, b, a, st->smx_tab)
+        if (cache->head_dim == 64) {
+            if (cache->int8) { CM_SHORT(64, true); } else { CM_SHORT(64, false); }
+        } else {
+            if (cache->int8) { CM_SHORT(128, true); } else { CM_SHORT(128, false); }
+        }
+#undef CM_SHORT
+        return CM_OK;
+    }
     const uint32_t steps = (b.cap + 63) / 64, wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20);
-    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M");
-    const uint32_t target = ev ? atoi(ev) : 1024, mn = em ? atoi(em) : 4;
+    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M"); const char* es = getenv("CMP_S");
+    const uint32_t target = ev ? atoi(ev) : few ? 1024 : 1536, mn = em ? atoi(em) : 4;
     const uint32_t want = std::max(target / wgs, 1u);
     const uint32_t per = std::min(std::max((steps + want - 1) / want, mn), kMaxPart / 64), splits = (steps + per - 1) / per;
-    if (splits > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits);
-    const size_t mx_bytes = round_up(rows * splits * 4, 256), sc_bytes = few ? round_up(rows * b.cap * 2, 256) : 0;
-    const size_t part_bytes = splits > 1 ? (few ? rows : slots * c.kv * R) * splits * (cache->head_dim + 1) * 8 : 0;
+    const uint32_t per_s = few ? std::min(per, es ? (uint32_t)atoi(es) : 8u) : per, splits_s = (steps + per_s - 1) / per_s;
+    if (splits > 65535u || splits_s > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits);
+    const size_t mx_bytes = round_up(rows * splits_s * 4, 256), sc_bytes = few ? round_up(rows * b.cap * 2, 256) : 0;
+    const size_t part_bytes = splits > 1 ? (few ? rows * splits * (cache->head_dim + 2) : slots * c.kv * R * splits * (cache->head_dim + 1)) * 8 : 0;
     void* ws;
     if ((rc = workspace(st, mx_bytes + sc_bytes + part_bytes, &ws, s))) return rc;
     Work wk;
@@ -1215,13 +1376,15 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     wk.part = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(ws) + mx_bytes + sc_bytes);
     wk.splits = splits;
     wk.per = per;
-    const dim3 grid((unsigned)slots, c.kv, splits), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
+    wk.splits_s = splits_s;
+    wk.per_s = per_s;
+    const dim3 grid((unsigned)slots, c.kv, splits), sgrid((unsigned)slots, c.kv, splits_s), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
 #define CM_FEW(HD, I8)                                                                                                  \
-    CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk);                \
+    CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), sgrid, dim3(256), 0, s, c, b, a, wk);                \
     CM_LAUNCH("paged_few_kernel", (paged_few_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);         \
     if (splits > 1) { CM_LAUNCH("paged_join_kernel", paged_join_kernel<HD>, jgrid, dim3(256), 0, s, b, a, wk); }
 #define CM_ROWS(HD, I8, QB)                                                                                             \
-    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk);                  \
+    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), sgrid, dim3(256), 0, s, c, b, a, wk);                  \
     CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);   \
     if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), dim3((unsigned)slots, c.kv, HD / 16), dim3(256), 0, s, c, b, a, wk); }
     if (cache->head_dim == 64) {

@@ -90,6 +90,16 @@ def test_attention(paged, lens, new, page, G, hd, int8):
     check_attention(paged, c, *regs(hd))
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens,new,G,window", [([700, 90, 1], [1, 1, 1], 3, 0), ([530, 300], [2, 1], 16, 0),
+                                               ([700, 5], [40, 5], 3, 0), ([650, 333], [70, 1], 4, 200)])
+def test_attention_in_parts(paged, lens, new, G, window, hd, int8):
+    """Tables of more than 2048 rows: a sequence's keys over several workgroups."""
+    c = Case(np.random.default_rng(sum(lens) + hd), lens, new, kv=2, G=G, hd=hd, int8=int8, tail=1, wide=150)
+    check_attention(paged, c, *regs(hd), window=window)
+
+
 @pytest.mark.parametrize("window", [1, 2, 15, 64, 100, 1 << 20])
 @pytest.mark.parametrize("int8", [False, True])
 def test_attention_window(paged, window, int8):
