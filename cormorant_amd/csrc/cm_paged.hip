@@ -87,9 +87,11 @@ __device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const
     d += d & 1;
     const uint32_t Dm = (uint32_t)(d >= 0 ? D >> d : D << -d);
     const uint32_t y0 = *reinterpret_cast<const uint32_t*>(tab + 32768 + 4 * ((Dm >> 19) & 8191u));
-    const uint32_t u = __umulhi(__umulhi(Dm, y0), y0);
-    const __int128 y1 = (__int128)y0 + (((__int128)y0 * (((int64_t)1 << 30) - (int64_t)u)) >> 31);
-    const __int128 lo = (__int128)1 << 31, hi = ((__int128)1 << 32) - 1;
+    const int64_t r = ((int64_t)1 << 30) - (int64_t)__umulhi(__umulhi(Dm, y0), y0);     // above -2^32
+    // y0 r >> 31 in 64 bits where r is below 2^31 (the unit's own table: below 2^18), else in two halves of y0
+    const int64_t step = r >= -((int64_t)1 << 31) ? ((int64_t)y0 * r) >> 31
+                                                  : ((int64_t)(y0 >> 16) * r + (((int64_t)(y0 & 0xFFFFu) * r) >> 16)) >> 15;
+    const int64_t y1 = (int64_t)y0 + step, lo = (int64_t)1 << 31, hi = ((int64_t)1 << 32) - 1;
     Rm = (uint64_t)(y1 < lo ? lo : y1 > hi ? hi : y1);
     sh = 47 + d / 2;
 }
@@ -97,6 +99,11 @@ __device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const
 __device__ __forceinline__ int rne_sat(int64_t v, uint32_t sc) {
     return (int)(sc <= 61 ? ro::sat16(ro::rne_shr_fast(v, sc)) : ro::sat16(ro::rne_shr((__int128)v, (int)sc)));
 }
+// v / 2^sc rounded half to even and saturated, of a whole number |v| <= 2^53 (v_rndne_f64; the scaling is exact)
+__device__ __forceinline__ int rne_sat_f64(double v, double scale) {
+    return sat16i((int)__builtin_rint(fmin(fmax(v * scale, -65536.0), 65536.0)));
+}
+__device__ __forceinline__ double pow2(int e) { return __builtin_bit_cast(double, (uint64_t)(1023 + e) << 52); }
 
 template <uint32_t L>
 __device__ __forceinline__ int64_t row_sum64(int64_t x) {     // over the L lanes of a row
@@ -105,163 +112,316 @@ __device__ __forceinline__ int64_t row_sum64(int64_t x) {     // over the L lane
     return x;
 }
 
-// HD / 8 lanes a head row, 8 columns a lane; a wavefront takes consecutive rows of
-// [token][q heads, k heads, v heads].
-template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep a) {
-    constexpr uint32_t L = HD / 8, RW = 64 / L;
-    const uint32_t lane = threadIdx.x & 63, u = lane % L, d0 = 8 * u;
-    const uint32_t per = a.heads + 2 * c.kv;
-    const uint64_t item = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * RW + lane / L;
-    const uint64_t items = (uint64_t)bt.start(bt.batch) * per;
-    if (((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * RW >= items) return;
-    const bool on = item < items;
-    const uint32_t tok = on ? (uint32_t)(item / per) : 0u, head = on ? (uint32_t)(item - (uint64_t)tok * per) : 0u;
-    // the wavefront's tokens lie in a few sequences: the first by search, then the rows after it one by one
-    const uint32_t tok0 = __builtin_amdgcn_readfirstlane(tok);
-    uint32_t b = find_le(bt.batch, tok0, [&](uint32_t i) { return bt.start(i); });
-    while (b + 1 < bt.batch && bt.start(b + 1) <= tok) b++;
-    const int n = (int)bt.start(b + 1) - (int)bt.start(b);
-    const int64_t pos = (int64_t)bt.len(b) - n + (int)(tok - bt.start(b));
-    const bool isq = head < a.heads, isv = head >= a.heads + c.kv;
-    const uint32_t g = isq ? head : isv ? head - a.heads - c.kv : head - a.heads;
-    const int16_t* src = isq ? a.q + tok * a.q_ld : isv ? a.v + tok * a.v_ld : a.k + tok * a.k_ld;
-    const int4 xw = on ? *reinterpret_cast<const int4*>(src + g * HD + d0) : make_int4(0, 0, 0, 0);
-    int x[8];
+// The 8-bit form of a row held by L lanes of 8 columns: its shift, and the codes in place
+template <uint32_t L>
+__device__ __forceinline__ uint32_t quantise(int (&x)[8]) {
+    int m = 0;
 #pragma unroll
-    for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&xw)[l];
-
-    const uint8_t* np = isq ? a.norm_q : isv ? nullptr : a.norm_k;
-    int64_t s2 = 0;
+    for (uint32_t l = 0; l < 8; l++) m = max(m, x[l] ^ (x[l] >> 31));
 #pragma unroll
-    for (uint32_t l = 0; l < 8; l++) s2 += (int64_t)x[l] * x[l];
-    s2 = row_sum64<L>(s2);
-    if (np != nullptr) {
-        const int64_t D = s2 + (isq ? a.eps_q : a.eps_k);
-        uint64_t Rm;
-        int sh;
-        rsqrt64((uint64_t)(D > 0 ? D : 1), Rm, sh, a.tab);
-#pragma unroll
-        for (uint32_t l = 0; l < 8; l++) {
-            const ro::Param p = ro::ld_param(np, d0 + l, false);
-            const int64_t P1 = ((int64_t)x[l] * (int64_t)Rm) >> (sh - 24);
-            x[l] = rne_sat(P1 * p.g + p.bq, (uint32_t)p.sc);
-        }
-    }
-    // rotation: the partner column's value from this or another lane of the row
-    const uint32_t half = a.rotary / 2;
-    const uint32_t row = (uint32_t)min(max(pos, (int64_t)0), (int64_t)a.rope_rows - 1);
-    const int32_t* cs = a.rope + (uint64_t)row * 2 * a.rotary;
-    const bool rot = d0 < a.rotary;
-    const uint32_t pl = a.interleaved ? lane : d0 < half ? lane + half / 8 : lane - half / 8;
-    int y[8];
+    for (uint32_t o = 1; o < L; o <<= 1) m = max(m, __shfl_xor(m, (int)o, 64));
+    const int e = max(0, 25 - __clz(m));                       // bits(m) - 7
 #pragma unroll
     for (uint32_t l = 0; l < 8; l++) {
-        const int other = __shfl(x[l], (int)(rot ? pl : lane), 64);
-        y[l] = a.interleaved ? (l & 1 ? x[l - 1] : -x[l + 1]) : d0 < half ? -other : other;
+        // round half to even in 32 bits: x + 2^(e-1) - 1 + bit e, shifted
+        x[l] = min(127, e ? (x[l] + (1 << (e - 1)) - 1 + ((x[l] >> e) & 1)) >> e : x[l]);
     }
-    if (!isv) {
-        const uint8_t* rp = isq ? a.rope_q : a.rope_k;
-        const bool cols = (isq ? a.rope_q_cols : a.rope_k_cols) != 0;
+    return (uint32_t)e;
+}
+
+// 64-row chunks of the sequences' new positions, aligned to 64 (so to pages and 16-row groups): sequence b's have the
+// slots from floor(start(b) / 64) + 2 b on.
+struct Chunk {
+    uint32_t b, q0;
+    int base, at, beg, end;                 // position of token q0; the chunk's first position; its valid rows [beg, end)
+    const int32_t* tb;
+    __device__ __forceinline__ Chunk(const Batch& bt, uint32_t slot) {
+        b = find_le(bt.batch, slot, [&](uint32_t i) { return bt.start(i) / 64 + 2 * i; });
+        q0 = bt.start(b);
+        const int n = max((int)bt.start(b + 1) - (int)q0, 0), len = bt.len(b);
+        base = len - n;
+        const int ci = (int)(slot - (q0 / 64 + 2 * b));
+        at = (base >> 6) * 64 + 64 * ci;
+        beg = max(max(base, 0) - at, 0);
+        end = min(min(len, (int)bt.cap) - at, 64);
+        tb = bt.table + b * bt.table_ld;
+    }
+};
+inline uint64_t chunk_slots(const Batch& b) { return (uint64_t)b.tokens / 64 + 2 * (uint64_t)b.batch; }
+
+// One launch, two kinds of workgroups.  q and k: HD / 8 lanes a head row, 8 columns a lane; a wavefront takes 64 / L
+// of a token's rows and `tpw` tokens, so that a lane's parameters stay in registers.  Its arithmetic is the row-ops
+// unit's, in double where every product is a whole number below 2^53 (the norm's x Rm and P1 G, the rotation's two
+// products; rounded by v_rndne_f64), about 10 instructions an element instead of 40 in 64-bit integers.  V: a chunk
+// of 64 positions of a head, transposed through LDS and stored as whole 16-key pieces where all 16 are new.
+template <uint32_t HD, bool I8>
+__global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep a, uint32_t qk_blocks, uint32_t passes, uint32_t tpw) {
+    constexpr uint32_t L = HD / 8, RW = 64 / L;
+    typedef Block<HD, I8> B;
+    __shared__ int16_t vt[64][HD + 2];
+    const uint32_t t = threadIdx.x, lane = t & 63, u = lane % L, d0 = 8 * u;
+    if (blockIdx.x >= qk_blocks) {
+        const uint32_t vb = blockIdx.x - qk_blocks, head = vb % c.kv;
+        const Chunk ch(bt, vb / c.kv);
+        if (ch.beg >= ch.end) return;
+        for (uint32_t i = t; i < 64 * L; i += 256) {
+            const int j = (int)(i / L);
+            const bool on = j >= ch.beg && j < ch.end;
+            if (__ballot(on) == 0) continue;
+            const int64_t tok = (int64_t)ch.q0 + ch.at + j - ch.base;
+            const int4 w = on ? *reinterpret_cast<const int4*>(a.v + tok * a.v_ld + head * HD + d0) : make_int4(0, 0, 0, 0);
+            int x[8];
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&w)[l];
+            if constexpr (I8) {
+                const uint32_t e = quantise<L>(x);
+                if (on && u == 0) {
+                    const uint32_t id = (uint32_t)ch.tb[(uint32_t)(ch.at + j) >> c.lg];
+                    if (id < c.pages)
+                        c.data[((uint64_t)id * c.kv + head) * c.block + B::ve(c.page) + ((uint32_t)(ch.at + j) & (c.page - 1))] = (uint8_t)e;
+                }
+            }
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) vt[j][d0 + l] = (int16_t)x[l];
+        }
+        __syncthreads();
+        for (uint32_t i = t; i < 4 * HD; i += 256) {
+            const uint32_t d = i % HD, j0 = 16 * (i / HD);
+            const int gb = max(ch.beg - (int)j0, 0), ge = min(ch.end - (int)j0, 16);
+            if (gb >= ge) continue;
+            const uint32_t p0 = (uint32_t)(ch.at + (int)j0), id = (uint32_t)ch.tb[p0 >> c.lg];
+            if (id >= c.pages) continue;
+            uint8_t* dst = c.data + ((uint64_t)id * c.kv + head) * c.block + B::v(c.page, 0) + d * c.page + (p0 & (c.page - 1));
+            uint32_t h[4], lo[4];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; q++) {
+                h[q] = lo[q] = 0;
+#pragma unroll
+                for (uint32_t l = 0; l < 4; l++) {
+                    const uint32_t x = (uint16_t)vt[j0 + 4 * q + l][d];
+                    h[q] |= ((I8 ? x : x >> 8) & 255u) << (8 * l);
+                    lo[q] |= ((x & 255u) ^ 128u) << (8 * l);
+                }
+            }
+            if (gb == 0 && ge == 16) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (!I8) *reinterpret_cast<uint4*>(dst + HD * c.page) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+#pragma unroll
+                for (int l = 0; l < 16; l++) {
+                    if (l < gb || l >= ge) continue;
+                    dst[l] = (uint8_t)(h[l / 4] >> (8 * (l & 3)));
+                    if constexpr (!I8) dst[HD * c.page + l] = (uint8_t)(lo[l / 4] >> (8 * (l & 3)));
+                }
+            }
+        }
+        return;
+    }
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (t >> 6)), ps = wv % passes, t0 = wv / passes * tpw;
+    const uint32_t total = bt.start(bt.batch);
+    if (t0 >= total) return;
+    const uint32_t t1 = min(t0 + tpw, total), rows = a.heads + c.kv;
+    const uint32_t r = ps * RW + lane / L;
+    const bool on = r < rows, isq = r < a.heads;
+    const uint32_t g = isq ? r : on ? r - a.heads : 0u;
+    const int16_t* src = (isq ? a.q : a.k) + g * HD + d0;
+    const uint64_t ld = isq ? a.q_ld : a.k_ld;
+    const uint8_t *np = isq ? a.norm_q : a.norm_k, *rp = isq ? a.rope_q : a.rope_k;
+    const bool cols = (isq ? a.rope_q_cols : a.rope_k_cols) != 0;
+    const int64_t eps = isq ? a.eps_q : a.eps_k;
+    const uint32_t half = a.rotary / 2;
+    const bool rot = d0 < a.rotary, upper = !a.interleaved && d0 >= half;
+    const int pl = (int)(!rot || a.interleaved ? lane : d0 < half ? lane + half / 8 : lane - half / 8);
+
+    // the double forms: a lane's 8 columns at the same shifts, the norm's Bq 0
+    int nG[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const ro::Param r0 = ro::ld_param(rp, g * HD + d0, !cols);
+    ro::Param n0{0, 0, 0, 0, 0};
+    bool plain = r0.sa <= 5 && r0.sb <= 5, nplain = true;    // int16 x int32 tables: two terms below 2^46 2^5
+    if (cols) {
+#pragma unroll
+        for (uint32_t l = 1; l < 8; l++) {
+            const ro::Param p = ro::ld_param(rp, g * HD + d0 + l, false);
+            plain = plain && p.sa == r0.sa && p.sb == r0.sb && p.sc == r0.sc;
+        }
+    }
+    if (np != nullptr) {
+        n0 = ro::ld_param(np, d0, false);
 #pragma unroll
         for (uint32_t l = 0; l < 8; l++) {
-            const ro::Param p = ro::ld_param(rp, g * HD + d0 + l, !cols);
-            const int co = rot ? cs[d0 + l] : 1 << 23, si = rot ? cs[a.rotary + d0 + l] : 0;
-            x[l] = ro::rope_elem(x[l], rot ? y[l] : 0, co, si, p);
+            const ro::Param n = ro::ld_param(np, d0 + l, false);
+            nG[l] = (int)n.g;
+            nplain = nplain && n.sc == n0.sc && n.bq == 0 && n.g < (1 << 27) && n.g > -(1 << 27);
         }
     }
-    if (isq) {
-        if (on) *reinterpret_cast<int4*>(a.qr + tok * a.qr_ld + g * HD + d0) = ro::pack16(x);
-        // fall through: the lanes of other rows of this wavefront share the shuffles below
-    }
-    // the int8 form's shift and codes, and the key's term
-    uint32_t e = 0;
-    if constexpr (I8) {
-        int m = 0;
-#pragma unroll
-        for (uint32_t l = 0; l < 8; l++) m = max(m, x[l] ^ (x[l] >> 31));
-#pragma unroll
-        for (uint32_t o = 1; o < L; o <<= 1) m = max(m, __shfl_xor(m, (int)o, 64));
-        e = (uint32_t)max(0, 32 - __clz(m) - 7);
-#pragma unroll
-        for (uint32_t l = 0; l < 8; l++) x[l] = min(127, (int)ro::rne_shr_fast(x[l], e));
-    }
-    int s = 0;
-#pragma unroll
-    for (uint32_t l = 0; l < 8; l++) s += x[l];
-#pragma unroll
-    for (uint32_t o = 1; o < L; o <<= 1) s += __shfl_xor(s, (int)o, 64);
-    if (isq || !on || pos < 0 || pos >= (int64_t)bt.cap) return;
-    const uint32_t id = (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)], slot = (uint32_t)pos & (c.page - 1);
-    if (id >= c.pages) return;
-    uint8_t* blk = c.data + ((uint64_t)id * c.kv + g) * c.block;
-    typedef Block<HD, I8> B;
-    uint32_t h[2], lo[2];                  // bytes of the two planes (the codes alone in int8)
-#pragma unroll
-    for (uint32_t w = 0; w < 2; w++) {
-        h[w] = lo[w] = 0;
-#pragma unroll
-        for (uint32_t l = 0; l < 4; l++) {
-            const uint32_t z = (uint32_t)x[4 * w + l];
-            h[w] |= ((I8 ? z : z >> 8) & 255u) << (8 * l);
-            lo[w] |= ((z & 255u) ^ 128u) << (8 * l);
+    const double rA = pow2(r0.sa), rB = pow2(r0.sb), rS = pow2(-r0.sc), nS = pow2(-n0.sc);
+    uint32_t b = find_le(bt.batch, t0, [&](uint32_t i) { return bt.start(i); });
+    uint32_t next = bt.start(b + 1);
+    int64_t base = (int64_t)bt.len(b) - next;                 // position = base + token
+    for (uint32_t tok = t0; tok < t1; tok++) {
+        while (tok >= next && b + 1 < bt.batch) {
+            next = bt.start(++b + 1);
+            base = (int64_t)bt.len(b) - next;
         }
-    }
-    if (!isv) {
-        *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = make_uint2(h[0], h[1]);
-        if constexpr (!I8) *reinterpret_cast<uint2*>(blk + B::k(c.page, 1) + slot * HD + d0) = make_uint2(lo[0], lo[1]);
+        const int64_t pos = base + tok;
+        const int4 xw = on ? *reinterpret_cast<const int4*>(src + tok * ld) : make_int4(0, 0, 0, 0);
+        const uint32_t trow = (uint32_t)min(max(pos, (int64_t)0), (int64_t)a.rope_rows - 1);
+        const int32_t* cs = a.rope + (uint64_t)trow * 2 * a.rotary + d0;
+        int co[8], si[8];
+        if (rot) {
+            const int4 c0 = *reinterpret_cast<const int4*>(cs), c1 = *reinterpret_cast<const int4*>(cs + 4);
+            const int4 s0 = *reinterpret_cast<const int4*>(cs + a.rotary), s1 = *reinterpret_cast<const int4*>(cs + a.rotary + 4);
+            co[0] = c0.x; co[1] = c0.y; co[2] = c0.z; co[3] = c0.w; co[4] = c1.x; co[5] = c1.y; co[6] = c1.z; co[7] = c1.w;
+            si[0] = s0.x; si[1] = s0.y; si[2] = s0.z; si[3] = s0.w; si[4] = s1.x; si[5] = s1.y; si[6] = s1.z; si[7] = s1.w;
+        } else {
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) {
+                co[l] = 1 << 23;
+                si[l] = 0;
+            }
+        }
+        int x[8];
+#pragma unroll
+        for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&xw)[l];
+        if (a.norm_q != nullptr || a.norm_k != nullptr) {     // every lane: the shuffles are the wavefront's
+            int64_t s2 = 0;
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) s2 += (int64_t)x[l] * x[l];
+            s2 = row_sum64<L>(s2);
+            if (np != nullptr) {
+                const int64_t D = s2 + eps;
+                uint64_t Rm;
+                int sh;
+                rsqrt64((uint64_t)(D > 0 ? D : 1), Rm, sh, a.tab);
+                const double scale = (double)Rm * pow2(24 - sh);        // x scale: below 2^48 of whole 2^(24 - sh)
+                double P1[8];
+                bool small = nplain;
+#pragma unroll
+                for (uint32_t l = 0; l < 8; l++) {
+                    P1[l] = __builtin_floor((double)x[l] * scale);
+                    small = small && __builtin_fabs(P1[l]) < 33554432.0;   // 2^25, so P1 G below 2^52
+                }
+                if (small) {
+#pragma unroll
+                    for (uint32_t l = 0; l < 8; l++) x[l] = rne_sat_f64(P1[l] * (double)nG[l], nS);
+                } else {
+#pragma unroll 1
+                    for (uint32_t l = 0; l < 8; l++) {
+                        const ro::Param p = ro::ld_param(np, d0 + l, false);
+                        x[l] = rne_sat((((int64_t)x[l] * (int64_t)Rm) >> (sh - 24)) * p.g + p.bq, (uint32_t)p.sc);
+                    }
+                }
+            }
+        }
+        int y[8];
+#pragma unroll
+        for (uint32_t l = 0; l < 8; l++) {
+            const int other = a.interleaved ? x[l ^ 1] : __shfl(x[l], pl, 64);
+            y[l] = (a.interleaved ? (l & 1) != 0 : upper) ? other : -other;
+        }
+        if (plain) {
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++)
+                x[l] = rne_sat_f64(__builtin_fma((double)x[l] * (double)co[l], rA, (double)y[l] * (double)si[l] * rB), rS);
+        } else {
+#pragma unroll 1
+            for (uint32_t l = 0; l < 8; l++) x[l] = ro::rope_elem(x[l], y[l], co[l], si[l], ro::ld_param(rp, g * HD + d0 + l, !cols));
+        }
+        if (on && isq) *reinterpret_cast<int4*>(a.qr + tok * a.qr_ld + g * HD + d0) = ro::pack16(x);
+        if (ps * RW + RW <= a.heads) continue;                // no k row in this wavefront's
+        uint32_t e = 0;
+        if constexpr (I8) e = quantise<L>(x);
+        int s = 0;
+#pragma unroll
+        for (uint32_t l = 0; l < 8; l++) s += x[l];
+#pragma unroll
+        for (uint32_t o = 1; o < L; o <<= 1) s += __shfl_xor(s, (int)o, 64);
+        if (!on || isq || pos < 0 || pos >= (int64_t)bt.cap) continue;
+        const uint32_t id = (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)], slot = (uint32_t)pos & (c.page - 1);
+        if (id >= c.pages) continue;
+        uint8_t* blk = c.data + ((uint64_t)id * c.kv + g) * c.block;
+        if constexpr (I8) {
+            uint32_t h[2];
+#pragma unroll
+            for (uint32_t w = 0; w < 2; w++)
+                h[w] = (x[4 * w] & 255) | (x[4 * w + 1] & 255) << 8 | (x[4 * w + 2] & 255) << 16 | (uint32_t)x[4 * w + 3] << 24;
+            *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = make_uint2(h[0], h[1]);
+        } else {
+            uint2 h, lo;
+            split8(ro::pack16(x), h, lo);
+            *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = h;
+            *reinterpret_cast<uint2*>(blk + B::k(c.page, 1) + slot * HD + d0) = lo;
+        }
         if (u == 0) {
             reinterpret_cast<int32_t*>(blk + B::term(c.page))[slot] = 128 * s - (I8 ? 0 : 16384 * (int)HD);
             if constexpr (I8) blk[B::ke(c.page) + slot] = (uint8_t)e;
         }
-    } else {
-#pragma unroll
-        for (uint32_t l = 0; l < 8; l++) {
-            blk[B::v(c.page, 0) + (d0 + l) * c.page + slot] = (uint8_t)(h[l / 4] >> (8 * (l & 3)));
-            if constexpr (!I8) blk[B::v(c.page, 1) + (d0 + l) * c.page + slot] = (uint8_t)(lo[l / 4] >> (8 * (l & 3)));
-        }
-        if constexpr (I8)
-            if (u == 0) blk[B::ve(c.page) + slot] = (uint8_t)e;
     }
 }
 
 // ---------------------------------------------------------------- read
+// A workgroup per 64-position chunk of a head: K rows as they lie, V 16 keys a lane through LDS.
 template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256) void paged_read_kernel(Cache c, Batch bt, int16_t* k, int16_t* v, uint64_t k_ld,
-                                                         uint64_t v_ld) {
-    constexpr uint32_t L = HD / 8, RW = 64 / L;
-    const uint32_t lane = threadIdx.x & 63, d0 = 8 * (lane % L);
-    const uint64_t first = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * RW;
-    const uint64_t items = (uint64_t)bt.start(bt.batch) * c.kv;
-    if (first >= items) return;
-    const uint64_t item = min(first + lane / L, items - 1);
-    const uint32_t tok = (uint32_t)(item / c.kv), g = (uint32_t)(item - (uint64_t)tok * c.kv);
-    uint32_t b = find_le(bt.batch, __builtin_amdgcn_readfirstlane(tok), [&](uint32_t i) { return bt.start(i); });
-    while (b + 1 < bt.batch && bt.start(b + 1) <= tok) b++;
-    const int n = (int)bt.start(b + 1) - (int)bt.start(b);
-    const int64_t pos = (int64_t)bt.len(b) - n + (int)(tok - bt.start(b));
-    const bool in = pos >= 0 && pos < (int64_t)bt.cap;
-    const uint32_t id = in ? (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)] : 0xFFFFFFFFu;
-    int kx[8] = {0, 0, 0, 0, 0, 0, 0, 0}, vx[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (id < c.pages) {
-        const uint32_t slot = (uint32_t)pos & (c.page - 1);
-        const uint8_t* blk = c.data + ((uint64_t)id * c.kv + g) * c.block;
-        typedef Block<HD, I8> B;
-        const int8_t *kp = reinterpret_cast<const int8_t*>(blk + B::k(c.page, 0) + slot * HD + d0),
-                     *vp = reinterpret_cast<const int8_t*>(blk + B::v(c.page, 0) + d0 * c.page + slot);
+__global__ __launch_bounds__(256) void paged_read_kernel(Cache c, Batch bt, int16_t* k, int16_t* v, uint64_t k_ld, uint64_t v_ld) {
+    constexpr uint32_t L = HD / 8;
+    typedef Block<HD, I8> B;
+    __shared__ int16_t vt[64][HD + 2];
+    const uint32_t t = threadIdx.x, head = blockIdx.y;
+    const Chunk ch(bt, blockIdx.x);
+    const int n = (int)bt.start(ch.b + 1) - (int)ch.q0;
+    const int rb = max(ch.base - ch.at, 0), re = min(ch.base + n - ch.at, 64);     // the chunk's tokens (without a row: zeros)
+    if (rb >= re) return;
+    auto block = [&](int j) -> const uint8_t* {
+        if (j < ch.beg || j >= ch.end) return nullptr;
+        const uint32_t id = (uint32_t)ch.tb[(uint32_t)(ch.at + j) >> c.lg];
+        return id < c.pages ? c.data + ((uint64_t)id * c.kv + head) * c.block : nullptr;
+    };
+    for (uint32_t i = t; i < 4 * HD; i += 256) {
+        const uint32_t d = i % HD, j0 = 16 * (i / HD);
+        const int gb = max(ch.beg - (int)j0, 0), ge = min(ch.end - (int)j0, 16);
+        uint32_t h[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, es[4] = {0, 0, 0, 0};
+        const uint8_t* blk = gb < ge ? block((int)j0 + gb) : nullptr;
+        if (blk != nullptr) {                                  // the whole 16-key piece lies in the page
+            const uint32_t in = (uint32_t)(ch.at + (int)j0) & (c.page - 1);
+            const uint8_t* p = blk + B::v(c.page, 0) + d * c.page + in;
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
+            const uint4 z = *reinterpret_cast<const uint4*>(I8 ? blk + B::ve(c.page) + in : p + HD * c.page);
+            (I8 ? es : lo)[0] = z.x; (I8 ? es : lo)[1] = z.y; (I8 ? es : lo)[2] = z.z; (I8 ? es : lo)[3] = z.w;
+        }
 #pragma unroll
-        for (uint32_t l = 0; l < 8; l++) {
-            if constexpr (I8) {
-                kx[l] = kp[l] << blk[B::ke(c.page) + slot];
-                vx[l] = vp[l * c.page] << blk[B::ve(c.page) + slot];
-            } else {
-                kx[l] = kp[l] * 256 + kp[c.page * HD + l] + 128;
-                vx[l] = vp[l * c.page] * 256 + vp[(HD + l) * c.page] + 128;
-            }
+        for (uint32_t l = 0; l < 16; l++) {
+            const int hb = (int8_t)(h[l / 4] >> (8 * (l & 3))), lb = (int8_t)(lo[l / 4] >> (8 * (l & 3)));
+            const int x = I8 ? hb << ((es[l / 4] >> (8 * (l & 3))) & 15u) : hb * 256 + lb + 128;
+            vt[j0 + l][d] = (int16_t)((int)l >= gb && (int)l < ge && blk != nullptr ? x : 0);
         }
     }
-    *reinterpret_cast<int4*>(k + tok * k_ld + g * HD + d0) = ro::pack16(kx);
-    *reinterpret_cast<int4*>(v + tok * v_ld + g * HD + d0) = ro::pack16(vx);
+    __syncthreads();
+    for (uint32_t i = t; i < 64 * L; i += 256) {
+        const int j = (int)(i / L);
+        const uint32_t d0 = 8 * (i % L);
+        if (j < rb || j >= re) continue;
+        const uint64_t tok = (uint64_t)((int64_t)ch.q0 + ch.at + j - ch.base);
+        int x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8];
+        if (const uint8_t* blk = block(j)) {
+            const uint32_t slot = (uint32_t)(ch.at + j) & (c.page - 1);
+            const uint8_t* kp = blk + B::k(c.page, 0) + slot * HD + d0;
+            const uint2 h = *reinterpret_cast<const uint2*>(kp);
+            uint2 lo = make_uint2(0, 0);
+            uint32_t e = 0;
+            if constexpr (I8) e = blk[B::ke(c.page) + slot] & 15u;
+            else lo = *reinterpret_cast<const uint2*>(kp + c.page * HD);
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) {
+                const int hb = (int8_t)((l < 4 ? h.x : h.y) >> (8 * (l & 3))), lb = (int8_t)((l < 4 ? lo.x : lo.y) >> (8 * (l & 3)));
+                x[l] = I8 ? hb << e : hb * 256 + lb + 128;
+            }
+        }
+#pragma unroll
+        for (uint32_t l = 0; l < 8; l++) y[l] = vt[j][d0 + l];
+        *reinterpret_cast<int4*>(k + tok * k_ld + head * HD + d0) = ro::pack16(x);
+        *reinterpret_cast<int4*>(v + tok * v_ld + head * HD + d0) = ro::pack16(y);
+    }
 }
 
 // ---------------------------------------------------------------- attention
@@ -575,45 +735,61 @@ struct Few {
         v4i acc[3][DB];
         uint32_t w;                         // the lane's weights: below 2^16 * 16 * kMaxPart / 64
     };
-    __device__ __forceinline__ void values(uint32_t i, uint32_t ido, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2, const Smx& smx,
-                                           const int32_t* stab, Sums& o) const {
-        const uint32_t kg = tl.lo + 64 * i + 16 * g, in = kg & (c.page - 1);
+    struct VRows {                          // the V operands of a step and the lane's keys' shifts
+        v4i h[DB], l[DB], es;
+    };
+    __device__ __forceinline__ void load_v(uint32_t i, uint32_t ido, VRows& v) const {
+        const uint32_t in = (tl.lo + 64 * i + 16 * g) & (c.page - 1);
         const uint8_t *vb = block(ido), *vp = vb + B::v(c.page, 0) + c16 * c.page + in;
-        v4i vh[DB], vl[DB], es = v4i{0, 0, 0, 0};
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
-            vh[m] = *reinterpret_cast<const v4i*>(vp + 16 * m * c.page);
-            if constexpr (!I8) vl[m] = *reinterpret_cast<const v4i*>(vp + (HD + 16 * m) * c.page);
+            v.h[m] = *reinterpret_cast<const v4i*>(vp + 16 * m * c.page);
+            if constexpr (!I8) v.l[m] = *reinterpret_cast<const v4i*>(vp + (HD + 16 * m) * c.page);
         }
-        if constexpr (I8) es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
-        uint32_t wp[8];
+        if constexpr (I8) v.es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
+        else v.es = v4i{0, 0, 0, 0};
+    }
+    // the weights of step i's scores in pairs, and their sum on top of sum
+    __device__ __forceinline__ void weights(uint32_t i, uint32_t ido, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2, const Smx& smx,
+                                            const int32_t* stab, uint32_t (&wp)[8], uint32_t& sum) const {
+        const uint32_t kg = tl.lo + 64 * i + 16 * g;
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++) {
             const Exp2 x = exps((int)(int16_t)sw[j], (int)sw[j] >> 16, m2, dl2, smx, stab);
             auto on = [&](uint32_t key) { return ido != ~0u && key >= vbeg && key < vend; };
             wp[j] = pair16(on(kg + 2 * j) ? x.e0() : 0u, on(kg + 2 * j + 1) ? x.e1() : 0u);
-            o.w = add16(wp[j], o.w);
+            sum = add16(wp[j], sum);
         }
-        v4i p[I8 ? 3 : 2];
+    }
+    // their byte operands; the column of ones
+    __device__ __forceinline__ void operands(const uint32_t (&wp)[8], const v4i es, v4i (&p)[I8 ? 3 : 2]) const {
 #pragma unroll
         for (uint32_t q = 0; q < 4; q++) {
             weight_bytes<I8>(wp[2 * q], wp[2 * q + 1], (uint32_t)es[q], p, q);
 #pragma unroll
             for (uint32_t x = 0; x < (I8 ? 3u : 2u); x++) p[x][q] = c16 == kFewRows ? 0x01010101 : p[x][q];
         }
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            if constexpr (I8) {
-                o.acc[0][m] = mfma(vh[m], p[I8 ? 2 : 0], o.acc[0][m]);
-                o.acc[1][m] = mfma(vh[m], p[1], o.acc[1][m]);
-                o.acc[2][m] = mfma(vh[m], p[0], o.acc[2][m]);
-            } else {
-                o.acc[0][m] = mfma(vh[m], p[1], o.acc[0][m]);
-                o.acc[1][m] = mfma(vh[m], p[0], o.acc[1][m]);
-                o.acc[2][m] = mfma(vl[m], p[0], o.acc[2][m]);
-                o.acc[1][m] = mfma(vl[m], p[1], o.acc[1][m]);
-            }
+    }
+    static __device__ __forceinline__ void pv(const v4i vh, const v4i vl, const v4i (&p)[I8 ? 3 : 2], v4i& a0, v4i& a1, v4i& a2) {
+        if constexpr (I8) {
+            a0 = mfma(vh, p[I8 ? 2 : 0], a0);
+            a1 = mfma(vh, p[1], a1);
+            a2 = mfma(vh, p[0], a2);
+        } else {
+            a0 = mfma(vh, p[1], a0);
+            a1 = mfma(vh, p[0], a1);
+            a2 = mfma(vl, p[0], a2);
+            a1 = mfma(vl, p[1], a1);
         }
+    }
+    __device__ __forceinline__ void values(uint32_t i, uint32_t ido, const VRows& v, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2,
+                                           const Smx& smx, const int32_t* stab, Sums& o) const {
+        uint32_t wp[8];
+        weights(i, ido, sw, m2, dl2, smx, stab, wp, o.w);
+        v4i p[I8 ? 3 : 2];
+        operands(wp, v.es, p);
+#pragma unroll
+        for (uint32_t m = 0; m < DB; m++) pv(v.h[m], v.l[m], p, o.acc[0][m], o.acc[1][m], o.acc[2][m]);
     }
 };
 
@@ -624,23 +800,32 @@ struct FewSums {
     __device__ __forceinline__ void clear() {
         for (uint32_t i = threadIdx.x; i < sizeof(FewSums) / 8; i += blockDim.x) reinterpret_cast<int64_t*>(this)[i] = 0;
     }
-    // a wavefront's sums added (LDS atomics of integers: the order is free)
+    static __device__ __forceinline__ void put(int64_t* p, int64_t x) {
+        atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)x);
+    }
+    // a wavefront's sums added (LDS atomics of integers: the order is free): of its weights, and of 16 columns m
     template <bool I8>
-    __device__ __forceinline__ void add(const Few<HD, I8>& f, const typename Few<HD, I8>::Sums& o) {
-        int64_t ws = o.w;
+    __device__ __forceinline__ void add_w(const Few<HD, I8>& f, uint32_t sum) {
+        int64_t ws = sum;
         ws += (int64_t)ro::shfl64((uint64_t)ws, 16);
         ws += (int64_t)ro::shfl64((uint64_t)ws, 32);
-        auto put = [](int64_t* p, int64_t x) { atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)x); };
         if (f.mine && f.g == 0) put(&w[f.c16], ws);
+    }
+    template <bool I8>
+    __device__ __forceinline__ void add_v(const Few<HD, I8>& f, uint32_t m, const v4i a0, const v4i a1, const v4i a2) {
 #pragma unroll
-        for (uint32_t m = 0; m < HD / 16; m++)
+        for (uint32_t r = 0; r < 4; r++) {
+            const uint32_t d = 16 * m + 4 * f.g + r;
+            const int64_t hh = a0[r], mid = a1[r], ll = a2[r];
+            if (f.mine) put(&part[f.c16][d], hh * 65536 + mid * 256 + ll);
+            else if (f.c16 == kFewRows) put(&v[d], I8 ? hh : hh * 256 + ll);
+        }
+    }
+    template <bool I8>
+    __device__ __forceinline__ void add(const Few<HD, I8>& f, const typename Few<HD, I8>::Sums& o) {
+        add_w<I8>(f, o.w);
 #pragma unroll
-            for (uint32_t r = 0; r < 4; r++) {
-                const uint32_t d = 16 * m + 4 * f.g + r;
-                const int64_t hh = o.acc[0][m][r], mid = o.acc[1][m][r], ll = o.acc[2][m][r];
-                if (f.mine) put(&part[f.c16][d], hh * 65536 + mid * 256 + ll);
-                else if (f.c16 == kFewRows) put(&v[d], I8 ? hh : hh * 256 + ll);
-            }
+        for (uint32_t m = 0; m < HD / 16; m++) add_v<I8>(f, m, o.acc[0][m], o.acc[1][m], o.acc[2][m]);
     }
     template <bool I8>
     __device__ __forceinline__ int64_t sum(uint32_t r, uint32_t d) const {
@@ -659,32 +844,51 @@ struct FewSums {
     }
 };
 
-// Caches of at most kShort keys in one launch: a tile's steps over the wavefronts of one workgroup (16, or 8 at 128 d
-// for its registers), at most NS each, their scores kept between the maximum and the weights.
+// Caches of at most kShort keys in one launch of 16 wavefronts a tile.  For the scores a wavefront takes steps w, w + 16;
+// the weights go through LDS (16 steps a round), and for P.V a wavefront takes 16 columns of V over 4 of the round's
+// steps (8 at 128 d): its sums are 12 registers, and 4 (2) of them meet in LDS instead of 16.  V's first round is read
+// beside K: one memory latency for both.  16 sequences of 1024 rows, 15 heads: us with V's columns undivided 11.5.
 constexpr uint32_t kShort = 2048;
 
 template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(HD == 64 ? 1024 : 512) void paged_short_kernel(Cache c, Batch bt, Attn a, const int32_t* __restrict__ tab) {
-    constexpr uint32_t NW = HD == 64 ? 16 : 8, NS = kShort / 64 / NW;
+__global__ __launch_bounds__(1024) void paged_short_kernel(Cache c, Batch bt, Attn a, const int32_t* __restrict__ tab) {
     typedef Few<HD, I8> F;
+    typedef Block<HD, I8> B;
+    constexpr uint32_t NW = 16, NS = kShort / 64 / NW, DB = HD / 16, KG = NW / DB, SP = NW / KG;   // SP steps a wavefront and round
     __shared__ __attribute__((aligned(16))) int32_t stab[4096];
+    __shared__ __attribute__((aligned(16))) uint4 wts[NW][2][64];
     __shared__ int32_t redm[NW][16];
     __shared__ FewSums<HD> sums;
     const Tile<kFewRows> tl(bt, a, blockIdx.x);
     if (!tl.on) return;
     const F f(c, bt, a, tl, blockIdx.y);
-#pragma unroll
-    for (uint32_t i = 0; i < 16 / NW; i++)
-        __builtin_amdgcn_global_load_lds(tab + 4 * (threadIdx.x + 64 * NW * i),
-                                         (__attribute__((address_space(3))) void*)(stab + 4 * (64 * f.w + 64 * NW * i)), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(tab + 4 * threadIdx.x, (__attribute__((address_space(3))) void*)(stab + 256 * f.w), 16, 0, 0);
     sums.clear();
-    uint32_t idr[NS], ido[NS], sw[NS][8];
+    const uint32_t vm = f.w % DB, vk = f.w / DB;     // the wavefront's columns of V, and its steps vk, vk + KG, .. of a round
+    constexpr uint32_t PF = HD == 64 || I8 ? 4 : 2;    // steps of V read ahead: 32 registers at most
+    uint32_t idr[NS], ido[NS], sw[NS][8], idv[PF];
 #pragma unroll
     for (uint32_t k = 0; k < NS; k++) {
         idr[k] = f.id_row(f.w + NW * k, tl.nt);
         ido[k] = f.id_own(f.w + NW * k, tl.nt);
     }
+#pragma unroll
+    for (uint32_t k = 0; k < PF; k++) idv[k] = f.id_own(vk + KG * k, tl.nt);
+    struct VCols {
+        v4i h, l, es;
+    } v[PF];
+    auto load_v = [&](uint32_t i, uint32_t id, VCols& x) {
+        const uint32_t in = (tl.lo + 64 * i + 16 * f.g) & (c.page - 1);
+        const uint8_t *vb = f.block(id), *vp = vb + B::v(c.page, 0) + (16 * vm + f.c16) * c.page + in;
+        x.h = *reinterpret_cast<const v4i*>(vp);
+        if constexpr (!I8) x.l = *reinterpret_cast<const v4i*>(vp + HD * c.page);
+        if constexpr (I8) x.es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
+        else x.es = v4i{0, 0, 0, 0};
+    };
     const typename F::Query q = f.query(a);
+#pragma unroll
+    for (uint32_t k = 0; k < PF; k++)
+        if (vk + KG * k < tl.nt) load_v(vk + KG * k, idv[k], v[k]);
     int mx = kNone;
 #pragma unroll
     for (uint32_t k = 0; k < NS; k++)
@@ -697,14 +901,33 @@ __global__ __launch_bounds__(HD == 64 ? 1024 : 512) void paged_short_kernel(Cach
 #pragma unroll
     for (uint32_t k = 0; k < NW; k++) mx = max(mx, redm[k][f.c16]);
     const uint32_t m2 = twice((uint32_t)sat16i(mx >> 8)), dl2 = twice(a.smx.dlim);
-    typename F::Sums o;
+    v4i acc[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
+    uint32_t wsum = 0;
 #pragma unroll
-    for (uint32_t m = 0; m < F::DB; m++) o.acc[0][m] = o.acc[1][m] = o.acc[2][m] = v4i{0, 0, 0, 0};
-    o.w = 0;
+    for (uint32_t k = 0; k < NS; k++) {
+        if (k && NW * k >= tl.nt) break;
+        if (k) __syncthreads();                        // the round before read
+        if (f.w + NW * k < tl.nt) {
+            uint32_t wp[8];
+            f.weights(f.w + NW * k, ido[k], sw[k], m2, dl2, a.smx, stab, wp, wsum);
+            wts[f.w][0][f.lane] = make_uint4(wp[0], wp[1], wp[2], wp[3]);
+            wts[f.w][1][f.lane] = make_uint4(wp[4], wp[5], wp[6], wp[7]);
+        }
+        __syncthreads();
 #pragma unroll
-    for (uint32_t k = 0; k < NS; k++)
-        if (f.w + NW * k < tl.nt) f.values(f.w + NW * k, ido[k], sw[k], m2, dl2, a.smx, stab, o);
-    if (f.w < tl.nt) sums.template add<I8>(f, o);
+        for (uint32_t j = 0; j < SP; j++) {
+            const uint32_t st = vk + KG * j, i = st + NW * k;
+            if (i >= tl.nt) break;
+            if (k || j >= PF) load_v(i, f.id_own(i, tl.nt), v[j % PF]);
+            const uint4 w0 = wts[st][0][f.lane], w1 = wts[st][1][f.lane];
+            const uint32_t wp[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            v4i p[I8 ? 3 : 2];
+            f.operands(wp, v[j % PF].es, p);
+            F::pv(v[j % PF].h, v[j % PF].l, p, acc[0], acc[1], acc[2]);
+        }
+    }
+    if (f.w < tl.nt) sums.template add_w<I8>(f, wsum);
+    if (vk < tl.nt) sums.template add_v<I8>(f, vm, acc[0], acc[1], acc[2]);
     __syncthreads();
     sums.template store<I8>(a, tl, blockIdx.y);
 }
@@ -783,6 +1006,8 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(Cache c, Batch bt, At
     };
     uint32_t ido = f.id_own(beg, end), sw[8];
     load(beg, sw);
+    typename F::VRows v;
+    f.load_v(beg, ido, v);                 // a wavefront without a step: block 0
     const uint32_t m2 = twice((uint32_t)row_max(wk, f.wrow, tl.parts(wk.per_s), f.g)), dl2 = twice(a.smx.dlim);
     __builtin_amdgcn_s_waitcnt(0x0070);               // the TAB's copies
     __syncthreads();
@@ -794,7 +1019,10 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(Cache c, Batch bt, At
         const uint32_t no = f.id_own(i + 4, end);
         uint32_t ns[8];
         load(i + 4, ns);
-        f.values(i, ido, sw, m2, dl2, a.smx, stab, o);
+        typename F::VRows nv;
+        f.load_v(i + 4, no, nv);           // past the end: block 0, not used
+        f.values(i, ido, v, sw, m2, dl2, a.smx, stab, o);
+        v = nv;
         ido = no;
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) sw[k] = ns[k];
@@ -1278,10 +1506,14 @@ int run_prep(const cm_paged_cache* cache, const cm_paged_batch* batch, const cm_
                  p.rope, static_cast<const uint8_t*>(p.rope_q), static_cast<const uint8_t*>(p.rope_k),
                  static_cast<const uint8_t*>(p.norm_q), static_cast<const uint8_t*>(p.norm_k), p.rope_q_cols,
                  p.rope_k_cols, p.eps_q, p.eps_k, st->ro_tables};
-    const uint64_t items = (uint64_t)b.tokens * (p.heads + 2 * c.kv), per = 4 * (64 / (cache->head_dim / 8));
-    const dim3 grid((unsigned)((items + per - 1) / per));
+    // q and k: `tpw` tokens a wavefront once there are 4096 wavefronts; V: a workgroup a chunk and head
+    const uint32_t rw = 64 / (cache->head_dim / 8), passes = (p.heads + c.kv + rw - 1) / rw;
+    const uint32_t tpw = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)b.tokens * passes / 4096, 1), 8);
+    const uint64_t waves = (uint64_t)((b.tokens + tpw - 1) / tpw) * passes, qk = (waves + 3) / 4, vb = chunk_slots(b) * c.kv;
+    if (qk + vb > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged prep: %u tokens of %u heads", b.tokens, p.heads);
+    const dim3 grid((unsigned)(qk + vb));
 #define CM_PREP(HD, I8)                                                                                     \
-    CM_LAUNCH("paged_prep_kernel", (paged_prep_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a)
+    CM_LAUNCH("paged_prep_kernel", (paged_prep_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, (uint32_t)qk, passes, tpw)
     if (cache->head_dim == 64) {
         if (cache->int8) { CM_PREP(64, true); } else { CM_PREP(64, false); }
     } else {
@@ -1305,8 +1537,7 @@ int run_read(const cm_paged_cache* cache, const cm_paged_batch* batch, int16_t* 
         return fail(CM_EINVAL, "paged read: rows of %llu columns overlap at their strides", (unsigned long long)kw);
     DeviceState* st;
     if ((rc = state(&st))) return rc;
-    const uint64_t items = (uint64_t)b.tokens * c.kv, per = 4 * (64 / (cache->head_dim / 8));
-    const dim3 grid((unsigned)((items + per - 1) / per));
+    const dim3 grid((unsigned)chunk_slots(b), c.kv);
 #define CM_READ(HD, I8) \
     CM_LAUNCH("paged_read_kernel", (paged_read_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, k, v, k_ld, v_ld)
     if (cache->head_dim == 64) {
@@ -1350,7 +1581,7 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     const dim3 tiles((unsigned)slots, c.kv);
     if (few && b.cap <= kShort) {
 #define CM_SHORT(HD, I8) \
-    CM_LAUNCH("paged_short_kernel", (paged_short_kernel<HD, I8>), tiles, dim3(HD == 64 ? 1024 : 512), 0, s, c, b, a, st->smx_tab)
+    CM_LAUNCH("paged_short_kernel", (paged_short_kernel<HD, I8>), tiles, dim3(1024), 0, s, c, b, a, st->smx_tab)
         if (cache->head_dim == 64) {
             if (cache->int8) { CM_SHORT(64, true); } else { CM_SHORT(64, false); }
         } else {
