@@ -80,13 +80,14 @@ struct Prep {
     const uint8_t* tab;                    // the row-ops table image (rsqrt entries)
 };
 
-// rsqrt_bf (cm_rowops_math.h) for D below 2^63
-__device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const uint8_t* tab) {
+// rsqrt_bf (cm_rowops_math.h) for D below 2^63; tab: the table image's entries from index 2048 on (Dm >= 2^30)
+constexpr uint32_t kRsqrt = 8192 - 2048;
+__device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const uint32_t* tab) {
     const int e = 64 - __clzll((long long)D);
     int d = e - 32;
     d += d & 1;
     const uint32_t Dm = (uint32_t)(d >= 0 ? D >> d : D << -d);
-    const uint32_t y0 = *reinterpret_cast<const uint32_t*>(tab + 32768 + 4 * ((Dm >> 19) & 8191u));
+    const uint32_t y0 = tab[(Dm >> 19) - 2048];
     const int64_t r = ((int64_t)1 << 30) - (int64_t)__umulhi(__umulhi(Dm, y0), y0);     // above -2^32
     // y0 r >> 31 in 64 bits where r is below 2^31 (the unit's own table: below 2^18), else in two halves of y0
     const int64_t step = r >= -((int64_t)1 << 31) ? ((int64_t)y0 * r) >> 31
@@ -99,17 +100,43 @@ __device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const
 __device__ __forceinline__ int rne_sat(int64_t v, uint32_t sc) {
     return (int)(sc <= 61 ? ro::sat16(ro::rne_shr_fast(v, sc)) : ro::sat16(ro::rne_shr((__int128)v, (int)sc)));
 }
-// v / 2^sc rounded half to even and saturated, of a whole number |v| <= 2^53 (v_rndne_f64; the scaling is exact)
+// v scale rounded half to even and saturated (|v scale| < 2^31): the sum with 1.5 2^52 has its units in the low word,
+// one v_fma_f64 for a product, a rounding and a conversion
 __device__ __forceinline__ int rne_sat_f64(double v, double scale) {
-    return sat16i((int)__builtin_rint(fmin(fmax(v * scale, -65536.0), 65536.0)));
+    return sat16i((int)(uint32_t)__builtin_bit_cast(uint64_t, __builtin_fma(v, scale, 0x1.8p52)));
+}
+// x as a double: the low word of 2^52 + 2^31 + x, less 2^52 + 2^31 (an exclusive or and a v_add_f64)
+__device__ __forceinline__ double f64(int x) {
+    return __builtin_bit_cast(double, (uint64_t)0x43300000u << 32 | ((uint32_t)x ^ 0x80000000u)) - 0x1.00000800p52;
 }
 __device__ __forceinline__ double pow2(int e) { return __builtin_bit_cast(double, (uint64_t)(1023 + e) << 52); }
 
-template <uint32_t L>
-__device__ __forceinline__ int64_t row_sum64(int64_t x) {     // over the L lanes of a row
-#pragma unroll
-    for (uint32_t o = 1; o < L; o <<= 1) x += (int64_t)ro::shfl64((uint64_t)x, (int)o);
+// Over the L = 8 or 16 lanes of a row (DPP, no LDS)
+template <uint32_t L, class F>
+__device__ __forceinline__ uint32_t row_all(uint32_t x, F f) {
+    x = f(x, ro::row16_step<0>(x));
+    x = f(x, ro::row16_step<1>(x));
+    x = f(x, ro::row16_step<2>(x));
+    if constexpr (L == 16) x = f(x, ro::row16_step<3>(x));
     return x;
+}
+template <uint32_t L>
+__device__ __forceinline__ uint64_t row_sum64(uint64_t x) {
+    auto add = [&](uint32_t lo, uint32_t hi) { x += (uint64_t)hi << 32 | lo; };
+    add(ro::row16_step<0>((uint32_t)x), ro::row16_step<0>((uint32_t)(x >> 32)));
+    add(ro::row16_step<1>((uint32_t)x), ro::row16_step<1>((uint32_t)(x >> 32)));
+    add(ro::row16_step<2>((uint32_t)x), ro::row16_step<2>((uint32_t)(x >> 32)));
+    if constexpr (L == 16) add(ro::row16_step<3>((uint32_t)x), ro::row16_step<3>((uint32_t)(x >> 32)));
+    return x;
+}
+// the sum of 8 int16 squares: two a v_dot2_i32_i16, at most 2^31 as an unsigned word
+__device__ __forceinline__ uint64_t squares8(const int4 v) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    auto sq = [](int w) {
+        const s16x2 x = __builtin_bit_cast(s16x2, w);
+        return (uint64_t)(uint32_t)__builtin_amdgcn_sdot2(x, x, 0, false);
+    };
+    return sq(v.x) + sq(v.y) + sq(v.z) + sq(v.w);
 }
 
 // The 8-bit form of a row held by L lanes of 8 columns: its shift, and the codes in place
@@ -118,8 +145,7 @@ __device__ __forceinline__ uint32_t quantise(int (&x)[8]) {
     int m = 0;
 #pragma unroll
     for (uint32_t l = 0; l < 8; l++) m = max(m, x[l] ^ (x[l] >> 31));
-#pragma unroll
-    for (uint32_t o = 1; o < L; o <<= 1) m = max(m, __shfl_xor(m, (int)o, 64));
+    m = (int)row_all<L>((uint32_t)m, [](uint32_t p, uint32_t q) { return max(p, q); });
     const int e = max(0, 25 - __clz(m));                       // bits(m) - 7
 #pragma unroll
     for (uint32_t l = 0; l < 8; l++) {
@@ -158,9 +184,11 @@ template <uint32_t HD, bool I8>
 __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep a, uint32_t qk_blocks, uint32_t passes, uint32_t tpw) {
     constexpr uint32_t L = HD / 8, RW = 64 / L;
     typedef Block<HD, I8> B;
-    __shared__ int16_t vt[64][HD + 2];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kRsqrt];       // the rsqrt table, or V's transposition
+    static_assert(64 * (HD + 2) * 2 <= sizeof(lds), "a chunk of V");
     const uint32_t t = threadIdx.x, lane = t & 63, u = lane % L, d0 = 8 * u;
     if (blockIdx.x >= qk_blocks) {
+        int16_t (*vt)[HD + 2] = reinterpret_cast<int16_t (*)[HD + 2]>(lds);
         const uint32_t vb = blockIdx.x - qk_blocks, head = vb % c.kv;
         const Chunk ch(bt, vb / c.kv);
         if (ch.beg >= ch.end) return;
@@ -217,63 +245,98 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         }
         return;
     }
-    const uint32_t wv = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (t >> 6)), ps = wv % passes, t0 = wv / passes * tpw;
-    const uint32_t total = bt.start(bt.batch);
-    if (t0 >= total) return;
-    const uint32_t t1 = min(t0 + tpw, total), rows = a.heads + c.kv;
-    const uint32_t r = ps * RW + lane / L;
+    // every load that needs no other comes first: the rsqrt table, the first token's x, the parameters, the batch
+    const bool norms = a.norm_q != nullptr || a.norm_k != nullptr;
+    if (norms) {
+#pragma unroll
+        for (uint32_t i = 0; i < kRsqrt / 1024; i++)
+            __builtin_amdgcn_global_load_lds(a.tab + 32768 + 4 * 2048 + 16 * (t + 256 * i),
+                                             (__attribute__((address_space(3))) void*)(lds + 16 * (64 * (t >> 6) + 256 * i)), 16, 0, 0);
+    }
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (t >> 6)), ps = wv % passes;
+    const uint32_t t0 = min(wv / passes * tpw, bt.tokens - 1);      // past the end: below
+    const bool idle = wv / passes * tpw >= bt.tokens;
+    const uint32_t rows = a.heads + c.kv, r = ps * RW + lane / L;
     const bool on = r < rows, isq = r < a.heads;
     const uint32_t g = isq ? r : on ? r - a.heads : 0u;
     const int16_t* src = (isq ? a.q : a.k) + g * HD + d0;
     const uint64_t ld = isq ? a.q_ld : a.k_ld;
     const uint8_t *np = isq ? a.norm_q : a.norm_k, *rp = isq ? a.rope_q : a.rope_k;
     const bool cols = (isq ? a.rope_q_cols : a.rope_k_cols) != 0;
-    const int64_t eps = isq ? a.eps_q : a.eps_k;
+    int4 xw = *reinterpret_cast<const int4*>(src + t0 * ld);
+    uint4 nw[8], rw[8];
+    rw[0] = *reinterpret_cast<const uint4*>(rp + (cols ? 16 * (g * HD + d0) : 0u));
+    if (cols) {
+#pragma unroll
+        for (uint32_t l = 1; l < 8; l++) rw[l] = *reinterpret_cast<const uint4*>(rp + 16 * (g * HD + d0 + l));
+    }
+#pragma unroll
+    for (uint32_t l = 0; l < 8; l++) nw[l] = np != nullptr ? *reinterpret_cast<const uint4*>(np + 16 * (d0 + l)) : make_uint4(0, 0, 22u << 16, 0);
+    uint32_t b, next, total;
+    int64_t base;                           // position = base + token
+    if (bt.batch <= 64) {
+        const uint32_t i = min(lane, bt.batch - 1), s0 = bt.start(i), s1 = bt.start(i + 1), l = (uint32_t)bt.len(i);
+        b = max((uint32_t)__popcll(__ballot(lane < bt.batch && s0 <= t0)), 1u) - 1;
+        next = (uint32_t)__builtin_amdgcn_readlane((int)s1, b);
+        base = (int64_t)__builtin_amdgcn_readlane((int)l, b) - next;
+        total = (uint32_t)__builtin_amdgcn_readlane((int)s1, bt.batch - 1);
+    } else {
+        b = find_le(bt.batch, t0, [&](uint32_t i) { return bt.start(i); });
+        next = bt.start(b + 1);
+        base = (int64_t)bt.len(b) - next;
+        total = bt.start(bt.batch);
+    }
+    if (norms) {
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        __syncthreads();
+    }
+    if (idle || t0 >= total) return;
+    const uint32_t t1 = min(t0 + tpw, total);
+    const uint64_t eps = (uint64_t)(isq ? a.eps_q : a.eps_k);
     const uint32_t half = a.rotary / 2;
     const bool rot = d0 < a.rotary, upper = !a.interleaved && d0 >= half;
     const int pl = (int)(!rot || a.interleaved ? lane : d0 < half ? lane + half / 8 : lane - half / 8);
+    const uint32_t minus = a.interleaved || upper ? 0u : 0x80000000u;     // the partner's sign, on its product's high word
 
-    // the double forms: a lane's 8 columns at the same shifts, the norm's Bq 0
-    int nG[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const ro::Param r0 = ro::ld_param(rp, g * HD + d0, !cols);
-    ro::Param n0{0, 0, 0, 0, 0};
-    bool plain = r0.sa <= 5 && r0.sb <= 5, nplain = true;    // int16 x int32 tables: two terms below 2^46 2^5
+    // The double forms: a lane's 8 columns at the same shifts, the norm's Bq 0.  x cos + y sin is below 2^47 for any
+    // int32 table, its rounded quotient below 2^30; |P1 G| below 2^52 (see below), its quotient below 2^30.
+    const ro::Param r0 = ro::param_of(rw[0]);
+    bool plain = r0.sa == r0.sb && r0.sc >= r0.sa + 17, nplain = true;
     if (cols) {
 #pragma unroll
-        for (uint32_t l = 1; l < 8; l++) {
-            const ro::Param p = ro::ld_param(rp, g * HD + d0 + l, false);
-            plain = plain && p.sa == r0.sa && p.sb == r0.sb && p.sc == r0.sc;
-        }
+        for (uint32_t l = 1; l < 8; l++) plain = plain && ((rw[l].z ^ rw[0].z) & 0x3F3F3Fu) == 0;
     }
-    if (np != nullptr) {
-        n0 = ro::ld_param(np, d0, false);
+    const double rS = pow2(r0.sa - r0.sc);
+    double nG[8];                           // G 2^-sc
 #pragma unroll
-        for (uint32_t l = 0; l < 8; l++) {
-            const ro::Param n = ro::ld_param(np, d0 + l, false);
-            nG[l] = (int)n.g;
-            nplain = nplain && n.sc == n0.sc && n.bq == 0 && n.g < (1 << 27) && n.g > -(1 << 27);
-        }
+    for (uint32_t l = 0; l < 8; l++) {
+        const ro::Param n = ro::param_of(nw[l]);
+        nG[l] = (double)(int)n.g * pow2(-n.sc);
+        nplain = nplain && n.sc >= 22 && n.bq == 0 && n.g < (1 << 27) && n.g > -(1 << 27);
     }
-    const double rA = pow2(r0.sa), rB = pow2(r0.sb), rS = pow2(-r0.sc), nS = pow2(-n0.sc);
-    uint32_t b = find_le(bt.batch, t0, [&](uint32_t i) { return bt.start(i); });
-    uint32_t next = bt.start(b + 1);
-    int64_t base = (int64_t)bt.len(b) - next;                 // position = base + token
-    for (uint32_t tok = t0; tok < t1; tok++) {
+    plain = __all(plain || !on);
+    // A token's loads are issued before the stores of the one before: a wait for a load is a wait for every older store
+    int64_t pos;
+    int4 c0, c1, s0, s1;
+    uint32_t id;
+    auto fetch = [&](uint32_t tok) {
         while (tok >= next && b + 1 < bt.batch) {
             next = bt.start(++b + 1);
             base = (int64_t)bt.len(b) - next;
         }
-        const int64_t pos = base + tok;
-        const int4 xw = on ? *reinterpret_cast<const int4*>(src + tok * ld) : make_int4(0, 0, 0, 0);
+        pos = base + tok;
         const uint32_t trow = (uint32_t)min(max(pos, (int64_t)0), (int64_t)a.rope_rows - 1);
-        const int32_t* cs = a.rope + (uint64_t)trow * 2 * a.rotary + d0;
-        int co[8], si[8];
-        if (rot) {
-            const int4 c0 = *reinterpret_cast<const int4*>(cs), c1 = *reinterpret_cast<const int4*>(cs + 4);
-            const int4 s0 = *reinterpret_cast<const int4*>(cs + a.rotary), s1 = *reinterpret_cast<const int4*>(cs + a.rotary + 4);
-            co[0] = c0.x; co[1] = c0.y; co[2] = c0.z; co[3] = c0.w; co[4] = c1.x; co[5] = c1.y; co[6] = c1.z; co[7] = c1.w;
-            si[0] = s0.x; si[1] = s0.y; si[2] = s0.z; si[3] = s0.w; si[4] = s1.x; si[5] = s1.y; si[6] = s1.z; si[7] = s1.w;
-        } else {
+        const int32_t* cs = a.rope + (uint64_t)trow * 2 * a.rotary + (rot ? d0 : 0u);
+        c0 = *reinterpret_cast<const int4*>(cs);
+        c1 = *reinterpret_cast<const int4*>(cs + 4);
+        s0 = *reinterpret_cast<const int4*>(cs + a.rotary);
+        s1 = *reinterpret_cast<const int4*>(cs + a.rotary + 4);
+        id = pos >= 0 && pos < (int64_t)bt.cap ? (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)] : ~0u;
+    };
+    fetch(t0);
+    for (uint32_t tok = t0; tok < t1; tok++) {
+        int co[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, si[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        if (!rot) {
 #pragma unroll
             for (uint32_t l = 0; l < 8; l++) {
                 co[l] = 1 << 23;
@@ -283,27 +346,18 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         int x[8];
 #pragma unroll
         for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&xw)[l];
-        if (a.norm_q != nullptr || a.norm_k != nullptr) {     // every lane: the shuffles are the wavefront's
-            int64_t s2 = 0;
-#pragma unroll
-            for (uint32_t l = 0; l < 8; l++) s2 += (int64_t)x[l] * x[l];
-            s2 = row_sum64<L>(s2);
+        if (norms) {                        // every lane: the sums are the wavefront's
+            const uint64_t s2 = row_sum64<L>(squares8(xw));
             if (np != nullptr) {
-                const int64_t D = s2 + eps;
+                const uint64_t D = max(s2 + eps, (uint64_t)1);
                 uint64_t Rm;
                 int sh;
-                rsqrt64((uint64_t)(D > 0 ? D : 1), Rm, sh, a.tab);
-                const double scale = (double)Rm * pow2(24 - sh);        // x scale: below 2^48 of whole 2^(24 - sh)
-                double P1[8];
-                bool small = nplain;
+                rsqrt64(D, Rm, sh, reinterpret_cast<const uint32_t*>(lds));
+                const double scale = (double)Rm * pow2(24 - sh);        // x scale: 48 bits, exact
+                // |x| <= sqrt(D), so |P1| <= sqrt(D) scale + 1; below 2^25 (the unit's own table: 2^24) P1 G is below 2^52
+                if (nplain && scale * scale * (double)D < 0x1p49) {
 #pragma unroll
-                for (uint32_t l = 0; l < 8; l++) {
-                    P1[l] = __builtin_floor((double)x[l] * scale);
-                    small = small && __builtin_fabs(P1[l]) < 33554432.0;   // 2^25, so P1 G below 2^52
-                }
-                if (small) {
-#pragma unroll
-                    for (uint32_t l = 0; l < 8; l++) x[l] = rne_sat_f64(P1[l] * (double)nG[l], nS);
+                    for (uint32_t l = 0; l < 8; l++) x[l] = rne_sat_f64(__builtin_floor(f64(x[l]) * scale), nG[l]);
                 } else {
 #pragma unroll 1
                     for (uint32_t l = 0; l < 8; l++) {
@@ -313,19 +367,28 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
                 }
             }
         }
-        int y[8];
+        int y[8];                           // the partners
 #pragma unroll
-        for (uint32_t l = 0; l < 8; l++) {
-            const int other = a.interleaved ? x[l ^ 1] : __shfl(x[l], pl, 64);
-            y[l] = (a.interleaved ? (l & 1) != 0 : upper) ? other : -other;
-        }
+        for (uint32_t l = 0; l < 8; l++) y[l] = a.interleaved ? x[l ^ 1] : __shfl(x[l], pl, 64);
         if (plain) {
 #pragma unroll
-            for (uint32_t l = 0; l < 8; l++)
-                x[l] = rne_sat_f64(__builtin_fma((double)x[l] * (double)co[l], rA, (double)y[l] * (double)si[l] * rB), rS);
+            for (uint32_t l = 0; l < 8; l++) {
+                const uint32_t m = a.interleaved && !(l & 1) ? 0x80000000u : minus;
+                const double ys = f64(y[l]) * f64(si[l]);
+                const double z = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, ys) ^ (uint64_t)m << 32);
+                x[l] = rne_sat_f64(__builtin_fma(f64(x[l]), f64(co[l]), z), rS);
+            }
         } else {
 #pragma unroll 1
-            for (uint32_t l = 0; l < 8; l++) x[l] = ro::rope_elem(x[l], y[l], co[l], si[l], ro::ld_param(rp, g * HD + d0 + l, !cols));
+            for (uint32_t l = 0; l < 8; l++) {
+                const bool neg = a.interleaved ? !(l & 1) : !upper;
+                x[l] = ro::rope_elem(x[l], neg ? -y[l] : y[l], co[l], si[l], ro::ld_param(rp, g * HD + d0 + l, !cols));
+            }
+        }
+        const uint32_t slot = (uint32_t)pos & (c.page - 1), page = id;
+        if (tok + 1 < t1) {
+            xw = *reinterpret_cast<const int4*>(src + (tok + 1) * ld);
+            fetch(tok + 1);
         }
         if (on && isq) *reinterpret_cast<int4*>(a.qr + tok * a.qr_ld + g * HD + d0) = ro::pack16(x);
         if (ps * RW + RW <= a.heads) continue;                // no k row in this wavefront's
@@ -334,12 +397,9 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         int s = 0;
 #pragma unroll
         for (uint32_t l = 0; l < 8; l++) s += x[l];
-#pragma unroll
-        for (uint32_t o = 1; o < L; o <<= 1) s += __shfl_xor(s, (int)o, 64);
-        if (!on || isq || pos < 0 || pos >= (int64_t)bt.cap) continue;
-        const uint32_t id = (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)], slot = (uint32_t)pos & (c.page - 1);
-        if (id >= c.pages) continue;
-        uint8_t* blk = c.data + ((uint64_t)id * c.kv + g) * c.block;
+        s = (int)row_all<L>((uint32_t)s, [](uint32_t p, uint32_t q) { return p + q; });
+        if (!on || isq || page >= c.pages) continue;
+        uint8_t* blk = c.data + ((uint64_t)page * c.kv + g) * c.block;
         if constexpr (I8) {
             uint32_t h[2];
 #pragma unroll
@@ -425,29 +485,36 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Cache c, Batch bt, int1
 }
 
 // ---------------------------------------------------------------- attention
-// The exponential of d = max - s: y = (d Cm) >> Cs, e = TAB[y & 4095] >> (y >> 12).  The kernels take
-// 4 y (a byte offset into TAB) = (min(d, dlim) cm) >> cs from two 24-bit products; at dlim, the least d with
-// y >= 17 * 4096, e is 0, and y there stays below 2^17 (a shift below 32): the host replaces register pairs
-// whose single step passes 15 octaves by one of the same exponentials.
+// The exponential of d = max - s: y = (d Cm) >> Cs, e = TAB[y & 4095] >> (y >> 12).  The kernels take 4 y, a byte
+// offset into TAB, as the high word of (min(d, dlim) << sh) mul: one product.  At dlim, the least d with y >= 17 * 4096,
+// e is 0; y there stays below 2^17, a shift below 32 (the host replaces register pairs whose single step passes 15
+// octaves by one of the same exponentials).  Cm counts from its top bit (its pair is as good with both moved), so
+// mul = Cm 2^8 has 32 bits and sh = 26 - Cs with d below 2^(Cs - 5) or 2^16; Cs above 34 would need sh < -8: all 65535
+// steps of a score within 1/128 octave, which the host refuses.
 struct Smx {
-    uint32_t cm, cs, dlim;                     // dlim at most 65535: no d passes it
+    uint32_t mul, sh, dlim;                    // dlim at most 65535: no d passes it
 };
 
-Smx smx_of(uint32_t cm24, uint32_t cs) {
-    Smx r{cm24, cs, smx_dlim(cm24, cs)};
-    const uint32_t step = cs < 32 ? cm24 >> cs : 0u;
+bool smx_of(uint32_t cm24, uint32_t cs, Smx* r) {
+    r->mul = r->sh = 0;
+    r->dlim = 65535;
+    if (cm24 == 0) return true;                // e = TAB[0] for every d
+    const uint32_t dlim = smx_dlim(cm24, cs), step = cs < 32 ? cm24 >> cs : 0u;
+    r->dlim = dlim < 65535u ? dlim : 65535u;
     if (step >= 61440u) {                      // d = 1 has y = step, every d >= 2 gives 0
-        r.cs = 0;
-        r.dlim = step > 65536u ? 1u : 2u;      // above 2^16: e(1) = 0
-        r.cm = step > 65536u ? kSmxYZero : (step < 65535u ? step : 65535u);   // e(1) is 1 at 65535 as at 65536
+        cs = 0;
+        r->dlim = step > 65536u ? 1u : 2u;     // above 2^16: e(1) = 0
+        cm24 = step > 65536u ? kSmxYZero : (step < 65535u ? step : 65535u);   // e(1) is 1 at 65535 as at 65536
     }
-    r.dlim = r.dlim < 65535u ? r.dlim : 65535u;
-    if (r.cs >= 2) r.cs -= 2;
-    else {
-        r.cm <<= 2 - r.cs;                     // below 2^20: step < 61440 * 2^cs, or the pairs above
-        r.cs = 0;
-    }
-    return r;
+    const uint32_t up = (uint32_t)__builtin_clz(cm24) - 8;
+    cm24 <<= up;
+    cs += up;
+    // 4 y = (d cm24) >> (cs - 2) = (d 2^sh mul) >> 32, sh + log2(mul / cm24) = 34 - cs
+    if (cs > 34) return false;
+    const uint32_t total = 34 - cs, low = total < 8 ? total : 8u;
+    r->mul = cm24 << low;
+    r->sh = total - low;
+    return true;
 }
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -464,8 +531,7 @@ struct Exp2 {
 __device__ __forceinline__ Exp2 exps(int s0, int s1, uint32_t m2, uint32_t dl2, const Smx& x, const int32_t* tab) {
     const u16x2 s = __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pk_i16(s0, s1));
     const u16x2 d = __builtin_elementwise_min(__builtin_bit_cast(u16x2, m2) - s, __builtin_bit_cast(u16x2, dl2));
-    const uint32_t y0 = (uint32_t)(((uint64_t)d[0] * (x.cm & 0xFFFFFFu)) >> x.cs);
-    const uint32_t y1 = (uint32_t)(((uint64_t)d[1] * (x.cm & 0xFFFFFFu)) >> x.cs);
+    const uint32_t y0 = __umulhi((uint32_t)d[0] << x.sh, x.mul), y1 = __umulhi((uint32_t)d[1] << x.sh, x.mul);
     const uint8_t* tb = reinterpret_cast<const uint8_t*>(tab);
     return Exp2{*reinterpret_cast<const uint32_t*>(tb + (y0 & 0x3FFCu)), *reinterpret_cast<const uint32_t*>(tb + (y1 & 0x3FFCu)),
                 y0 >> 14, y1 >> 14};
@@ -1309,7 +1375,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
             typename RW::Frag f;
             v4i h[2], md[2], l[2];
             uint32_t es[2];
-            Exp2 e[2];
+            Exp2 x[2][2];
             rw.load(sm, 0, f);
 #pragma unroll
             for (uint32_t j = 0; j < NB + 2; j++) {
@@ -1318,8 +1384,19 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
                     es[j & 1] = f.es;
                     if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
                 }
+                if (j >= 1 && j <= NB) {
+                    const uint32_t y = j - 1, qb = y % QB;
+                    int z[4];
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++)
+                        z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
+                    x[y & 1][0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
+                    x[y & 1][1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 if (j >= 2) {
                     const uint32_t y = j - 2, kb = y / QB, qb = y % QB;
+                    const Exp2 *e = x[y & 1];
                     uint32_t v[4] = {e[0].e0(), e[0].e1(), e[1].e0(), e[1].e1()};
                     if constexpr (masked) {
 #pragma unroll
@@ -1333,15 +1410,6 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
                     uint32_t ve = 0;
                     if constexpr (I8) ve = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
                     weight_bytes<I8>(w01, w23, ve, p[qb], kb);
-                }
-                if (j >= 1 && j <= NB) {
-                    const uint32_t y = j - 1, qb = y % QB;
-                    int z[4];
-#pragma unroll
-                    for (uint32_t r = 0; r < 4; r++)
-                        z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
-                    e[0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
-                    e[1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -1560,6 +1628,9 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     const uint32_t fp = (smx_cfg >> 8) & 31u;
     if (fp < 1 || fp > 15) return fail(CM_EINVAL, "paged attention: softmax output bits %u (1 .. 15)", fp);
     if (window > 0x3FFFFFFFu) return fail(CM_EINVAL, "paged attention: a window of %u keys", window);
+    Smx smx;
+    if (!smx_of(smx_cm & 0xFFFFFFu, smx_cfg & 63u, &smx))
+        return fail(CM_EINVAL, "paged attention: softmax scale %u 2^-%u (65535 steps within 1/128 octave)", smx_cm & 0xFFFFFFu, smx_cfg & 63u);
     if (b.batch == 0 || b.tokens == 0) return CM_OK;
     if (q == nullptr || o == nullptr) return fail(CM_EINVAL, "paged attention: a null q or o");
     if (!aligned16(q) || !aligned16(o) || ((q_ld | o_ld) & 7))
@@ -1569,8 +1640,8 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
         return fail(CM_EINVAL, "paged attention: rows of %llu columns overlap at their strides", (unsigned long long)qw);
     DeviceState* st;
     if ((rc = state(&st))) return rc;
-    const uint32_t cm24 = smx_cm & 0xFFFFFFu, cs = smx_cfg & 63u, G = heads / c.kv;
-    const Attn a{q, o, q_ld, o_ld, G, window, fp, smx_of(cm24, cs)};
+    const uint32_t G = heads / c.kv;
+    const Attn a{q, o, q_ld, o_ld, G, window, fp, smx};
     // Few rows a sequence: tiles of 15 rows, in one launch for short caches, with kept scores for long ones (where those
     // fit kMaxScores); otherwise tiles of 64 or 128 rows that compute the scores twice
     const uint64_t rows = (uint64_t)b.tokens * heads;

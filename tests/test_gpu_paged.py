@@ -140,7 +140,9 @@ def test_attention_scales_and_large_values(paged, fs, fp, int8):
     check_attention(paged, c, *regs(64, fs, fp))
 
 
-@pytest.mark.parametrize("cm,cs", [(0, 20), (1, 0), ((1 << 24) - 1, 0), ((1 << 24) - 1, 63), (12102203, 31), (8388608, 40)])
+@pytest.mark.parametrize("cm,cs", [(0, 20), (0, 63), (1, 0), (7, 0), ((1 << 24) - 1, 0), ((1 << 24) - 1, 7),
+                                   (12345678, 8), ((1 << 24) - 1, 10), (65535, 0), (65536, 0), (69632, 0), (70000, 0), (12102203, 31),
+                                   (8388608, 34), (16777215, 34), (5, 13)])
 def test_attention_softmax_registers(paged, cm, cs):
     c = Case(np.random.default_rng(cs), [70], [7], amp=3000)
     check_attention(paged, c, cm, cs | (14 << 8))

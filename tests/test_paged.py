@@ -74,7 +74,7 @@ def test_bad_prep(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(q=0), dict(o=0), dict(q=OK + 2), dict(o_ld=380), dict(q_ld=320), dict(heads=0), dict(heads=5),
-                                dict(cfg=20), dict(cfg=20 | 16 << 8), dict(window=1 << 31)], ids=str)
+                                dict(cfg=20), dict(cfg=20 | 16 << 8), dict(cfg=35 | 14 << 8), dict(cm=1, cfg=12 | 14 << 8), dict(window=1 << 31)], ids=str)
 def test_bad_attention(lib, kw):
     a = {**dict(q=OK, o=OK, q_ld=384, o_ld=384, heads=6, window=0, cm=1 << 23, cfg=20 | 14 << 8), **kw}
     c, b = cache(), batch()
