@@ -593,6 +593,8 @@ __device__ __forceinline__ void store_out(int16_t* p, const Divide& q, const int
 // 64-key steps that any row of the tile sees go to workgroups in parts of `per` steps (the same for every tile: a short
 // sequence has fewer parts, not smaller ones).
 
+constexpr uint32_t kTileCost = 4;                 // what a tile of many rows costs beside its steps, in steps
+
 template <uint32_t R>
 struct Tile {
     uint32_t b, q0, n, row0, rows;         // sequence, its first token, tokens; the tile's first row, the sequence's rows
@@ -635,6 +637,22 @@ struct Tile {
         all_hi = __builtin_amdgcn_readfirstlane(seen(bt, tf));
         nt = hi > lo ? (hi - lo + 63) / 64 : 0u;
     }
+    // A lane's own tile: its steps, one at least (a tile without keys has zeros to write), 0 past the sequence's rows
+    static __device__ __forceinline__ uint32_t lane_steps(const Batch& bt, const Attn& a, uint32_t slot) {
+        uint32_t b = 0, e = bt.batch;
+        while (e - b > 1) {
+            const uint32_t m = (b + e) / 2;
+            const bool le = (uint32_t)((uint64_t)bt.start(m) * a.G / R) + m <= slot;
+            b = le ? m : b;
+            e = le ? e : m;
+        }
+        const uint32_t s0 = bt.start(b), n = (uint32_t)max((int)bt.start(b + 1) - (int)s0, 0);
+        const uint32_t row0 = (slot - ((uint32_t)((uint64_t)s0 * a.G / R) + b)) * R;
+        if (row0 >= n * a.G) return 0;
+        const int base = bt.len(b) - (int)n, tf = (int)(row0 / a.G), tl = (int)min((row0 + R - 1) / a.G, n - 1);
+        const int lo = a.window ? max(base + tf + 1 - (int)a.window, 0) & ~63 : 0, hi = min(max(base + tl + 1, 0), (int)bt.cap);
+        return kTileCost + (hi > lo ? (uint32_t)(hi - lo + 63) / 64 : 1u);
+    }
     __device__ __forceinline__ uint32_t seen(const Batch& bt, uint32_t tk) const {   // keys end
         return (uint32_t)min(max(base + (int)tk + 1, 0), (int)bt.cap);
     }
@@ -644,17 +662,17 @@ struct Tile {
     __device__ __forceinline__ uint32_t parts(uint32_t per) const { return max((nt + per - 1) / per, 1u); }
 };
 
-// The call's workspace: per row (head, token, head of the group: (head T + token) G + i) the maxima of its parts,
-// its scores (few rows), its partial sums of w V and of w.
+// Few rows, the call's workspace: per row (head, token, head of the group: (head T + token) G + i) the maxima of its
+// parts, its scores, its partial sums of w V and of w.
 struct Work {
     int32_t* mx;                           // [rows][splits] raw q.K^T sums, kNone: no key
     int16_t* sc;                           // [rows][cap]
-    int64_t* part;                         // few rows: [rows][splits][HD + 2]; many: [tile][splits][R HD + R], each
-                                           // tile in its lanes' order (1 KiB a store)
+    int64_t* part;                         // [rows][splits][HD + 2]
     uint32_t splits, per;                  // most parts of a tile, steps of a part
     uint32_t splits_s, per_s;              // the same of the maxima's parts
 };
 constexpr int kNone = (int)0x80000000;
+constexpr uint32_t kMaxPart = 32768;           // keys of a part of a tile: the int32 limb sums
 
 // V's sums and the bytes' offsets put back: the exact sum of w V (int16: hh, mid, ll of w's and V's bytes; int8: the
 // three bytes of w 2^e; every byte was taken less 128)
@@ -1277,20 +1295,106 @@ struct Rows {
     }
 };
 
+// ---- the work of many rows.  The 64-key steps of all tiles, one KV head after the other, are one list that is divided
+// evenly over the workgroups (shares): a causal prompt's tiles differ by the length of the prompt, and a share per tile
+// leaves the chip half empty behind the long ones.  A share covers the end of a tile, whole tiles, and the beginning of
+// one; sums of a tile that crosses shares are joined by a last kernel.
+struct Queue {
+    uint32_t* cum;                         // [slots + 1] steps before each tile of a KV head
+    int32_t* mx;                           // [rows] raw maxima, row (head T + token) G + i
+    int64_t* part;                         // [workgroups][2: a tile's later part, its first][R HD + R], in the lanes' order
+    uint32_t slots;
+};
+constexpr uint32_t kMaxMin = 4, kRowsMin = 4;   // steps of a share, at least
+
+struct Shares {
+    uint64_t all;                          // steps of every KV head
+    uint32_t head;                         // steps of one
+    uint32_t n;                            // shares
+    __device__ __forceinline__ Shares(const Queue& q, uint32_t kv, uint32_t least) {
+        head = __builtin_amdgcn_readfirstlane(q.cum[q.slots]);
+        all = (uint64_t)head * kv;
+        n = (uint32_t)min((uint64_t)gridDim.x, max(all / least, (uint64_t)1));
+        if (n > 8) n &= ~7u;
+        if (all == 0) n = 0;
+    }
+    __device__ __forceinline__ uint64_t first(uint32_t i) const { return (uint64_t)i * all / n; }
+    __device__ __forceinline__ uint32_t owner(uint64_t step) const { return (uint32_t)(((step + 1) * n - 1) / all); }
+    // workgroups are dealt round-robin to the 8 XCDs: each takes a contiguous run of the list (its keys in its L2)
+    __device__ __forceinline__ uint32_t order(uint32_t i) const { return n & 7 ? i : (i & 7) * (n >> 3) + (i >> 3); }
+};
+
+// The part of a tile from position `at` of the list to `stop` at most: a tile has kTileCost positions, then its steps
+struct Piece {
+    uint32_t head, slot, beg, end, steps;  // steps [beg, end) of the tile's
+    uint64_t next;                         // the list's position behind the piece
+    uint64_t tile;                         // the position of the tile's first step
+    bool whole;
+    __device__ __forceinline__ Piece(const Queue& q, const Shares& sh, uint64_t at, uint64_t stop) {
+        head = (uint32_t)(at / sh.head);
+        const uint32_t y = (uint32_t)(at - (uint64_t)head * sh.head);
+        slot = find_le(q.slots, y, [&](uint32_t i) { return q.cum[i]; });
+        const uint32_t c0 = __builtin_amdgcn_readfirstlane(q.cum[slot]), c1 = __builtin_amdgcn_readfirstlane(q.cum[slot + 1]);
+        steps = c1 - c0 - kTileCost;
+        tile = (uint64_t)head * sh.head + c0 + kTileCost;
+        next = min(stop, tile + steps);
+        beg = (uint32_t)(max(at, tile) - tile);
+        end = (uint32_t)(max(next, tile) - tile);
+        whole = beg == 0 && end == steps;
+    }
+};
+
+// cum by the first workgroup; no maximum yet, by the others
+template <uint32_t R>
+__global__ __launch_bounds__(1024) void paged_plan_kernel(Batch bt, Attn a, Queue qu, uint64_t rows) {
+    const uint32_t t = threadIdx.x, lane = t & 63, w = t >> 6;
+    if (blockIdx.x > 0) {
+        for (uint64_t i = (uint64_t)(blockIdx.x - 1) * 1024 + t; i < rows; i += (uint64_t)(gridDim.x - 1) * 1024) qu.mx[i] = kNone;
+        return;
+    }
+    __shared__ uint32_t wave[16];
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < qu.slots; s0 += 1024) {
+        const uint32_t n = s0 + t < qu.slots ? Tile<R>::lane_steps(bt, a, s0 + t) : 0u;
+        uint32_t sum = n;
+#pragma unroll
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint32_t x = (uint32_t)__shfl_up((int)sum, o, 64);
+            sum += lane >= o ? x : 0u;
+        }
+        if (lane == 63) wave[w] = sum;
+        __syncthreads();
+        uint32_t off = before, all = 0;
+        for (uint32_t i = 0; i < 16; i++) {
+            off += i < w ? wave[i] : 0u;
+            all += wave[i];
+        }
+        if (s0 + t < qu.slots) qu.cum[s0 + t] = off + sum - n;
+        before += all;
+        __syncthreads();
+    }
+    if (t == 0) qu.cum[qu.slots] = before;
+}
+
 template <uint32_t HD, bool I8, uint32_t QB>
-__global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, Attn a, Work wk) {
+__global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, Attn a, Queue qu) {
     typedef Rows<HD, I8, QB, false> RW;
     __shared__ __attribute__((aligned(1024))) uint8_t sm0[RW::S::BYTES];
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[RW::S::BYTES];
-    const uint32_t head = blockIdx.y, z = blockIdx.z;
-    const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);             // the long tiles first
-    const uint32_t per = wk.per_s;
-    if (!tl.on || z >= tl.parts(per)) return;
+    const Shares sh(qu, c.kv, kMaxMin);
+    if (blockIdx.x >= sh.n) return;
+    const uint32_t id = sh.order(blockIdx.x);
+    for (uint64_t at = sh.first(id), stop = sh.first(id + 1); at < stop;) {
+    const Piece pc(qu, sh, at, stop);
+    at = pc.next;
+    if (pc.beg == pc.end) continue;            // a tile's first positions alone
+    const uint32_t head = pc.head;
+    const Tile<RW::R> tl(bt, a, pc.slot);
     const RW rw(c, bt, a, tl, head);
     int mx[QB];
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) mx[qb] = kNone;
-    rw.run(sm0, sm1, z * per, min((z + 1) * per, tl.nt), [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
+    rw.run(sm0, sm1, pc.beg, pc.end, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
         const uint32_t kg = tl.lo + 64 * i + 16 * rw.g;
         constexpr uint32_t NB = 4 * QB;
         auto maxima = [&](auto masked) {
@@ -1329,12 +1433,13 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
         m = max(m, __shfl_xor(m, 16, 64));
         m = max(m, __shfl_xor(m, 32, 64));
         const uint32_t row = rw.row_of(qb);
-        if (rw.g == 0 && row < tl.rows) wk.mx[(((uint64_t)head * bt.tokens + tl.q0) * a.G + row) * wk.splits_s + z] = m;
+        if (rw.g == 0 && row < tl.rows) atomicMax(qu.mx + ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, m);
+    }
     }
 }
 
 template <uint32_t HD, bool I8, uint32_t QB>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, Attn a, Queue qu, const int32_t* __restrict__ tab) {
     constexpr uint32_t DB = HD / 16, NP = I8 ? 1 : 2, MW = DB / 4;
     typedef Rows<HD, I8, QB, true> RW;
     typedef typename RW::S S;
@@ -1342,23 +1447,37 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[S::BYTES];
     __shared__ __attribute__((aligned(16))) int32_t stab[4096];
     __shared__ int32_t vsum[NP][HD];
-    const uint32_t head = blockIdx.y, z = blockIdx.z;
-    const Tile<RW::R> tl(bt, a, gridDim.x - 1 - blockIdx.x);
-    const uint32_t per = wk.per, parts = tl.parts(per);
-    if (!tl.on || z >= parts) return;
+    const Shares sh(qu, c.kv, kRowsMin);
+    if (blockIdx.x >= sh.n) return;
+    const uint32_t id = sh.order(blockIdx.x);
     stage_tab(stab, tab);
+    for (uint64_t at = sh.first(id), stop = sh.first(id + 1); at < stop;) {
+    const Piece pc(qu, sh, at, stop);
+    at = pc.next;
+    if (pc.beg == pc.end) continue;            // a tile's first positions alone
+    const uint32_t head = pc.head;
+    const Tile<RW::R> tl(bt, a, pc.slot);
     const RW rw(c, bt, a, tl, head);
-    int64_t* part = wk.part + (((uint64_t)(gridDim.x - 1 - blockIdx.x) * c.kv + head) * wk.splits + z) * (RW::R * HD + RW::R);
-    const uint32_t g = rw.g, c16 = rw.c16, w = rw.w, beg = z * per, end = min((z + 1) * per, tl.nt);
+    int64_t* part = qu.part + (uint64_t)(2 * id + (pc.beg == 0 ? 1 : 0)) * (RW::R * HD + RW::R);
+    const uint32_t g = rw.g, c16 = rw.c16, w = rw.w;
     const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
     uint32_t m2[QB];
     const uint32_t dl2 = twice(a.smx.dlim);
+    int64_t total[QB];
+#pragma unroll
+    for (uint32_t qb = 0; qb < QB; qb++) {
+        const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
+        m2[qb] = twice((uint32_t)sat16i(qu.mx[((uint64_t)head * bt.tokens + tl.q0) * a.G + row] >> 8));
+        total[qb] = 0;
+    }
+    // at most kMaxPart keys in the int32 limb sums (a product is below 2^14, two a key in the middle ones): a longer
+    // piece adds to its partial sums
+    for (uint32_t beg = pc.beg; beg < pc.end;) {
+    const uint32_t end = min(pc.end, beg + kMaxPart / 64);
     v4i acc[3][DB][QB], vs[NP][MW];
     uint32_t wsum[QB];                         // the lane's keys' weights: below 2^16 * 16 * kMaxPart / 64
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
-        const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
-        m2[qb] = twice((uint32_t)row_max(wk, ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, tl.parts(wk.per_s), g));
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
         wsum[qb] = 0;
@@ -1451,17 +1570,18 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
 #pragma unroll
                 for (uint32_t r = 0; r < 4; r++) vsum[pl][16 * (w + 4 * m) + 4 * g + r] = vs[pl][m][r];
     }
-    __builtin_amdgcn_s_waitcnt(0x0070);                // the TAB's copies too, where there were no steps
     __syncthreads();
+    const bool last = end == pc.end;
 #pragma unroll
     for (uint32_t qb = 0; qb < QB; qb++) {
         int64_t sum = wsum[qb];
         sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
         sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
+        total[qb] += sum;
         const uint32_t row = rw.row_of(qb);
         const bool on = row < tl.rows;
         int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
-        const Divide quot(sum, a.fp);
+        const Divide quot(total[qb], a.fp);
 #pragma unroll
         for (uint32_t m = 0; m < DB; m++) {
             int64_t x[4];
@@ -1470,37 +1590,50 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
                 const uint32_t d = 16 * m + 4 * g + r;
                 x[r] = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
             }
-            if (parts > 1) {
-                longlong2* pp = reinterpret_cast<longlong2*>(part) + (((w * QB + qb) * DB + m) * 2) * 64 + rw.lane;
+            longlong2* pp = reinterpret_cast<longlong2*>(part) + (((w * QB + qb) * DB + m) * 2) * 64 + rw.lane;
+            if (beg != pc.beg) {
+                const longlong2 u = pp[0], v = pp[64];
+                x[0] += u.x;
+                x[1] += u.y;
+                x[2] += v.x;
+                x[3] += v.y;
+            }
+            if (!last || !pc.whole) {
                 pp[0] = make_longlong2(x[0], x[1]);
                 pp[64] = make_longlong2(x[2], x[3]);
             } else if (on) {
                 store_out(op + 16 * m + 4 * g, quot, x);
             }
         }
-        if (parts > 1 && g == 0) part[RW::R * HD + 16 * (w * QB + qb) + c16] = sum;
+        if (last && !pc.whole && g == 0) part[RW::R * HD + 16 * (w * QB + qb) + c16] = total[qb];
+    }
+    beg = end;
+    }
     }
 }
 
-// The parts' sums of a tile of many rows added and divided, in the lanes' order of paged_rows_kernel; a workgroup per
-// 16 columns, a wavefront's loads of four parts in flight at once.
+// The pieces' sums of a tile added and divided, in the lanes' order of paged_rows_kernel: a workgroup per boundary
+// between shares that is the first inside its tile, and 16 columns; loads of four pieces in flight.
 template <uint32_t HD, uint32_t QB>
-__global__ __launch_bounds__(256) void paged_rows_join_kernel(Cache c, Batch bt, Attn a, Work wk) {
+__global__ __launch_bounds__(256) void paged_rows_join_kernel(Cache c, Batch bt, Attn a, Queue qu) {
     constexpr uint32_t DB = HD / 16, R = 64 * QB;
-    const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, head = blockIdx.y, slot = blockIdx.x;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = blockIdx.z;
-    const Tile<R> tl(bt, a, slot);
-    const uint32_t parts = tl.parts(wk.per);
-    if (!tl.on || parts == 1) return;
-    const int64_t* part = wk.part + ((uint64_t)slot * c.kv + head) * wk.splits * (R * HD + R);
-#pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) {
-        const uint32_t wq = w * QB + qb, row = tl.row0 + 16 * wq + c16;
-        if (tl.row0 + 16 * wq >= tl.rows) break;
+    const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, m = blockIdx.y;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x + 1;
+    const Shares sh(qu, c.kv, kRowsMin);
+    if (id >= sh.n) return;
+    const uint64_t at = sh.first(id);
+    const Piece pc(qu, sh, at, at + 1);
+    if (pc.beg == 0) return;                   // before or at the tile's first step
+    if (sh.owner(pc.tile) + 1 != id) return;   // a later boundary inside this tile
+    const uint32_t pieces = sh.owner(pc.tile + pc.steps - 1) - (id - 1) + 1;
+    const Tile<R> tl(bt, a, pc.slot);
+    const uint32_t wq = w * QB + blockIdx.z, row = tl.row0 + 16 * wq + c16;
+    {
+        if (tl.row0 + 16 * wq >= tl.rows) return;
         int64_t x[4] = {0, 0, 0, 0}, S = 0;
 #pragma unroll 4
-        for (uint32_t i = 0; i < parts; i++) {
-            const int64_t* p = part + (uint64_t)i * (R * HD + R);
+        for (uint32_t i = 0; i < pieces; i++) {
+            const int64_t* p = qu.part + (uint64_t)(2 * (id - 1 + i) + (i == 0 ? 1 : 0)) * (R * HD + R);
             const longlong2* pp = reinterpret_cast<const longlong2*>(p) + (wq * DB + m) * 128 + lane;
             const longlong2 u = pp[0], v = pp[64];
             S += p[R * HD + 16 * wq + c16];
@@ -1509,15 +1642,14 @@ __global__ __launch_bounds__(256) void paged_rows_join_kernel(Cache c, Batch bt,
             x[2] += v.x;
             x[3] += v.y;
         }
-        if (row >= tl.rows) continue;
+        if (row >= tl.rows) return;
         const Divide quot(S, a.fp);
-        store_out(a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * m + 4 * g, quot, x);
+        store_out(a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(pc.head * a.G + row % a.G) * HD + 16 * m + 4 * g, quot, x);
     }
 }
 
 // ---------------------------------------------------------------- the host's checks
 constexpr uint32_t kMaxKeys = 1u << 20;
-constexpr uint32_t kMaxPart = 32768;           // keys of a part of a tile
 constexpr uint64_t kMaxScores = 1ull << 28;    // bytes of scores that a call keeps
 
 int view(const cm_paged_cache* cache, const cm_paged_batch* batch, Cache* c, Batch* b) {
@@ -1661,48 +1793,54 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
 #undef CM_SHORT
         return CM_OK;
     }
-    const uint32_t steps = (b.cap + 63) / 64, wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20);
-    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M"); const char* es = getenv("CMP_S");
-    const uint32_t target = ev ? atoi(ev) : few ? 1024 : 1536, mn = em ? atoi(em) : 4;
-    const uint32_t want = std::max(target / wgs, 1u);
-    const uint32_t per = std::min(std::max((steps + want - 1) / want, mn), kMaxPart / 64), splits = (steps + per - 1) / per;
-    const uint32_t per_s = few ? std::min(per, es ? (uint32_t)atoi(es) : 8u) : per, splits_s = (steps + per_s - 1) / per_s;
-    if (splits > 65535u || splits_s > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits);
-    const size_t mx_bytes = round_up(rows * splits_s * 4, 256), sc_bytes = few ? round_up(rows * b.cap * 2, 256) : 0;
-    const size_t part_bytes = splits > 1 ? (few ? rows * splits * (cache->head_dim + 2) : slots * c.kv * R * splits * (cache->head_dim + 1)) * 8 : 0;
-    void* ws;
-    if ((rc = workspace(st, mx_bytes + sc_bytes + part_bytes, &ws, s))) return rc;
-    Work wk;
-    wk.mx = static_cast<int32_t*>(ws);
-    wk.sc = reinterpret_cast<int16_t*>(static_cast<uint8_t*>(ws) + mx_bytes);
-    wk.part = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(ws) + mx_bytes + sc_bytes);
-    wk.splits = splits;
-    wk.per = per;
-    wk.splits_s = splits_s;
-    wk.per_s = per_s;
-    const dim3 grid((unsigned)slots, c.kv, splits), sgrid((unsigned)slots, c.kv, splits_s), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
-#define CM_FEW(HD, I8)                                                                                                  \
-    CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), sgrid, dim3(256), 0, s, c, b, a, wk);                \
-    CM_LAUNCH("paged_few_kernel", (paged_few_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);         \
+    const uint32_t steps = (b.cap + 63) / 64;
+    if (few) {
+        // parts of equal steps: about four workgroups a compute unit, two steps a wavefront for the scores; a part of at
+        // most kMaxPart keys (the int32 limb sums)
+        const uint32_t wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20), want = std::max(4u * (uint32_t)st->cus / wgs, 1u);
+        const uint32_t per = std::min(std::max((steps + want - 1) / want, 4u), kMaxPart / 64), splits = (steps + per - 1) / per;
+        const uint32_t per_s = std::min(per, 8u), splits_s = (steps + per_s - 1) / per_s;
+        if (splits_s > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits_s);
+        const size_t mx_bytes = round_up(rows * splits_s * 4, 256), sc_bytes = round_up(rows * b.cap * 2, 256);
+        const size_t part_bytes = splits > 1 ? rows * splits * (cache->head_dim + 2) * 8 : 0;
+        void* ws;
+        if ((rc = workspace(st, mx_bytes + sc_bytes + part_bytes, &ws, s))) return rc;
+        uint8_t* p = static_cast<uint8_t*>(ws);
+        const Work wk{reinterpret_cast<int32_t*>(p), reinterpret_cast<int16_t*>(p + mx_bytes),
+                      reinterpret_cast<int64_t*>(p + mx_bytes + sc_bytes), splits, per, splits_s, per_s};
+        const dim3 grid((unsigned)slots, c.kv, splits), sgrid((unsigned)slots, c.kv, splits_s), jgrid((unsigned)(((uint64_t)b.tokens * G + 3) / 4), c.kv);
+#define CM_FEW(HD, I8)                                                                                              \
+    CM_LAUNCH("paged_scores_kernel", (paged_scores_kernel<HD, I8>), sgrid, dim3(256), 0, s, c, b, a, wk);           \
+    CM_LAUNCH("paged_few_kernel", (paged_few_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);     \
     if (splits > 1) { CM_LAUNCH("paged_join_kernel", paged_join_kernel<HD>, jgrid, dim3(256), 0, s, b, a, wk); }
-#define CM_ROWS(HD, I8, QB)                                                                                             \
-    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), sgrid, dim3(256), 0, s, c, b, a, wk);                  \
-    CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), grid, dim3(256), 0, s, c, b, a, wk, st->smx_tab);   \
-    if (splits > 1) { CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), dim3((unsigned)slots, c.kv, HD / 16), dim3(256), 0, s, c, b, a, wk); }
-    if (cache->head_dim == 64) {
-        if (cache->int8) {
-            if (few) { CM_FEW(64, true) } else { CM_ROWS(64, true, 2) }
+        if (cache->head_dim == 64) {
+            if (cache->int8) { CM_FEW(64, true) } else { CM_FEW(64, false) }
         } else {
-            if (few) { CM_FEW(64, false) } else { CM_ROWS(64, false, 2) }
+            if (cache->int8) { CM_FEW(128, true) } else { CM_FEW(128, false) }
         }
-    } else {
-        if (cache->int8) {
-            if (few) { CM_FEW(128, true) } else { CM_ROWS(128, true, 1) }
-        } else {
-            if (few) { CM_FEW(128, false) } else { CM_ROWS(128, false, 1) }
-        }
-    }
 #undef CM_FEW
+        return CM_OK;
+    }
+    if (slots * steps > 0xFFFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens over %u rows", b.tokens, b.cap);
+    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M");
+    const uint32_t wgs = (ev ? atoi(ev) : 2) * st->cus, mwgs = (em ? atoi(em) : 4) * st->cus;
+    const size_t cum_bytes = round_up((slots + 1) * 4, 256), mx_bytes = round_up(rows * 4, 256);
+    void* ws;
+    if ((rc = workspace(st, cum_bytes + mx_bytes + (size_t)wgs * 2 * R * (cache->head_dim + 1) * 8, &ws, s))) return rc;
+    uint8_t* p = static_cast<uint8_t*>(ws);
+    const Queue qu{reinterpret_cast<uint32_t*>(p), reinterpret_cast<int32_t*>(p + cum_bytes),
+                   reinterpret_cast<int64_t*>(p + cum_bytes + mx_bytes), (uint32_t)slots};
+    const uint32_t plan = 1 + (uint32_t)std::min<uint64_t>((rows + 4095) / 4096, 64);
+#define CM_ROWS(HD, I8, QB)                                                                                                     \
+    CM_LAUNCH("paged_plan_kernel", (paged_plan_kernel<64 * QB>), dim3(plan), dim3(1024), 0, s, b, a, qu, rows);                 \
+    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), dim3(mwgs), dim3(256), 0, s, c, b, a, qu);                    \
+    CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), dim3(wgs), dim3(256), 0, s, c, b, a, qu, st->smx_tab);      \
+    CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), dim3(wgs, HD / 16, QB), dim3(256), 0, s, c, b, a, qu);
+    if (cache->head_dim == 64) {
+        if (cache->int8) { CM_ROWS(64, true, 2) } else { CM_ROWS(64, false, 2) }
+    } else {
+        if (cache->int8) { CM_ROWS(128, true, 1) } else { CM_ROWS(128, false, 1) }
+    }
 #undef CM_ROWS
     return CM_OK;
 }
