@@ -597,6 +597,16 @@ constexpr uint32_t kTileCost = 4;                 // what a tile of many rows co
 
 template <uint32_t R>
 struct Tile {
+    struct Seqs {                          // lane i: sequence i's first token, the next one's, its length (batch <= 64)
+        uint32_t s0, s1, len;
+        Seqs() = default;
+        __device__ __forceinline__ Seqs(const Batch& bt) {
+            const uint32_t i = min(threadIdx.x & 63, bt.batch - 1);
+            s0 = bt.start(i);
+            s1 = bt.start(i + 1);
+            len = (uint32_t)bt.len(i);
+        }
+    };
     uint32_t b, q0, n, row0, rows;         // sequence, its first token, tokens; the tile's first row, the sequence's rows
     uint32_t lo, hi, nt;                   // keys [lo, hi) that a row sees, lo a multiple of 64; 64-key steps
     uint32_t all_lo, all_hi;               // keys that every row sees
@@ -604,17 +614,16 @@ struct Tile {
     const int32_t* tb;
     bool on;
 
-    __device__ __forceinline__ Tile(const Batch& bt, const Attn& a, uint32_t slot) {
+    __device__ __forceinline__ Tile(const Batch& bt, const Attn& a, uint32_t slot) : Tile(bt, a, slot, Seqs(bt)) {}
+    __device__ __forceinline__ Tile(const Batch& bt, const Attn& a, uint32_t slot, const Seqs& sq) {
         uint32_t q1, first;
         int len;
-        if (bt.batch <= 64) {                  // one round of loads: lane i holds sequence i
-            const uint32_t i = min(threadIdx.x & 63, bt.batch - 1);
-            const uint32_t s0 = bt.start(i), s1 = bt.start(i + 1), l = (uint32_t)bt.len(i);
-            const uint32_t f = (uint32_t)((uint64_t)s0 * a.G / R) + i;
+        if (bt.batch <= 64) {
+            const uint32_t f = (uint32_t)((uint64_t)sq.s0 * a.G / R) + min(threadIdx.x & 63, bt.batch - 1);
             b = max((uint32_t)__popcll(__ballot((threadIdx.x & 63) < bt.batch && f <= slot)), 1u) - 1;
-            q0 = (uint32_t)__builtin_amdgcn_readlane((int)s0, b);
-            q1 = (uint32_t)__builtin_amdgcn_readlane((int)s1, b);
-            len = __builtin_amdgcn_readlane((int)l, b);
+            q0 = (uint32_t)__builtin_amdgcn_readlane((int)sq.s0, b);
+            q1 = (uint32_t)__builtin_amdgcn_readlane((int)sq.s1, b);
+            len = __builtin_amdgcn_readlane((int)sq.len, b);
             first = (uint32_t)__builtin_amdgcn_readlane((int)f, b);
         } else {
             auto at = [&](uint32_t i) { return (uint32_t)((uint64_t)bt.start(i) * a.G / R) + i; };
@@ -638,18 +647,19 @@ struct Tile {
         nt = hi > lo ? (hi - lo + 63) / 64 : 0u;
     }
     // A lane's own tile: its steps, one at least (a tile without keys has zeros to write), 0 past the sequence's rows
-    static __device__ __forceinline__ uint32_t lane_steps(const Batch& bt, const Attn& a, uint32_t slot) {
+    static __device__ __forceinline__ uint32_t lane_steps(const Batch& bt, const Attn& a, uint32_t slot, const Seqs* seqs) {
+        auto start = [&](uint32_t i) { return seqs ? seqs[i].s0 : bt.start(i); };
         uint32_t b = 0, e = bt.batch;
         while (e - b > 1) {
             const uint32_t m = (b + e) / 2;
-            const bool le = (uint32_t)((uint64_t)bt.start(m) * a.G / R) + m <= slot;
+            const bool le = (uint32_t)((uint64_t)start(m) * a.G / R) + m <= slot;
             b = le ? m : b;
             e = le ? e : m;
         }
-        const uint32_t s0 = bt.start(b), n = (uint32_t)max((int)bt.start(b + 1) - (int)s0, 0);
+        const uint32_t s0 = start(b), s1 = seqs ? seqs[b].s1 : bt.start(b + 1), n = (uint32_t)max((int)s1 - (int)s0, 0);
         const uint32_t row0 = (slot - ((uint32_t)((uint64_t)s0 * a.G / R) + b)) * R;
         if (row0 >= n * a.G) return 0;
-        const int base = bt.len(b) - (int)n, tf = (int)(row0 / a.G), tl = (int)min((row0 + R - 1) / a.G, n - 1);
+        const int base = (seqs ? (int)seqs[b].len : bt.len(b)) - (int)n, tf = (int)(row0 / a.G), tl = (int)min((row0 + R - 1) / a.G, n - 1);
         const int lo = a.window ? max(base + tf + 1 - (int)a.window, 0) & ~63 : 0, hi = min(max(base + tl + 1, 0), (int)bt.cap);
         return kTileCost + (hi > lo ? (uint32_t)(hi - lo + 63) / 64 : 1u);
     }
@@ -1190,6 +1200,8 @@ struct Rows {
         c16 = lane & 15;
         g = lane >> 4;
         w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    }
+    __device__ __forceinline__ void queries(const Attn& a) {
 #pragma unroll
         for (uint32_t qb = 0; qb < QB; qb++) {
             const uint32_t row = row_of(qb), rr = min(row, tl.rows - 1), tok = rr / a.G;
@@ -1273,10 +1285,11 @@ struct Rows {
     }
     // body(stage, step, ids) for the steps [i, end), two stages deep; an odd count is made even by a step without pages
     // (a loop that may end between its halves has the accumulators moved from registers to registers)
+    // id0, id1: ids of the first two steps, loaded by the caller ahead of the queries
     template <class F>
-    __device__ __forceinline__ void run(uint8_t* sm0, uint8_t* sm1, uint32_t i, uint32_t end, F body) const {
+    __device__ __forceinline__ void run(uint8_t* sm0, uint8_t* sm1, uint32_t i, uint32_t end, uint32_t id0, uint32_t id1,
+                                        F body) const {
         if (i >= end) return;
-        uint32_t id0 = ids(i, end), id1 = ids(i + 1, end);
         stage(sm0, i, id0);
         for (; i < end; i += 2) {
             __builtin_amdgcn_s_waitcnt(0x0070);        // this wavefront's copies
@@ -1298,30 +1311,92 @@ struct Rows {
 // ---- the work of many rows.  The 64-key steps of all tiles, one KV head after the other, are one list that is divided
 // evenly over the workgroups (shares): a causal prompt's tiles differ by the length of the prompt, and a share per tile
 // leaves the chip half empty behind the long ones.  A share covers the end of a tile, whole tiles, and the beginning of
-// one; sums of a tile that crosses shares are joined by a last kernel.
+// one; sums of a tile that crosses shares are joined by a last kernel.  Up to kPlan tiles of up to 64 sequences each
+// workgroup sums the tiles' steps for itself (1 us of LDS work in place of a launch and its wait, 5.5 us); more have
+// them from a kernel of their own.
+constexpr uint32_t kPlan = 256;
 struct Queue {
-    uint32_t* cum;                         // [slots + 1] steps before each tile of a KV head
-    int32_t* mx;                           // [rows] raw maxima, row (head T + token) G + i
-    int64_t* part;                         // [workgroups][2: a tile's later part, its first][R HD + R], in the lanes' order
-    uint32_t slots;
+    uint32_t* cum;                         // [slots + 1] steps before each tile of a KV head; null: each workgroup's own
+    int32_t* mx;                           // [max_shares][2: a tile's later part, its first][R] raw maxima
+    int64_t* part;                         // [shares][2][R HD + R], in the lanes' order
+    uint32_t slots, max_shares, shares;    // shares at most, both multiples of 8
 };
 constexpr uint32_t kMaxMin = 4, kRowsMin = 4;   // steps of a share, at least
 
+template <uint32_t R>
+struct PlanLds {                           // one workgroup's
+    typename Tile<R>::Seqs seqs[64];
+    uint32_t cum[kPlan + 1], wave[4];
+};
+
+template <uint32_t R>
+__device__ __forceinline__ uint32_t wave_scan(uint32_t n) {
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t x = (uint32_t)__shfl_up((int)n, o, 64);
+        n += lane >= o ? x : 0u;
+    }
+    return n;
+}
+
+// cum of at most kPlan slots by 256 threads; the sequences for Tile (every wavefront writes the same, and reads its own)
+template <uint32_t R>
+__device__ __forceinline__ void plan(PlanLds<R>& sm, const Batch& bt, const Attn& a, const Queue& q) {
+    const uint32_t t = threadIdx.x, lane = t & 63, w = t >> 6;
+    sm.seqs[lane] = typename Tile<R>::Seqs(bt);
+    if (q.cum != nullptr) return;
+    const uint32_t n = t < q.slots ? Tile<R>::lane_steps(bt, a, t, sm.seqs) : 0u, sum = wave_scan<R>(n);
+    if (lane == 63) sm.wave[w] = sum;
+    __syncthreads();
+    uint32_t off = sum;
+    for (uint32_t i = 0; i < w; i++) off += sm.wave[i];
+    sm.cum[t + 1] = off;
+    if (t == 0) sm.cum[0] = 0;
+    __syncthreads();
+}
+
+// The shares of at most `most`
+template <uint32_t R>
 struct Shares {
-    uint64_t all;                          // steps of every KV head
-    uint32_t head;                         // steps of one
-    uint32_t n;                            // shares
-    __device__ __forceinline__ Shares(const Queue& q, uint32_t kv, uint32_t least) {
-        head = __builtin_amdgcn_readfirstlane(q.cum[q.slots]);
+    const uint32_t* cum;
+    const PlanLds<R>& sm;
+    uint64_t all;                          // positions of every KV head
+    uint32_t slots, head, n;               // tiles and positions of one, shares
+    __device__ __forceinline__ Shares(const Queue& q, const PlanLds<R>& sm_, uint32_t kv, uint32_t most, uint32_t least)
+        : cum(q.cum), sm(sm_), slots(q.slots) {
+        head = __builtin_amdgcn_readfirstlane(at(slots));
         all = (uint64_t)head * kv;
-        n = (uint32_t)min((uint64_t)gridDim.x, max(all / least, (uint64_t)1));
-        if (n > 8) n &= ~7u;
-        if (all == 0) n = 0;
+        n = all ? (uint32_t)min((uint64_t)most, max(all / least, (uint64_t)1)) : 0u;
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t slot) const { return cum ? cum[slot] : sm.cum[slot]; }
+    // the last slot with cum <= y, its cum and the next one's: a round of loads, one more from 64 and from 4032 slots on
+    __device__ __forceinline__ uint32_t find(uint32_t y, uint32_t& c0, uint32_t& c1) const {
+        const uint32_t lane = threadIdx.x & 63, stride = slots / 64 + 1;
+        uint32_t v = at(min(lane * stride, slots)), base = 0;
+        uint32_t k = max((uint32_t)__popcll(__ballot(lane * stride < slots && v <= y)), 1u) - 1;
+        if (stride > 1) {
+            base = k * stride;
+            uint32_t m = min(stride, slots - base);
+            if (stride > 63) {
+                base += find_le(m, y, [&](uint32_t i) { return cum[base + i]; });
+                m = 1;
+            }
+            v = at(min(base + lane, slots));
+            k = max((uint32_t)__popcll(__ballot(lane < m && v <= y)), 1u) - 1;
+        }
+        c0 = (uint32_t)__builtin_amdgcn_readlane((int)v, k);
+        c1 = (uint32_t)__builtin_amdgcn_readlane((int)v, k + 1);
+        return base + k;
     }
     __device__ __forceinline__ uint64_t first(uint32_t i) const { return (uint64_t)i * all / n; }
-    __device__ __forceinline__ uint32_t owner(uint64_t step) const { return (uint32_t)(((step + 1) * n - 1) / all); }
-    // workgroups are dealt round-robin to the 8 XCDs: each takes a contiguous run of the list (its keys in its L2)
-    __device__ __forceinline__ uint32_t order(uint32_t i) const { return n & 7 ? i : (i & 7) * (n >> 3) + (i >> 3); }
+    __device__ __forceinline__ uint32_t owner(uint64_t pos) const { return (uint32_t)(((pos + 1) * n - 1) / all); }
+    // workgroups are dealt round-robin to the 8 XCDs: each takes a contiguous run of the list (its keys in its L2);
+    // ~0: none (a grid of a multiple of 8 and of n or more)
+    __device__ __forceinline__ uint32_t order(uint32_t i) const {
+        const uint32_t lo = (uint32_t)((uint64_t)(i & 7) * n >> 3), hi = (uint32_t)((uint64_t)((i & 7) + 1) * n >> 3);
+        return lo + (i >> 3) < hi ? lo + (i >> 3) : ~0u;
+    }
 };
 
 // The part of a tile from position `at` of the list to `stop` at most: a tile has kTileCost positions, then its steps
@@ -1330,11 +1405,11 @@ struct Piece {
     uint64_t next;                         // the list's position behind the piece
     uint64_t tile;                         // the position of the tile's first step
     bool whole;
-    __device__ __forceinline__ Piece(const Queue& q, const Shares& sh, uint64_t at, uint64_t stop) {
+    template <uint32_t R>
+    __device__ __forceinline__ Piece(const Shares<R>& sh, uint64_t at, uint64_t stop) {
         head = (uint32_t)(at / sh.head);
-        const uint32_t y = (uint32_t)(at - (uint64_t)head * sh.head);
-        slot = find_le(q.slots, y, [&](uint32_t i) { return q.cum[i]; });
-        const uint32_t c0 = __builtin_amdgcn_readfirstlane(q.cum[slot]), c1 = __builtin_amdgcn_readfirstlane(q.cum[slot + 1]);
+        uint32_t c0, c1;
+        slot = sh.find((uint32_t)(at - (uint64_t)head * sh.head), c0, c1);
         steps = c1 - c0 - kTileCost;
         tile = (uint64_t)head * sh.head + c0 + kTileCost;
         next = min(stop, tile + steps);
@@ -1344,24 +1419,13 @@ struct Piece {
     }
 };
 
-// cum by the first workgroup; no maximum yet, by the others
 template <uint32_t R>
-__global__ __launch_bounds__(1024) void paged_plan_kernel(Batch bt, Attn a, Queue qu, uint64_t rows) {
+__global__ __launch_bounds__(1024) void paged_plan_kernel(Batch bt, Attn a, Queue qu) {
     const uint32_t t = threadIdx.x, lane = t & 63, w = t >> 6;
-    if (blockIdx.x > 0) {
-        for (uint64_t i = (uint64_t)(blockIdx.x - 1) * 1024 + t; i < rows; i += (uint64_t)(gridDim.x - 1) * 1024) qu.mx[i] = kNone;
-        return;
-    }
     __shared__ uint32_t wave[16];
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < qu.slots; s0 += 1024) {
-        const uint32_t n = s0 + t < qu.slots ? Tile<R>::lane_steps(bt, a, s0 + t) : 0u;
-        uint32_t sum = n;
-#pragma unroll
-        for (uint32_t o = 1; o < 64; o <<= 1) {
-            const uint32_t x = (uint32_t)__shfl_up((int)sum, o, 64);
-            sum += lane >= o ? x : 0u;
-        }
+        const uint32_t n = s0 + t < qu.slots ? Tile<R>::lane_steps(bt, a, s0 + t, nullptr) : 0u, sum = wave_scan<R>(n);
         if (lane == 63) wave[w] = sum;
         __syncthreads();
         uint32_t off = before, all = 0;
@@ -1381,60 +1445,64 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
     typedef Rows<HD, I8, QB, false> RW;
     __shared__ __attribute__((aligned(1024))) uint8_t sm0[RW::S::BYTES];
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[RW::S::BYTES];
-    const Shares sh(qu, c.kv, kMaxMin);
-    if (blockIdx.x >= sh.n) return;
+    __shared__ PlanLds<RW::R> spl;
+    plan(spl, bt, a, qu);
+    const Shares<RW::R> sh(qu, spl, c.kv, qu.max_shares, kMaxMin);
     const uint32_t id = sh.order(blockIdx.x);
+    if (id == ~0u) return;
     for (uint64_t at = sh.first(id), stop = sh.first(id + 1); at < stop;) {
-    const Piece pc(qu, sh, at, stop);
-    at = pc.next;
-    if (pc.beg == pc.end) continue;            // a tile's first positions alone
-    const uint32_t head = pc.head;
-    const Tile<RW::R> tl(bt, a, pc.slot);
-    const RW rw(c, bt, a, tl, head);
-    int mx[QB];
+        const Piece pc(sh, at, stop);
+        at = pc.next;
+        if (pc.beg == pc.end) continue;            // a tile's first positions alone
+        const uint32_t head = pc.head;
+        const Tile<RW::R> tl(bt, a, pc.slot, spl.seqs[threadIdx.x & 63]);
+        if (!tl.on) continue;
+        RW rw(c, bt, a, tl, head);
+        int mx[QB];
 #pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) mx[qb] = kNone;
-    rw.run(sm0, sm1, pc.beg, pc.end, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
-        const uint32_t kg = tl.lo + 64 * i + 16 * rw.g;
-        constexpr uint32_t NB = 4 * QB;
-        auto maxima = [&](auto masked) {
-            typename RW::Frag f;
-            v4i h[2], md[2], l[2];
-            uint32_t es[2];
-            rw.load(sm, 0, f);
+        for (uint32_t qb = 0; qb < QB; qb++) mx[qb] = kNone;
+        const uint32_t id0 = rw.ids(pc.beg, pc.end), id1 = rw.ids(pc.beg + 1, pc.end);
+        rw.queries(a);
+        rw.run(sm0, sm1, pc.beg, pc.end, id0, id1, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
+            const uint32_t kg = tl.lo + 64 * i + 16 * rw.g;
+            constexpr uint32_t NB = 4 * QB;
+            auto maxima = [&](auto masked) {
+                typename RW::Frag f;
+                v4i h[2], md[2], l[2];
+                uint32_t es[2];
+                rw.load(sm, 0, f);
 #pragma unroll
-            for (uint32_t j = 0; j < NB + 1; j++) {
-                if (j < NB) {
-                    rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
-                    es[j & 1] = f.es;
-                    if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
-                }
-                if (j >= 1) {
-                    const uint32_t y = j - 1, qb = y % QB;
-#pragma unroll
-                    for (uint32_t r = 0; r < 4; r++) {
-                        int z = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]);
-                        if constexpr (masked) {
-                            const uint32_t key = kg + 4 * (y / QB) + r;
-                            z = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? z : kNone;
-                        }
-                        mx[qb] = max(mx[qb], z);
+                for (uint32_t j = 0; j < NB + 1; j++) {
+                    if (j < NB) {
+                        rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
+                        es[j & 1] = f.es;
+                        if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
                     }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        if (rw.whole(i, ids)) maxima(std::false_type{});
-        else maxima(std::true_type{});
-    });
+                    if (j >= 1) {
+                        const uint32_t y = j - 1, qb = y % QB;
 #pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) {
-        int m = mx[qb];
-        m = max(m, __shfl_xor(m, 16, 64));
-        m = max(m, __shfl_xor(m, 32, 64));
-        const uint32_t row = rw.row_of(qb);
-        if (rw.g == 0 && row < tl.rows) atomicMax(qu.mx + ((uint64_t)head * bt.tokens + tl.q0) * a.G + row, m);
-    }
+                        for (uint32_t r = 0; r < 4; r++) {
+                            int z = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]);
+                            if constexpr (masked) {
+                                const uint32_t key = kg + 4 * (y / QB) + r;
+                                z = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? z : kNone;
+                            }
+                            mx[qb] = max(mx[qb], z);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            if (rw.whole(i, ids)) maxima(std::false_type{});
+            else maxima(std::true_type{});
+        });
+#pragma unroll
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            int m = mx[qb];
+            m = max(m, __shfl_xor(m, 16, 64));
+            m = max(m, __shfl_xor(m, 32, 64));
+            if (rw.g == 0) qu.mx[(2 * id + (pc.beg == 0 ? 1 : 0)) * RW::R + rw.row_of(qb) - tl.row0] = m;
+        }
     }
 }
 
@@ -1447,205 +1515,228 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[S::BYTES];
     __shared__ __attribute__((aligned(16))) int32_t stab[4096];
     __shared__ int32_t vsum[NP][HD];
-    const Shares sh(qu, c.kv, kRowsMin);
-    if (blockIdx.x >= sh.n) return;
+    __shared__ PlanLds<RW::R> spl;
+    plan(spl, bt, a, qu);
+    const Shares<RW::R> sh(qu, spl, c.kv, qu.shares, kRowsMin);
     const uint32_t id = sh.order(blockIdx.x);
+    if (id == ~0u) return;
     stage_tab(stab, tab);
     for (uint64_t at = sh.first(id), stop = sh.first(id + 1); at < stop;) {
-    const Piece pc(qu, sh, at, stop);
-    at = pc.next;
-    if (pc.beg == pc.end) continue;            // a tile's first positions alone
-    const uint32_t head = pc.head;
-    const Tile<RW::R> tl(bt, a, pc.slot);
-    const RW rw(c, bt, a, tl, head);
-    int64_t* part = qu.part + (uint64_t)(2 * id + (pc.beg == 0 ? 1 : 0)) * (RW::R * HD + RW::R);
-    const uint32_t g = rw.g, c16 = rw.c16, w = rw.w;
-    const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-    uint32_t m2[QB];
-    const uint32_t dl2 = twice(a.smx.dlim);
-    int64_t total[QB];
+        const Piece pc(sh, at, stop);
+        at = pc.next;
+        if (pc.beg == pc.end) continue;            // a tile's first positions alone
+        const uint32_t head = pc.head;
+        const Tile<RW::R> tl(bt, a, pc.slot, spl.seqs[threadIdx.x & 63]);
+        if (!tl.on) continue;
+        RW rw(c, bt, a, tl, head);
+        int64_t* part = qu.part + (uint64_t)(2 * id + (pc.beg == 0 ? 1 : 0)) * (RW::R * HD + RW::R);
+        const uint32_t g = rw.g, c16 = rw.c16, w = rw.w;
+        const v4i zero = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+        uint32_t id0 = rw.ids(pc.beg, pc.end), id1 = rw.ids(pc.beg + 1, pc.end);
+        uint32_t m2[QB];
+        const uint32_t dl2 = twice(a.smx.dlim);
+        int64_t total[QB];
 #pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) {
-        const uint32_t row = min(rw.row_of(qb), tl.rows - 1);
-        m2[qb] = twice((uint32_t)sat16i(qu.mx[((uint64_t)head * bt.tokens + tl.q0) * a.G + row] >> 8));
-        total[qb] = 0;
-    }
-    // at most kMaxPart keys in the int32 limb sums (a product is below 2^14, two a key in the middle ones): a longer
-    // piece adds to its partial sums
-    for (uint32_t beg = pc.beg; beg < pc.end;) {
-    const uint32_t end = min(pc.end, beg + kMaxPart / 64);
-    v4i acc[3][DB][QB], vs[NP][MW];
-    uint32_t wsum[QB];                         // the lane's keys' weights: below 2^16 * 16 * kMaxPart / 64
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            m2[qb] = (uint32_t)kNone;
+            total[qb] = 0;
+        }
+        {                                          // the tile's maxima: its pieces' in the list of paged_max_kernel
+            const Shares<RW::R> shm(qu, spl, c.kv, qu.max_shares, kMaxMin);
+            const uint32_t i0 = shm.owner(pc.tile), i1 = shm.owner(pc.tile + pc.steps - 1);
+#pragma unroll 4
+            for (uint32_t i = i0 + g; i <= i1; i += 4) {
+                const int32_t* mp = qu.mx + (2 * i + (i == i0 ? 1 : 0)) * RW::R + rw.row_of(0) - tl.row0;
 #pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) {
+                for (uint32_t qb = 0; qb < QB; qb++) m2[qb] = (uint32_t)max((int)m2[qb], mp[16 * qb]);
+            }
+        }
 #pragma unroll
-        for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
-        wsum[qb] = 0;
-    }
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            int m = max((int)m2[qb], __shfl_xor((int)m2[qb], 16, 64));
+            m = max(m, __shfl_xor(m, 32, 64));
+            m2[qb] = twice((uint32_t)sat16i(m >> 8));
+        }
+        rw.queries(a);
+        // at most kMaxPart keys in the int32 limb sums (a product is below 2^14, two a key in the middle ones): a longer
+        // piece adds to its partial sums
+        for (uint32_t beg = pc.beg; beg < pc.end;) {
+        const uint32_t end = min(pc.end, beg + kMaxPart / 64);
+        v4i acc[3][DB][QB], vs[NP][MW];
+        uint32_t wsum[QB];                         // the lane's keys' weights: below 2^16 * 16 * kMaxPart / 64
 #pragma unroll
-    for (uint32_t m = 0; m < MW; m++) vs[0][m] = vs[NP - 1][m] = zero;
-    rw.run(sm0, sm1, beg, end, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
-        const uint32_t kg = tl.lo + 64 * i + 16 * g;
-        v4i p[QB][I8 ? 3 : 2];
-        // the step's blocks (16 keys x 16 rows) in three stages, a block's products under the exponentials of the one
-        // before and the packing of the one before that
-        constexpr uint32_t NB = 4 * QB;
-        auto weights = [&](auto masked) {
-            typename RW::Frag f;
-            v4i h[2], md[2], l[2];
-            uint32_t es[2];
-            Exp2 x[2][2];
-            rw.load(sm, 0, f);
+        for (uint32_t qb = 0; qb < QB; qb++) {
 #pragma unroll
-            for (uint32_t j = 0; j < NB + 2; j++) {
-                if (j < NB) {
-                    rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
-                    es[j & 1] = f.es;
-                    if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
-                }
-                if (j >= 1 && j <= NB) {
-                    const uint32_t y = j - 1, qb = y % QB;
-                    int z[4];
+            for (uint32_t m = 0; m < DB; m++) acc[0][m][qb] = acc[1][m][qb] = acc[2][m][qb] = zero;
+            wsum[qb] = 0;
+        }
 #pragma unroll
-                    for (uint32_t r = 0; r < 4; r++)
-                        z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
-                    x[y & 1][0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
-                    x[y & 1][1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (j >= 2) {
-                    const uint32_t y = j - 2, kb = y / QB, qb = y % QB;
-                    const Exp2 *e = x[y & 1];
-                    uint32_t v[4] = {e[0].e0(), e[0].e1(), e[1].e0(), e[1].e1()};
-                    if constexpr (masked) {
+        for (uint32_t m = 0; m < MW; m++) vs[0][m] = vs[NP - 1][m] = zero;
+        rw.run(sm0, sm1, beg, end, id0, id1, [&](const uint8_t* sm, uint32_t i, uint32_t ids) {
+            const uint32_t kg = tl.lo + 64 * i + 16 * g;
+            v4i p[QB][I8 ? 3 : 2];
+            // the step's blocks (16 keys x 16 rows) in three stages, a block's products under the exponentials of the one
+            // before and the packing of the one before that
+            constexpr uint32_t NB = 4 * QB;
+            auto weights = [&](auto masked) {
+                typename RW::Frag f;
+                v4i h[2], md[2], l[2];
+                uint32_t es[2];
+                Exp2 x[2][2];
+                rw.load(sm, 0, f);
 #pragma unroll
-                        for (uint32_t r = 0; r < 4; r++) {
-                            const uint32_t key = kg + 4 * kb + r;
-                            v[r] = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? v[r] : 0u;
-                        }
+                for (uint32_t j = 0; j < NB + 2; j++) {
+                    if (j < NB) {
+                        rw.products(f, j % QB, h[j & 1], md[j & 1], l[j & 1]);
+                        es[j & 1] = f.es;
+                        if (j % QB == QB - 1 && j / QB + 1 < 4) rw.load(sm, j / QB + 1, f);
                     }
-                    const uint32_t w01 = pair16(v[0], v[1]), w23 = pair16(v[2], v[3]);
-                    wsum[qb] = add16(w01, add16(w23, wsum[qb]));
-                    uint32_t ve = 0;
-                    if constexpr (I8) ve = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
-                    weight_bytes<I8>(w01, w23, ve, p[qb], kb);
+                    if (j >= 1 && j <= NB) {
+                        const uint32_t y = j - 1, qb = y % QB;
+                        int z[4];
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; r++)
+                            z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
+                        x[y & 1][0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
+                        x[y & 1][1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j >= 2) {
+                        const uint32_t y = j - 2, kb = y / QB, qb = y % QB;
+                        const Exp2 *e = x[y & 1];
+                        uint32_t v[4] = {e[0].e0(), e[0].e1(), e[1].e0(), e[1].e1()};
+                        if constexpr (masked) {
+#pragma unroll
+                            for (uint32_t r = 0; r < 4; r++) {
+                                const uint32_t key = kg + 4 * kb + r;
+                                v[r] = ids != ~0u && key >= rw.vbeg[qb] && key < rw.vend[qb] ? v[r] : 0u;
+                            }
+                        }
+                        const uint32_t w01 = pair16(v[0], v[1]), w23 = pair16(v[2], v[3]);
+                        wsum[qb] = add16(w01, add16(w23, wsum[qb]));
+                        uint32_t ve = 0;
+                        if constexpr (I8) ve = *reinterpret_cast<const uint32_t*>(sm + S::TERM + 320 + 16 * g + 4 * kb);
+                        weight_bytes<I8>(w01, w23, ve, p[qb], kb);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        if (rw.whole(i, ids)) weights(std::false_type{});
-        else weights(std::true_type{});
+            };
+            if (rw.whole(i, ids)) weights(std::false_type{});
+            else weights(std::true_type{});
 #pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * m + c16) * 16;
-            const v4i vh = *reinterpret_cast<const v4i*>(vp);
-            v4i vl = zero;
-            if constexpr (!I8) vl = *reinterpret_cast<const v4i*>(vp + 64 * HD);
+            for (uint32_t m = 0; m < DB; m++) {
+                const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * m + c16) * 16;
+                const v4i vh = *reinterpret_cast<const v4i*>(vp);
+                v4i vl = zero;
+                if constexpr (!I8) vl = *reinterpret_cast<const v4i*>(vp + 64 * HD);
 #pragma unroll
-            for (uint32_t qb = 0; qb < QB; qb++) {
-                if constexpr (I8) {
-                    acc[0][m][qb] = mfma(vh, p[qb][I8 ? 2 : 0], acc[0][m][qb]);
-                    acc[1][m][qb] = mfma(vh, p[qb][1], acc[1][m][qb]);
-                    acc[2][m][qb] = mfma(vh, p[qb][0], acc[2][m][qb]);
-                } else {
-                    acc[0][m][qb] = mfma(vh, p[qb][1], acc[0][m][qb]);
-                    acc[1][m][qb] = mfma(vh, p[qb][0], acc[1][m][qb]);
-                    acc[2][m][qb] = mfma(vl, p[qb][0], acc[2][m][qb]);
-                    acc[1][m][qb] = mfma(vl, p[qb][1], acc[1][m][qb]);
+                for (uint32_t qb = 0; qb < QB; qb++) {
+                    if constexpr (I8) {
+                        acc[0][m][qb] = mfma(vh, p[qb][I8 ? 2 : 0], acc[0][m][qb]);
+                        acc[1][m][qb] = mfma(vh, p[qb][1], acc[1][m][qb]);
+                        acc[2][m][qb] = mfma(vh, p[qb][0], acc[2][m][qb]);
+                    } else {
+                        acc[0][m][qb] = mfma(vh, p[qb][1], acc[0][m][qb]);
+                        acc[1][m][qb] = mfma(vh, p[qb][0], acc[1][m][qb]);
+                        acc[2][m][qb] = mfma(vl, p[qb][0], acc[2][m][qb]);
+                        acc[1][m][qb] = mfma(vl, p[qb][1], acc[1][m][qb]);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (uint32_t m = 0; m < MW; m++) {    // V's sums: each wavefront its share of d
-            const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * (w + 4 * m) + c16) * 16;
-            vs[0][m] = mfma(*reinterpret_cast<const v4i*>(vp), ones, vs[0][m]);
-            if constexpr (!I8) vs[NP - 1][m] = mfma(*reinterpret_cast<const v4i*>(vp + 64 * HD), ones, vs[NP - 1][m]);
-        }
-    });
-    if (c16 == 0) {
-#pragma unroll
-        for (uint32_t m = 0; m < MW; m++)
-#pragma unroll
-            for (uint32_t pl = 0; pl < NP; pl++)
-#pragma unroll
-                for (uint32_t r = 0; r < 4; r++) vsum[pl][16 * (w + 4 * m) + 4 * g + r] = vs[pl][m][r];
-    }
-    __syncthreads();
-    const bool last = end == pc.end;
-#pragma unroll
-    for (uint32_t qb = 0; qb < QB; qb++) {
-        int64_t sum = wsum[qb];
-        sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
-        sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
-        total[qb] += sum;
-        const uint32_t row = rw.row_of(qb);
-        const bool on = row < tl.rows;
-        int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
-        const Divide quot(total[qb], a.fp);
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            int64_t x[4];
-#pragma unroll
-            for (uint32_t r = 0; r < 4; r++) {
-                const uint32_t d = 16 * m + 4 * g + r;
-                x[r] = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
+            for (uint32_t m = 0; m < MW; m++) {    // V's sums: each wavefront its share of d
+                const uint8_t* vp = sm + S::KBYTES + (g * HD + 16 * (w + 4 * m) + c16) * 16;
+                vs[0][m] = mfma(*reinterpret_cast<const v4i*>(vp), ones, vs[0][m]);
+                if constexpr (!I8) vs[NP - 1][m] = mfma(*reinterpret_cast<const v4i*>(vp + 64 * HD), ones, vs[NP - 1][m]);
             }
-            longlong2* pp = reinterpret_cast<longlong2*>(part) + (((w * QB + qb) * DB + m) * 2) * 64 + rw.lane;
-            if (beg != pc.beg) {
-                const longlong2 u = pp[0], v = pp[64];
-                x[0] += u.x;
-                x[1] += u.y;
-                x[2] += v.x;
-                x[3] += v.y;
-            }
-            if (!last || !pc.whole) {
-                pp[0] = make_longlong2(x[0], x[1]);
-                pp[64] = make_longlong2(x[2], x[3]);
-            } else if (on) {
-                store_out(op + 16 * m + 4 * g, quot, x);
-            }
+        });
+        if (c16 == 0) {
+#pragma unroll
+            for (uint32_t m = 0; m < MW; m++)
+#pragma unroll
+                for (uint32_t pl = 0; pl < NP; pl++)
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) vsum[pl][16 * (w + 4 * m) + 4 * g + r] = vs[pl][m][r];
         }
-        if (last && !pc.whole && g == 0) part[RW::R * HD + 16 * (w * QB + qb) + c16] = total[qb];
-    }
-    beg = end;
-    }
+        __syncthreads();
+        const bool last = end == pc.end;
+#pragma unroll
+        for (uint32_t qb = 0; qb < QB; qb++) {
+            int64_t sum = wsum[qb];
+            sum += (int64_t)ro::shfl64((uint64_t)sum, 16);
+            sum += (int64_t)ro::shfl64((uint64_t)sum, 32);
+            total[qb] += sum;
+            const uint32_t row = rw.row_of(qb);
+            const bool on = row < tl.rows;
+            int16_t* op = a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD;
+            const Divide quot(total[qb], a.fp);
+#pragma unroll
+            for (uint32_t m = 0; m < DB; m++) {
+                int64_t x[4];
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) {
+                    const uint32_t d = 16 * m + 4 * g + r;
+                    x[r] = whole_sum<I8>(acc[0][m][qb][r], acc[1][m][qb][r], acc[2][m][qb][r], vsum[0][d], vsum[NP - 1][d], sum);
+                }
+                longlong2* pp = reinterpret_cast<longlong2*>(part) + (((w * QB + qb) * DB + m) * 2) * 64 + rw.lane;
+                if (beg != pc.beg) {
+                    const longlong2 u = pp[0], v = pp[64];
+                    x[0] += u.x;
+                    x[1] += u.y;
+                    x[2] += v.x;
+                    x[3] += v.y;
+                }
+                if (!last || !pc.whole) {
+                    pp[0] = make_longlong2(x[0], x[1]);
+                    pp[64] = make_longlong2(x[2], x[3]);
+                } else if (on) {
+                    store_out(op + 16 * m + 4 * g, quot, x);
+                }
+            }
+            if (last && !pc.whole && g == 0) part[RW::R * HD + 16 * (w * QB + qb) + c16] = total[qb];
+        }
+        beg = end;
+        if (beg < pc.end) {
+            id0 = rw.ids(beg, pc.end);
+            id1 = rw.ids(beg + 1, pc.end);
+        }
+        }
     }
 }
 
-// The pieces' sums of a tile added and divided, in the lanes' order of paged_rows_kernel: a workgroup per boundary
-// between shares that is the first inside its tile, and 16 columns; loads of four pieces in flight.
+// The pieces' sums of a tile added and divided, in the lanes' order of paged_rows_kernel: a workgroup per tile, 64 rows
+// and 16 columns; loads of four pieces in flight.
 template <uint32_t HD, uint32_t QB>
 __global__ __launch_bounds__(256) void paged_rows_join_kernel(Cache c, Batch bt, Attn a, Queue qu) {
     constexpr uint32_t DB = HD / 16, R = 64 * QB;
-    const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, m = blockIdx.y;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x + 1;
-    const Shares sh(qu, c.kv, kRowsMin);
-    if (id >= sh.n) return;
-    const uint64_t at = sh.first(id);
-    const Piece pc(qu, sh, at, at + 1);
-    if (pc.beg == 0) return;                   // before or at the tile's first step
-    if (sh.owner(pc.tile) + 1 != id) return;   // a later boundary inside this tile
-    const uint32_t pieces = sh.owner(pc.tile + pc.steps - 1) - (id - 1) + 1;
-    const Tile<R> tl(bt, a, pc.slot);
-    const uint32_t wq = w * QB + blockIdx.z, row = tl.row0 + 16 * wq + c16;
-    {
-        if (tl.row0 + 16 * wq >= tl.rows) return;
-        int64_t x[4] = {0, 0, 0, 0}, S = 0;
+    __shared__ PlanLds<R> spl;
+    plan(spl, bt, a, qu);
+    const Shares<R> sh(qu, spl, c.kv, qu.shares, kRowsMin);
+    const uint32_t slot = blockIdx.x, head = blockIdx.y, m = blockIdx.z % DB, qb = blockIdx.z / DB;
+    const uint32_t c0 = __builtin_amdgcn_readfirstlane(sh.at(slot)), c1 = __builtin_amdgcn_readfirstlane(sh.at(slot + 1));
+    if (c0 == c1) return;
+    const uint64_t tile = (uint64_t)head * sh.head + c0 + kTileCost;
+    const uint32_t i0 = sh.owner(tile), i1 = sh.owner(tile + (c1 - c0 - kTileCost) - 1);
+    if (i0 == i1) return;                      // one piece: written
+    const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Tile<R> tl(bt, a, slot, spl.seqs[lane]);
+    const uint32_t wq = w * QB + qb, row = tl.row0 + 16 * wq + c16;
+    if (tl.row0 + 16 * wq >= tl.rows) return;
+    int64_t x[4] = {0, 0, 0, 0}, S = 0;
 #pragma unroll 4
-        for (uint32_t i = 0; i < pieces; i++) {
-            const int64_t* p = qu.part + (uint64_t)(2 * (id - 1 + i) + (i == 0 ? 1 : 0)) * (R * HD + R);
-            const longlong2* pp = reinterpret_cast<const longlong2*>(p) + (wq * DB + m) * 128 + lane;
-            const longlong2 u = pp[0], v = pp[64];
-            S += p[R * HD + 16 * wq + c16];
-            x[0] += u.x;
-            x[1] += u.y;
-            x[2] += v.x;
-            x[3] += v.y;
-        }
-        if (row >= tl.rows) return;
-        const Divide quot(S, a.fp);
-        store_out(a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(pc.head * a.G + row % a.G) * HD + 16 * m + 4 * g, quot, x);
+    for (uint32_t i = i0; i <= i1; i++) {
+        const int64_t* p = qu.part + (uint64_t)(2 * i + (i == i0 ? 1 : 0)) * (R * HD + R);
+        const longlong2* pp = reinterpret_cast<const longlong2*>(p) + (wq * DB + m) * 128 + lane;
+        const longlong2 u = pp[0], v = pp[64];
+        S += p[R * HD + 16 * wq + c16];
+        x[0] += u.x;
+        x[1] += u.y;
+        x[2] += v.x;
+        x[3] += v.y;
     }
+    if (row >= tl.rows) return;
+    const Divide quot(S, a.fp);
+    store_out(a.o + (uint64_t)(tl.q0 + row / a.G) * a.o_ld + (uint64_t)(head * a.G + row % a.G) * HD + 16 * m + 4 * g, quot, x);
 }
 
 // ---------------------------------------------------------------- the host's checks
@@ -1821,21 +1912,23 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
 #undef CM_FEW
         return CM_OK;
     }
-    if (slots * steps > 0xFFFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens over %u rows", b.tokens, b.cap);
-    const char* ev = getenv("CMP_T"); const char* em = getenv("CMP_M");
-    const uint32_t wgs = (ev ? atoi(ev) : 2) * st->cus, mwgs = (em ? atoi(em) : 4) * st->cus;
-    const size_t cum_bytes = round_up((slots + 1) * 4, 256), mx_bytes = round_up(rows * 4, 256);
+    if (slots * (steps + kTileCost) > 0xFFFFFFFFu)
+        return fail(CM_EINVAL, "paged attention: %u tokens over %u rows", b.tokens, b.cap);
+    const bool planned = slots > kPlan || b.batch > 64;
+    const uint32_t shares = 2 * (uint32_t)st->cus / 8 * 8, max_shares = 2 * shares;
+    const size_t cum_bytes = planned ? round_up((slots + 1) * 4, 256) : 0, mx_bytes = (size_t)max_shares * 2 * R * 4;
     void* ws;
-    if ((rc = workspace(st, cum_bytes + mx_bytes + (size_t)wgs * 2 * R * (cache->head_dim + 1) * 8, &ws, s))) return rc;
+    if ((rc = workspace(st, cum_bytes + mx_bytes + (size_t)shares * 2 * R * (cache->head_dim + 1) * 8, &ws, s))) return rc;
     uint8_t* p = static_cast<uint8_t*>(ws);
-    const Queue qu{reinterpret_cast<uint32_t*>(p), reinterpret_cast<int32_t*>(p + cum_bytes),
-                   reinterpret_cast<int64_t*>(p + cum_bytes + mx_bytes), (uint32_t)slots};
-    const uint32_t plan = 1 + (uint32_t)std::min<uint64_t>((rows + 4095) / 4096, 64);
-#define CM_ROWS(HD, I8, QB)                                                                                                     \
-    CM_LAUNCH("paged_plan_kernel", (paged_plan_kernel<64 * QB>), dim3(plan), dim3(1024), 0, s, b, a, qu, rows);                 \
-    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), dim3(mwgs), dim3(256), 0, s, c, b, a, qu);                    \
-    CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), dim3(wgs), dim3(256), 0, s, c, b, a, qu, st->smx_tab);      \
-    CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), dim3(wgs, HD / 16, QB), dim3(256), 0, s, c, b, a, qu);
+    const Queue qu{planned ? reinterpret_cast<uint32_t*>(p) : nullptr, reinterpret_cast<int32_t*>(p + cum_bytes),
+                   reinterpret_cast<int64_t*>(p + cum_bytes + mx_bytes), (uint32_t)slots, max_shares, shares};
+    const dim3 jgrid((unsigned)slots, c.kv, cache->head_dim / 16 * (R / 64));
+#define CM_ROWS(HD, I8, QB)                                                                                         \
+    if (planned) { CM_LAUNCH("paged_plan_kernel", paged_plan_kernel<64 * QB>, dim3(1), dim3(1024), 0, s, b, a, qu); } \
+    CM_LAUNCH("paged_max_kernel", (paged_max_kernel<HD, I8, QB>), dim3(max_shares), dim3(256), 0, s, c, b, a, qu);  \
+    CM_LAUNCH("paged_rows_kernel", (paged_rows_kernel<HD, I8, QB>), dim3(shares), dim3(256), 0, s, c, b, a, qu,     \
+              st->smx_tab);                                                                                         \
+    CM_LAUNCH("paged_join_kernel", (paged_rows_join_kernel<HD, QB>), jgrid, dim3(256), 0, s, c, b, a, qu);
     if (cache->head_dim == 64) {
         if (cache->int8) { CM_ROWS(64, true, 2) } else { CM_ROWS(64, false, 2) }
     } else {
