@@ -34,6 +34,8 @@ reference's attention chains, which it runs as one fused node each: ``VitAttenti
 LlmAttnScores, VitAttnSoftmax on the unit, LlmAttnPV, LlmAttnMerge: vit.py:19-32 -> AttentionNode)
 and ``LlmDecodeAttention`` (LlmAttnPrep's RoPE and cache-row writes, the scores, LlmAttnSoftmax,
 P.V: llm_nodes.py:1012-1030, rowops_nodes.py:893-1236 -> DecodePrepNode + DecodeAttentionNode).
+``LlmPagedAttention`` (no reference op) is the same over a paged cache and packed tokens:
+PagedPrepNode + PagedAttentionNode.
 """
 from __future__ import annotations
 
@@ -45,11 +47,12 @@ import numpy as np
 
 from . import units
 from .graph import (KEY_QUANTUM, AttentionNode, AttnMergeNode, AttnSoftmaxNode, ConvNode, DecodeAttentionNode, Graph,
-                    LlmAttnConvNode, MatmulNode, PoolNode, ReshapeNode, ScheduledNode, SchedulerError, SelectRowNode,
-                    SoftmaxVopNode, TensorInfo, conv_out, fuse_activations, softmax_regs)
+                    LlmAttnConvNode, MatmulNode, PagedAttentionNode, PoolNode, ReshapeNode, ScheduledNode,
+                    SchedulerError, SelectRowNode, SoftmaxVopNode, TensorInfo, conv_out, fuse_activations, softmax_regs)
 from .host_ops import (GeluNode, LayerNormNode, LlmAttentionNode, LlmDequantNode, LlmEmbedNode, LlmResAddNode,
                        LlmRMSNormNode, LlmSiluMulNode, LlmToHostNode, SoftmaxNode, TransposeNode)
-from .rowops_nodes import (N_MAX, P1_BITS, AttnPrepRoNode, DecodePrepNode, DequantRoNode, VitAttnPrepRoNode, LayerNorm32RoNode, LayerNormRoNode,
+from .rowops_nodes import (N_MAX, P1_BITS, AttnPrepRoNode, DecodePrepNode, DequantRoNode, PagedPrepNode,
+                           VitAttnPrepRoNode, LayerNorm32RoNode, LayerNormRoNode,
                            ResAddBiasRoNode, ResAddRoNode, RMSNormRoNode, SiluMulRoNode, TransposeRoNode, beta_bits,
                            collapse, gamma_scale, transpose_job)
 
@@ -473,6 +476,24 @@ def _llm_decode_attention(op, ctx):
     return [prep, att]
 
 
+def _llm_paged_attention(op, ctx):
+    """inputs [q, k, v, pool, q_start, kv_len, table], outputs [q after RoPE, o]: PagedPrepNode then
+    PagedAttentionNode."""
+    if not (ctx.platform.rowops and ctx.platform.softmax):
+        raise SchedulerError(f"LlmPagedAttention node '{op.label}': needs the row-ops and softmax units")
+    a = op.attrs
+    ins = ctx.ins(op)
+    qr, o = ctx.t(op.outputs[0], op), ctx.t(op.outputs[1], op)
+    geo = dict(heads=int(a["heads"]), kv_heads=int(a["kv_heads"]), head_dim=int(a["head_dim"]), page=int(a["page"]),
+               int8=bool(a.get("int8", False)), f_v=int(a["f_v"]))
+    prep = PagedPrepNode(ins, qr, f_k=int(a["f_k"]), cos=a["cos"], sin=a["sin"],
+                         interleaved=bool(a.get("interleaved", False)), gamma_q=a.get("gamma_q"),
+                         gamma_k=a.get("gamma_k"), eps=float(a.get("eps", 1e-5)), **geo)
+    att = PagedAttentionNode([qr] + list(ins[3:]), o, window=int(a.get("window", 0)), cm=int(a["cm"]),
+                             cfg=int(a["cfg"]), **geo)
+    return [prep, att]
+
+
 def _heads(op):
     a = op.attrs
     H, KV, HD = int(a["num_heads"]), int(a["num_kv_heads"]), int(a["head_dim"])
@@ -573,7 +594,8 @@ LLM_FACTORIES: Dict[str, Callable] = {
     "LlmEmbed": _llm_embed, "LlmRMSNorm": _llm_rmsnorm, "LlmResAdd": _llm_resadd, "LlmSiluMul": _llm_silu_mul,
     "LlmDequant": _llm_dequant, "LlmToHost": _llm_dequant, "LlmAttention": _llm_attention,
     "VitLayerNorm": _vit_layernorm, "VitResAdd": _llm_resadd, "VitGelu": _vit_gelu, "VitAttention": _vit_attention,
-    "LlmDecodeAttention": _llm_decode_attention, "LlmAttnPrep": _llm_attn_prep, "LlmAttnScores": _llm_attn_conv,
+    "LlmDecodeAttention": _llm_decode_attention, "LlmPagedAttention": _llm_paged_attention,
+    "LlmAttnPrep": _llm_attn_prep, "LlmAttnScores": _llm_attn_conv,
     "LlmAttnPV": _llm_attn_conv, "LlmAttnSoftmax": _llm_attn_softmax, "LlmAttnMerge": _llm_attn_merge,
     "LlmSelectRow": _llm_select_row, "VitAttnPrep": _vit_attn_prep, "VitAttnSoftmax": _vit_attn_softmax,
 }

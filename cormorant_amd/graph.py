@@ -313,6 +313,67 @@ class DecodeAttentionNode(KernelNode):
         return head_dim in (32, 64) and ctx % 64 == 0 and 0 < ctx <= 8192 and 0 < group <= 8
 
 
+@dataclass
+class PagedAttentionNode(KernelNode):
+    """Causal attention of packed tokens over a paged cache (paged.paged_attention): q [tokens][heads
+    hd] against the cache rows of each token's sequence up to its own position (the last ``window``
+    of them, 0: all).  inputs: q, the pool, q_start, kv_len, table as PagedPrepNode's.  Scores and
+    exponentials are the softmax unit's; the sums are exact and o rounded once.  ``cm`` / ``cfg`` the
+    softmax unit's registers, o at f_p + f_v - 8 (``f_v`` the V cache's exponent).  Output rows of no
+    sequence are zeros."""
+    inputs: List[TensorInfo]
+    output: TensorInfo
+    heads: int = 1
+    kv_heads: int = 1
+    head_dim: int = 64
+    page: int = 16
+    int8: bool = False
+    window: int = 0
+    cm: int = 12102203
+    cfg: int = 0x0813
+    f_v: int = 8
+
+    def __post_init__(self):
+        what = f"paged attention '{self.output.onnx_name}'"
+        q = self.inputs[0]
+        if list(q.shape) != [int(q.shape[0]), self.heads * self.head_dim] or list(self.output.shape) != list(q.shape):
+            raise SchedulerError(f"{what}: q {list(q.shape)} -> o {list(self.output.shape)}")
+        check_paged(what, self)
+        if self.window < 0:
+            raise SchedulerError(f"{what}: window {self.window}")
+
+
+def paged_pool(name: str, pages: int, page: int, kv_heads: int, head_dim: int, int8: bool = False) -> TensorInfo:
+    """The state tensor of a paged cache's pool: its bytes as int32 words [pages][kv_heads][block / 4]
+    (paged.block_bytes; zeros are valid rows of zeros)."""
+    return TensorInfo(name, [pages, kv_heads, page * (2 * head_dim + 6 if int8 else 4 * head_dim + 4) // 4], exp=0,
+                      kind="i32", state=True)
+
+
+def one_exponent(e, what: str):
+    e = np.asarray(e).reshape(-1)
+    if (e != e[0]).any():
+        raise SchedulerError(f"{what}: one exponent an operand")
+    return e[0]
+
+
+def check_paged(what: str, sn) -> None:
+    """A paged node's heads, pool (the input before q_start, kv_len and table) and batch tensors."""
+    pool, qs, kl, tb = sn.inputs[-4:]
+    if sn.head_dim not in (64, 128) or sn.page < 16 or sn.page > 4096 or sn.page & (sn.page - 1):
+        raise SchedulerError(f"{what}: head dim {sn.head_dim} (64 or 128), pages of {sn.page} rows (a power of two, "
+                             "16 .. 4096)")
+    if sn.kv_heads < 1 or sn.heads % sn.kv_heads:
+        raise SchedulerError(f"{what}: {sn.heads} heads over {sn.kv_heads} KV heads")
+    want = paged_pool("", int(pool.shape[0]), sn.page, sn.kv_heads, sn.head_dim, sn.int8)
+    if pool.kind != "i32" or list(pool.shape) != want.shape:
+        raise SchedulerError(f"{what}: a pool of shape {list(pool.shape)}, not {want.shape}")
+    if any(t.kind != "i32" for t in (qs, kl, tb)) or len(tb.shape) != 2 or list(kl.shape) != [int(tb.shape[0])] or \
+            list(qs.shape) != [int(tb.shape[0]) + 1]:
+        raise SchedulerError(f"{what}: q_start {list(qs.shape)}, kv_len {list(kl.shape)}, table {list(tb.shape)} "
+                             "(int32 [batch + 1], [batch], [batch][max_pages])")
+
+
 def softmax_regs(f_s: int, sigma: float, f_p: int):
     """(smx_cm, smx_cfg) of scores at 2^-f_s with logit scale ``sigma`` and P at 2^-f_p
     (vectorop_smx.scale_regs + smx_nodes.regs, vectorop_smx.py:37-47, smx_nodes.py:64-76):
@@ -655,7 +716,8 @@ def conv_out(size: int, k: int, stride: int, pad_lo: int, pad_hi: int, dil: int 
 
 
 __all__ = ["SchedulerError", "KernelNode", "TensorInfo", "HeadView", "ScheduledNode", "MatmulNode", "MatmulConvNode", "ConvNode", "PoolNode",
-           "ReshapeNode", "SoftmaxVopNode", "DecodeAttentionNode", "RowOpsNode", "LlmAttnConvNode", "KvWriteNode", "AttentionNode", "attn_keys",
+           "ReshapeNode", "SoftmaxVopNode", "DecodeAttentionNode", "PagedAttentionNode", "paged_pool", "RowOpsNode",
+           "LlmAttnConvNode", "KvWriteNode", "AttentionNode", "attn_keys",
            "AttnSoftmaxNode", "AttnMergeNode", "SelectRowNode", "KEY_QUANTUM", "SMX_MAX_KEYS",
            "Graph", "conv_out", "OP_ADD", "OP_SUB",
            "OP_MUL", "OP_DIV", "OP_RELU", "OP_RELU6", "OP_SOFTMAX", "OP_SOFTMAX_T", "POOL_MAX",

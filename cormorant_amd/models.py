@@ -773,6 +773,49 @@ def smollm2_decode(shape: LlamaShape = LlamaShape(), seed: int = 0, calib_seqs: 
     encode_matmul_weights(g.nodes, AP_FIXED_16_8)
     return g, inputs, exps
 
+
+def _llama_mlp(add, p, L, e, S, T, om, hcur):
+    """A layer behind its attention: the o MatMul, ResAdd, RMSNorm, gate / up, SiluMul, down, ResAdd."""
+    from .rowops_nodes import RMSNormRoNode, ResAddRoNode, SiluMulRoNode
+    T_ = TensorInfo
+    a = T_(p + "a", [T, S.d], exp=e["a"])
+    add(MatmulNode([om, T_(p + "wo", [S.heads * S.hd, S.d], data=L["wo"])], a), "MatMul", domain="")
+    h1 = T_(p + "h1", [T, S.d], exp=RES_BITS, kind="i32")
+    add(ResAddRoNode([hcur, a], h1), "LlmResAdd")
+    x2 = T_(p + "x2", [T, S.d], exp=e["x2"])
+    add(RMSNormRoNode([h1], x2, gamma=L["g2"], eps=S.eps), "LlmRMSNorm", gamma=L["g2"], eps=S.eps)
+    gt = T_(p + "g", [T, S.ff], exp=e["g"])
+    add(MatmulNode([x2, T_(p + "wg", [S.d, S.ff], data=L["wg"])], gt), "MatMul", domain="")
+    up = T_(p + "u", [T, S.ff], exp=e["u"])
+    add(MatmulNode([x2, T_(p + "wu", [S.d, S.ff], data=L["wu"])], up), "MatMul", domain="")
+    mm = T_(p + "m", [T, S.ff], exp=e["m"])
+    add(SiluMulRoNode([gt, up], mm), "LlmSiluMul")
+    dd = T_(p + "d", [T, S.d], exp=e["d"])
+    add(MatmulNode([mm, T_(p + "wd", [S.ff, S.d], data=L["wd"])], dd), "MatMul", domain="")
+    hn = T_(p + "h", [T, S.d], exp=RES_BITS, kind="i32")
+    add(ResAddRoNode([h1, dd], hn), "LlmResAdd")
+    return hn
+
+
+def _llama_head(add, S, rows, emb, gf, fin, h):
+    """The final RMSNorm, the tied head and the dequant of ``rows`` rows to float32 logits."""
+    from .rowops_nodes import DequantRoNode, RMSNormRoNode
+    T_ = TensorInfo
+    xf = T_("xf", [rows, S.d], exp=fin["xf"])
+    add(RMSNormRoNode([h], xf, gamma=gf, eps=S.eps), "LlmRMSNorm", gamma=gf, eps=S.eps)
+    lq = T_("logits_q", [rows, S.vocab], exp=fin["logits"])
+    add(MatmulNode([xf, T_("w.lm_head", [S.d, S.vocab], data=np.ascontiguousarray(emb.T))], lq), "MatMul",
+        domain="")
+    chunk = next(c for c in range(4096, 0, -8) if S.vocab % c == 0)
+    lr = T_("logits_rows", [rows * S.vocab // chunk, chunk], exp=fin["logits"])
+    add(ReshapeNode([lq], lr), "Reshape", domain="")
+    lf = T_("logits_f32", [rows * S.vocab // chunk, chunk], kind="f32")
+    add(DequantRoNode([lr], lf), "LlmDequant")
+    lo = T_("logits", [rows, S.vocab], kind="f32")
+    add(ReshapeNode([lf], lo), "Reshape", domain="")
+    return lo
+
+
 def smollm2_prefill(shape: LlamaShape, T: int, exps, weights, with_head: bool = False, as_ops: bool = False):
     """The prefill_T entry of one sequence (llama.py:28-33; the layers :404-450 with the FPGA
     prefill attention :329-402; the entry :465-497): ids [T] (int32), pos and n (host) -> every
@@ -799,7 +842,7 @@ def smollm2_prefill(shape: LlamaShape, T: int, exps, weights, with_head: bool = 
     from .frontend import LLM_DOMAIN, OpDesc
     from .graph import AttnMergeNode, AttnSoftmaxNode, LlmAttnConvNode, SelectRowNode, SMX_MAX_KEYS
     from .numeric import encode_matmul_weights
-    from .rowops_nodes import AttnPrepRoNode, DequantRoNode, RMSNormRoNode, ResAddRoNode, SiluMulRoNode
+    from .rowops_nodes import AttnPrepRoNode, RMSNormRoNode
 
     S = shape
     if T % 16 or S.ctx % 16 or S.ctx > SMX_MAX_KEYS or S.heads % S.kv or S.hd % 16:
@@ -859,45 +902,88 @@ def smollm2_prefill(shape: LlamaShape, T: int, exps, weights, with_head: bool = 
             outs.append(og)
         om = T_(p + "om", [T, A], exp=e["o"])
         add(AttnMergeNode(outs, om, T=T, H=H, KV=KV, HD=HD), "LlmAttnMerge", **heads)
-        a = T_(p + "a", [T, D], exp=e["a"])
-        add(MatmulNode([om, T_(p + "wo", [A, D], data=L["wo"])], a), "MatMul", domain="")
-        h1 = T_(p + "h1", [T, D], exp=RES_BITS, kind="i32")
-        add(ResAddRoNode([hcur, a], h1), "LlmResAdd")
-        x2 = T_(p + "x2", [T, D], exp=e["x2"])
-        add(RMSNormRoNode([h1], x2, gamma=L["g2"], eps=S.eps), "LlmRMSNorm", gamma=L["g2"], eps=S.eps)
-        gt = T_(p + "g", [T, S.ff], exp=e["g"])
-        add(MatmulNode([x2, T_(p + "wg", [D, S.ff], data=L["wg"])], gt), "MatMul", domain="")
-        up = T_(p + "u", [T, S.ff], exp=e["u"])
-        add(MatmulNode([x2, T_(p + "wu", [D, S.ff], data=L["wu"])], up), "MatMul", domain="")
-        mm = T_(p + "m", [T, S.ff], exp=e["m"])
-        add(SiluMulRoNode([gt, up], mm), "LlmSiluMul")
-        dd = T_(p + "d", [T, D], exp=e["d"])
-        add(MatmulNode([mm, T_(p + "wd", [S.ff, D], data=L["wd"])], dd), "MatMul", domain="")
-        hn = T_(p + "h", [T, D], exp=RES_BITS, kind="i32")
-        add(ResAddRoNode([h1, dd], hn), "LlmResAdd")
-        hcur = hn
+        hcur = _llama_mlp(add, p, L, e, S, T, om, hcur)
     h_last = T_("h_last", [1, D], exp=RES_BITS, kind="i32", state=True)
     add(SelectRowNode([hcur, n_t], h_last), "LlmSelectRow")
     outputs = [h_last]
     if with_head:
-        fin = exps[-1]
-        xf = T_("xf", [1, D], exp=fin["xf"])
-        add(RMSNormRoNode([h_last], xf, gamma=gf, eps=S.eps), "LlmRMSNorm", gamma=gf, eps=S.eps)
-        lq = T_("logits_q", [1, S.vocab], exp=fin["logits"])
-        add(MatmulNode([xf, T_("w.lm_head", [D, S.vocab], data=np.ascontiguousarray(emb.T))], lq), "MatMul",
-            domain="")
-        chunk = next(c for c in range(4096, 0, -8) if S.vocab % c == 0)
-        lr = T_("logits_rows", [S.vocab // chunk, chunk], exp=fin["logits"])
-        add(ReshapeNode([lq], lr), "Reshape", domain="")
-        lf = T_("logits_f32", [S.vocab // chunk, chunk], kind="f32")
-        add(DequantRoNode([lr], lf), "LlmDequant")
-        lo = T_("logits", [1, S.vocab], kind="f32")
-        add(ReshapeNode([lf], lo), "Reshape", domain="")
-        outputs.append(lo)
+        outputs.append(_llama_head(add, S, 1, emb, gf, exps[-1], h_last))
     graph_inputs = [ids_t, pos_t, n_t]
     if as_ops:
         return ops, reg, [t.onnx_name for t in graph_inputs], [t.onnx_name for t in outputs]
     g = Graph(nodes, input_tensors=graph_inputs, output_tensors=outputs)
+    encode_matmul_weights(g.nodes, AP_FIXED_16_8)
+    return g
+
+
+def smollm2_paged(shape: LlamaShape, tokens: int, batch: int, pages: int, page: int, max_pages: int, exps, weights,
+                  int8: bool = False, window: int = 0, with_head: bool = False, as_ops: bool = False):
+    """The serving entry over paged caches: ``tokens`` packed rows of ``batch`` sequences -- whole
+    prompts, chunks of prompts and single decode tokens in one step, each sequence at its own length.
+    Inputs (int32): ids [tokens], q_start [batch + 1], kv_len [batch], table [batch][max_pages] (as
+    paged.PagedBatch's); states: every layer's pool ``l<i>.pool`` (graph.paged_pool: ``pages`` pages of
+    ``page`` rows, ``int8``: half the bytes), written in place.  Output: the residual rows ``h``
+    [tokens][d], with ``with_head`` their float32 logits.  Rows behind the last sequence write nothing
+    to the pools; their output rows mean nothing.
+
+    Weights, exponents and every node but the attention are smollm2_decode's and smollm2_prefill's
+    (head dim 64 or 128; the rope tables reach max_pages * page positions): RMSNorm; q / k / v; the
+    prep and the attention over the pages (PagedPrepNode, PagedAttentionNode); o, ResAdd, RMSNorm,
+    gate / up, SiluMul, down, ResAdd.  ``window``: the keys a row sees (0: all).  ``as_ops``: (ops,
+    tensors, inputs, outputs) in place of the graph, the attention as LlmPagedAttention."""
+    from .dtype import AP_FIXED_16_8
+    from .frontend import LLM_DOMAIN, OpDesc
+    from .graph import PagedAttentionNode, paged_pool
+    from .numeric import encode_matmul_weights
+    from .rowops_nodes import PagedPrepNode, RMSNormRoNode
+
+    S = shape
+    if tokens < 1 or batch < 1 or max_pages < 1:
+        raise ValueError(f"paged entry: {tokens} tokens of {batch} sequences over {max_pages} pages")
+    D, H, KV, HD = S.d, S.heads, S.kv, S.hd
+    A, KD = H * HD, KV * HD
+    emb, Ls, gf = weights
+    cos, sin = rope_half_tables(S.theta, HD, max_pages * page)
+    T_ = TensorInfo
+    nodes, ops, reg = [], [], {}
+
+    def add(node, kind, domain=LLM_DOMAIN, ins=None, outs=None, **attrs):
+        nodes.append(node)
+        if kind is None:
+            return
+        ins = [t for t in node.inputs if t is not None] if ins is None else ins
+        outs = [node.output] if outs is None else outs
+        for t in ins + outs:
+            reg[t.onnx_name] = t
+        ops.append(OpDesc(kind, [t.onnx_name for t in ins], [t.onnx_name for t in outs], attrs, domain))
+
+    ids_t = T_("ids", [tokens], exp=0, kind="i32")
+    step = [T_("q_start", [batch + 1], exp=0, kind="i32"), T_("kv_len", [batch], exp=0, kind="i32"),
+            T_("table", [batch, max_pages], exp=0, kind="i32")]
+    hcur = T_("h0", [tokens, D], exp=RES_BITS, kind="i32")
+    add(LlmEmbedNode([ids_t], hcur, table=emb), "LlmEmbed", table=emb)
+    geo = dict(heads=H, kv_heads=KV, head_dim=HD, page=page, int8=int8)
+    for li, (L, e) in enumerate(zip(Ls, exps)):
+        p = f"l{li}."
+        pool = paged_pool(p + "pool", pages, page, KV, HD, int8)
+        x = T_(p + "x", [tokens, D], exp=e["x"])
+        add(RMSNormRoNode([hcur], x, gamma=L["g1"], eps=S.eps), "LlmRMSNorm", gamma=L["g1"], eps=S.eps)
+        q, k, v = (T_(p + c, [tokens, n], exp=e[c]) for c, n in (("q", A), ("k", KD), ("v", KD)))
+        for t, w in ((q, "wq"), (k, "wk"), (v, "wv")):
+            add(MatmulNode([x, T_(p + w, [D, t.shape[1]], data=L[w])], t), "MatMul", domain="")
+        qr, om = T_(p + "qr", [tokens, A], exp=e["q"]), T_(p + "om", [tokens, A], exp=e["o"])
+        cmr, cfg = softmax_regs(e["s"], 1.0 / math.sqrt(HD), e["p"])
+        ins = [q, k, v, pool] + step
+        add(PagedPrepNode(ins, qr, f_k=e["k"], f_v=e["v"], cos=cos, sin=sin, **geo), None)
+        add(PagedAttentionNode([qr] + ins[3:], om, window=window, cm=cmr, cfg=cfg, f_v=e["v"], **geo),
+            "LlmPagedAttention", ins=ins, outs=[qr, om], f_k=e["k"], f_v=e["v"], cos=cos, sin=sin, window=window,
+            cm=cmr, cfg=cfg, **geo)
+        hcur = _llama_mlp(add, p, L, e, S, tokens, om, hcur)
+    out = _llama_head(add, S, tokens, emb, gf, exps[-1], hcur) if with_head else hcur
+    graph_inputs = [ids_t] + step
+    if as_ops:
+        return ops, reg, [t.onnx_name for t in graph_inputs], [out.onnx_name]
+    g = Graph(nodes, input_tensors=graph_inputs, output_tensors=[out])
     encode_matmul_weights(g.nodes, AP_FIXED_16_8)
     return g
 

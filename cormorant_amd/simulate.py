@@ -14,15 +14,15 @@ from typing import Dict, Iterable, Optional
 import numpy as np
 import torch
 
-from . import residuals, units
+from . import paged, residuals, units
 from .dtype import AP_FIXED_16_8, ApFixed16
 from .graph import (AttentionNode, AttnContractNode, AttnMergeNode, AttnSoftmaxNode, ConvNode, DecodeAttentionNode, Graph,
-                    KvWriteNode, LlmAttnConvNode, MatmulConvNode, SelectRowNode,
+                    KvWriteNode, LlmAttnConvNode, MatmulConvNode, PagedAttentionNode, SelectRowNode,
                     MatmulNode, PermuteNode, PoolNode, ReshapeNode, RowOpsNode, ScheduledNode, SchedulerError, SoftmaxVopNode,
-                    SMX_MAX_KEYS, TensorInfo, attn_keys)
+                    SMX_MAX_KEYS, TensorInfo, attn_keys, one_exponent)
 from .packing import conv_bias_image, conv_lowered_b_image, conv_weight_image, pack_matmul_b
 from .host_ops import HostNode, LlmEmbedNode
-from .rowops_nodes import DecodePrepNode, RoCallNode, RoJob, RowOpsAdapter
+from .rowops_nodes import DecodePrepNode, PagedPrepNode, RoCallNode, RoJob, RowOpsAdapter
 
 def node_reference(node, ins, dtype: Optional[ApFixed16] = None, device: str = "cuda",
                    host: Optional[Dict[str, np.ndarray]] = None) -> np.ndarray:
@@ -255,6 +255,10 @@ class Simulator:
             raw[sn.output.onnx_name] = self._decode_attention(sn, raw)
         elif isinstance(sn, DecodePrepNode):
             raw[sn.output.onnx_name] = self._decode_prep(sn, raw)
+        elif isinstance(sn, PagedPrepNode):
+            raw[sn.output.onnx_name] = self._paged_prep(sn, raw)
+        elif isinstance(sn, PagedAttentionNode):
+            raw[sn.output.onnx_name] = self._paged_attention(sn, raw)
         elif isinstance(sn, AttentionNode):
             raw[sn.output.onnx_name] = self._attention(sn, raw)
         elif isinstance(sn, ScheduledNode):
@@ -1460,6 +1464,40 @@ class Simulator:
                           self._get(vc, raw).reshape(-1), B, sn.heads, KV, HD, pos, tab[jq.b_row0], params[0], jq.op,
                           params[1], jk.op)
         return qr
+
+    def _paged(self, sn, raw):
+        """The cache and batch of a paged node (one PagedBatch for all the layers of a pass)."""
+        pool, qs, kl, tb = sn.inputs[-4:]
+        data = self._get(pool, raw).reshape(-1).view(torch.uint8)
+        cache = paged.PagedCache(int(pool.shape[0]), sn.page, sn.kv_heads, sn.head_dim, sn.int8, data)
+        tokens = int(sn.inputs[0].shape[0])
+        key = f"{qs.onnx_name},{kl.onnx_name},{tb.onnx_name},{tokens}#paged"
+        if key not in raw:
+            raw[key] = paged.PagedBatch(self._get(qs, raw).reshape(-1), self._get(kl, raw).reshape(-1),
+                                        self._get(tb, raw).reshape(tb.shape), tokens)
+        return cache, raw[key]
+
+    def _paged_prep(self, sn: PagedPrepNode, raw) -> torch.Tensor:
+        """The norms and rotations of q (into the output) and k, k and v into the pages, one launch."""
+        q, k, v = (self._get(t, raw).reshape(t.shape) for t in sn.inputs[:3])
+        prep = self._params.get(id(sn))
+        if prep is None:
+            dev = lambda p: None if p is None else torch.from_numpy(p).to(self.device)      # noqa: E731
+            prep = paged.PagedPrep(self._get(sn.table, raw).reshape(sn.table.shape), dev(sn.rope_q), dev(sn.rope_k),
+                                   sn.interleaved, dev(sn.norm_q), dev(sn.norm_k), sn.eps_q, sn.eps_k)
+            self._params[id(sn)] = prep
+        cache, batch = self._paged(sn, raw)
+        return paged.paged_prep(cache, batch, prep, q, k, v, torch.zeros_like(q))
+
+    def _paged_attention(self, sn: PagedAttentionNode, raw) -> torch.Tensor:
+        qt, ot = sn.inputs[0], sn.output
+        what = f"paged attention '{ot.onnx_name}'"
+        one_exponent(self._exp_b(qt), what)
+        if int(one_exponent(self._exp_b(ot), what)) != ((sn.cfg >> 8) & 31) + sn.f_v - self._dtype.frac_bits:
+            raise SchedulerError(f"{what}: the output exponent is not f_p + f_v - {self._dtype.frac_bits}")
+        q = self._get(qt, raw).reshape(qt.shape)
+        cache, batch = self._paged(sn, raw)
+        return paged.paged_attention(cache, batch, q, torch.zeros_like(q), sn.heads, sn.cm, sn.cfg, sn.window)
 
     def _kv_write(self, sn: KvWriteNode, raw) -> torch.Tensor:
         """Row ``pos`` of every sequence's group-major cache from the step's rows, in place."""
