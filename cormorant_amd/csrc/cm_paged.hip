@@ -1864,6 +1864,8 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     DeviceState* st;
     if ((rc = state(&st))) return rc;
     const uint32_t G = heads / c.kv;
+    if ((uint64_t)b.tokens * G > 0x7FFFFFFFu)
+        return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
     const Attn a{q, o, q_ld, o_ld, G, window, fp, smx};
     // Few rows a sequence: tiles of 15 rows, in one launch for short caches, with kept scores for long ones (where those
     // fit kMaxScores); otherwise tiles of 64 or 128 rows that compute the scores twice

@@ -130,7 +130,7 @@ def test_captured_pass_replayed(torch_gpu):
         graph.replay()
         torch.cuda.synchronize()
         want = og.forward(g, f, states=ref)
-        np.testing.assert_array_equal(sim._to_values(sim._tensor(name), out), np.asarray(want[name]).reshape(out.shape))
+        np.testing.assert_array_equal(sim._to_values(sim._tensor(name), out), np.asarray(want[name]).reshape(2, -1))
         for nm in ref:
             np.testing.assert_array_equal(pools[nm].cpu().numpy().astype(np.float64), ref[nm].reshape(pools[nm].shape))
         sim.forward_raw({**{k: sim._to_device(sim._tensor(k), v) for k, v in f.items()},
