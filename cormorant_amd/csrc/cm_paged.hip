@@ -155,6 +155,8 @@ __device__ __forceinline__ uint32_t quantise(int (&x)[8]) {
     return (uint32_t)e;
 }
 
+constexpr uint32_t kPrepGroup = 4;
+
 // 64-row chunks of the sequences' new positions, aligned to 64 (so to pages and 16-row groups): sequence b's have the
 // slots from floor(start(b) / 64) + 2 b on.
 struct Chunk {
@@ -175,12 +177,14 @@ struct Chunk {
 };
 inline uint64_t chunk_slots(const Batch& b) { return (uint64_t)b.tokens / 64 + 2 * (uint64_t)b.batch; }
 
-// One launch, two kinds of workgroups.  q and k: HD / 8 lanes a head row, 8 columns a lane; a wavefront takes 64 / L
-// of a token's rows and `tpw` tokens, so that a lane's parameters stay in registers.  Its arithmetic is the row-ops
-// unit's, in double where every product is a whole number below 2^53 (the norm's x Rm and P1 G, the rotation's two
-// products; rounded by v_rndne_f64), about 10 instructions an element instead of 40 in 64-bit integers.  V: a chunk
-// of 64 positions of a head, transposed through LDS and stored as whole 16-key pieces where all 16 are new.
-template <uint32_t HD, bool I8>
+// One launch, two kinds of workgroups.  q and k: HD / 8 lanes a head row, 8 columns a lane; a wavefront takes PG passes
+// of 64 / L of a token's rows and `tpw` tokens, so that PG rows' loads are in flight and a token's table row is
+// converted once for them.  Its arithmetic is the row-ops unit's, in double where every product is a whole number below
+// 2^53 (the norm's x Rm and P1 G, the rotation's two products; rounded by the sum with 1.5 2^52).  V: a chunk of 64
+// positions of a head, transposed through LDS and stored as whole 16-key pieces where all 16 are new.
+// 8192 tokens of 15 + 5 heads of 64 with norms: 31 us for 63 MB (2.0 TB/s, a copy's rate 5.2); without the norms'
+// arithmetic 23, without the rotation's 21, V's part alone 5.5: bound by the doubles at 2 wavefronts a SIMD.
+template <uint32_t HD, bool I8, uint32_t PG>
 __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep a, uint32_t qk_blocks, uint32_t passes, uint32_t tpw) {
     constexpr uint32_t L = HD / 8, RW = 64 / L;
     typedef Block<HD, I8> B;
@@ -246,6 +250,7 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         return;
     }
     // every load that needs no other comes first: the rsqrt table, the first token's x, the parameters, the batch
+    __shared__ double nG[2][HD];            // the norms' G 2^-sc
     const bool norms = a.norm_q != nullptr || a.norm_k != nullptr;
     if (norms) {
 #pragma unroll
@@ -253,25 +258,47 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
             __builtin_amdgcn_global_load_lds(a.tab + 32768 + 4 * 2048 + 16 * (t + 256 * i),
                                              (__attribute__((address_space(3))) void*)(lds + 16 * (64 * (t >> 6) + 256 * i)), 16, 0, 0);
     }
-    const uint32_t wv = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (t >> 6)), ps = wv % passes;
-    const uint32_t t0 = min(wv / passes * tpw, bt.tokens - 1);      // past the end: below
-    const bool idle = wv / passes * tpw >= bt.tokens;
-    const uint32_t rows = a.heads + c.kv, r = ps * RW + lane / L;
-    const bool on = r < rows, isq = r < a.heads;
-    const uint32_t g = isq ? r : on ? r - a.heads : 0u;
-    const int16_t* src = (isq ? a.q : a.k) + g * HD + d0;
-    const uint64_t ld = isq ? a.q_ld : a.k_ld;
-    const uint8_t *np = isq ? a.norm_q : a.norm_k, *rp = isq ? a.rope_q : a.rope_k;
-    const bool cols = (isq ? a.rope_q_cols : a.rope_k_cols) != 0;
-    int4 xw = *reinterpret_cast<const int4*>(src + t0 * ld);
-    uint4 nw[8], rw[8];
-    rw[0] = *reinterpret_cast<const uint4*>(rp + (cols ? 16 * (g * HD + d0) : 0u));
-    if (cols) {
+    const uint32_t groups = (passes + PG - 1) / PG;
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (t >> 6)), ps0 = wv % groups * PG;
+    const uint32_t t0 = min(wv / groups * tpw, bt.tokens - 1);      // past the end: below
+    const bool idle = wv / groups * tpw >= bt.tokens;
+    const uint32_t rows = a.heads + c.kv;
+    // the lane's row of pass p: on, of q or of k, its head
+    auto row = [&](uint32_t p) { return (ps0 + p) * RW + lane / L; };
+    auto on = [&](uint32_t p) { return row(p) < rows; };
+    auto isq = [&](uint32_t p) { return row(p) < a.heads; };
+    auto head = [&](uint32_t p) { return isq(p) ? row(p) : on(p) ? row(p) - a.heads : 0u; };
+    int4 xn[PG], c0, c1, s0, s1;            // the next token's
+    auto load_x = [&](uint32_t tok) {
 #pragma unroll
-        for (uint32_t l = 1; l < 8; l++) rw[l] = *reinterpret_cast<const uint4*>(rp + 16 * (g * HD + d0 + l));
+        for (uint32_t p = 0; p < PG; p++)
+            xn[p] = *reinterpret_cast<const int4*>((isq(p) ? a.q + tok * a.q_ld : a.k + tok * a.k_ld) + head(p) * HD + d0);
+    };
+    load_x(t0);
+    // The double forms: a lane's 8 columns at the same shifts, the norm's Bq 0.  x cos + y sin is below 2^47 for any
+    // int32 table, its rounded quotient below 2^30; |P1 G| below 2^52 (see below), its quotient below 2^30.
+    double rS[PG];
+    uint32_t plain = 0;                     // a bit a pass
+    {
+        uint4 rw[PG];
+#pragma unroll
+        for (uint32_t p = 0; p < PG; p++)
+            rw[p] = *reinterpret_cast<const uint4*>(isq(p) ? a.rope_q + (a.rope_q_cols ? 16 * (head(p) * HD + d0) : 0u)
+                                                           : a.rope_k + (a.rope_k_cols ? 16 * (head(p) * HD + d0) : 0u));
+#pragma unroll
+        for (uint32_t p = 0; p < PG; p++) {
+            const ro::Param r0 = ro::param_of(rw[p]);
+            bool ok = r0.sa == r0.sb && r0.sc >= r0.sa + 17;
+            if (isq(p) ? a.rope_q_cols : a.rope_k_cols) {
+                const uint8_t* rp = (isq(p) ? a.rope_q : a.rope_k) + 16 * (head(p) * HD + d0);
+#pragma unroll
+                for (uint32_t l = 1; l < 8; l++)
+                    ok = ok && ((reinterpret_cast<const uint4*>(rp)[l].z ^ rw[p].z) & 0x3F3F3Fu) == 0;
+            }
+            rS[p] = pow2(r0.sa - r0.sc);
+            plain |= __all(ok || !on(p)) ? 1u << p : 0u;
+        }
     }
-#pragma unroll
-    for (uint32_t l = 0; l < 8; l++) nw[l] = np != nullptr ? *reinterpret_cast<const uint4*>(np + 16 * (d0 + l)) : make_uint4(0, 0, 22u << 16, 0);
     uint32_t b, next, total;
     int64_t base;                           // position = base + token
     if (bt.batch <= 64) {
@@ -286,38 +313,30 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         base = (int64_t)bt.len(b) - next;
         total = bt.start(bt.batch);
     }
+    bool nplain[2] = {true, true};
     if (norms) {
+#pragma unroll
+        for (uint32_t k = 0; k < 2; k++) {
+            const uint8_t* np = k == 0 ? a.norm_q : a.norm_k;
+            bool ok = true;
+            if (np != nullptr && t < HD) {
+                const ro::Param n = ro::ld_param(np, t, false);
+                nG[k][t] = (double)(int)n.g * pow2(-n.sc);
+                ok = n.sc >= 22 && n.bq == 0 && n.g < (1 << 27) && n.g > -(1 << 27);
+            }
+            nplain[k] = __syncthreads_and(ok) != 0;
+        }
         __builtin_amdgcn_s_waitcnt(0x0070);
         __syncthreads();
     }
     if (idle || t0 >= total) return;
-    const uint32_t t1 = min(t0 + tpw, total);
-    const uint64_t eps = (uint64_t)(isq ? a.eps_q : a.eps_k);
-    const uint32_t half = a.rotary / 2;
+    const uint32_t t1 = min(t0 + tpw, total), half = a.rotary / 2;
     const bool rot = d0 < a.rotary, upper = !a.interleaved && d0 >= half;
     const int pl = (int)(!rot || a.interleaved ? lane : d0 < half ? lane + half / 8 : lane - half / 8);
     const uint32_t minus = a.interleaved || upper ? 0u : 0x80000000u;     // the partner's sign, on its product's high word
-
-    // The double forms: a lane's 8 columns at the same shifts, the norm's Bq 0.  x cos + y sin is below 2^47 for any
-    // int32 table, its rounded quotient below 2^30; |P1 G| below 2^52 (see below), its quotient below 2^30.
-    const ro::Param r0 = ro::param_of(rw[0]);
-    bool plain = r0.sa == r0.sb && r0.sc >= r0.sa + 17, nplain = true;
-    if (cols) {
-#pragma unroll
-        for (uint32_t l = 1; l < 8; l++) plain = plain && ((rw[l].z ^ rw[0].z) & 0x3F3F3Fu) == 0;
-    }
-    const double rS = pow2(r0.sa - r0.sc);
-    double nG[8];                           // G 2^-sc
-#pragma unroll
-    for (uint32_t l = 0; l < 8; l++) {
-        const ro::Param n = ro::param_of(nw[l]);
-        nG[l] = (double)(int)n.g * pow2(-n.sc);
-        nplain = nplain && n.sc >= 22 && n.bq == 0 && n.g < (1 << 27) && n.g > -(1 << 27);
-    }
-    plain = __all(plain || !on);
     // A token's loads are issued before the stores of the one before: a wait for a load is a wait for every older store
     int64_t pos;
-    int4 c0, c1, s0, s1;
+    const int32_t* cs;
     uint32_t id;
     auto fetch = [&](uint32_t tok) {
         while (tok >= next && b + 1 < bt.batch) {
@@ -326,95 +345,121 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep
         }
         pos = base + tok;
         const uint32_t trow = (uint32_t)min(max(pos, (int64_t)0), (int64_t)a.rope_rows - 1);
-        const int32_t* cs = a.rope + (uint64_t)trow * 2 * a.rotary + (rot ? d0 : 0u);
+        cs = a.rope + (uint64_t)trow * 2 * a.rotary + (rot ? d0 : 0u);
         c0 = *reinterpret_cast<const int4*>(cs);
         c1 = *reinterpret_cast<const int4*>(cs + 4);
         s0 = *reinterpret_cast<const int4*>(cs + a.rotary);
         s1 = *reinterpret_cast<const int4*>(cs + a.rotary + 4);
         id = pos >= 0 && pos < (int64_t)bt.cap ? (uint32_t)bt.table[b * bt.table_ld + (uint32_t)(pos >> c.lg)] : ~0u;
     };
+    // x[l] = f(l, x[l]) one column at a time, in the lane's LDS words: a loop's index into registers costs 60 of them
+    __shared__ __attribute__((aligned(16))) int16_t slow_x[256][8], slow_y[256][8];
+    auto slow = [&](int (&x)[8], auto f) {
+        *reinterpret_cast<int4*>(slow_x[t]) = ro::pack16(x);
+#pragma unroll 1
+        for (uint32_t l = 0; l < 8; l++) slow_x[t][l] = (int16_t)f(l, (int)slow_x[t][l]);
+        const int4 w = *reinterpret_cast<const int4*>(slow_x[t]);
+#pragma unroll
+        for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&w)[l];
+    };
     fetch(t0);
     for (uint32_t tok = t0; tok < t1; tok++) {
-        int co[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, si[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        if (!rot) {
+        double co[8], si[8];
+        {
+            const int ci[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sj[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
             for (uint32_t l = 0; l < 8; l++) {
-                co[l] = 1 << 23;
-                si[l] = 0;
+                co[l] = rot ? f64(ci[l]) : 0x1p23;
+                si[l] = rot ? f64(sj[l]) : 0.0;
             }
         }
-        int x[8];
+        int4 xc[PG];
 #pragma unroll
-        for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&xw)[l];
-        if (norms) {                        // every lane: the sums are the wavefront's
-            const uint64_t s2 = row_sum64<L>(squares8(xw));
-            if (np != nullptr) {
-                const uint64_t D = max(s2 + eps, (uint64_t)1);
-                uint64_t Rm;
-                int sh;
-                rsqrt64(D, Rm, sh, reinterpret_cast<const uint32_t*>(lds));
-                const double scale = (double)Rm * pow2(24 - sh);        // x scale: 48 bits, exact
-                // |x| <= sqrt(D), so |P1| <= sqrt(D) scale + 1; below 2^25 (the unit's own table: 2^24) P1 G is below 2^52
-                if (nplain && scale * scale * (double)D < 0x1p49) {
+        for (uint32_t p = 0; p < PG; p++) xc[p] = xn[p];
+        const uint32_t slot = (uint32_t)pos & (c.page - 1), page = id;
+        const int32_t* trow = cs;
+        if (tok + 1 < t1) {
+            load_x(tok + 1);
+            fetch(tok + 1);
+        }
 #pragma unroll
-                    for (uint32_t l = 0; l < 8; l++) x[l] = rne_sat_f64(__builtin_floor(f64(x[l]) * scale), nG[l]);
-                } else {
-#pragma unroll 1
-                    for (uint32_t l = 0; l < 8; l++) {
-                        const ro::Param p = ro::ld_param(np, d0 + l, false);
-                        x[l] = rne_sat((((int64_t)x[l] * (int64_t)Rm) >> (sh - 24)) * p.g + p.bq, (uint32_t)p.sc);
+        for (uint32_t p = 0; p < PG; p++) {
+            if (p && ps0 + p >= passes) break;
+            const uint32_t g = head(p);
+            const bool q_row = isq(p), live = on(p);
+            int x[8];
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) x[l] = (int)reinterpret_cast<const int16_t*>(&xc[p])[l];
+            if (norms) {                    // every lane: the sums are the wavefront's
+                const uint64_t s2 = row_sum64<L>(squares8(xc[p]));
+                const uint8_t* np = q_row ? a.norm_q : a.norm_k;
+                if (np != nullptr) {
+                    const uint64_t D = max(s2 + (uint64_t)(q_row ? a.eps_q : a.eps_k), (uint64_t)1);
+                    uint64_t Rm;
+                    int sh;
+                    rsqrt64(D, Rm, sh, reinterpret_cast<const uint32_t*>(lds));
+                    const double scale = (double)Rm * pow2(24 - sh);        // x scale: 48 bits, exact
+                    // |x| <= sqrt(D), so |P1| <= sqrt(D) scale + 1; below 2^25 (the unit's own table: 2^24) P1 G is below 2^52
+                    if (nplain[q_row ? 0 : 1] && scale * scale * (double)D < 0x1p49) {
+#pragma unroll
+                        for (uint32_t l = 0; l < 8; l++)
+                            x[l] = rne_sat_f64(__builtin_floor(f64(x[l]) * scale), nG[q_row ? 0 : 1][d0 + l]);
+                    } else {
+                        slow(x, [&](uint32_t l, int v) {
+                            const ro::Param n = ro::ld_param(np, d0 + l, false);
+                            return rne_sat((((int64_t)v * (int64_t)Rm) >> (sh - 24)) * n.g + n.bq, (uint32_t)n.sc);
+                        });
                     }
                 }
             }
-        }
-        int y[8];                           // the partners
+            int y[8];                       // the partners
 #pragma unroll
-        for (uint32_t l = 0; l < 8; l++) y[l] = a.interleaved ? x[l ^ 1] : __shfl(x[l], pl, 64);
-        if (plain) {
+            for (uint32_t l = 0; l < 8; l++) y[l] = a.interleaved ? x[l ^ 1] : __shfl(x[l], pl, 64);
+            if (plain >> p & 1) {
 #pragma unroll
-            for (uint32_t l = 0; l < 8; l++) {
-                const uint32_t m = a.interleaved && !(l & 1) ? 0x80000000u : minus;
-                const double ys = f64(y[l]) * f64(si[l]);
-                const double z = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, ys) ^ (uint64_t)m << 32);
-                x[l] = rne_sat_f64(__builtin_fma(f64(x[l]), f64(co[l]), z), rS);
+                for (uint32_t l = 0; l < 8; l++) {
+                    const uint32_t m = a.interleaved && !(l & 1) ? 0x80000000u : minus;
+                    const double ys = f64(y[l]) * si[l];
+                    const double z = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, ys) ^ (uint64_t)m << 32);
+                    x[l] = rne_sat_f64(__builtin_fma(f64(x[l]), co[l], z), rS[p]);
+                }
+            } else {
+                const uint8_t* rp = q_row ? a.rope_q : a.rope_k;
+                const bool cols = (q_row ? a.rope_q_cols : a.rope_k_cols) != 0;
+                *reinterpret_cast<int4*>(slow_y[t]) = ro::pack16(y);
+                slow(x, [&](uint32_t l, int v) {
+                    const bool neg = a.interleaved ? !(l & 1) : !upper;
+                    const int w = slow_y[t][l];
+                    return ro::rope_elem(v, neg ? -w : w, rot ? trow[l] : 1 << 23, rot ? trow[a.rotary + l] : 0,
+                                         ro::ld_param(rp, g * HD + d0 + l, !cols));
+                });
             }
-        } else {
-#pragma unroll 1
-            for (uint32_t l = 0; l < 8; l++) {
-                const bool neg = a.interleaved ? !(l & 1) : !upper;
-                x[l] = ro::rope_elem(x[l], neg ? -y[l] : y[l], co[l], si[l], ro::ld_param(rp, g * HD + d0 + l, !cols));
+            if (live && q_row) *reinterpret_cast<int4*>(a.qr + tok * a.qr_ld + g * HD + d0) = ro::pack16(x);
+            if ((ps0 + p + 1) * RW <= a.heads) continue;      // no k row in this pass
+            uint32_t e = 0;
+            if constexpr (I8) e = quantise<L>(x);
+            int s = 0;
+#pragma unroll
+            for (uint32_t l = 0; l < 8; l++) s += x[l];
+            s = (int)row_all<L>((uint32_t)s, [](uint32_t p, uint32_t q) { return p + q; });
+            if (!live || q_row || page >= c.pages) continue;
+            uint8_t* blk = c.data + ((uint64_t)page * c.kv + g) * c.block;
+            if constexpr (I8) {
+                uint32_t h[2];
+#pragma unroll
+                for (uint32_t w = 0; w < 2; w++)
+                    h[w] = (x[4 * w] & 255) | (x[4 * w + 1] & 255) << 8 | (x[4 * w + 2] & 255) << 16 | (uint32_t)x[4 * w + 3] << 24;
+                *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = make_uint2(h[0], h[1]);
+            } else {
+                uint2 h, lo;
+                split8(ro::pack16(x), h, lo);
+                *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = h;
+                *reinterpret_cast<uint2*>(blk + B::k(c.page, 1) + slot * HD + d0) = lo;
             }
-        }
-        const uint32_t slot = (uint32_t)pos & (c.page - 1), page = id;
-        if (tok + 1 < t1) {
-            xw = *reinterpret_cast<const int4*>(src + (tok + 1) * ld);
-            fetch(tok + 1);
-        }
-        if (on && isq) *reinterpret_cast<int4*>(a.qr + tok * a.qr_ld + g * HD + d0) = ro::pack16(x);
-        if (ps * RW + RW <= a.heads) continue;                // no k row in this wavefront's
-        uint32_t e = 0;
-        if constexpr (I8) e = quantise<L>(x);
-        int s = 0;
-#pragma unroll
-        for (uint32_t l = 0; l < 8; l++) s += x[l];
-        s = (int)row_all<L>((uint32_t)s, [](uint32_t p, uint32_t q) { return p + q; });
-        if (!on || isq || page >= c.pages) continue;
-        uint8_t* blk = c.data + ((uint64_t)page * c.kv + g) * c.block;
-        if constexpr (I8) {
-            uint32_t h[2];
-#pragma unroll
-            for (uint32_t w = 0; w < 2; w++)
-                h[w] = (x[4 * w] & 255) | (x[4 * w + 1] & 255) << 8 | (x[4 * w + 2] & 255) << 16 | (uint32_t)x[4 * w + 3] << 24;
-            *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = make_uint2(h[0], h[1]);
-        } else {
-            uint2 h, lo;
-            split8(ro::pack16(x), h, lo);
-            *reinterpret_cast<uint2*>(blk + B::k(c.page, 0) + slot * HD + d0) = h;
-            *reinterpret_cast<uint2*>(blk + B::k(c.page, 1) + slot * HD + d0) = lo;
-        }
-        if (u == 0) {
-            reinterpret_cast<int32_t*>(blk + B::term(c.page))[slot] = 128 * s - (I8 ? 0 : 16384 * (int)HD);
-            if constexpr (I8) blk[B::ke(c.page) + slot] = (uint8_t)e;
+            if (u == 0) {
+                reinterpret_cast<int32_t*>(blk + B::term(c.page))[slot] = 128 * s - (I8 ? 0 : 16384 * (int)HD);
+                if constexpr (I8) blk[B::ke(c.page) + slot] = (uint8_t)e;
+            }
         }
     }
 }
@@ -1317,7 +1362,7 @@ struct Rows {
 constexpr uint32_t kPlan = 256;
 struct Queue {
     uint32_t* cum;                         // [slots + 1] steps before each tile of a KV head; null: each workgroup's own
-    int32_t* mx;                           // [max_shares][2: a tile's later part, its first][R] raw maxima
+    int32_t* mx;                           // [max_shares + KV heads slots][R] raw maxima, a piece's at share + tile
     int64_t* part;                         // [shares][2][R HD + R], in the lanes' order
     uint32_t slots, max_shares, shares;    // shares at most, both multiples of 8
 };
@@ -1405,6 +1450,10 @@ struct Piece {
     uint64_t next;                         // the list's position behind the piece
     uint64_t tile;                         // the position of the tile's first step
     bool whole;
+    // a piece's maxima: along the list either the share or the tile grows from piece to piece
+    static __device__ __forceinline__ uint64_t maxima(const Queue& q, uint32_t share, uint32_t head, uint32_t slot) {
+        return share + (uint64_t)head * q.slots + slot;
+    }
     template <uint32_t R>
     __device__ __forceinline__ Piece(const Shares<R>& sh, uint64_t at, uint64_t stop) {
         head = (uint32_t)(at / sh.head);
@@ -1501,7 +1550,7 @@ __global__ __launch_bounds__(256, 2) void paged_max_kernel(Cache c, Batch bt, At
             int m = mx[qb];
             m = max(m, __shfl_xor(m, 16, 64));
             m = max(m, __shfl_xor(m, 32, 64));
-            if (rw.g == 0) qu.mx[(2 * id + (pc.beg == 0 ? 1 : 0)) * RW::R + rw.row_of(qb) - tl.row0] = m;
+            if (rw.g == 0) qu.mx[Piece::maxima(qu, id, head, pc.slot) * RW::R + rw.row_of(qb) - tl.row0] = m;
         }
     }
 }
@@ -1546,7 +1595,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
             const uint32_t i0 = shm.owner(pc.tile), i1 = shm.owner(pc.tile + pc.steps - 1);
 #pragma unroll 4
             for (uint32_t i = i0 + g; i <= i1; i += 4) {
-                const int32_t* mp = qu.mx + (2 * i + (i == i0 ? 1 : 0)) * RW::R + rw.row_of(0) - tl.row0;
+                const int32_t* mp = qu.mx + Piece::maxima(qu, i, head, pc.slot) * RW::R + rw.row_of(0) - tl.row0;
 #pragma unroll
                 for (uint32_t qb = 0; qb < QB; qb++) m2[qb] = (uint32_t)max((int)m2[qb], mp[16 * qb]);
             }
@@ -1797,18 +1846,28 @@ int run_prep(const cm_paged_cache* cache, const cm_paged_batch* batch, const cm_
                  p.rope, static_cast<const uint8_t*>(p.rope_q), static_cast<const uint8_t*>(p.rope_k),
                  static_cast<const uint8_t*>(p.norm_q), static_cast<const uint8_t*>(p.norm_k), p.rope_q_cols,
                  p.rope_k_cols, p.eps_q, p.eps_k, st->ro_tables};
-    // q and k: `tpw` tokens a wavefront once there are 4096 wavefronts; V: a workgroup a chunk and head
+    // q and k: a pass of a token a wavefront until those are 4096 wavefronts (16 decode tokens 3.8 us, in groups 6.0),
+    // then kPrepGroup passes and `tpw` tokens (1610 packed tokens of 12 + 4 heads of 128: 11.7 us, a pass alone 14.6;
+    // 8192 tokens of 15 + 5 heads of 64: 31 either way).  V: a workgroup a chunk and head.
     const uint32_t rw = 64 / (cache->head_dim / 8), passes = (p.heads + c.kv + rw - 1) / rw;
-    const uint32_t tpw = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)b.tokens * passes / 4096, 1), 8);
-    const uint64_t waves = (uint64_t)((b.tokens + tpw - 1) / tpw) * passes, qk = (waves + 3) / 4, vb = chunk_slots(b) * c.kv;
+    const bool grouped = (uint64_t)b.tokens * passes > 4096u;
+    const uint32_t groups = grouped ? (passes + kPrepGroup - 1) / kPrepGroup : passes;
+    const uint32_t tpw = grouped ? (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)b.tokens * groups / 2048, 1), 8) : 1;
+    const uint64_t waves = (uint64_t)((b.tokens + tpw - 1) / tpw) * groups, qk = (waves + 3) / 4, vb = chunk_slots(b) * c.kv;
     if (qk + vb > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged prep: %u tokens of %u heads", b.tokens, p.heads);
     const dim3 grid((unsigned)(qk + vb));
-#define CM_PREP(HD, I8)                                                                                     \
-    CM_LAUNCH("paged_prep_kernel", (paged_prep_kernel<HD, I8>), grid, dim3(256), 0, s, c, b, a, (uint32_t)qk, passes, tpw)
+#define CM_PREP(HD, I8)                                                                                               \
+    if (grouped) {                                                                                                    \
+        CM_LAUNCH("paged_prep_kernel", (paged_prep_kernel<HD, I8, kPrepGroup>), grid, dim3(256), 0, s, c, b, a,       \
+                  (uint32_t)qk, passes, tpw);                                                                         \
+    } else {                                                                                                          \
+        CM_LAUNCH("paged_prep_kernel", (paged_prep_kernel<HD, I8, 1>), grid, dim3(256), 0, s, c, b, a, (uint32_t)qk,  \
+                  passes, tpw);                                                                                       \
+    }
     if (cache->head_dim == 64) {
-        if (cache->int8) { CM_PREP(64, true); } else { CM_PREP(64, false); }
+        if (cache->int8) { CM_PREP(64, true) } else { CM_PREP(64, false) }
     } else {
-        if (cache->int8) { CM_PREP(128, true); } else { CM_PREP(128, false); }
+        if (cache->int8) { CM_PREP(128, true) } else { CM_PREP(128, false) }
     }
 #undef CM_PREP
     return CM_OK;
@@ -1918,7 +1977,7 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
         return fail(CM_EINVAL, "paged attention: %u tokens over %u rows", b.tokens, b.cap);
     const bool planned = slots > kPlan || b.batch > 64;
     const uint32_t shares = 2 * (uint32_t)st->cus / 8 * 8, max_shares = 2 * shares;
-    const size_t cum_bytes = planned ? round_up((slots + 1) * 4, 256) : 0, mx_bytes = (size_t)max_shares * 2 * R * 4;
+    const size_t cum_bytes = planned ? round_up((slots + 1) * 4, 256) : 0, mx_bytes = (max_shares + slots * c.kv) * R * 4;
     void* ws;
     if ((rc = workspace(st, cum_bytes + mx_bytes + (size_t)shares * 2 * R * (cache->head_dim + 1) * 8, &ws, s))) return rc;
     uint8_t* p = static_cast<uint8_t*>(ws);

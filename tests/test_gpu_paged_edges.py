@@ -34,6 +34,15 @@ def test_more_than_256_tiles(paged, batch, int8):  # noqa: F811
     check_attention(paged, c, *regs(128), window=30)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hd,batch,kv", [(64, 300, 8), (64, 60, 40), (128, 300, 8)])
+def test_several_tiles_a_share(paged, hd, batch, kv, int8):  # noqa: F811
+    """2400 tiles of one or two steps: every workgroup has several whole ones between the ends of others."""
+    rng = np.random.default_rng(batch)
+    c = Case(rng, [int(x) for x in rng.integers(4, 100, batch)], [4] * batch, kv=kv, G=8, hd=hd, int8=int8)
+    check_attention(paged, c, *regs(hd))
+
+
 @pytest.mark.parametrize("kv,G,T", [(1, 1, 200), (5, 1, 3), (1, 40, 33), (2, 33, 1)])
 def test_head_groups(paged, kv, G, T):  # noqa: F811
     c = Case(np.random.default_rng(G), [T + 70, 1], [T, 1], kv=kv, G=G)
