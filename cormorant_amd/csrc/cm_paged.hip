@@ -986,7 +986,9 @@ struct FewSums {
 // Caches of at most kShort keys in one launch of 16 wavefronts a tile.  For the scores a wavefront takes steps w, w + 16;
 // the weights go through LDS (16 steps a round), and for P.V a wavefront takes 16 columns of V over 4 of the round's
 // steps (8 at 128 d): its sums are 12 registers, and 4 (2) of them meet in LDS instead of 16.  V's first round is read
-// beside K: one memory latency for both.  16 sequences of 1024 rows, 15 heads: us with V's columns undivided 11.5.
+// beside K: one memory latency for both.  16 sequences of 1024 rows, 15 heads: 10.2 us
+// (V's columns undivided 11.5, with the three kernels of long caches 14.3), on 80 CUs: a CU reads 262 KB in 4 us, the
+// rest is the chain of launch, batch, page ids, K, maxima, V.
 constexpr uint32_t kShort = 2048;
 
 template <uint32_t HD, bool I8>
@@ -1071,7 +1073,9 @@ __global__ __launch_bounds__(1024) void paged_short_kernel(Cache c, Batch bt, At
     sums.template store<I8>(a, tl, blockIdx.y);
 }
 
-// Long caches.  A workgroup takes `per_s` steps, its four wavefronts in turn.
+// Long caches.  A workgroup takes `per_s` steps, its four wavefronts in turn.  24 sequences of 300 .. 8192 rows, 8 x 128
+// in 8 bits: 20 us for 64 MB (3.2 TB/s), the weights and V 25 us for as much; two steps' rows in flight a wavefront
+// 29 (fewer wavefronts), 4 or 16 steps a workgroup 21.5.
 template <uint32_t HD, bool I8>
 __global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
     typedef Few<HD, I8> F;
@@ -1926,12 +1930,22 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     if ((uint64_t)b.tokens * G > 0x7FFFFFFFu)
         return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
     const Attn a{q, o, q_ld, o_ld, G, window, fp, smx};
-    // Few rows a sequence: tiles of 15 rows, in one launch for short caches, with kept scores for long ones (where those
-    // fit kMaxScores); otherwise tiles of 64 or 128 rows that compute the scores twice
-    const uint64_t rows = (uint64_t)b.tokens * heads;
-    const bool few = (uint64_t)b.tokens * G < 32u * (uint64_t)b.batch && (b.cap <= kShort || rows * b.cap * 2 <= kMaxScores);
-    const uint32_t R = few ? kFewRows : cache->head_dim == 64 ? 128 : 64;
-    const uint64_t slots = (uint64_t)b.tokens * G / R + b.batch;
+    // Tiles of 15 rows in one launch (tables of at most kShort rows), tiles of 15 rows whose scores are kept (where those
+    // fit kMaxScores), or tiles of 64 or 128 rows that compute the scores twice: the least of three estimates in ns, from
+    // the tiles' count for sequences of equal rows, fitted to these (15 + 5 heads of 64, us of few and of many): 16
+    // sequences of 1024 rows, 1 / 16 / 32 tokens each 11.4 / 29 / 45 and 37 / 41 / 43; of 4096, 8 / 12 / 16 tokens
+    // 48 / 63 / 84 and 75 / 78 / 76; one of 1000, 40 tokens 12.6 and 27.7; one of 200, 100 tokens 8.5 and 31; one of 4000,
+    // 20 tokens 21 and 36.
+    const uint64_t rows = (uint64_t)b.tokens * heads, packed = (uint64_t)b.tokens * G, each = (packed + b.batch - 1) / b.batch;
+    const uint32_t steps = (b.cap + 63) / 64, big = cache->head_dim == 64 ? 128 : 64, wide = cache->head_dim / 64;
+    auto tiles_of = [&](uint32_t r) { return (each + r - 1) / r * b.batch * c.kv; };
+    const uint64_t many_ns = 27000 + tiles_of(big) * steps * (cache->int8 ? 11 : 19) / 2;
+    const uint64_t rounds = ((packed / kFewRows + b.batch) * c.kv + st->cus - 1) / st->cus;
+    const uint64_t few_ns = b.cap <= kShort ? rounds * (6500 + 8 * b.cap) * (wide + 1) / 2
+                                            : 8000 + tiles_of(kFewRows) * steps * wide * (cache->int8 ? 25 : 37) / 10;
+    const bool few = few_ns <= many_ns && (b.cap <= kShort || rows * b.cap * 2 <= kMaxScores);
+    const uint32_t R = few ? kFewRows : big;
+    const uint64_t slots = packed / R + b.batch;
     if (slots > 0x7FFFFFFFu) return fail(CM_EINVAL, "paged attention: %u tokens of %u heads", b.tokens, heads);
     const dim3 tiles((unsigned)slots, c.kv);
     if (few && b.cap <= kShort) {
@@ -1945,7 +1959,6 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
 #undef CM_SHORT
         return CM_OK;
     }
-    const uint32_t steps = (b.cap + 63) / 64;
     if (few) {
         // parts of equal steps: about four workgroups a compute unit, two steps a wavefront for the scores; a part of at
         // most kMaxPart keys (the int32 limb sums)

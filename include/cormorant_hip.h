@@ -488,7 +488,9 @@ typedef struct cm_paged_cache {
  * table[b table_ld + j / page] (device int32, max_pages entries a sequence, max_pages page <= 2^20).
  * Checked on the device: a page id outside the pool (or a position past max_pages) is not written,
  * and its rows are not attended to and read back as 0; a token at a negative position is not
- * written, attends to nothing and reads back as 0. */
+ * written, attends to nothing and reads back as 0; a negative kv_len counts as 0; q_start is held to 0 .. tokens (a
+ * q_start that falls gives unspecified rows of o and kv).  Sequences may share pages that no token of the call is
+ * written to.  The arrays may change between the replays of a captured call, max_pages and tokens not. */
 typedef struct cm_paged_batch {
     const int32_t *q_start, *kv_len, *table;
     uint32_t batch, tokens, max_pages;
@@ -499,7 +501,8 @@ size_t cm_paged_block_bytes(uint32_t page, uint32_t head_dim, uint32_t int8);
 
 /* What stands before a step's attention, in one launch.  For the token at position p, per head:
  *   y = x, or with norm_q / norm_k the row-ops NORM job (RMS, int16 in and out, rows of head_dim,
- *       the 16-byte parameter entries [head_dim], eps in 0 .. 2^61; ROWOPS_RTL_KERNEL.md section 1);
+ *       the 16-byte parameter entries [head_dim], Bq' added as it stands (bq_sh 0), eps in 0 .. 2^61;
+ *       ROWOPS_RTL_KERNEL.md section 1);
  *   z = the ROPE job's element rule over the head's first `rotary` columns (a multiple of 16) with
  *       row min(max(p, 0), rope_rows - 1) of `rope` (int32 cos [rotary] then sin [rotary] at 2^-23),
  *       the partner of column c being c +- rotary / 2 (interleaved 0) or c ^ 1 (interleaved 1), negated
@@ -532,7 +535,11 @@ int cm_paged_prep(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
  *   o_d = sat16(floor(2^(f_p - 8) sum_j w_j V_j,d / sum_j w_j + 1/2)), f_p = (smx_cfg >> 8) & 31 in 1 .. 15
  * with the sums exact: the scale of o is that of the unit's P . V at P's 2^-f_p, but P itself is never
  * rounded to f_p bits (at f_p = 14 a flat row of 16384 keys would have P = 1 of 16384).  A token that
- * attends to nothing gives zeros.  q / o rows q_ld / o_ld elements apart, 16-byte aligned; o apart from q. */
+ * attends to nothing gives zeros.  q / o rows q_ld / o_ld elements apart, 16-byte aligned; o apart from q.
+ * smx_cm 2^-shift is a scale (graph.softmax_regs); one whose 24-bit normalised form has a shift above 34 (weights that
+ * stay 1 over all 65536 score steps) is refused.  Calls of 32 or more rows (tokens times group) a sequence on average,
+ * or over tables of more than 2048 rows, keep maxima, scores and partial sums in the device's workspace: run such a
+ * call once before a stream captures it; calls on different streams of one device must not overlap. */
 int cm_paged_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, const int16_t* q, int16_t* o,
                        uint64_t q_ld, uint64_t o_ld, uint32_t heads, uint32_t window, uint32_t smx_cm,
                        uint32_t smx_cfg, void* stream);
