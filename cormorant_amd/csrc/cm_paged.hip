@@ -638,7 +638,9 @@ __device__ __forceinline__ void store_out(int16_t* p, const Divide& q, const int
 // 64-key steps that any row of the tile sees go to workgroups in parts of `per` steps (the same for every tile: a short
 // sequence has fewer parts, not smaller ones).
 
-constexpr uint32_t kTileCost = 4;                 // what a tile of many rows costs beside its steps, in steps
+// What a tile of many rows costs beside its steps, in steps: its queries, maxima and first keys, its sums' end.  A prompt
+// of 4096 tokens: 1, 2, 3, 6 for 4 take 188, 183, 169, 168 us for 161.
+constexpr uint32_t kTileCost = 4;
 
 template <uint32_t R>
 struct Tile {
@@ -1220,6 +1222,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work 
 // weights and P.V with the scores computed again: a weight needs the final maximum (its shift drops bits, so a sum
 // over another maximum cannot be rescaled), and the scores of many rows are dearer to keep than to compute twice.
 //
+// Bound by the VALU at two wavefronts a SIMD (the accumulators' registers): a prompt of 4096 tokens of 15 + 5 heads of
+// 64 takes 45 us for the maxima, 120 for the weights and P.V and 14 for the join of the pieces, of which the byte
+// products are 13 and 26 at the matrix rate; without the exponentials' arithmetic the 120 are 89, without their table
+// reads 111, with one of P.V's four products 114, without the copies into LDS 115.  Tiles of 64 rows at three wavefronts
+// a SIMD: 123.  256 tokens on 4096 rows: 11 + 27 + 9, half of it the pieces' first loads and 33 MB of partial sums.
+//
 // LDS layouts.  K: row = key, its 16-byte chunks XORed by the key's place so that the 16 rows of a fragment (keys
 // 16 a + 4 kb + i) fall on 16 bank groups.  V: [plane][16-key group][d][16 bytes], a fragment's lanes consecutive.
 // Wavefront w copies the step's 16-key group w, of one page: a direct copy moves 1 KiB, lane l to 16 l (16 key rows,
@@ -1370,7 +1378,8 @@ struct Queue {
     int64_t* part;                         // [shares][2][R HD + R], in the lanes' order
     uint32_t slots, max_shares, shares;    // shares at most, both multiples of 8
 };
-constexpr uint32_t kMaxMin = 4, kRowsMin = 4;   // steps of a share, at least
+constexpr uint32_t kMaxMin = 4, kRowsMin = 4;   // steps of a share, at least: 6, 8, 12 for 4 in 256 tokens on 4096 rows
+                                                // 52, 49, 55 us for 47
 
 template <uint32_t R>
 struct PlanLds {                           // one workgroup's
