@@ -573,11 +573,17 @@ struct Exp2 {
     __device__ __forceinline__ uint32_t e0() const { return t0 >> k0; }
     __device__ __forceinline__ uint32_t e1() const { return t1 >> k1; }
 };
+// HALF: tab holds TAB - 1 in 16 bits
+template <bool HALF = false>
 __device__ __forceinline__ Exp2 exps(int s0, int s1, uint32_t m2, uint32_t dl2, const Smx& x, const int32_t* tab) {
     const u16x2 s = __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pk_i16(s0, s1));
     const u16x2 d = __builtin_elementwise_min(__builtin_bit_cast(u16x2, m2) - s, __builtin_bit_cast(u16x2, dl2));
-    const uint32_t y0 = __umulhi((uint32_t)d[0] << x.sh, x.mul), y1 = __umulhi((uint32_t)d[1] << x.sh, x.mul);
+    const uint32_t mul = HALF ? x.mul >> 1 : x.mul;        // its low 8 bits are 0
+    const uint32_t y0 = __umulhi((uint32_t)d[0] << x.sh, mul), y1 = __umulhi((uint32_t)d[1] << x.sh, mul);
     const uint8_t* tb = reinterpret_cast<const uint8_t*>(tab);
+    if constexpr (HALF)
+        return Exp2{*reinterpret_cast<const uint16_t*>(tb + (y0 & 0x1FFEu)) + 1u,
+                    *reinterpret_cast<const uint16_t*>(tb + (y1 & 0x1FFEu)) + 1u, y0 >> 13, y1 >> 13};
     return Exp2{*reinterpret_cast<const uint32_t*>(tb + (y0 & 0x3FFCu)), *reinterpret_cast<const uint32_t*>(tb + (y1 & 0x3FFCu)),
                 y0 >> 14, y1 >> 14};
 }
@@ -639,7 +645,7 @@ __device__ __forceinline__ void store_out(int16_t* p, const Divide& q, const int
 // sequence has fewer parts, not smaller ones).
 
 // What a tile of many rows costs beside its steps, in steps: its queries, maxima and first keys, its sums' end.  A prompt
-// of 4096 tokens: 1, 2, 3, 6 for 4 take 188, 183, 169, 168 us for 161.
+// of 4096 tokens: 3 and 6 for 4 take 169 and 168 us for 161 (the weights' kernel alone: 1 and 2 for 4, 140 and 135 for 120).
 constexpr uint32_t kTileCost = 4;
 
 template <uint32_t R>
@@ -782,6 +788,16 @@ __device__ __forceinline__ void stage_tab(int32_t* stab, const int32_t* tab) {
     for (uint32_t i = 0; i < 4; i++)
         __builtin_amdgcn_global_load_lds(tab + 4 * (t + 256 * i),
                                          (__attribute__((address_space(3))) void*)(stab + 4 * (64 * w + 256 * i)), 16, 0, 0);
+}
+
+// TAB - 1 in 16 bits (TAB is 32774 .. 65536)
+__device__ __forceinline__ void stage_tab_half(int32_t* stab, const int32_t* tab) {
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < 1024; i += 256) {
+        const int4 v = reinterpret_cast<const int4*>(tab)[i];
+        reinterpret_cast<uint2*>(stab)[i] = make_uint2((uint32_t)(v.x - 1) | (uint32_t)(v.y - 1) << 16,
+                                                       (uint32_t)(v.z - 1) | (uint32_t)(v.w - 1) << 16);
+    }
 }
 
 // ---------------------------------------------------------------- attention of few rows
@@ -1575,14 +1591,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
     typedef typename RW::S S;
     __shared__ __attribute__((aligned(1024))) uint8_t sm0[S::BYTES];
     __shared__ __attribute__((aligned(1024))) uint8_t sm1[S::BYTES];
-    __shared__ __attribute__((aligned(16))) int32_t stab[4096];
+    // int16 rows of 128 take 66 KB of stages: with TAB in 16 bits two workgroups fit a CU
+    constexpr bool HALF = HD == 128 && !I8;
+    __shared__ __attribute__((aligned(16))) int32_t stab[HALF ? 2048 : 4096];
     __shared__ int32_t vsum[NP][HD];
     __shared__ PlanLds<RW::R> spl;
     plan(spl, bt, a, qu);
     const Shares<RW::R> sh(qu, spl, c.kv, qu.shares, kRowsMin);
     const uint32_t id = sh.order(blockIdx.x);
     if (id == ~0u) return;
-    stage_tab(stab, tab);
+    if constexpr (HALF) stage_tab_half(stab, tab);
+    else stage_tab(stab, tab);
     for (uint64_t at = sh.first(id), stop = sh.first(id + 1); at < stop;) {
         const Piece pc(sh, at, stop);
         at = pc.next;
@@ -1659,8 +1678,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Cache c, Batch bt, A
 #pragma unroll
                         for (uint32_t r = 0; r < 4; r++)
                             z[r] = raw_sum<I8>(h[y & 1][r], md[y & 1][r], l[y & 1][r], es[y & 1], r, rw.qterm[qb]) >> 8;
-                        x[y & 1][0] = exps(z[0], z[1], m2[qb], dl2, a.smx, stab);
-                        x[y & 1][1] = exps(z[2], z[3], m2[qb], dl2, a.smx, stab);
+                        x[y & 1][0] = exps<HALF>(z[0], z[1], m2[qb], dl2, a.smx, stab);
+                        x[y & 1][1] = exps<HALF>(z[2], z[3], m2[qb], dl2, a.smx, stab);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     if (j >= 2) {
@@ -1944,14 +1963,16 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     // the tiles' count for sequences of equal rows, fitted to these (15 + 5 heads of 64, us of few and of many): 16
     // sequences of 1024 rows, 1 / 16 / 32 tokens each 11.4 / 29 / 45 and 37 / 41 / 43; of 4096, 8 / 12 / 16 tokens
     // 48 / 63 / 84 and 75 / 78 / 76; one of 1000, 40 tokens 12.6 and 27.7; one of 200, 100 tokens 8.5 and 31; one of 4000,
-    // 20 tokens 21 and 36.
+    // 20 tokens 21 and 36.  (16 + 4 heads of 128, int16 / int8) 16 of 4096, 8 tokens 90 / 70 and 69 / 55; 1 token in int8
+    // 39 and 53.
     const uint64_t rows = (uint64_t)b.tokens * heads, packed = (uint64_t)b.tokens * G, each = (packed + b.batch - 1) / b.batch;
     const uint32_t steps = (b.cap + 63) / 64, big = cache->head_dim == 64 ? 128 : 64, wide = cache->head_dim / 64;
     auto tiles_of = [&](uint32_t r) { return (each + r - 1) / r * b.batch * c.kv; };
-    const uint64_t many_ns = 27000 + tiles_of(big) * steps * (cache->int8 ? 11 : 19) / 2;
+    const uint64_t many_ns = 31000 + tiles_of(big) * steps * (cache->int8 ? 55 : 85) / 10;
     const uint64_t rounds = ((packed / kFewRows + b.batch) * c.kv + st->cus - 1) / st->cus;
     const uint64_t few_ns = b.cap <= kShort ? rounds * (6500 + 8 * b.cap) * (wide + 1) / 2
-                                            : 8000 + tiles_of(kFewRows) * steps * wide * (cache->int8 ? 25 : 37) / 10;
+                                            : wide == 1 ? 12000 + tiles_of(kFewRows) * steps * (cache->int8 ? 26 : 35) / 10
+                                                        : 26000 + tiles_of(kFewRows) * steps * (cache->int8 ? 37 : 50) / 10;
     const bool few = few_ns <= many_ns && (b.cap <= kShort || rows * b.cap * 2 <= kMaxScores);
     const uint32_t R = few ? kFewRows : big;
     const uint64_t slots = packed / R + b.batch;
