@@ -578,12 +578,11 @@ template <bool HALF = false>
 __device__ __forceinline__ Exp2 exps(int s0, int s1, uint32_t m2, uint32_t dl2, const Smx& x, const int32_t* tab) {
     const u16x2 s = __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pk_i16(s0, s1));
     const u16x2 d = __builtin_elementwise_min(__builtin_bit_cast(u16x2, m2) - s, __builtin_bit_cast(u16x2, dl2));
-    const uint32_t mul = HALF ? x.mul >> 1 : x.mul;        // its low 8 bits are 0
-    const uint32_t y0 = __umulhi((uint32_t)d[0] << x.sh, mul), y1 = __umulhi((uint32_t)d[1] << x.sh, mul);
+    const uint32_t y0 = __umulhi((uint32_t)d[0] << x.sh, x.mul), y1 = __umulhi((uint32_t)d[1] << x.sh, x.mul);
     const uint8_t* tb = reinterpret_cast<const uint8_t*>(tab);
     if constexpr (HALF)
-        return Exp2{*reinterpret_cast<const uint16_t*>(tb + (y0 & 0x1FFEu)) + 1u,
-                    *reinterpret_cast<const uint16_t*>(tb + (y1 & 0x1FFEu)) + 1u, y0 >> 13, y1 >> 13};
+        return Exp2{*reinterpret_cast<const uint16_t*>(tb + (y0 >> 1 & 0x1FFEu)) + 1u,
+                    *reinterpret_cast<const uint16_t*>(tb + (y1 >> 1 & 0x1FFEu)) + 1u, y0 >> 14, y1 >> 14};
     return Exp2{*reinterpret_cast<const uint32_t*>(tb + (y0 & 0x3FFCu)), *reinterpret_cast<const uint32_t*>(tb + (y1 & 0x3FFCu)),
                 y0 >> 14, y1 >> 14};
 }

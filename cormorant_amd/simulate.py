@@ -88,6 +88,7 @@ class Simulator:
         self._staging: Dict[tuple, torch.Tensor] = {}     # row-ops nodes' staging buffers
         self._plan = None                                  # MatMuls fed byte planes by their A's producer
         self._keep = None                                  # forward_raw's keep (None: every tensor)
+        self._batches: Dict[tuple, paged.PagedBatch] = {}
         self._planes_only_names = None                     # tensors only plane-path MatMuls read
         self._errors = None                                # residual statistics being collected
         for t in graph.input_tensors + graph.output_tensors:
@@ -155,6 +156,7 @@ class Simulator:
         tensor that only plane-path MatMuls read, as the byte planes its producer writes, is not
         written at all and is absent from the result."""
         self._keep = None if keep is None else set(keep)
+        self._batches = {}                          # the pass's PagedBatches, one for all the layers of a step
         raw: Dict[str, torch.Tensor] = dict(raw_inputs)
         nodes = self._graph.nodes
         fuse = self._errors is None                 # residual statistics read every node's own output
@@ -1471,11 +1473,11 @@ class Simulator:
         data = self._get(pool, raw).reshape(-1).view(torch.uint8)
         cache = paged.PagedCache(int(pool.shape[0]), sn.page, sn.kv_heads, sn.head_dim, sn.int8, data)
         tokens = int(sn.inputs[0].shape[0])
-        key = f"{qs.onnx_name},{kl.onnx_name},{tb.onnx_name},{tokens}#paged"
-        if key not in raw:
-            raw[key] = paged.PagedBatch(self._get(qs, raw).reshape(-1), self._get(kl, raw).reshape(-1),
-                                        self._get(tb, raw).reshape(tb.shape), tokens)
-        return cache, raw[key]
+        key = (qs.onnx_name, kl.onnx_name, tb.onnx_name, tokens)
+        if key not in self._batches:
+            self._batches[key] = paged.PagedBatch(self._get(qs, raw).reshape(-1), self._get(kl, raw).reshape(-1),
+                                                  self._get(tb, raw).reshape(tb.shape), tokens)
+        return cache, self._batches[key]
 
     def _paged_prep(self, sn: PagedPrepNode, raw) -> torch.Tensor:
         """The norms and rotations of q (into the output) and k, k and v into the pages, one launch."""

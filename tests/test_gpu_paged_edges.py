@@ -130,6 +130,20 @@ def test_prep_and_read_of_many_sequences(paged, int8):  # noqa: F811
     check_read(paged, c, cache, batch, pad=8)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hd,rotary,interleaved,cols,norm,amp,in_place", [
+    (64, 64, False, False, True, 400, False), (64, 32, True, True, True, 400, True), (128, 128, False, True, False, 40000, False),
+    (128, 64, False, False, True, 40000, True), (64, 64, True, False, False, 400, False), (128, 128, True, True, True, 3, False),
+])
+def test_prep_of_many_tokens(paged, hd, rotary, interleaved, cols, norm, amp, in_place, int8):  # noqa: F811
+    """5 passes a token, several passes and tokens a wavefront."""
+    rng = np.random.default_rng(hd + rotary)
+    kv, G = (4, 9) if hd == 64 else (4, 4)
+    c = Case(rng, [700, 40, 1, 300], [600, 40, 1, 290], kv=kv, G=G, hd=hd, page=32, int8=int8, tail=5)
+    cache, batch = check_prep(paged, c, rng, rotary, interleaved, cols, norm, amp=amp, in_place=in_place, pad=16)
+    check_read(paged, c, cache, batch)
+
+
 def test_two_captured_graphs_share_the_workspace(paged):  # noqa: F811
     """A graph of many rows and one of few over long tables, replayed in turn on one stream with other
     calls between them: each replay equal to its eager call."""

@@ -83,6 +83,14 @@ def test_softmax_registers(paged, way, cm, cs):  # noqa: F811
     check(paged, c, way, cm, cs | (14 << 8))
 
 
+@pytest.mark.parametrize("cm,cs", [(0, 20), (1, 0), (7, 0), ((1 << 24) - 1, 0), ((1 << 24) - 1, 7), (12345678, 8), (65535, 0),
+                                   (65536, 0), (69632, 0), (12102203, 31), (8388608, 34), (16777215, 34), (5, 13)])
+def test_many_rows_softmax_registers_128(paged, cm, cs):  # noqa: F811
+    """Int16 rows of 128: the exponential's table in 16 bits."""
+    c = Case(np.random.default_rng(cs), [70, 64], [50, 50], kv=4, hd=128, amp=2000)
+    check(paged, c, "many", cm, cs | (14 << 8))
+
+
 @pytest.mark.parametrize("way", ["short", "kept", "many"])
 def test_strided_rows(paged, way):  # noqa: F811
     n = 1 if way == "kept" else 50
