@@ -1091,7 +1091,7 @@ __global__ __launch_bounds__(1024) void paged_short_kernel(Cache c, Batch bt, At
 }
 
 // Long caches.  A workgroup takes `per_s` steps, its four wavefronts in turn.  24 sequences of 300 .. 8192 rows, 8 x 128
-// in 8 bits: 20 us for 64 MB (3.2 TB/s), the weights and V 25 us for as much; two steps' rows in flight a wavefront
+// in 8 bits: 20 us for 64 MB (3.2 TB/s), the weights and V 22.4 for as much; two steps' rows in flight a wavefront
 // 29 (fewer wavefronts), 4 or 16 steps a workgroup 21.5.
 template <uint32_t HD, bool I8>
 __global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
@@ -1140,21 +1140,27 @@ __device__ __forceinline__ int row_max(const Work& wk, uint64_t wrow, uint32_t p
     return sat16i(m >> 8);
 }
 
+// A round is four steps: each wavefront makes one step's weights (its byte operands meet in LDS, two rounds deep), then
+// takes a quarter of V's columns over all four, so that no sums meet and a part ends in its lanes' stores (a step a
+// wavefront, all columns, the sums joined by LDS atomics: 24.5; 16 sequences of 4096 rows in int16 47 us a call for 39).
+// Parts of about eight workgroups a compute unit: four 30, six 24, twelve 23.6.
 template <uint32_t HD, bool I8>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
+__global__ __launch_bounds__(256) void paged_few_kernel(Cache c, Batch bt, Attn a, Work wk, const int32_t* __restrict__ tab) {
     typedef Few<HD, I8> F;
+    typedef Block<HD, I8> B;
+    constexpr uint32_t NB = HD / 64, NP = I8 ? 3 : 2;          // column blocks a wavefront; byte operands of the weights
     __shared__ __attribute__((aligned(16))) int32_t stab[4096];
-    __shared__ FewSums<HD> sums;
+    __shared__ v4i ops[2][4][NP][64];
+    __shared__ int64_t wsum[4][16];
     const uint32_t z = blockIdx.z;
     const Tile<kFewRows> tl(bt, a, blockIdx.x);
     const uint32_t parts = tl.parts(wk.per);
     if (!tl.on || z >= parts) return;
     stage_tab(stab, tab);
-    sums.clear();
     const F f(c, bt, a, tl, blockIdx.y);
-    const uint32_t beg = z * wk.per + f.w, end = min((z + 1) * wk.per, tl.nt);
+    const uint32_t beg = z * wk.per, end = min((z + 1) * wk.per, tl.nt), g = f.g, w = f.w;
     auto load = [&](uint32_t i, uint32_t (&x)[8]) {
-        const uint32_t kg = tl.lo + 64 * i + 16 * f.g;
+        const uint32_t kg = tl.lo + 64 * i + 16 * g;
         uint4 s0 = make_uint4(0, 0, 0, 0), s1 = s0;
         if (f.mine && i < end && kg < bt.cap) {
             const uint4* sp = reinterpret_cast<const uint4*>(wk.sc + f.wrow * bt.cap + kg);
@@ -1164,42 +1170,93 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(Cache c, Batch bt, At
         x[0] = s0.x; x[1] = s0.y; x[2] = s0.z; x[3] = s0.w;
         x[4] = s1.x; x[5] = s1.y; x[6] = s1.z; x[7] = s1.w;
     };
-    uint32_t ido = f.id_own(beg, end), sw[8];
-    load(beg, sw);
-    typename F::VRows v;
-    f.load_v(beg, ido, v);                 // a wavefront without a step: block 0
-    const uint32_t m2 = twice((uint32_t)row_max(wk, f.wrow, tl.parts(wk.per_s), f.g)), dl2 = twice(a.smx.dlim);
+    v4i vh[4][NB], vl[4][I8 ? 1 : NB], es = {0, 0, 0, 0};
+    auto load_v = [&](uint32_t i, const uint32_t (&id)[4]) {   // past the end: block 0, not used
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t in = (tl.lo + 64 * (i + j) + 16 * g) & (c.page - 1);
+            const uint8_t *vb = f.block(id[j]), *vp = vb + B::v(c.page, 0) + (16 * NB * w + f.c16) * c.page + in;
+#pragma unroll
+            for (uint32_t m = 0; m < NB; m++) {
+                vh[j][m] = *reinterpret_cast<const v4i*>(vp + 16 * m * c.page);
+                if constexpr (!I8) vl[j][m] = *reinterpret_cast<const v4i*>(vp + (HD + 16 * m) * c.page);
+            }
+        }
+    };
+    auto load_e = [&](uint32_t i, uint32_t id) {               // the shifts of the wavefront's own step's keys
+        if constexpr (I8) es = *reinterpret_cast<const v4i*>(f.block(id) + B::ve(c.page) + ((tl.lo + 64 * i + 16 * g) & (c.page - 1)));
+    };
+    uint32_t id[4], sw[8];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) id[j] = f.id_own(beg + j, end);
+    uint32_t ido = f.id_own(beg + w, end);
+    load(beg + w, sw);
+    load_e(beg + w, ido);
+    load_v(beg, id);
+    const uint32_t m2 = twice((uint32_t)row_max(wk, f.wrow, tl.parts(wk.per_s), g)), dl2 = twice(a.smx.dlim);
     __builtin_amdgcn_s_waitcnt(0x0070);               // the TAB's copies
     __syncthreads();
-    typename F::Sums o;
+    v4i acc[3][NB];
 #pragma unroll
-    for (uint32_t m = 0; m < F::DB; m++) o.acc[0][m] = o.acc[1][m] = o.acc[2][m] = v4i{0, 0, 0, 0};
-    o.w = 0;
-    for (uint32_t i = beg; i < end; i += 4) {
-        const uint32_t no = f.id_own(i + 4, end);
-        uint32_t ns[8];
-        load(i + 4, ns);
-        typename F::VRows nv;
-        f.load_v(i + 4, no, nv);           // past the end: block 0, not used
-        f.values(i, ido, v, sw, m2, dl2, a.smx, stab, o);
-        v = nv;
-        ido = no;
+    for (uint32_t m = 0; m < NB; m++) acc[0][m] = acc[1][m] = acc[2][m] = v4i{0, 0, 0, 0};
+    uint32_t sum = 0;
+    for (uint32_t i = beg, buf = 0; i < end; i += 4, buf ^= 1) {
+        if (i + w < end) {
+            uint32_t wp[8];
+            f.weights(i + w, ido, sw, m2, dl2, a.smx, stab, wp, sum);
+            v4i p[NP];
+            f.operands(wp, es, p);
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) sw[k] = ns[k];
+            for (uint32_t x = 0; x < NP; x++) ops[buf][w][x][f.lane] = p[x];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) id[j] = f.id_own(i + 4 + j, end);
+        ido = f.id_own(i + 4 + w, end);
+        load(i + 4 + w, sw);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            if (i + j >= end) break;
+            v4i p[NP];
+#pragma unroll
+            for (uint32_t x = 0; x < NP; x++) p[x] = ops[buf][j][x][f.lane];
+#pragma unroll
+            for (uint32_t m = 0; m < NB; m++) F::pv(vh[j][m], vl[j][I8 ? 0 : m], p, acc[0][m], acc[1][m], acc[2][m]);
+        }
+        if (i + 4 < end) {
+            load_e(i + 4 + w, ido);
+            load_v(i + 4, id);
+        }
     }
-    if (beg < end) sums.template add<I8>(f, o);
+    int64_t ws = sum;
+    ws += (int64_t)ro::shfl64((uint64_t)ws, 16);
+    ws += (int64_t)ro::shfl64((uint64_t)ws, 32);
+    if (g == 0) wsum[w][f.c16] = ws;
     __syncthreads();
-    if (parts == 1) {
-        sums.template store<I8>(a, tl, blockIdx.y);
-        return;
+    const int64_t total = wsum[0][f.c16] + wsum[1][f.c16] + wsum[2][f.c16] + wsum[3][f.c16];
+    const Divide quot(total, a.fp);
+    int64_t* pp = wk.part + (f.wrow * wk.splits + z) * (HD + 2);
+#pragma unroll
+    for (uint32_t m = 0; m < NB; m++) {
+        const uint32_t d = 16 * (NB * w + m) + 4 * g;
+        int64_t x[4];
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) {
+            // in lane 15 V's sum, below 2^30
+            const int vs = I8 ? acc[0][m][r] : (int)((uint32_t)acc[0][m][r] * 256u + (uint32_t)acc[2][m][r]);
+            const int64_t v = __shfl(vs, 16 * g + kFewRows, 64);
+            x[r] = (int64_t)acc[0][m][r] * 65536 + (int64_t)acc[1][m][r] * 256 + acc[2][m][r] +
+                   (I8 ? v * (128 * 65793) : v * 32896 + 128 * total);
+        }
+        if (!f.mine) continue;
+        if (parts == 1) {
+            store_out(a.o + (uint64_t)(tl.q0 + f.row / a.G) * a.o_ld + (uint64_t)(f.head * a.G + f.row % a.G) * HD + d, quot, x);
+        } else {
+            *reinterpret_cast<longlong2*>(pp + d) = make_longlong2(x[0], x[1]);
+            *reinterpret_cast<longlong2*>(pp + d + 2) = make_longlong2(x[2], x[3]);
+        }
     }
-    const uint32_t rows = min(kFewRows, tl.rows - tl.row0);
-    for (uint32_t i = threadIdx.x; i < rows * (HD / 2); i += 256) {
-        const uint32_t r = i / (HD / 2), d = 2 * (i % (HD / 2));
-        int64_t* pp = wk.part + ((((uint64_t)blockIdx.y * bt.tokens + tl.q0) * a.G + tl.row0 + r) * wk.splits + z) * (HD + 2);
-        *reinterpret_cast<longlong2*>(pp + d) = make_longlong2(sums.template sum<I8>(r, d), sums.template sum<I8>(r, d + 1));
-        if (d == 0) pp[HD] = sums.w[r];
-    }
+    if (parts > 1 && f.mine && w == 0 && g == 0) pp[HD] = total;
 }
 
 // The parts' sums of a row added and divided: a wavefront per row, loads of four parts in flight.
@@ -1971,7 +2028,7 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     const uint64_t rounds = ((packed / kFewRows + b.batch) * c.kv + st->cus - 1) / st->cus;
     const uint64_t few_ns = b.cap <= kShort ? rounds * (6500 + 8 * b.cap) * (wide + 1) / 2
                                             : wide == 1 ? 12000 + tiles_of(kFewRows) * steps * (cache->int8 ? 26 : 35) / 10
-                                                        : 26000 + tiles_of(kFewRows) * steps * (cache->int8 ? 37 : 50) / 10;
+                                                        : 18000 + tiles_of(kFewRows) * steps * (cache->int8 ? 37 : 50) / 10;
     const bool few = few_ns <= many_ns && (b.cap <= kShort || rows * b.cap * 2 <= kMaxScores);
     const uint32_t R = few ? kFewRows : big;
     const uint64_t slots = packed / R + b.batch;
@@ -1989,9 +2046,9 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
         return CM_OK;
     }
     if (few) {
-        // parts of equal steps: about four workgroups a compute unit, two steps a wavefront for the scores; a part of at
+        // parts of equal steps: about eight workgroups a compute unit, two steps a wavefront for the scores; a part of at
         // most kMaxPart keys (the int32 limb sums)
-        const uint32_t wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20), want = std::max(4u * (uint32_t)st->cus / wgs, 1u);
+        const uint32_t wgs = (uint32_t)std::min<uint64_t>(slots * c.kv, 1u << 20), want = std::max(8u * (uint32_t)st->cus / wgs, 1u);
         const uint32_t per = std::min(std::max((steps + want - 1) / want, 4u), kMaxPart / 64), splits = (steps + per - 1) / per;
         const uint32_t per_s = std::min(per, 8u), splits_s = (steps + per_s - 1) / per_s;
         if (splits_s > 65535u) return fail(CM_EINVAL, "paged attention: %u parts", splits_s);
