@@ -14,6 +14,7 @@ they are given and enqueue on the current torch stream of the cache's device.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -45,7 +46,7 @@ class PagedCache:
         nbytes = pages * kv_heads * block_bytes(page, head_dim, self.int8)
         self.data = torch.zeros(nbytes, dtype=torch.uint8, device=device) if data is None else data
         _require(self.data, "PagedCache: data", torch.uint8, nbytes)
-        self.width, self.device = kv_heads * head_dim, self.data.device
+        self.width, self.device, self.index = kv_heads * head_dim, self.data.device, self.data.get_device()
         self._c = _lib.CmPagedCache(self.data.data_ptr(), pages, page, kv_heads, head_dim, int(self.int8))
         self._ref = ctypes.byref(self._c)
 
@@ -77,7 +78,7 @@ class PagedBatch:
 
 class PagedPrep:
     """A layer's rotation and norms: ``table`` int32 [positions][2 rotary] (cos then sin at 2^-23:
-    rowops_nodes.rope_table's rows, or with ``interleaved`` each angle on a pair of neighbouring
+    rowops_nodes.rope_table's rows; with ``interleaved`` its own, each angle on a pair of neighbouring
     columns), ``params_q`` / ``params_k`` the ROPE jobs' parameter bytes (one 16-byte entry, or one
     per column), ``norm_q`` / ``norm_k`` the per-head RMSNorms' entries [head_dim] (None: no norm)
     with ``eps_q`` / ``eps_k`` (rowops_nodes.norm_params, rms)."""
@@ -102,6 +103,7 @@ class PagedPrep:
                                           rope_k=params_k.data_ptr(), rope_q_cols=int(params_q.numel() != 16),
                                           rope_k_cols=int(params_k.numel() != 16), norm_q=ptr(norm_q),
                                           norm_k=ptr(norm_k), eps_q=self.eps_q, eps_k=self.eps_k)
+        self._tail = bytes(self._args)[_OPERANDS.size:]
         self._checked = None
 
     def _check(self, heads: int, kv_heads: int, head_dim: int) -> None:
@@ -117,9 +119,12 @@ class PagedPrep:
         self._checked = (heads, kv_heads, head_dim)
 
 
+_OPERANDS = struct.Struct("@4P4QI")         # cm_paged_prep_args up to heads: q, k, v, qr, their strides, heads
+
+
 def _rows(t: torch.Tensor, name: str, tokens: int, width: int) -> int:
     """The row stride of a [tokens][>= width] int16 operand (rows of contiguous columns)."""
-    if t.dtype != torch.int16 or not t.is_cuda:
+    if t.dtype is not torch.int16 or not t.is_cuda:
         raise ValueError(f"{name} must be a GPU int16 tensor")
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[0] < tokens or shape[1] < width or stride[1] != 1 and shape[1] > 1:
@@ -128,15 +133,15 @@ def _rows(t: torch.Tensor, name: str, tokens: int, width: int) -> int:
     return stride[0] if shape[0] > 1 else shape[1]
 
 
-def _on(cache: PagedCache, *devices: torch.device) -> int:
+def _on(cache: PagedCache, *on) -> int:
     """The current stream of the cache's device, which every operand must be on and which must be current."""
-    dev = cache.device
-    for d in devices:
-        if d != dev:
-            raise ValueError(f"the cache is on {dev}, an operand on {d}")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"the cache is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(dev.index)         # torch.cuda.current_stream() takes 2.8 us of a 10 us call
+    index = cache.index
+    for t in on:
+        if t.get_device() != index:
+            raise ValueError(f"the cache is on {cache.device}, an operand on {t.device}")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {cache.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(index)         # torch.cuda.current_stream() takes 2.8 us of a 10 us call
 
 
 def paged_prep(cache: PagedCache, batch: PagedBatch, prep: PagedPrep, q: torch.Tensor, k: torch.Tensor,
@@ -154,12 +159,9 @@ def paged_prep(cache: PagedCache, batch: PagedBatch, prep: PagedPrep, q: torch.T
         prep._check(heads, cache.kv_heads, hd)
     if q.data_ptr() == qr.data_ptr() and lds[0] != lds[3]:
         raise ValueError("paged_prep: qr is q at another stride")
-    stream = _on(cache, batch.device, prep.device, q.device, k.device, v.device, qr.device)
-    a = _lib.CmPagedPrepArgs.from_buffer_copy(prep._args)
-    a.q, a.k, a.v, a.qr = q.data_ptr(), k.data_ptr(), v.data_ptr(), qr.data_ptr()
-    a.q_ld, a.k_ld, a.v_ld, a.qr_ld = lds
-    a.heads = heads
-    _lib.check(_lib.lib().cm_paged_prep(cache._ref, batch._ref, ctypes.byref(a), stream), "cm_paged_prep")
+    stream = _on(cache, batch.kv_len, prep.table, q, k, v, qr)
+    a = _OPERANDS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), qr.data_ptr(), *lds, heads) + prep._tail
+    _lib.check(_lib.lib().cm_paged_prep(cache._ref, batch._ref, a, stream), "cm_paged_prep")
     return qr
 
 
@@ -173,7 +175,7 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: to
     if heads < 1 or heads % cache.kv_heads or window < 0:
         raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window}")
     q_ld, o_ld = _rows(q, "q", n, heads * hd), _rows(o, "o", n, heads * hd)
-    stream = _on(cache, batch.device, q.device, o.device)
+    stream = _on(cache, batch.kv_len, q, o)
     _lib.check(_lib.lib().cm_paged_attention(cache._ref, batch._ref, q.data_ptr(), o.data_ptr(), q_ld, o_ld, heads,
                                              window, smx_cm & 0xFFFFFFFF, smx_cfg & 0xFFFFFFFF, stream),
                "cm_paged_attention")
@@ -184,7 +186,7 @@ def paged_read(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.T
     """cm_paged_read: the cache rows of the batch's tokens as int16 rows k / v [tokens][kv_heads hd]."""
     n = batch.tokens
     lds = _rows(k, "k", n, cache.width), _rows(v, "v", n, cache.width)
-    stream = _on(cache, batch.device, k.device, v.device)
+    stream = _on(cache, batch.kv_len, k, v)
     _lib.check(_lib.lib().cm_paged_read(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), *lds, stream),
                "cm_paged_read")
 

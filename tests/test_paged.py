@@ -143,3 +143,12 @@ def test_oracle_quantise_and_pool():
                     codes, e = O.quantise(x)
                     x = codes << e
                 np.testing.assert_array_equal(x, y)
+
+
+def test_prep_operands_pack_as_the_structure(lib):
+    """paged_prep packs the call's operands itself: the structure's leading fields, byte for byte."""
+    from cormorant_amd import _lib as L
+    from cormorant_amd import paged as P
+    a = L.CmPagedPrepArgs(q=1, k=2, v=3, qr=1 << 40, q_ld=5, k_ld=6, v_ld=7, qr_ld=1 << 33, heads=9)
+    assert bytes(a)[:P._OPERANDS.size] == P._OPERANDS.pack(1, 2, 3, 1 << 40, 5, 6, 7, 1 << 33, 9)
+    assert L.CmPagedPrepArgs.heads.offset + L.CmPagedPrepArgs.heads.size == P._OPERANDS.size
