@@ -886,26 +886,7 @@ struct Few {
             out[2 * kb + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_i16(x[2] >> 8, x[3] >> 8));
         }
     }
-    // the weights of those scores and their products with V
-    struct Sums {
-        v4i acc[3][DB];
-        uint32_t w;                         // the lane's weights: below 2^16 * 16 * kMaxPart / 64
-    };
-    struct VRows {                          // the V operands of a step and the lane's keys' shifts
-        v4i h[DB], l[DB], es;
-    };
-    __device__ __forceinline__ void load_v(uint32_t i, uint32_t ido, VRows& v) const {
-        const uint32_t in = (tl.lo + 64 * i + 16 * g) & (c.page - 1);
-        const uint8_t *vb = block(ido), *vp = vb + B::v(c.page, 0) + c16 * c.page + in;
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) {
-            v.h[m] = *reinterpret_cast<const v4i*>(vp + 16 * m * c.page);
-            if constexpr (!I8) v.l[m] = *reinterpret_cast<const v4i*>(vp + (HD + 16 * m) * c.page);
-        }
-        if constexpr (I8) v.es = *reinterpret_cast<const v4i*>(vb + B::ve(c.page) + in);
-        else v.es = v4i{0, 0, 0, 0};
-    }
-    // the weights of step i's scores in pairs, and their sum on top of sum
+    // the weights of step i's scores in pairs, and their sum on top of sum (a lane's: below 2^16 * 16 * kMaxPart / 64)
     __device__ __forceinline__ void weights(uint32_t i, uint32_t ido, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2, const Smx& smx,
                                             const int32_t* stab, uint32_t (&wp)[8], uint32_t& sum) const {
         const uint32_t kg = tl.lo + 64 * i + 16 * g;
@@ -938,15 +919,6 @@ struct Few {
             a1 = mfma(vl, p[1], a1);
         }
     }
-    __device__ __forceinline__ void values(uint32_t i, uint32_t ido, const VRows& v, const uint32_t (&sw)[8], uint32_t m2, uint32_t dl2,
-                                           const Smx& smx, const int32_t* stab, Sums& o) const {
-        uint32_t wp[8];
-        weights(i, ido, sw, m2, dl2, smx, stab, wp, o.w);
-        v4i p[I8 ? 3 : 2];
-        operands(wp, v.es, p);
-#pragma unroll
-        for (uint32_t m = 0; m < DB; m++) pv(v.h[m], v.l[m], p, o.acc[0][m], o.acc[1][m], o.acc[2][m]);
-    }
 };
 
 // The workgroup's sums of a tile: products [row][d] (the bytes' offsets out), weights [row], V's [d].
@@ -976,12 +948,6 @@ struct FewSums {
             if (f.mine) put(&part[f.c16][d], hh * 65536 + mid * 256 + ll);
             else if (f.c16 == kFewRows) put(&v[d], I8 ? hh : hh * 256 + ll);
         }
-    }
-    template <bool I8>
-    __device__ __forceinline__ void add(const Few<HD, I8>& f, const typename Few<HD, I8>::Sums& o) {
-        add_w<I8>(f, o.w);
-#pragma unroll
-        for (uint32_t m = 0; m < HD / 16; m++) add_v<I8>(f, m, o.acc[0][m], o.acc[1][m], o.acc[2][m]);
     }
     template <bool I8>
     __device__ __forceinline__ int64_t sum(uint32_t r, uint32_t d) const {

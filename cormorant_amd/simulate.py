@@ -9,7 +9,7 @@ conversion happens once at the graph's inputs, weights and returned tensors.
 """
 from __future__ import annotations
 
-from typing import Dict, Iterable, Optional
+from typing import Dict, Iterable, List, Optional
 
 import numpy as np
 import torch
@@ -86,9 +86,12 @@ class Simulator:
         self._infos: Dict[str, TensorInfo] = {}
         self._params: Dict[int, list] = {}                # row-ops parameter blocks on the device
         self._staging: Dict[tuple, torch.Tensor] = {}     # row-ops nodes' staging buffers
+        self._private = None                               # _step_private's set
         self._plan = None                                  # MatMuls fed byte planes by their A's producer
         self._keep = None                                  # forward_raw's keep (None: every tensor)
-        self._batches: Dict[tuple, paged.PagedBatch] = {}
+        self._batches: Dict[tuple, paged.PagedBatch] = {}  # a pass's, one for all the layers of a step
+        self._shared: Dict[tuple, torch.Tensor] = {}       # a pass's rows that the layers' paged nodes write in turn
+        self._passing: List[str] = []                      # the tensors in them
         self._planes_only_names = None                     # tensors only plane-path MatMuls read
         self._errors = None                                # residual statistics being collected
         for t in graph.input_tensors + graph.output_tensors:
@@ -156,7 +159,7 @@ class Simulator:
         tensor that only plane-path MatMuls read, as the byte planes its producer writes, is not
         written at all and is absent from the result."""
         self._keep = None if keep is None else set(keep)
-        self._batches = {}                          # the pass's PagedBatches, one for all the layers of a step
+        self._batches, self._shared, self._passing = {}, {}, []
         raw: Dict[str, torch.Tensor] = dict(raw_inputs)
         nodes = self._graph.nodes
         fuse = self._errors is None                 # residual statistics read every node's own output
@@ -213,6 +216,8 @@ class Simulator:
                 i += 1
                 continue
             self._dispatch(sn, raw)
+        for name in self._passing:                  # overwritten by the next layer's: absent from the result
+            raw.pop(name, None)
         return raw
 
     def _dispatch(self, sn, raw: Dict[str, torch.Tensor]) -> None:
@@ -1479,6 +1484,35 @@ class Simulator:
                                                   self._get(tb, raw).reshape(tb.shape), tokens)
         return cache, self._batches[key]
 
+    def _paged_rows(self, sn) -> torch.Tensor:
+        """The output rows of a paged node, zeros behind the last sequence (the calls leave those rows alone): where
+        the caller does not read the tensor, one buffer for the layers in turn, filled once."""
+        t = sn.output
+
+        def zeros():
+            return torch.zeros([int(d) for d in t.shape], dtype=torch.int16, device=self.device)
+        if self._keep is None or t.onnx_name in self._keep or any(t is o for o in self._graph.output_tensors) or \
+                t.onnx_name not in self._step_private():
+            return zeros()
+        key = (type(sn), tuple(t.shape)) + tuple(u.onnx_name for u in sn.inputs[-3:])
+        if key not in self._shared:
+            self._shared[key] = zeros()
+        self._passing.append(t.onnx_name)
+        return self._shared[key]
+
+    def _step_private(self) -> set:
+        """The paged nodes' outputs that only the node behind them reads: overwritten safely by the next layer's."""
+        if self._private is None:
+            nodes, readers = self._graph.nodes, {}
+            for i, sn in enumerate(nodes):
+                for u in sn.inputs:
+                    if u is not None:
+                        readers.setdefault(u.onnx_name, []).append(i)
+            self._private = {sn.output.onnx_name for i, sn in enumerate(nodes)
+                             if isinstance(sn, (PagedPrepNode, PagedAttentionNode)) and readers.get(sn.output.onnx_name) == [i + 1]
+                             and not isinstance(nodes[i + 1], ReshapeNode)}
+        return self._private
+
     def _paged_prep(self, sn: PagedPrepNode, raw) -> torch.Tensor:
         """The norms and rotations of q (into the output) and k, k and v into the pages, one launch."""
         q, k, v = (self._get(t, raw).reshape(t.shape) for t in sn.inputs[:3])
@@ -1489,7 +1523,7 @@ class Simulator:
                                    sn.interleaved, dev(sn.norm_q), dev(sn.norm_k), sn.eps_q, sn.eps_k)
             self._params[id(sn)] = prep
         cache, batch = self._paged(sn, raw)
-        return paged.paged_prep(cache, batch, prep, q, k, v, torch.zeros_like(q))
+        return paged.paged_prep(cache, batch, prep, q, k, v, self._paged_rows(sn))
 
     def _paged_attention(self, sn: PagedAttentionNode, raw) -> torch.Tensor:
         qt, ot = sn.inputs[0], sn.output
@@ -1499,7 +1533,7 @@ class Simulator:
             raise SchedulerError(f"{what}: the output exponent is not f_p + f_v - {self._dtype.frac_bits}")
         q = self._get(qt, raw).reshape(qt.shape)
         cache, batch = self._paged(sn, raw)
-        return paged.paged_attention(cache, batch, q, torch.zeros_like(q), sn.heads, sn.cm, sn.cfg, sn.window)
+        return paged.paged_attention(cache, batch, q, self._paged_rows(sn), sn.heads, sn.cm, sn.cfg, sn.window)
 
     def _kv_write(self, sn: KvWriteNode, raw) -> torch.Tensor:
         """Row ``pos`` of every sequence's group-major cache from the step's rows, in place."""

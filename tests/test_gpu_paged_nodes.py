@@ -61,6 +61,23 @@ def test_serving_steps(torch_gpu, int8, window):
             np.testing.assert_array_equal(st[nm], ref[nm], err_msg=f"step {step}: {nm}")
 
 
+def test_lean_pass(torch_gpu):
+    """A pass whose caller reads the output alone (the layers' rows in one buffer): h and the pools as in a
+    pass that keeps every tensor, padded rows among them; a kept row tensor is its layer's own."""
+    from cormorant_amd.simulate import Simulator
+    w = models.smollm2_weights(SHAPE, 3)
+    exps = models.smollm2_decode(SHAPE, seed=3, weights=w)[2]
+    g = models.smollm2_paged(SHAPE, 30, 2, 8, 16, 3, exps, w)
+    sim = Simulator(g)
+    f = feeds(np.random.default_rng(1).integers(0, SHAPE.vocab, 30), [18, 9], [18, 9], [[3, 1, 6], [0, 7, 2]])
+    every = sim._forward_pass(f)
+    dev = {nm: sim._to_device(sim._tensor(nm), v) for nm, v in {**f, **sim.initial_states()}.items()}
+    raw = sim.forward_raw(dict(dev), keep=["l1.h", "l0.om"])
+    assert "l0.om" in raw and not {"l0.qr", "l1.qr", "l1.om"} & set(raw)
+    for nm in ("l1.h", "l0.om", "l0.pool", "l1.pool"):
+        np.testing.assert_array_equal(sim._to_values(sim._tensor(nm), raw[nm]), every[nm])
+
+
 def layer(T, B, H, KV, HD, rotary, interleaved, norm, int8, page=16, max_pages=4, pages=11):
     """A prep and the attention of its rows as a graph."""
     fq, fk, fv = 11, 10, 9
