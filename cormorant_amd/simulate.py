@@ -218,6 +218,7 @@ class Simulator:
             self._dispatch(sn, raw)
         for name in self._passing:                  # overwritten by the next layer's: absent from the result
             raw.pop(name, None)
+        self._batches, self._shared, self._passing = {}, {}, []
         return raw
 
     def _dispatch(self, sn, raw: Dict[str, torch.Tensor]) -> None:
@@ -1475,7 +1476,7 @@ class Simulator:
     def _paged(self, sn, raw):
         """The cache and batch of a paged node (one PagedBatch for all the layers of a pass)."""
         pool, qs, kl, tb = sn.inputs[-4:]
-        data = self._get(pool, raw).reshape(-1).view(torch.uint8)
+        data = self._get(pool, raw).view(-1).view(torch.uint8)     # written in place: never a copy
         cache = paged.PagedCache(int(pool.shape[0]), sn.page, sn.kv_heads, sn.head_dim, sn.int8, data)
         tokens = int(sn.inputs[0].shape[0])
         key = (qs.onnx_name, kl.onnx_name, tb.onnx_name, tokens)
