@@ -166,7 +166,9 @@ struct Chunk {
     __device__ __forceinline__ Chunk(const Batch& bt, uint32_t slot) {
         b = find_le(bt.batch, slot, [&](uint32_t i) { return bt.start(i) / 64 + 2 * i; });
         q0 = bt.start(b);
-        const int n = max((int)bt.start(b + 1) - (int)q0, 0), len = bt.len(b);
+        // A length past 2^30 stands for any past the table (2^20 rows at most): the places below stay within int32 whatever
+        // kv_len holds (a length near 2^31 with more than a table's rows of padding wrapped to places outside q, k and v).
+        const int n = max((int)bt.start(b + 1) - (int)q0, 0), len = min(bt.len(b), 1 << 30);
         base = len - n;
         const int ci = (int)(slot - (q0 / 64 + 2 * b));
         at = (base >> 6) * 64 + 64 * ci;
