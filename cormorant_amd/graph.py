@@ -339,8 +339,8 @@ class PagedAttentionNode(KernelNode):
         if list(q.shape) != [int(q.shape[0]), self.heads * self.head_dim] or list(self.output.shape) != list(q.shape):
             raise SchedulerError(f"{what}: q {list(q.shape)} -> o {list(self.output.shape)}")
         check_paged(what, self)
-        if self.window < 0:
-            raise SchedulerError(f"{what}: window {self.window}")
+        if not 0 <= self.window < 1 << 30:
+            raise SchedulerError(f"{what}: window {self.window} (0, or below 2^30)")
 
 
 def paged_pool(name: str, pages: int, page: int, kv_heads: int, head_dim: int, int8: bool = False) -> TensorInfo:

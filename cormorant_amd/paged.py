@@ -172,8 +172,8 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: to
     unit's registers (graph.softmax_regs), o at 2^-(f_p + f_v - 8) as the unit's P . V.  Long tables and many
     rows use the device's workspace: one such call at a time a device, and once before a capture."""
     n, hd = batch.tokens, cache.head_dim
-    if heads < 1 or heads % cache.kv_heads or window < 0:
-        raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window}")
+    if heads < 1 or heads % cache.kv_heads or not 0 <= window < 1 << 30:       # the ABI's word would drop bits from 2^32 on
+        raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window} (below 2^30)")
     q_ld, o_ld = _rows(q, "q", n, heads * hd), _rows(o, "o", n, heads * hd)
     stream = _on(cache, batch.kv_len, q, o)
     _lib.check(_lib.lib().cm_paged_attention(cache._ref, batch._ref, q.data_ptr(), o.data_ptr(), q_ld, o_ld, heads,

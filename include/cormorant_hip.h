@@ -529,7 +529,7 @@ int cm_paged_prep(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
 
 /* The causal attention of the batch's tokens over their sequences' cache rows (the tokens' own among
  * them), `heads` query heads in groups of heads / kv_heads per KV head.  For the token at position p and
- * keys j in max(0, p - window + 1) .. p (window 0: from 0):
+ * keys j in max(0, p - window + 1) .. p (window below 2^30; 0: from 0):
  *   s_j = sat16(wrap32(sum_d q_d K_j,d) >> 8)                      (the Matmul unit's pow2 arithmetic)
  *   w_j = min(e_j, 65535), e_j the softmax unit's exponential of max s - s_j (smx_cm, smx_cfg's shift)
  *   o_d = sat16(floor(2^(f_p - 8) sum_j w_j V_j,d / sum_j w_j + 1/2)), f_p = (smx_cfg >> 8) & 31 in 1 .. 15

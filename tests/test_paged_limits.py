@@ -1,0 +1,20 @@
+"""What the paged cache's Python layer refuses before a C type could drop bits of it, without a GPU."""
+from types import SimpleNamespace
+
+import pytest
+
+from cormorant_amd import paged as P
+from cormorant_amd.graph import PagedAttentionNode, SchedulerError, TensorInfo, paged_pool
+
+
+@pytest.mark.parametrize("window", [-1, 1 << 30, 1 << 32, (1 << 32) + 5, 1 << 64])
+def test_windows(window):
+    """A window of 2^32 + 5 keys would reach the library as one of 5."""
+    cache, batch = SimpleNamespace(kv_heads=2, head_dim=64), SimpleNamespace(tokens=1)
+    with pytest.raises(ValueError, match="window"):
+        P.paged_attention(cache, batch, None, None, 4, 1 << 23, 20 | 14 << 8, window=window)
+    T = TensorInfo
+    ins = [T("q", [4, 128], exp=8), paged_pool("pool", 4, 16, 1, 64), T("qs", [3], kind="i32"), T("kl", [2], kind="i32"),
+           T("tb", [2, 2], kind="i32")]
+    with pytest.raises(SchedulerError, match="window"):
+        PagedAttentionNode(ins, T("o", [4, 128], exp=8), heads=2, kv_heads=1, head_dim=64, page=16, window=window)
