@@ -86,6 +86,8 @@ class PagedPrep:
     def __init__(self, table: torch.Tensor, params_q: torch.Tensor, params_k: torch.Tensor, interleaved: bool = False,
                  norm_q: Optional[torch.Tensor] = None, norm_k: Optional[torch.Tensor] = None, eps_q: int = 0,
                  eps_k: int = 0):
+        if not (0 <= eps_q <= 1 << 61 and 0 <= eps_k <= 1 << 61):            # the ABI's words would drop bits from 2^63 on
+            raise ValueError(f"PagedPrep: eps {eps_q}, {eps_k} outside 0 .. 2^61")
         if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 32 or table.shape[1] % 32:
             raise ValueError("PagedPrep: a table [positions][2 rotary], rotary a multiple of 16")
         _require(table, "PagedPrep: table", torch.int32, 2)

@@ -18,3 +18,13 @@ def test_windows(window):
            T("tb", [2, 2], kind="i32")]
     with pytest.raises(SchedulerError, match="window"):
         PagedAttentionNode(ins, T("o", [4, 128], exp=8), heads=2, kv_heads=1, head_dim=64, page=16, window=window)
+
+
+@pytest.mark.parametrize("eps", [-1, (1 << 61) + 1, 1 << 63, (1 << 64) + 5])
+def test_eps(eps):
+    """An eps of 2^64 + 5 would reach the library as 5."""
+    import torch
+    table, entry = torch.zeros(4, 32, dtype=torch.int32), torch.zeros(16, dtype=torch.uint8)
+    for kw in (dict(eps_q=eps), dict(eps_k=eps)):
+        with pytest.raises(ValueError, match="eps"):
+            P.PagedPrep(table, entry, entry, **kw)
