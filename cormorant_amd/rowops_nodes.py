@@ -12,6 +12,7 @@ reference's ``reference()`` of the node bit for bit.
 """
 from __future__ import annotations
 
+import hashlib
 import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
@@ -171,6 +172,14 @@ def rope_table(cos, sin, interleaved: bool = False) -> np.ndarray:
     both = (lambda t: np.repeat(t, 2, 1)) if interleaved else (lambda t: np.concatenate([t, t], 1))
     cr, sr = rope_tables_raw(both(cos).astype(np.float64), both(sin).astype(np.float64))
     return np.ascontiguousarray(np.concatenate([cr, sr], axis=1).astype(np.int32))
+
+
+def rope_tensor(tab: np.ndarray) -> TensorInfo:
+    """A rope_table as a constant tensor, named by what it holds: device constants are kept by name, one
+    for the layers of a graph and the entries that share its weights, and the entries' tables differ
+    (in their rows, a cache's context or a page table's; in their layout)."""
+    name = hashlib.blake2b(tab.tobytes(), digest_size=16).hexdigest()
+    return TensorInfo(f"rope_table_{tab.shape[0]}x{tab.shape[1]}_{name}", list(tab.shape), data=tab, kind="i32", raw=True)
 
 
 # ---------------------------------------------------------------- jobs
@@ -527,7 +536,7 @@ class RopeRoNode(RowOpsAdapter):
         self._span = 1 if self.same_pos else self.rows
         _require(tab.shape[1] == 2 * HD and 0 <= self.pos and self.pos + self._span <= tab.shape[0], what,
                  "cos / sin tables [C][HD/2] covering the rows' positions")
-        self.table = TensorInfo(f"{y.onnx_name}__rope_table", list(tab.shape), data=tab, kind="i32", raw=True)
+        self.table = rope_tensor(tab)
         self._params, self.bcast = pblock(0, 0, sa.reshape(-1), sb.reshape(-1), sc.reshape(-1), n)
 
     def jobs(self, pos: Optional[int] = None):
@@ -625,7 +634,7 @@ class PagedPrepNode(KernelNode):
         tab = rope_table(self.cos, self.sin, self.interleaved)
         _require(tab.shape[1] % 32 == 0 and tab.shape[1] <= 2 * HD, what, "cos / sin of rotary / 2 columns, rotary a "
                  "multiple of 16 up to the head dim")
-        self.table = TensorInfo(f"{self.output.onnx_name}__rope_table", list(tab.shape), data=tab, kind="i32", raw=True)
+        self.table = rope_tensor(tab)
         self.norm_q, self.eps_q, self.rope_q = self._params(self.gamma_q, fq, fo, what)
         self.norm_k, self.eps_k, self.rope_k = self._params(self.gamma_k, fk, self.f_k, what)
 
@@ -1040,5 +1049,6 @@ ADAPTERS = (LayerNormRoNode, LayerNorm32RoNode, RMSNormRoNode, ResAddRoNode, Res
 __all__ = ["RoJob", "RowOpsAdapter", "RoCall", "RoCallNode", "TransposeRoNode", "AttnPrepRoNode", "VitAttnPrepRoNode",
            "DecodePrepNode", "PagedPrepNode", "collapse",
            "transpose_job", "opword", "gamma_scale", "beta_bits", "bias_bits", "quant_bias", "bias_exp",
-           "bias_params", "norm_params", "param_block", "pblock", "rope_tables_raw", "rope_table"] + \
+           "bias_params", "norm_params", "param_block", "pblock", "rope_tables_raw", "rope_table",
+           "rope_tensor"] + \
           [c.__name__ for c in ADAPTERS]

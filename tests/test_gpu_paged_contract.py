@@ -42,3 +42,31 @@ def attends_to_the_table(P, c, lengths):
         cache, batch = c.device(P)
         P.paged_attention(cache, batch, q, out, c.heads, *regs(c.hd))
     assert torch.equal(o, want) and o[:c.new[0]].any()
+
+
+@pytest.mark.parametrize("first", ["decode", "paged", "wide"])
+def test_entries_that_share_weights(paged, first):  # noqa: F811
+    """A decode entry and paged entries over tables of 3 and 6 pages with one set of device weights, whichever comes first:
+    each one's pass is the oracle's."""
+    from cormorant_amd import models
+    from cormorant_amd.simulate import Simulator
+    from oracle import graph_sim as og
+    from test_gpu_paged_nodes import SHAPE, feeds, same
+    w = models.smollm2_weights(SHAPE, 3)
+    decode, inputs, exps = models.smollm2_decode(SHAPE, seed=3, weights=w, runtime_pos=True)
+    graphs = {"decode": decode, **{k: models.smollm2_paged(SHAPE, 9, 2, 14, 16, n, exps, w) for k, n in (("paged", 3), ("wide", 6))}}
+    rng = np.random.default_rng(2)
+    sims, held = {}, None
+    for k in sorted(graphs, key=lambda k: k != first):
+        g = graphs[k]
+        sims[k] = held = Simulator(g, share=held)
+        states = {t.onnx_name: np.zeros(t.shape) for t in g.state_tensors}
+        n = 0 if k == "decode" else int(g.input_tensors[-1].shape[1])
+        f = feeds(rng.integers(0, SHAPE.vocab, 9), [8, 1], [16 * n, 8 * n], rng.permutation(14)[:2 * n].reshape(2, n)) if n else \
+            {t.onnx_name: inputs[t.onnx_name] for t in g.input_tensors if t.onnx_name not in states}
+        ref = {nm: v.copy() for nm, v in states.items()}
+        print(f"{k} behind {first}", flush=True)
+        got, want = sims[k]._forward_pass(f, states=states), og.forward(g, f, states=ref)
+        same(got, want, k)
+        for nm in ref:
+            np.testing.assert_array_equal(states[nm], ref[nm], err_msg=f"{k}: {nm}")
