@@ -171,8 +171,9 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: to
                     smx_cfg: int, window: int = 0) -> torch.Tensor:
     """cm_paged_attention: the causal attention of the batch's tokens, q / o [tokens][heads hd], over
     their sequences' cache rows (the last ``window`` of them, 0: all); smx_cm / smx_cfg as the softmax
-    unit's registers (graph.softmax_regs), o at 2^-(f_p + f_v - 8) as the unit's P . V.  Long tables and many
-    rows use the device's workspace: one such call at a time a device, and once before a capture."""
+    unit's registers (graph.softmax_regs), o at 2^-(f_p + f_v - 8) as the unit's P . V.  Any call may use the
+    device's workspace: one at a time a device, and one of the same sizes before a capture.  The kernels are
+    chosen by the sizes (the table's width among them), not by the sequences' lengths."""
     n, hd = batch.tokens, cache.head_dim
     if heads < 1 or heads % cache.kv_heads or not 0 <= window < 1 << 30:       # the ABI's word would drop bits from 2^32 on
         raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window} (below 2^30)")

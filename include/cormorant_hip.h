@@ -537,9 +537,11 @@ int cm_paged_prep(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
  * rounded to f_p bits (at f_p = 14 a flat row of 16384 keys would have P = 1 of 16384).  A token that
  * attends to nothing gives zeros.  q / o rows q_ld / o_ld elements apart, 16-byte aligned; o apart from q.
  * smx_cm 2^-shift is a scale (graph.softmax_regs); one whose 24-bit normalised form has a shift above 34 (weights that
- * stay 1 over all 65536 score steps) is refused.  Calls of 32 or more rows (tokens times group) a sequence on average,
- * or over tables of more than 2048 rows, keep maxima, scores and partial sums in the device's workspace: run such a
- * call once before a stream captures it; calls on different streams of one device must not overlap. */
+ * stay 1 over all 65536 score steps) is refused.  Any call may keep maxima, scores and partial sums in the device's
+ * workspace, single tokens over short tables of many sequences among them: run a call of the same sizes once before a
+ * stream captures it; calls on different streams of one device must not overlap.  Which kernels run, and how much
+ * workspace they take, follows from tokens, batch, the heads and max_pages * page alone, never from the arrays'
+ * contents (nor from window): tables much wider than their sequences (above all past 2048 rows) take more launches. */
 int cm_paged_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, const int16_t* q, int16_t* o,
                        uint64_t q_ld, uint64_t o_ld, uint32_t heads, uint32_t window, uint32_t smx_cm,
                        uint32_t smx_cfg, void* stream);

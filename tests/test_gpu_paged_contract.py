@@ -70,3 +70,41 @@ def test_entries_that_share_weights(paged, first):  # noqa: F811
         same(got, want, k)
         for nm in ref:
             np.testing.assert_array_equal(states[nm], ref[nm], err_msg=f"{k}: {nm}")
+
+
+@pytest.mark.parametrize("hd,kv,G,batch,page,int8", [(128, 8, 4, 128, 64, True), (128, 8, 4, 128, 128, False), (64, 5, 3, 512, 64, False),
+                                                     (64, 8, 1, 512, 64, True)])
+def test_single_tokens_in_the_workspace(paged, hd, kv, G, batch, page, int8):  # noqa: F811
+    """Decode steps of many sequences over tables of one page: few rows a sequence, short tables, and yet the kernels that
+    share the device's workspace.  One call, then captured and replayed as the lengths change, beside other calls there."""
+    import torch
+    from cormorant_amd import _lib
+    from oracle import paged as O
+    rng = np.random.default_rng(batch + hd)
+    c = Case(rng, [int(x) for x in rng.integers(1, page + 1, batch)], [1] * batch, kv=kv, G=G, hd=hd, page=page, int8=int8)
+    other = Case(rng, [70], [50], kv=4)
+    q, oq = dev(c.q), dev(other.q)
+    o, oo = torch.zeros_like(q), torch.zeros_like(oq)
+    cache, step = c.device(paged)
+    beside = other.device(paged)
+    call = lambda: paged.paged_attention(cache, step, q, o, c.heads, *regs(hd))     # noqa: E731
+    _lib.timing_reset()
+    _lib.timing_enable(True)
+    try:
+        call()
+        assert _lib.timing_read("paged_rows_kernel")[1] == 1 and _lib.timing_read("paged_short_kernel")[1] == 0
+    finally:
+        _lib.timing_enable(False)
+        _lib.timing_reset()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call()
+    for i in range(3):
+        print(f"replay {i}", flush=True)
+        step.kv_len.copy_(dev(np.maximum(c.kv_len - 7 * i, 1).astype(np.int32)))
+        o.zero_()
+        graph.replay()
+        want = O.attend(c.pool, c.q_start, np.maximum(c.kv_len - 7 * i, 1), c.table, c.q, c.heads, *regs(hd))
+        np.testing.assert_array_equal(o.cpu().numpy(), want)
+        paged.paged_attention(*beside, oq, oo, other.heads, *regs())
