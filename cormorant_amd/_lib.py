@@ -52,6 +52,7 @@ SIGNATURES = {
     "cm_last_error": (ctypes.c_char_p, []),
     "cm_init": (_I32, []),
     "cm_host_act_table": (_I32, [_I32, _P]),
+    "cm_host_workspace_growth": (ctypes.c_size_t, [ctypes.c_size_t] * 2),
     "cm_host_rowops_table_image": (_I32, [_P]),
     "cm_act_table_init": (_I32, [_P]),
     "cm_rowops_tables_init": (_I32, [_P]),

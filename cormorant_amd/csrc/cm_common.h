@@ -71,9 +71,10 @@ int state(DeviceState** out);
 // The calling thread's current device if cm_init (or any earlier call) has prepared it;
 // CM_EINVAL otherwise.  Allocates nothing.
 int state_ready(DeviceState** out);
-// At least `bytes` of workspace on the current device.  Growth allocates a larger buffer and
-// keeps the old one until the process ends (work already queued, or a captured graph, may
-// still use it); it is refused (CM_EINVAL) while the stream `s` is capturing a graph.
+// At least `bytes` of workspace on the current device.  Growth allocates a buffer of at least
+// twice the size (cm_host_workspace_growth) and keeps the old one until the process ends (work
+// already queued, or a captured graph, may still use it); it is refused (CM_EINVAL) while the
+// stream `s` is capturing a graph.
 int workspace(DeviceState* st, size_t bytes, void** out, hipStream_t s);
 
 // A call's workspace: the grow-only buffer above (fixed == nullptr) or a fixed region of

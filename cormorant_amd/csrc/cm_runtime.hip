@@ -179,11 +179,15 @@ int workspace(DeviceState* st, size_t bytes, void** out, hipStream_t s) {
         if (cap != hipStreamCaptureStatusNone)
             return fail(CM_EINVAL, "workspace of %zu bytes needed while the stream captures a graph (%zu held): "
                                    "run the call once before the capture", bytes, st->ws_size);
-        size_t sz = round_up(bytes, (size_t)1 << 21);
+        size_t sz = cm_host_workspace_growth(st->ws_size, bytes);
         void* p = nullptr;
         if (hipMalloc(&p, sz) != hipSuccess) {
             (void)hipGetLastError();
-            return fail(CM_ENOMEM, "workspace of %zu bytes", sz);
+            sz = cm_host_workspace_growth(0, bytes);      // a device nearly full: what the call needs
+            if (hipMalloc(&p, sz) != hipSuccess) {
+                (void)hipGetLastError();
+                return fail(CM_ENOMEM, "workspace of %zu bytes", sz);
+            }
         }
         // the old buffer stays allocated: queued work and captured graphs may still use it
         if (st->ws) st->ws_retired.push_back(st->ws);
@@ -358,6 +362,12 @@ int cm_host_act_table(int act, int16_t* out65536) {
     cm::build_act_tables_full(full);
     std::memcpy(out65536, full[act - 4], sizeof(full[0]));
     return CM_OK;
+}
+
+// Outgrown buffers stay allocated, and a server's requests grow by a page at a time: each buffer at least doubles the one
+// before it, so that all the outgrown ones together are no larger than the one in use.
+size_t cm_host_workspace_growth(size_t held, size_t bytes) {
+    return cm::round_up(std::max(bytes, 2 * held), (size_t)1 << 21);
 }
 
 int cm_host_rowops_table_image(uint8_t* out65536) {

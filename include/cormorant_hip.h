@@ -15,7 +15,8 @@
  *     overlap on one device -- from two host threads, or queued on two streams whose work
  *     may run concurrently -- therefore race; order them (one stream, or events).
  *   - Workspace growth allocates (and keeps every outgrown buffer until the process ends,
- *     so graphs captured earlier stay valid); a call that would grow it while its stream
+ *     so graphs captured earlier stay valid; each buffer at least doubles the one before, so
+ *     the outgrown ones are together no larger); a call that would grow it while its stream
  *     captures a HIP graph fails with CM_EINVAL -- run that call once before the capture.
  *   - Return value: CM_OK (0) or a negative CM_E* status; cm_last_error() describes the
  *     last failure of the calling thread.  Nothing throws across the ABI.
@@ -57,6 +58,10 @@ int cm_init(void);
  * (rowops_spec.table_image, rowops_spec.py:605-616). */
 int cm_host_act_table(int act, int16_t* out65536);
 int cm_host_rowops_table_image(uint8_t* out65536);
+
+/* The bytes that a workspace of `held` bytes (0: none) grows to for a call that needs `bytes`, more than it holds (no
+ * device work): at least twice `held`. */
+size_t cm_host_workspace_growth(size_t held, size_t bytes);
 
 /* The current device's unit tables from the caller (the role of cm_act_table_init /
  * cm_rowops_tables_init in the boundary the reference's simulator mirrors; cm_init builds

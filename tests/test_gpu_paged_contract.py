@@ -108,3 +108,25 @@ def test_single_tokens_in_the_workspace(paged, hd, kv, G, batch, page, int8):  #
         want = O.attend(c.pool, c.q_start, np.maximum(c.kv_len - 7 * i, 1), c.table, c.q, c.heads, *regs(hd))
         np.testing.assert_array_equal(o.cpu().numpy(), want)
         paged.paged_attention(*beside, oq, oo, other.heads, *regs())
+
+
+def test_steps_over_growing_tables(paged):  # noqa: F811
+    """24 single tokens of 32 + 8 heads over tables that widen by a page at a time: the workspaces allocated on the way
+    stay within four of the last request (each at least doubles the one before; one twice the request at most)."""
+    import torch
+    B, kv, G, hd, page = 24, 8, 4, 128, 4096
+    heads = kv * G
+    cache = paged.PagedCache(1, page, kv, hd, int8=True)
+    q = torch.zeros((B, heads * hd), dtype=torch.int16, device="cuda")
+    o = torch.ones_like(q)
+    step = [dev(np.arange(B + 1, dtype=np.int32)), dev(np.full(B, 5, np.int32))]
+    tables = [dev(np.zeros((B, n), np.int32)) for n in range(8, 33)]
+    torch.cuda.synchronize()
+    before, last = torch.cuda.mem_get_info()[0], 0
+    for table in tables:
+        cap = table.shape[1] * page
+        paged.paged_attention(cache, paged.PagedBatch(*step, table, B), q, o, heads, *regs(hd))
+        last = B * heads * 2 * cap * 1.1        # the scores; the maxima and eight parts' sums are less than a tenth of them
+    torch.cuda.synchronize()
+    grown = before - torch.cuda.mem_get_info()[0]
+    assert not o.any() and grown <= 4 * last + (64 << 20), (grown, last)
