@@ -1492,8 +1492,8 @@ class Simulator:
 
         def zeros():
             return torch.zeros([int(d) for d in t.shape], dtype=torch.int16, device=self.device)
-        if self._keep is None or t.onnx_name in self._keep or any(t is o for o in self._graph.output_tensors) or \
-                t.onnx_name not in self._step_private():
+        if self._keep is None or t.onnx_name in self._keep or t.onnx_name not in self._step_private() or \
+                t.onnx_name in {o.onnx_name for o in self._graph.output_tensors}:
             return zeros()
         key = (type(sn), tuple(t.shape)) + tuple(u.onnx_name for u in sn.inputs[-3:])
         if key not in self._shared:

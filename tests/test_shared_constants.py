@@ -46,3 +46,21 @@ def test_one_copy_for_the_layers():
     for g in entries():
         sim = constants()
         assert len({sim._get(t, {}).data_ptr() for t in tables(g)}) == len(sim._weights) == 1
+
+
+def test_outputs_by_name_are_kept():
+    """A graph output described by a tensor of its own: forward_raw keeps the graph's outputs whatever ``keep`` holds, so a
+    paged node's rows of that name are not the layers' shared buffer."""
+    import torch
+    from cormorant_amd.graph import Graph
+    w = models.smollm2_weights(SHAPE, 3)
+    exps = models.smollm2_decode(SHAPE, seed=3, weights=w)[2]
+    g = models.smollm2_paged(SHAPE, 4, 2, 8, 16, 3, exps, w)
+    preps = [sn for sn in g.nodes if type(sn).__name__ == "PagedPrepNode"]
+    t = preps[0].output
+    own = TensorInfo(t.onnx_name, list(t.shape), exp=t.exp)
+    sim = object.__new__(Simulator)
+    sim.device, sim._private, sim._keep, sim._shared, sim._passing = torch.device("cpu"), None, set(), {}, []
+    sim._graph = Graph(g.nodes, input_tensors=g.input_tensors, output_tensors=g.output_tensors + [own])
+    rows = [sim._paged_rows(sn) for sn in preps]
+    assert sim._passing == [preps[1].output.onnx_name] and rows[0].data_ptr() != rows[1].data_ptr()
