@@ -185,7 +185,8 @@ inline uint64_t chunk_slots(const Batch& b) { return (uint64_t)b.tokens / 64 + 2
 // 2^53 (the norm's x Rm and P1 G, the rotation's two products; rounded by the sum with 1.5 2^52).  V: a chunk of 64
 // positions of a head, transposed through LDS and stored as whole 16-key pieces where all 16 are new.
 // 8192 tokens of 15 + 5 heads of 64 with norms: 31 us for 63 MB (2.0 TB/s, a copy's rate 5.2); without the norms'
-// arithmetic 23, without the rotation's 21, V's part alone 5.5: bound by the doubles at 2 wavefronts a SIMD.
+// arithmetic 23, without the rotation's 21, V's part alone 5.5: bound by the doubles at 2 wavefronts a SIMD (four passes
+// take 235 registers; 56 SGPRs go to vector lanes, no register to memory).
 template <uint32_t HD, bool I8, uint32_t PG>
 __global__ __launch_bounds__(256) void paged_prep_kernel(Cache c, Batch bt, Prep a, uint32_t qk_blocks, uint32_t passes, uint32_t tpw) {
     constexpr uint32_t L = HD / 8, RW = 64 / L;
@@ -973,7 +974,8 @@ struct FewSums {
 // steps (8 at 128 d): its sums are 12 registers, and 4 (2) of them meet in LDS instead of 16.  V's first round is read
 // beside K: one memory latency for both.  16 sequences of 1024 rows, 15 heads: 10.2 us
 // (V's columns undivided 11.5, with the three kernels of long caches 14.3), on 80 CUs: a CU reads 262 KB in 4 us, the
-// rest is the chain of launch, batch, page ids, K, maxima, V.
+// rest is the chain of launch, batch, page ids, K, maxima, V.  At 128 int16 columns 8 of the 128 registers that 16
+// wavefronts leave a lane spill.
 constexpr uint32_t kShort = 2048;
 
 template <uint32_t HD, bool I8>
@@ -1059,8 +1061,8 @@ __global__ __launch_bounds__(1024) void paged_short_kernel(Cache c, Batch bt, At
 }
 
 // Long caches.  A workgroup takes `per_s` steps, its four wavefronts in turn.  24 sequences of 300 .. 8192 rows, 8 x 128
-// in 8 bits: 20 us for 64 MB (3.2 TB/s), the weights and V 22.4 for as much; two steps' rows in flight a wavefront
-// 29 (fewer wavefronts), 4 or 16 steps a workgroup 21.5.
+// in 8 bits: 20 us for 64 MB (3.2 TB/s; 22 with the first, cold call among ten), the weights and V 22.5 (23) for as much;
+// two steps' rows in flight a wavefront 29 (fewer wavefronts), 4 or 16 steps a workgroup 21.5.
 template <uint32_t HD, bool I8>
 __global__ __launch_bounds__(256) void paged_scores_kernel(Cache c, Batch bt, Attn a, Work wk) {
     typedef Few<HD, I8> F;
@@ -1262,11 +1264,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Batch bt, Attn a, Work 
 // weights and P.V with the scores computed again: a weight needs the final maximum (its shift drops bits, so a sum
 // over another maximum cannot be rescaled), and the scores of many rows are dearer to keep than to compute twice.
 //
-// Bound by the VALU at two wavefronts a SIMD (the accumulators' registers): a prompt of 4096 tokens of 15 + 5 heads of
-// 64 takes 45 us for the maxima, 120 for the weights and P.V and 14 for the join of the pieces, of which the byte
-// products are 13 and 26 at the matrix rate; without the exponentials' arithmetic the 120 are 89, without their table
-// reads 111, with one of P.V's four products 114, without the copies into LDS 115.  Tiles of 64 rows at three wavefronts
-// a SIMD: 123.  256 tokens on 4096 rows: 11 + 27 + 9, half of it the pieces' first loads and 33 MB of partial sums.
+// Two wavefronts a SIMD (the accumulators' registers; the second kernel takes all 256 and spills 18 of them with int16
+// rows of 64, 12 with int16 rows of 128, 2 with int8 rows of 64, and 42 .. 50 SGPRs).  A prompt of 4096 tokens of 15 + 5
+// heads of 64 takes 45 us for the maxima, 121 for the weights and P.V and 14 for the join of the pieces; the byte products
+// of the first two are 13 and 26 at the matrix rate.  What the 121 lose, a part taken out at a time: the exponentials'
+// arithmetic 31, their table reads 9, the sums of the score limbs 10, the weights' sum 4, the weights' bytes 3, V's sums 3,
+// one of P.V's four products 6, the copies into LDS 5: 71 in all, the other seven products and the spilled registers not
+// among them; they have not been taken apart.  Tiles of 64 rows at three wavefronts a SIMD: 123.  256 tokens on 4096 rows:
+// 11 + 27 + 9, half of it the pieces' first loads and 33 MB of partial sums.
 //
 // LDS layouts.  K: row = key, its 16-byte chunks XORed by the key's place so that the 16 rows of a fragment (keys
 // 16 a + 4 kb + i) fall on 16 bank groups.  V: [plane][16-key group][d][16 bytes], a fragment's lanes consecutive.
@@ -1984,11 +1989,12 @@ int run_attention(const cm_paged_cache* cache, const cm_paged_batch* batch, cons
     const Attn a{q, o, q_ld, o_ld, G, window, fp, smx};
     // Tiles of 15 rows in one launch (tables of at most kShort rows), tiles of 15 rows whose scores are kept (where those
     // fit kMaxScores), or tiles of 64 or 128 rows that compute the scores twice: the least of three estimates in ns, from
-    // the tiles' count for sequences of equal rows, fitted to these (15 + 5 heads of 64, us of few and of many): 16
-    // sequences of 1024 rows, 1 / 16 / 32 tokens each 11.4 / 29 / 45 and 37 / 41 / 43; of 4096, 8 / 12 / 16 tokens
-    // 48 / 63 / 84 and 75 / 78 / 76; one of 1000, 40 tokens 12.6 and 27.7; one of 200, 100 tokens 8.5 and 31; one of 4000,
-    // 20 tokens 21 and 36.  (16 + 4 heads of 128, int16 / int8) 16 of 4096, 8 tokens 90 / 70 and 69 / 55; 1 token in int8
-    // 39 and 53.
+    // the tiles' count for sequences of equal rows.  They decide as the present kernels' times do, within 3 % (15 + 5 heads
+    // of 64, us of few and of many): 16 sequences of 1024 rows, 1 / 16 / 32 tokens each 11.5 / 29.5 / 45 and 38 / 41 / 43;
+    // of 4096, 8 / 12 / 16 tokens 47 / 65 / 81 and 74 / 74 / 73; one of 1000, 40 tokens 12.3 and 27; one of 200, 100 tokens
+    // 8.3 and 31; one of 4000, 20 tokens 18 and 36.  (16 + 4 heads of 128, int16 / int8) 16 of 4096, 8 tokens 83 / 62 and
+    // 68 / 55; 1 token 38 / 33 and 66 / 52.  All of it counts the table's width (cap), the lengths being on the device: 16
+    // sequences of 1024 rows, a token each, take 11.4 us under tables of 2048 rows, 16.6 of 8192 and 19.4 of 16384.
     const uint64_t rows = (uint64_t)b.tokens * heads, packed = (uint64_t)b.tokens * G, each = (packed + b.batch - 1) / b.batch;
     const uint32_t steps = (b.cap + 63) / 64, big = cache->head_dim == 64 ? 128 : 64, wide = cache->head_dim / 64;
     auto tiles_of = [&](uint32_t r) { return (each + r - 1) / r * b.batch * c.kv; };
