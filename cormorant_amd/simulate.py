@@ -9,6 +9,7 @@ conversion happens once at the graph's inputs, weights and returned tensors.
 """
 from __future__ import annotations
 
+import hashlib
 from typing import Dict, Iterable, List, Optional
 
 import numpy as np
@@ -86,6 +87,7 @@ class Simulator:
         self._infos: Dict[str, TensorInfo] = {}
         self._params: Dict[int, list] = {}                # row-ops parameter blocks on the device
         self._staging: Dict[tuple, torch.Tensor] = {}     # row-ops nodes' staging buffers
+        self._constants: Dict[tuple, torch.Tensor] = {}   # nodes' constants, in _images by what they hold
         self._private = None                               # _step_private's set
         self._plan = None                                  # MatMuls fed byte planes by their A's producer
         self._keep = None                                  # forward_raw's keep (None: every tensor)
@@ -459,6 +461,21 @@ class Simulator:
             self._weights[t.onnx_name] = w
         return w
 
+    def _constant(self, sn, what: str, lanes) -> torch.Tensor:
+        """The device copy of a node's constant lanes() (a host array): the simulator's nodes know their own,
+        simulators that share weights find it by what it holds, whichever of their nodes came first and
+        whether or not its graph still lives."""
+        t = self._constants.get((id(sn), what))
+        if t is None:
+            a = np.ascontiguousarray(lanes())
+            key = f"constant {a.dtype.str} {a.shape} {hashlib.blake2b(a.view(np.uint8).reshape(-1), digest_size=16).hexdigest()}"
+            t = self._images.get(key)
+            if t is None:
+                t = torch.from_numpy(a.copy()).to(self.device)
+                self._images[key] = t
+            self._constants[id(sn), what] = t
+        return t
+
     def _upload(self, arr: np.ndarray) -> torch.Tensor:
         """A weight on the device in a buffer whose last 8-lane word is whole (zero lanes past
         the data), so that the VectorOP unit reads it in place (_padded)."""
@@ -729,11 +746,7 @@ class Simulator:
 
     def _embed(self, sn: LlmEmbedNode, raw) -> torch.Tensor:
         """The embedding rows gathered on the device from the output-lane image of the table."""
-        key = f"{id(sn)}#embed"
-        img = self._images.get(key)
-        if img is None:
-            img = torch.from_numpy(sn.image()).to(self.device)
-            self._images[key] = img
+        img = self._constant(sn, "embed", sn.image)
         ids = self._get(sn.inputs[0], raw)
         if not isinstance(ids, torch.Tensor):                 # host ids (an i32 host tensor)
             ids = torch.from_numpy(np.asarray(ids, np.int64).reshape(-1).astype(np.int32)).to(self.device)
@@ -1569,10 +1582,7 @@ class Simulator:
                 self._staging[(key, k)] = b
             bufs["node:" + k] = b
         for k, lanes in sn.tables().items():
-            b = self._images.get(f"{key}:{k}")
-            if b is None:
-                b = torch.from_numpy(np.ascontiguousarray(lanes).reshape(-1).view(np.uint8).copy()).to(self.device)
-                self._images[f"{key}:{k}"] = b
+            b = self._constant(sn, "table " + k, lambda lanes=lanes: np.ascontiguousarray(lanes).reshape(-1).view(np.uint8))
             bufs["node:" + k] = b
         params = self._params.setdefault(key, {})
         for j in sn.calls(host):

@@ -28,7 +28,7 @@ def constants():
     """A simulator's constants alone (the units need a GPU)."""
     import torch
     sim = object.__new__(Simulator)
-    sim.device, sim._dtype, sim._weights = torch.device("cpu"), AP_FIXED_16_8, {}
+    sim.device, sim._dtype, sim._weights, sim._images, sim._constants = torch.device("cpu"), AP_FIXED_16_8, {}, {}, {}
     return sim
 
 
@@ -64,3 +64,30 @@ def test_outputs_by_name_are_kept():
     sim._graph = Graph(g.nodes, input_tensors=g.input_tensors, output_tensors=g.output_tensors + [own])
     rows = [sim._paged_rows(sn) for sn in preps]
     assert sim._passing == [preps[1].output.onnx_name] and rows[0].data_ptr() != rows[1].data_ptr()
+
+
+def embedding(rows, seed):
+    from cormorant_amd.host_ops import LlmEmbedNode
+    table = np.random.default_rng(seed).standard_normal((rows, 8)).astype(np.float32)
+    return LlmEmbedNode([TensorInfo("ids", [2], exp=0, kind="i32")], TensorInfo("h0", [2, 8], exp=15, kind="i32"), table=table)
+
+
+def test_embeddings_of_entries_that_come_and_go(monkeypatch):
+    """Entries share one dict of images that outlives their graphs: a node made where a dropped entry's was (the same id)
+    reads its own table, and equal tables are one copy."""
+    import torch
+    from cormorant_amd import simulate, units
+    read = []
+    monkeypatch.setattr(units, "embed_rows", lambda img, ids, out, rows, d: read.append(img.numpy()))
+    images = {}
+
+    def run(node):
+        sim = constants()
+        sim._images = images
+        sim._embed(node, {"ids": torch.zeros(2, dtype=torch.int32)})
+        np.testing.assert_array_equal(read.pop(), node.image())
+
+    monkeypatch.setattr(simulate, "id", lambda node: 7, raising=False)     # each node where the one before it was
+    for rows, seed in ((9, 0), (6, 1), (9, 0), (9, 2), (6, 1)):
+        run(embedding(rows, seed))
+    assert len(images) == 3
