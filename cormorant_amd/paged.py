@@ -169,7 +169,7 @@ def paged_prep(cache: PagedCache, batch: PagedBatch, prep: PagedPrep, q: torch.T
 
 def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: torch.Tensor, heads: int, smx_cm: int,
                     smx_cfg: int, window: int = 0) -> torch.Tensor:
-    """cm_paged_attention: the causal attention of the batch's tokens, q / o [tokens][heads hd], over
+    """cm_paged_attention: the causal attention of the batch's tokens, q / o [tokens][heads hd] (apart), over
     their sequences' cache rows (the last ``window`` of them, 0: all); smx_cm / smx_cfg as the softmax
     unit's registers (graph.softmax_regs), o at 2^-(f_p + f_v - 8) as the unit's P . V.  Any call may use the
     device's workspace: one at a time a device, and one of the same sizes before a capture.  The kernels are
@@ -178,8 +178,11 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, o: to
     if heads < 1 or heads % cache.kv_heads or not 0 <= window < 1 << 30:       # the ABI's word would drop bits from 2^32 on
         raise ValueError(f"paged_attention: {heads} heads over {cache.kv_heads} KV heads, window {window} (below 2^30)")
     q_ld, o_ld = _rows(q, "q", n, heads * hd), _rows(o, "o", n, heads * hd)
+    q_at, o_at = q.data_ptr(), o.data_ptr()
+    if q_at == o_at and n:                      # a tile's rows are read by several workgroups, and by two kernels
+        raise ValueError("paged_attention: o is q")
     stream = _on(cache, batch.kv_len, q, o)
-    _lib.check(_lib.lib().cm_paged_attention(cache._ref, batch._ref, q.data_ptr(), o.data_ptr(), q_ld, o_ld, heads,
+    _lib.check(_lib.lib().cm_paged_attention(cache._ref, batch._ref, q_at, o_at, q_ld, o_ld, heads,
                                              window, smx_cm & 0xFFFFFFFF, smx_cfg & 0xFFFFFFFF, stream),
                "cm_paged_attention")
     return o

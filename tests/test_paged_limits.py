@@ -28,3 +28,12 @@ def test_eps(eps):
     for kw in (dict(eps_q=eps), dict(eps_k=eps)):
         with pytest.raises(ValueError, match="eps"):
             P.PagedPrep(table, entry, entry, **kw)
+
+
+def test_o_apart_from_q():
+    """The many-row kernels read q again after other workgroups have written o."""
+    import torch
+    rows = SimpleNamespace(dtype=torch.int16, is_cuda=True, shape=(3, 256), stride=lambda: (256, 1), data_ptr=lambda: 4096)
+    cache, batch = SimpleNamespace(kv_heads=2, head_dim=64), SimpleNamespace(tokens=3)
+    with pytest.raises(ValueError, match="o is q"):
+        P.paged_attention(cache, batch, rows, rows, 4, 1 << 23, 20 | 14 << 8)
