@@ -46,6 +46,12 @@ class CmPagedPrepArgs(ctypes.Structure):
                 ("eps_q", ctypes.c_int64), ("eps_k", ctypes.c_int64)]
 
 
+class CmLinear8Weight(ctypes.Structure):
+    """cm_linear8_weight: an 8-bit weight's image and, of a gated one, its activation."""
+    _fields_ = [("image", _P), ("k", _U32), ("m", _U32), ("gated", _U32), ("act", _U32), ("gate_shift", _U32),
+                ("out_shift", _U32)]
+
+
 # name -> (restype, argtypes); every symbol include/cormorant_hip.h declares
 SIGNATURES = {
     "cm_abi_version": (_I32, []),
@@ -95,6 +101,12 @@ SIGNATURES = {
     "cm_paged_prep": (_I32, [_P] * 4),
     "cm_paged_attention": (_I32, [_P] * 4 + [ctypes.c_uint64] * 2 + [_U32] * 4 + [_P]),
     "cm_paged_read": (_I32, [_P] * 4 + [ctypes.c_uint64] * 2 + [_P]),
+    "cm_linear8_image_bytes": (ctypes.c_size_t, [_U32] * 3),
+    "cm_linear8_pack": (_I32, [_P] + [ctypes.c_uint64] * 2 + [_P] * 3 + [_U32] * 3 + [_P]),
+    "cm_linear8_rows_bytes": (ctypes.c_size_t, [_U32] * 2),
+    "cm_linear8_rows": (_I32, [_P, ctypes.c_uint64, _P, _U32, _U32, _P]),
+    "cm_linear8": (_I32, [_P, _P, ctypes.c_uint64, _P, _U32, _P, ctypes.c_uint64, _P, ctypes.c_uint64, _U32, _P]),
+    "cm_linear8_gated": (_I32, [_P, _P, ctypes.c_uint64, _P, _U32, _P, ctypes.c_uint64, _P]),
     "cm_timing_enable": (_I32, [_I32]),
     "cm_timing_read": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                               ctypes.POINTER(ctypes.c_uint64)]),

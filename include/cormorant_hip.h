@@ -557,6 +557,48 @@ int cm_paged_attention(const cm_paged_cache* cache, const cm_paged_batch* batch,
 int cm_paged_read(const cm_paged_cache* cache, const cm_paged_batch* batch, int16_t* k, int16_t* v, uint64_t k_ld,
                   uint64_t v_ld, void* stream);
 
+/* ---------------------------------------------------------------- 8-bit linear layers
+ * A decoder's linear layers on int16 rows with 8-bit weights (no counterpart in the reference, whose
+ * MatmulKernel takes int16 weights).  All arithmetic is in whole numbers and one rounding an output:
+ *   a row's codes:   a = max_k |x|, R = floor((127 2^24 + floor(a / 2)) / a), c = (x R + 2^23) >> 24 (a = 0: zeros);
+ *                    the row stands for c a / 127
+ *   a product:       o = sat16(rne(a mu_j sum_k c w_kj + b_j)), rne to the nearest whole number, ties to even;
+ *                    mu_j (a double, |mu_j| <= 64) the channel's scale at the output's exponent over 127
+ *   with a residual: sat32(h + (o << shift)), the ADDX of LlmResAdd (rowops_nodes.py:401-447)
+ *   a gate:          g and u two products of the same rows; y = sat16(rne(act(g) u 2^-out_shift));
+ *                    act 0: SiLU at 2^-20 of g << gate_shift at 2^-14, the MULACT job's rule (rowops_nodes.py:540-563);
+ *                    1 / 2: GELU / GELU-tanh of g, the activation unit's table (2^-8 in and out).
+ * k up to 32768, m up to 2^20, n up to 2^22 rows.  A multiplier outside its range (or not a number) gives unspecified
+ * values in its column.
+ *
+ * A weight's image (cm_linear8_image_bytes, 256-byte aligned): cm_linear8_pack lays out w [k][m], element
+ * (kk, j) at w + kk k_stride + j m_stride, with its multipliers [m] and an int32 bias [m] or NULL; `part` 0
+ * the weight, 1 / 2 the gate / up half of a gated image (gated 1, two calls).  Rows' codes
+ * (cm_linear8_rows_bytes, 256-byte aligned): cm_linear8_rows, for rows that several products read. */
+typedef struct cm_linear8_weight {
+    const void* image;
+    uint32_t k, m;
+    uint32_t gated;                     /* 0: a product, 1: gate and up */
+    uint32_t act, gate_shift, out_shift; /* gated: the activation, its shift (0 .. 14), the output's (0 .. 63) */
+} cm_linear8_weight;
+
+size_t cm_linear8_image_bytes(uint32_t k, uint32_t m, uint32_t gated);
+int cm_linear8_pack(const int8_t* w, uint64_t k_stride, uint64_t m_stride, const double* mult, const int32_t* bias,
+                    void* image, uint32_t k, uint32_t m, uint32_t part, void* stream);
+size_t cm_linear8_rows_bytes(uint32_t n, uint32_t k);
+int cm_linear8_rows(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, void* stream);
+
+/* o of n rows: x (rows x_ld elements apart, 2-byte aligned) or, x NULL, their codes.  out int16 rows out_ld apart; with a
+ * residual (int32, shift 0 .. 16) int32 rows, which may be the residual's own.  out is apart from x otherwise.  Called
+ * with x, the codes may stand in the device's workspace: a call of the same sizes before a stream captures it, and no
+ * two on different streams at once; with codes the workspace may still hold partial sums. */
+int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n, void* out,
+               uint64_t out_ld, const int32_t* residual, uint64_t residual_ld, uint32_t shift, void* stream);
+
+/* y of n rows, x and its codes as above: both products, the activation and their product in one kernel. */
+int cm_linear8_gated(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n,
+                     int16_t* out, uint64_t out_ld, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
