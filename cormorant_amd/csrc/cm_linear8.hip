@@ -202,6 +202,168 @@ __global__ __launch_bounds__(256) void linear8_tile_kernel(Prod p) {
     }
 }
 
+// ---------------------------------------------------------------- few rows
+// At most 16 RF rows: the weight is read once and the time is the latency of a launch, of x and of a
+// weight's bytes.  A workgroup of W wavefronts takes NF fragments of 16 columns (kGated: half gate, half up) at
+// all of k, the wavefronts its 64-k steps in turn; their sums meet in LDS (integer adds: any order).  With
+// x (DIRECT) a wavefront loads its own steps' pieces of the rows in the operand's layout, keeps them
+// in registers while the rows' maxima meet in LDS, and turns them into codes there: x is read once, no launch
+// and no memory between (S steps a wavefront, all of k).  Without, the codes are read, S steps at a time.
+// Further units of columns reuse a direct call's codes.
+constexpr uint32_t kFewWaves = 16, kFewSteps = 4;
+
+template <uint32_t NF>
+__device__ __forceinline__ void load_weights(v4i (&b)[NF], const int8_t* const (&w)[NF], uint32_t step) {
+#pragma unroll
+    for (uint32_t f = 0; f < NF; f++) b[f] = *reinterpret_cast<const v4i*>(w[f] + (uint64_t)step * kPiece);
+}
+
+template <uint32_t MODE, uint32_t RF, uint32_t NF, uint32_t S, bool DIRECT>
+__global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k) {
+    constexpr uint32_t R = 16 * RF, COLS = 16 * NF, OUT = MODE == kGated ? COLS / 2 : COLS;
+    constexpr uint32_t LD = COLS + 4;                // the four k groups' rows in different banks
+    __shared__ int32_t red[R * LD];                  // the unit's sums, zeros between units
+    __shared__ int32_t part[R * kFewWaves], top[R];  // the rows' maxima: of a wavefront's pieces, and all
+    const uint32_t W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const uint32_t units = (p.m + OUT - 1) / OUT;
+    const int8_t* w[NF];
+    // fragment f of unit u: its column block and half (kGated: gate and up blocks alternate)
+    auto weights_of = [&](uint32_t u) {
+#pragma unroll
+        for (uint32_t f = 0; f < NF; f++) {
+            constexpr uint32_t per = MODE == kGated ? NF / 2 : NF;
+            const uint32_t q = u * per + f % per;
+            const uint32_t blk = MODE == kGated ? 2 * (q >> 1) + f / per : q >> 1;
+            // columns past the last block: any, never stored
+            w[f] = p.w + (uint64_t)min(blk, p.cblocks - 1) * p.steps * kPiece + g * 512 + (q & 1) * 256 + c * 16;
+        }
+    };
+    uint32_t u = blockIdx.x;
+    weights_of(u);
+    v4i a[S][RF], b[S][NF];
+    for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
+    if constexpr (DIRECT) {
+        int4 xv[S][RF][2];
+        const int16_t* xr[RF];
+#pragma unroll
+        for (uint32_t f = 0; f < RF; f++) xr[f] = x + (uint64_t)min(16 * f + c, p.n - 1) * ld;
+#pragma unroll
+        for (uint32_t i = 0; i < S; i++) {
+            const uint32_t k0 = (wave + i * W) * kStep + 16 * g;
+#pragma unroll
+            for (uint32_t f = 0; f < RF; f++) {
+                if (k0 + 16 <= k) {
+                    xv[i][f][0] = load8(xr[f] + k0);
+                    xv[i][f][1] = load8(xr[f] + k0 + 8);
+                } else {
+                    int16_t e[16];
+#pragma unroll
+                    for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? xr[f][k0 + q] : (int16_t)0;
+                    __builtin_memcpy(&xv[i][f][0], e, 32);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < S; i++)
+            if (wave + i * W < p.steps) load_weights<NF>(b[i], w, wave + i * W);
+        // the rows' maxima: this wavefront's pieces, its four k groups, then the wavefronts
+#pragma unroll
+        for (uint32_t f = 0; f < RF; f++) {
+            int32_t t = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < S; i++) {
+                const int16_t* e = reinterpret_cast<const int16_t*>(&xv[i][f][0]);
+#pragma unroll
+                for (int q = 0; q < 16; q++) t = max(t, abs((int32_t)e[q]));
+            }
+            t = max(t, __shfl_xor(t, 16, 64));
+            t = max(t, __shfl_xor(t, 32, 64));
+            if (g == 0) part[(16 * f + c) * kFewWaves + wave] = t;
+        }
+        lds_barrier();
+#pragma unroll
+        for (uint32_t f = 0; f < RF; f++) {
+            int32_t am = 0;
+            for (uint32_t i = 0; i < W; i++) am = max(am, part[(16 * f + c) * kFewWaves + i]);
+            if (wave == 0 && g == 0) top[16 * f + c] = am;
+            const int32_t rc = (int32_t)recip((uint32_t)am);
+#pragma unroll
+            for (uint32_t i = 0; i < S; i++) {
+                const int16_t* e = reinterpret_cast<const int16_t*>(&xv[i][f][0]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t word = 0;               // four codes: the top bytes of four sums
+#pragma unroll
+                    for (int h = 0; h < 4; h++) word |= ((uint32_t)(e[4 * q + h] * rc + (1 << 23)) >> 24) << (8 * h);
+                    a[i][f][q] = (int)word;
+                }
+            }
+        }
+    } else {
+        lds_barrier();                               // red is zeros
+    }
+    for (;;) {
+        v4i sum[RF][NF];
+#pragma unroll
+        for (uint32_t f = 0; f < RF; f++)
+#pragma unroll
+            for (uint32_t q = 0; q < NF; q++) sum[f][q] = v4i{0, 0, 0, 0};
+        // one round of S steps if direct, else as many as k takes
+        for (uint32_t s0 = wave; s0 < p.steps; s0 += S * W) {
+            if constexpr (!DIRECT) {
+#pragma unroll
+                for (uint32_t i = 0; i < S; i++) {
+                    const uint32_t st = min(s0 + i * W, p.steps - 1);
+                    load_weights<NF>(b[i], w, st);
+#pragma unroll
+                    for (uint32_t f = 0; f < RF; f++)
+                        a[i][f] = *reinterpret_cast<const v4i*>(p.a + (uint64_t)st * kPiece + g * 512 + f * 256 + c * 16);
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < S; i++) {
+                if (s0 + i * W >= p.steps) break;
+#pragma unroll
+                for (uint32_t q = 0; q < NF; q++)
+#pragma unroll
+                    for (uint32_t f = 0; f < RF; f++)
+                        sum[f][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][f], b[i][q], sum[f][q], 0, 0, 0);
+            }
+        }
+        const uint32_t next = u + gridDim.x;
+        if (next < units) {                          // the next unit's weights travel while this one's sums meet
+            weights_of(next);
+            if constexpr (DIRECT) {
+#pragma unroll
+                for (uint32_t i = 0; i < S; i++)
+                    if (wave + i * W < p.steps) load_weights<NF>(b[i], w, wave + i * W);
+            }
+        }
+#pragma unroll
+        for (uint32_t f = 0; f < RF; f++)
+#pragma unroll
+            for (uint32_t q = 0; q < NF; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    __hip_atomic_fetch_add(&red[(16 * f + 4 * g + i) * LD + 16 * q + c], sum[f][q][i], __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+        lds_barrier();
+        for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
+            const uint32_t row = e / OUT, cl = e % OUT, col = u * OUT + cl;
+            const int32_t s0 = red[row * LD + cl], s1 = MODE == kGated ? red[row * LD + OUT + cl] : 0;
+            red[row * LD + cl] = 0;
+            if (MODE == kGated) red[row * LD + OUT + cl] = 0;
+            if (row >= p.n || col >= p.m) continue;
+            const double am = (double)(DIRECT ? top[row] : p.amax[row]);
+            const uint32_t at = MODE == kGated ? (col >> 5) * 64 + (col & 31) : col;
+            store<MODE>(p, row, col, s0, s1, am, p.cols[at], MODE == kGated ? p.cols[at + 32] : double2{});
+        }
+        if (next >= units) return;
+        u = next;
+        lds_barrier();                               // red is zeros again
+    }
+}
+
 // ---------------------------------------------------------------- calls
 int check_weight(const char* what, const cm_linear8_weight* w, bool gated) {
     if (w == nullptr || w->image == nullptr) return fail(CM_EINVAL, "%s: a null weight", what);
@@ -232,13 +394,37 @@ int check_rows(const char* what, const int16_t* x, uint64_t x_ld, const void* ro
     return CM_OK;
 }
 
+// Few rows: fragments of columns a workgroup, and the grid.
+template <uint32_t MODE, uint32_t RF, uint32_t NF>
+int few_rows_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, uint32_t grid, hipStream_t s) {
+    const uint32_t W = std::min(kFewWaves, p.steps), per = (p.steps + W - 1) / W;
+#define CM_FEW(S, D) \
+    CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D>), dim3(grid), dim3(64 * W), 0, s, p, x, ld, k)
+    if (x == nullptr) { CM_FEW(kFewSteps, false); }
+    else if (per == 1) { CM_FEW(1, true); }
+    else if (per == 2) { CM_FEW(2, true); }
+    else { CM_FEW(kFewSteps, true); }
+#undef CM_FEW
+    return CM_OK;
+}
+
+template <uint32_t MODE>
+int few_rows(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipStream_t s) {
+    constexpr uint32_t P = MODE == kGated ? 2 : 1;
+    const uint32_t cap = 2 * (uint32_t)st->cus;
+    if (p.n > 16) return few_rows_at<MODE, 2, P>(p, x, ld, k, std::min(ceil_div(p.m, 16), cap), s);
+    if (p.m <= 16 * cap) return few_rows_at<MODE, 1, P>(p, x, ld, k, ceil_div(p.m, 16), s);
+    return few_rows_at<MODE, 1, 2 * P>(p, x, ld, k, std::min(ceil_div(p.m, 32), cap), s);
+}
+
 // The product behind its checks: the rows' codes (the caller's, or made in the workspace), then the kernel.
 template <uint32_t MODE>
 int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const void* rows, Prod p, hipStream_t s) {
     DeviceState* st;
     int rc = state(&st);
     if (rc) return rc;
-    if (rows == nullptr) {
+    const bool few = p.n <= 32, direct = few && rows == nullptr && steps_of(w->k) <= kFewSteps * kFewWaves;
+    if (rows == nullptr && !direct) {
         void* ws;
         if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;
         if ((rc = quantise(x, x_ld, ws, p.n, w->k, s))) return rc;
@@ -248,8 +434,10 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.steps = steps_of(w->k);
     p.rblocks = blocks_of(p.n);
     p.cblocks = blocks_of(w->m) * (MODE == kGated ? 2 : 1);
-    p.a = static_cast<const int8_t*>(rows);
-    p.amax = reinterpret_cast<const int32_t*>(p.a + codes_bytes(p.rblocks, w->k));
+    if (!direct) {
+        p.a = static_cast<const int8_t*>(rows);
+        p.amax = reinterpret_cast<const int32_t*>(p.a + codes_bytes(p.rblocks, w->k));
+    }
     p.w = static_cast<const int8_t*>(w->image);
     p.cols = reinterpret_cast<const double2*>(p.w + codes_bytes(p.cblocks, w->k));
     if (MODE == kGated) {
@@ -258,6 +446,10 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
         p.scale = __builtin_ldexp(1.0, -(int)w->out_shift);
         p.tab = w->act == kSilu ? st->ro_tables : st->act_tab + w->act * kActTabBytes;
         p.len = w->act == kSilu ? 0 : st->act_len[w->act];
+    }
+    if (few) {
+        const int16_t* src = direct ? x : nullptr;
+        return few_rows<MODE>(st, p, src, x_ld, w->k, s);
     }
     const dim3 grid(ceil_div(p.cblocks, 4), ceil_div(p.rblocks, 2));
     if (grid.y > 65535u) return fail(CM_EINVAL, "linear8: %u rows", p.n);
