@@ -15,6 +15,9 @@
 #include "cm_common.h"
 #include "cm_rowops_math.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace cm {
 namespace {
 
@@ -25,14 +28,20 @@ constexpr uint32_t kLine = 32, kStep = 64, kPiece = kLine * kStep;      // lines
 constexpr uint32_t kMaxK = 32768, kMaxM = 1u << 20, kMaxN = 1u << 22;
 constexpr double kMagic = 6755399441055744.0;                           // 1.5 2^52: a whole number added to it is its low word
 
-enum : uint32_t { kOut16 = 0, kOut32 = 1, kGated = 2 };
-enum : uint32_t { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
+// What a product becomes: int16 rows, the int32 residual with them, or a gate by the sigmoid's pieces or a byte table.
+enum : uint32_t { kOut16 = 0, kOut32 = 1, kSiluGate = 2, kTableGate = 3 };
+constexpr bool gated(uint32_t mode) { return mode >= kSiluGate; }
+enum : uint32_t { kSilu = 0, kGelu = 1, kGeluTanh = 2 };             // cm_linear8_weight's act
+constexpr uint32_t kPieces = 4096;                                    // of the sigmoid, 8 bytes each
 
 inline uint32_t steps_of(uint32_t k) { return ceil_div(k, kStep); }
 inline uint32_t blocks_of(uint32_t lines) { return ceil_div(lines, kLine); }
 
 // Where a rows image's maxima and a weight image's channel parameters start (behind the blocks).
-inline size_t codes_bytes(uint32_t blocks, uint32_t k) { return (size_t)blocks * steps_of(k) * kPiece; }
+// Blocks of lines start an odd number of 2 KiB pieces apart: at a power of two, all that the workgroups read at one time
+// would lie in the same few channels of the L2s and of the memory.
+__host__ __device__ inline uint32_t pitch_of(uint32_t steps) { return (steps | 1u) * kPiece; }
+inline size_t codes_bytes(uint32_t blocks, uint32_t k) { return (size_t)blocks * pitch_of(steps_of(k)); }
 inline size_t rows_bytes(uint32_t n, uint32_t k) { return codes_bytes(blocks_of(n), k) + (size_t)blocks_of(n) * kLine * 4; }
 inline size_t image_bytes(uint32_t k, uint32_t m, bool gated) {
     const uint32_t b = blocks_of(m) * (gated ? 2 : 1);
@@ -51,40 +60,43 @@ struct Prod {
     const int32_t* res;              // kOut32
     uint64_t res_ld;
     uint32_t shift;
-    const uint8_t* tab;              // kGated: the sigmoid's pieces, or the activation's bytes (`len` of them)
-    uint32_t act, len, sa;
-    double scale;                    // 2^-sc
+    const uint8_t* tab;              // a gate's: the sigmoid's pieces, or the activation's bytes (`len` of them)
+    uint32_t len, sa;
+    double gscale, scale;            // 2^(sa - 18), 2^-sc
 };
 
-// rne(acc a mu + b), saturated to int16.
-__device__ __forceinline__ int32_t out16(int32_t acc, double a, double2 c) {
+// 1.5 2^52 + sat16(rne(acc a mu + b)): the low word is the result.
+__device__ __forceinline__ double scaled(int32_t acc, double a, double2 c) {
     const double z = __builtin_fma((double)acc * a, c.x, c.y);
-    return __double2loint(__builtin_fmin(__builtin_fmax(z, kMagic - 32768.0), kMagic + 32767.0));
+    return __builtin_fmin(__builtin_fmax(z, kMagic - 32768.0), kMagic + 32767.0);
 }
 
+// sat32(h + (o << shift)), o of 16 bits and shift at most 16.
 __device__ __forceinline__ int32_t add_res(int32_t h, int32_t o, uint32_t shift) {
-    const int64_t s = (int64_t)h + ((int64_t)o << shift);
-    return (int32_t)(s > 2147483647 ? 2147483647 : s < -2147483648ll ? -2147483648ll : s);
+    return __builtin_elementwise_add_sat(h, (int32_t)((uint32_t)o << shift));
 }
 
-// act(g) u 2^-sc, rounded to even and saturated.  SiLU by the row-ops rule (MULACT): sigma at 2^-24 from the
-// piece of |g| at 2^-14, silu at 2^-20.  gv sigma is exact in a double (below 2^18 2^26, or a power of two
-// times g), so is silu u (2^35 2^15), and each sum onto 1.5 2^52 is its one rounding.
-__device__ __forceinline__ int32_t gate16(int32_t g, int32_t u, const Prod& p) {
+// act(g) u 2^-sc, rounded to even and saturated, of the two products zg, zu as `scaled` gives them.  SiLU by the row-ops
+// rule (MULACT): sigma at 2^-24 from the piece of |g| at 2^-14, silu at 2^-20.  gv sigma is exact in a double (below
+// 2^18 2^26, or a power of two times g), so is silu u (2^35 2^15), and each sum onto 1.5 2^52 is its one rounding.
+template <uint32_t MODE, class Tab>
+__device__ __forceinline__ int32_t gate16(double zg, double zu, Tab tab, const Prod& p) {
+    const int32_t g = __double2loint(zg), a = max(g, -g);
     double f;
-    const uint32_t a = (uint32_t)(g < 0 ? -g : g);
-    if (p.act == kSilu) {
-        const uint32_t av = a << p.sa, ai = min(av, (1u << 18) - 1), fr = ai & 63;
-        const uint64_t e = *reinterpret_cast<const uint64_t*>(p.tab + 8 * (ai >> 6));
-        const uint32_t T = (uint32_t)e & 0x1FFFFFFu, D = (uint32_t)(e >> 25) & 0xFFFFFFu;
-        int32_t sg = av >= (1u << 18) ? 1 << 24 : (int32_t)(T + ((D * fr) >> 6));
+    if (MODE == kSiluGate) {
+        const uint32_t av = (uint32_t)a << p.sa, ai = min(av, (1u << 18) - 1), fr = ai & 63;
+        const uint2 e = *reinterpret_cast<const uint2*>(tab + 8 * (ai >> 6));        // {D << 25 | T}: 24 and 25 bits
+        const uint32_t T = e.x & 0x1FFFFFFu, D = (e.x >> 25 | e.y << 7) & 0xFFFFFFu;
+        int32_t sg = (int32_t)(T + ((D * fr) >> 6));
+        asm("" : "+v"(sg));                              // for every lane: a branch around it costs more
+        sg = av >= (1u << 18) ? 1 << 24 : sg;
         if (g < 0) sg = (1 << 24) - sg;
-        f = __builtin_fma((double)(g << p.sa), (double)sg * 0x1p-18, kMagic) - kMagic;
+        f = __builtin_fma((zg - kMagic) * p.gscale, (double)sg, kMagic) - kMagic;
     } else {
-        f = (double)(max(g, 0) - (a < p.len ? (int32_t)p.tab[a] : 0));
+        f = (double)(max(g, 0) - ((uint32_t)a < p.len ? (int32_t)tab[a] : 0));
     }
-    const double v = __builtin_fmin(__builtin_fmax(f * (double)u * p.scale, -65536.0), 65536.0);
-    return min(max(__double2loint(v + kMagic), -32768), 32767);
+    const double z = __builtin_fma(f * (zu - kMagic), p.scale, kMagic);
+    return __double2loint(__builtin_fmin(__builtin_fmax(z, kMagic - 32768.0), kMagic + 32767.0));
 }
 
 // ---------------------------------------------------------------- a weight's image
@@ -106,7 +118,7 @@ __global__ __launch_bounds__(256) void linear8_pack_kernel(const int8_t* __restr
         const uint32_t kk = st * kStep + kg * 16 + e;
         v[e] = kk < k && j < m ? w[kk * ks + j * js] : (int8_t)0;
     }
-    *reinterpret_cast<int4*>(codes + ((uint64_t)to * steps + st) * kPiece + kg * 512 + line * 16) = *reinterpret_cast<const int4*>(v);
+    *reinterpret_cast<int4*>(codes + (uint64_t)to * pitch_of(steps) + st * kPiece + kg * 512 + line * 16) = *reinterpret_cast<const int4*>(v);
     if (st == 0 && kg == 0)
         cols[(uint64_t)to * kLine + line] = j < m ? make_double2(mult[j], kMagic + (bias ? (double)bias[j] : 0.0)) : make_double2(0.0, kMagic);
 }
@@ -119,92 +131,399 @@ __device__ __forceinline__ int4 load8(const int16_t* p) {                   // 8
 }
 
 __device__ __forceinline__ uint32_t recip(uint32_t a) { return a ? (127u * (1u << 24) + (a >> 1)) / a : 0u; }
-__device__ __forceinline__ int32_t code(int32_t x, uint32_t r) { return (x * (int32_t)r + (1 << 23)) >> 24; }
 
-// A wavefront a row: its maximum, then its codes, 16 elements a lane.
-__global__ __launch_bounds__(256) void linear8_rows_kernel(const int16_t* __restrict__ x, uint64_t ld, uint32_t n, uint32_t k,
-                                                           int8_t* __restrict__ codes, int32_t* __restrict__ amax, uint32_t steps) {
-    const uint32_t lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= n) return;
-    const int16_t* r = x + (uint64_t)row * ld;
-    const uint32_t kp = steps * kStep;
-    auto load = [&](uint32_t k0, int16_t (&e)[16]) {
-        if (k0 + 16 <= k) {
-            const int4 v[2] = {load8(r + k0), load8(r + k0 + 8)};
-            __builtin_memcpy(e, v, 32);
-        } else {
-            for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? r[k0 + q] : (int16_t)0;
-        }
-    };
-    int32_t top = 0;
-    int16_t e[16];
-    for (uint32_t k0 = 16 * lane; k0 < kp; k0 += 1024) {
-        load(k0, e);
-        for (int q = 0; q < 16; q++) top = max(top, abs((int32_t)e[q]));
+typedef short v2s __attribute__((ext_vector_type(2)));
+
+// 16 elements from k0 of a row of k (zeros past its end), as they come from memory.
+struct Piece {
+    int4 v[2];
+};
+__device__ __forceinline__ Piece load_piece(const int16_t* row, uint32_t k0, uint32_t k) {
+    Piece p;
+    if (k0 + 16 <= k) {
+        p.v[0] = load8(row + k0);
+        p.v[1] = load8(row + k0 + 8);
+    } else {
+        int16_t e[16];
+#pragma unroll
+        for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? row[k0 + q] : (int16_t)0;
+        __builtin_memcpy(&p, e, 32);
     }
+    return p;
+}
+
+// The largest and the smallest elements so far, two lanes of 16 bits each: |-32768| has no int16.
+struct Range {
+    v2s hi{0, 0}, lo{0, 0};
+    __device__ __forceinline__ void add(const Piece& p) {
+        const v2s* e = reinterpret_cast<const v2s*>(&p);
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            hi = __builtin_elementwise_max(hi, e[q]);
+            lo = __builtin_elementwise_min(lo, e[q]);
+        }
+    }
+    __device__ __forceinline__ int32_t top() const {
+        return max(max((int32_t)hi[0], (int32_t)hi[1]), -min((int32_t)lo[0], (int32_t)lo[1]));
+    }
+};
+
+// The 16 codes of a piece: the top bytes of x R + 2^23.  `small`: every R of the wavefront is below 2^23 (maxima from 255 on),
+// so that a 24-bit multiply-add does (full rate; a 32-bit product a quarter of it).
+__device__ __forceinline__ v4i codes_of(const Piece& p, int32_t r, bool small) {
+    const v2s* e = reinterpret_cast<const v2s*>(&p);
+    v4i out;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        int32_t t[4];
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+            const int32_t x = e[2 * q + (h >> 1)][h & 1];
+            t[h] = (small ? __mul24(x, r) : x * r) + (1 << 23);
+        }
+        const uint32_t a = __builtin_amdgcn_perm((uint32_t)t[1], (uint32_t)t[0], 0x0C0C0703u);
+        const uint32_t b = __builtin_amdgcn_perm((uint32_t)t[3], (uint32_t)t[2], 0x0C0C0703u);
+        out[q] = (int)(a | b << 16);
+    }
+    return out;
+}
+
+// 16 rows a workgroup, a wavefront a row: its maximum, then its codes, 16 elements a lane and pass of 1024; rows of up to 1024 U
+// elements stay in registers, U = 0: longer ones are read twice.  A pass's codes go through LDS, so that 16 lanes
+// write 256 consecutive bytes of a block.  Bound by memory for many rows.
+template <int U>
+__global__ __launch_bounds__(1024) void linear8_rows_kernel(const int16_t* __restrict__ x, uint64_t ld, uint32_t n, uint32_t k,
+                                                           int8_t* __restrict__ codes, int32_t* __restrict__ amax, uint32_t steps) {
+    constexpr uint32_t PL = 16 * 16 + 16;                  // bytes of a piece of 16 rows in LDS: pieces in different banks
+    __shared__ __attribute__((aligned(16))) int8_t sm[2][64 * PL];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row0 = blockIdx.x * 16, row = row0 + wave;
+    const int16_t* r = x + (uint64_t)min(row, n - 1) * ld;
+    Range range;
+    Piece e[U ? U : 1];
+    if constexpr (U != 0) {
+#pragma unroll
+        for (int i = 0; i < U; i++) e[i] = load_piece(r, 16 * lane + 1024 * i, k);
+#pragma unroll
+        for (int i = 0; i < U; i++) range.add(e[i]);
+    } else {
+        for (uint32_t k0 = 16 * lane; k0 < k; k0 += 1024) range.add(load_piece(r, k0, k));
+    }
+    int32_t top = range.top();
     for (int off = 32; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
-    if (lane == 0) amax[row] = top;
-    const uint32_t rc = recip((uint32_t)top);
-    for (uint32_t k0 = 16 * lane; k0 < kp; k0 += 1024) {
-        load(k0, e);
-        int8_t c[16];
-        for (int q = 0; q < 16; q++) c[q] = (int8_t)code(e[q], rc);
-        const uint32_t st = k0 >> 6, kg = (k0 >> 4) & 3;
-        *reinterpret_cast<int4*>(codes + ((uint64_t)(row >> 5) * steps + st) * kPiece + kg * 512 + (row & 31) * 16) =
-            *reinterpret_cast<const int4*>(c);
+    top = __builtin_amdgcn_readfirstlane(top);
+    if (lane == 0 && row < n) amax[row] = top;
+    const int32_t rc = (int32_t)recip((uint32_t)top);
+    int8_t* to = codes + (uint64_t)(row0 >> 5) * pitch_of(steps) + (row0 & 31) * 16;
+    const uint32_t piece = threadIdx.x >> 4, line = threadIdx.x & 15;
+    auto pass = [&](int i, const Piece& p) {
+        *reinterpret_cast<v4i*>(&sm[i & 1][lane * PL + wave * 16]) = codes_of(p, rc, rc < 1 << 23);
+        lds_barrier();                                     // two buffers: one barrier a pass
+        const uint32_t q = 64 * i + piece;
+        if (q < 4 * steps && row0 + line < n)
+            *reinterpret_cast<v4i*>(to + q * 512 + line * 16) = *reinterpret_cast<const v4i*>(&sm[i & 1][piece * PL + line * 16]);
+    };
+    if constexpr (U != 0) {
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (1024 * i < (int)k) pass(i, e[i]);          // the same for the whole workgroup
+    } else {
+        for (int i = 0; 1024 * i < (int)k; i++) pass(i, load_piece(r, 16 * lane + 1024 * i, k));
     }
 }
 
 // ---------------------------------------------------------------- products
-// The value of one output element from the sums of its columns (kGated: gate and up).
+// One output element from the sums of its column (a gate: of both).
 template <uint32_t MODE>
 __device__ __forceinline__ void store(const Prod& p, uint32_t row, uint32_t col, int32_t acc0, int32_t acc1, double a,
                                       double2 c0, double2 c1) {
-    if (row >= p.n || col >= p.m) return;
-    const int32_t o = out16(acc0, a, c0);
-    if (MODE == kOut16) {
-        static_cast<int16_t*>(p.out)[row * p.out_ld + col] = (int16_t)o;
-    } else if (MODE == kOut32) {
-        static_cast<int32_t*>(p.out)[row * p.out_ld + col] = add_res(p.res[row * p.res_ld + col], o, p.shift);
+    const double z = scaled(acc0, a, c0);
+    if (MODE == kOut32) {
+        static_cast<int32_t*>(p.out)[row * p.out_ld + col] = add_res(p.res[row * p.res_ld + col], __double2loint(z), p.shift);
     } else {
-        static_cast<int16_t*>(p.out)[row * p.out_ld + col] = (int16_t)gate16(o, out16(acc1, a, c1), p);
+        const int32_t o = gated(MODE) ? gate16<MODE>(z, scaled(acc1, a, c1), p.tab, p) : __double2loint(z);
+        static_cast<int16_t*>(p.out)[row * p.out_ld + col] = (int16_t)o;
     }
 }
 
-// 64 rows by two pairs of column blocks a workgroup, a wavefront 32 rows and a pair, operands straight from memory.
-template <uint32_t MODE>
-__global__ __launch_bounds__(256) void linear8_tile_kernel(Prod p) {
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
-    const uint32_t rb = blockIdx.y * 2 + (wave >> 1), pair = blockIdx.x * 2 + (wave & 1);
-    if (rb >= p.rblocks || 2 * pair >= p.cblocks) return;
-    const uint32_t cb[2] = {2 * pair, min(2 * pair + 1, p.cblocks - 1)};
-    const int8_t* a = p.a + (uint64_t)rb * p.steps * kPiece + lane * 16;
-    const int8_t* w0 = p.w + (uint64_t)cb[0] * p.steps * kPiece + lane * 16;
-    const int8_t* w1 = p.w + (uint64_t)cb[1] * p.steps * kPiece + lane * 16;
-    v16i s0{}, s1{};
-    for (uint32_t i = 0; i < 2 * p.steps; i++) {
-        const uint64_t at = (uint64_t)i * 1024;
-        const v4i av = *reinterpret_cast<const v4i*>(a + at);
-        s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, *reinterpret_cast<const v4i*>(w0 + at), s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, *reinterpret_cast<const v4i*>(w1 + at), s1, 0, 0, 0);
-    }
-    const double2 c0 = p.cols[cb[0] * kLine + l32], c1 = p.cols[cb[1] * kLine + l32];
+// ---------------------------------------------------------------- many rows
+// LDS reads, LDS copies and vector memory each move 64 bytes a cycle and compute unit (measured), an i8 MFMA of 32 x
+// 32 x 32 takes 32 cycles: what bounds a product is how often its operands pass through those two ports.  So a
+// wavefront takes 64 rows by 128 columns, WR of them side by side over the same columns: x's fragments, which no other wavefront
+// reads, go from memory straight into registers, three steps ahead; the weight's 128 columns go through a ring of
+// three LDS stages, copied three steps ahead.  A 64-k step of two such workgroups on a compute unit (WR = 4) is 1024 cycles of MFMA
+// on each SIMD, 64 KiB of LDS reads, 16 KiB of copies and 32 KiB of loads.  Operand pieces lie in memory, in LDS and in the
+// registers in one order (a lane's 16 bytes at 16 lane): whole lines, no bank conflict.
+// Buffer accesses: a block's base in scalar registers, the lane's 16 bytes in one vector register, the step's offset
+// scalar.  Copies to LDS go this way and not as global_load_lds, which the compiler counts as a flat access: every wait
+// for a register load or an LDS read behind one becomes a wait for all (8192 x 4096 x 8192: 268 us, 260 this way).
+// Both are marked volatile: a wait below counts the accesses behind a copy, so none of them may move over another.
+typedef __amdgpu_buffer_rsrc_t Buf;
+constexpr int kVolatile = (int)0x80000000;
+__device__ __forceinline__ Buf buffer_of(const int8_t* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, (int)bytes, 0x00027000);
+}
+__device__ __forceinline__ void lds_copy16(Buf b, uint32_t lane_at, uint32_t at, int8_t* lds_wave_base) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)lds_wave_base, 16, (int)lane_at, (int)at, 0, kVolatile);
+}
+__device__ __forceinline__ v4i load16(Buf b, uint32_t lane_at, uint32_t at) {
+    return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(b, (int)lane_at, (int)at, kVolatile));
+}
+
+template <int N>
+__device__ __forceinline__ void wait_copies() {            // at most N of this wavefront's copies outstanding, LDS reads done
+    static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+}
+
+// The output tile of workgroup x: the workgroups of an XCD (one residue mod 8) take a contiguous run of an order that
+// walks strips of xw tile columns row by row, so that its L2 holds the operands of a block of tiles.
+struct Tile {
+    uint32_t r, c;
+};
+__device__ __forceinline__ Tile tile_of(uint32_t x, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
+    const uint32_t tiles = tiles_r * tiles_c, q = tiles >> 3, res = x & 7;
+    const uint32_t at = res * q + min(res, tiles & 7) + (x >> 3);
+    const uint32_t strip = at / (tiles_r * xw), in = at - strip * tiles_r * xw;
+    const uint32_t w = min(xw, tiles_c - strip * xw), row = in / w;
+    return Tile{row, strip * xw + in - row * w};
+}
+
+// The outputs of a wavefront's RB x CB blocks: a lane holds column l32 of a block, its rows 8 (r / 4) + 4 lh + r % 4.  Through
+// buffer accesses, which drop what lies past the last row and, at an offset past every row, past the last column.
+template <uint32_t MODE, int RB, int CB, class Tab>
+__device__ __forceinline__ void epilogue(const Prod& p, const v16i (&acc)[RB][CB], uint32_t rb0, uint32_t cb0, uint32_t l32,
+                                         uint32_t lh, Tab tab) {
+    constexpr uint32_t E = MODE == kOut32 ? 4 : 2;
+    constexpr int ST = gated(MODE) ? 2 : 1;
+    const uint32_t ld = (uint32_t)p.out_ld, rld = (uint32_t)p.res_ld;
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const uint32_t row = rb * kLine + 8 * (r >> 2) + 4 * lh + (r & 3);
-        const double am = (double)p.amax[min(row, p.n - 1)];
-        if (MODE == kGated) {
-            store<MODE>(p, row, pair * kLine + l32, s0[r], s1[r], am, c0, c1);
-        } else {
-            store<MODE>(p, row, cb[0] * kLine + l32, s0[r], 0, am, c0, c0);
-            if (cb[1] != cb[0]) store<MODE>(p, row, cb[1] * kLine + l32, s1[r], 0, am, c1, c1);
+    for (int i = 0; i < RB; i++) {
+        const uint32_t row0 = (rb0 + i) * kLine;
+        if (row0 >= p.n) break;
+        const uint32_t rows = min(p.n - row0, kLine);
+        const Buf ob = buffer_of(static_cast<int8_t*>(p.out) + (uint64_t)row0 * p.out_ld * E, ((rows - 1) * ld + p.m) * E);
+        Buf hb;
+        if constexpr (MODE == kOut32)
+            hb = buffer_of(reinterpret_cast<const int8_t*>(p.res) + (uint64_t)row0 * p.res_ld * E, ((rows - 1) * rld + p.m) * E);
+        double am[16];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int4 v = *reinterpret_cast<const int4*>(p.amax + row0 + 8 * q + 4 * lh);
+            am[4 * q] = v.x, am[4 * q + 1] = v.y, am[4 * q + 2] = v.z, am[4 * q + 3] = v.w;
         }
+#pragma unroll
+        for (int j = 0; j < CB; j += ST) {
+            const uint32_t blk = cb0 + j, col = (gated(MODE) ? blk >> 1 : blk) * kLine + l32;
+            const double2 c0 = p.cols[min(blk, p.cblocks - 1) * kLine + l32];
+            const double2 c1 = gated(MODE) ? p.cols[min(blk + 1, p.cblocks - 1) * kLine + l32] : double2{};
+            const uint32_t at = col < p.m ? (4 * lh * ld + col) * E : 0x80000000u;
+            int32_t h[16];
+            if constexpr (MODE == kOut32) {
+                const uint32_t rat = col < p.m ? (4 * lh * rld + col) * E : 0x80000000u;
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    h[r] = __builtin_amdgcn_raw_buffer_load_b32(hb, (int)(rat + (8 * (r >> 2) + (r & 3)) * rld * E), 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const double z = scaled(acc[i][j][r], am[r], c0);
+                const int to = (int)(at + (8 * (r >> 2) + (r & 3)) * ld * E);
+                if constexpr (MODE == kOut32) {
+                    __builtin_amdgcn_raw_buffer_store_b32(add_res(h[r], __double2loint(z), p.shift), ob, to, 0, 0);
+                } else {
+                    int32_t o = __double2loint(z);
+                    if constexpr (gated(MODE)) o = gate16<MODE>(z, scaled(acc[i][j + 1][r], am[r], c1), tab, p);
+                    __builtin_amdgcn_raw_buffer_store_b16((short)o, ob, to, 0, 0);
+                }
+            }
+            if constexpr (MODE == kOut32) __builtin_amdgcn_sched_barrier(0);     // a block's residuals in registers at a time
+        }
+    }
+}
+
+template <uint32_t MODE, int CB>
+__global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
+    constexpr int WR = 4, RB = 2, NC = 2 * CB / WR;        // wavefronts; blocks of one; copies a wavefront and step
+    __shared__ __attribute__((aligned(1024))) int8_t sm0[2 * CB * 1024];
+    __shared__ __attribute__((aligned(1024))) int8_t sm1[2 * CB * 1024];
+    __shared__ __attribute__((aligned(1024))) int8_t sm2[2 * CB * 1024];
+    // a gate's table, for gathers of 64 lanes; it lands before the ring's first copies
+    constexpr int TAB = MODE == kSiluGate ? 8 * kPieces : MODE == kTableGate ? kActTabBytes : 16;
+    __shared__ __attribute__((aligned(1024))) int8_t tab[TAB];
+    const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t l32 = lane & 31, lh = lane >> 5;
+    const uint32_t rb0 = (t.r * WR + wave) * RB, cb0 = t.c * CB;
+    // blocks past the last: any, never stored
+    const uint32_t line = pitch_of(p.steps);               // bytes of a block of lines
+    Buf xa[RB];
+#pragma unroll
+    for (int i = 0; i < RB; i++) xa[i] = buffer_of(p.a + (uint64_t)min(rb0 + i, p.rblocks - 1) * line, line);
+    const Buf wb = buffer_of(p.w + (uint64_t)cb0 * line, min(p.cblocks - cb0, (uint32_t)CB) * line);
+    uint32_t wq[NC];
+#pragma unroll
+    for (int i = 0; i < NC; i++) {                         // piece q of a stage: block q / 2, substep q % 2
+        const uint32_t q = wave * NC + i;
+        wq[i] = min(q >> 1, p.cblocks - 1 - cb0) * line + (q & 1) * 1024;
+    }
+    const uint32_t l16 = lane * 16;
+    v16i acc[RB][CB];
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) acc[i][j] = v16i{};
+    v4i a[3][2][RB], b[2][CB];
+    auto at = [&](uint32_t step) { return min(step, p.steps - 1) * kPiece; };       // past the last step: any, never used
+    auto issue = [&](int8_t* sm, uint32_t step) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) lds_copy16(wb, l16, wq[i] + at(step), sm + (wave * NC + i) * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load = [&](int slot, int s, uint32_t step) {
+#pragma unroll
+        for (int i = 0; i < RB; i++) a[slot][s][i] = load16(xa[i], l16, at(step) + s * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto fragments = [&](const int8_t* sm, int s) {
+#pragma unroll
+        for (int j = 0; j < CB; j++) b[s][j] = *reinterpret_cast<const v4i*>(sm + (2 * j + s) * 1024 + l16);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto products = [&](int slot, int s) {
+#pragma unroll
+        for (int j = 0; j < CB; j++)
+#pragma unroll
+            for (int i = 0; i < RB; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[slot][s][i], b[s][j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Step kt (slot kt % 3), its first weight fragments read: the second ones are read under the first products, the next
+    // step's first ones under the second, behind the barrier that frees `cur` for step kt + 3 and says that step
+    // kt + 1 (`next`) has landed.  Behind that step's copies this wavefront has copied once more (NC) and, in the
+    // loop, loaded x twice (4 RB: the loads of a later step that feed no product may be left out by the compiler, so the
+    // steps behind the loop count none).  No copy is conditional: with a path that skips one the compiler waits for
+    // every copy in flight before it reads a stage.
+    auto step = [&](int8_t* cur, const int8_t* next, int slot, uint32_t kt, auto loads) {
+        fragments(cur, 1);
+        products(slot, 0);
+        wait_copies<NC + loads.value>();
+        __builtin_amdgcn_s_barrier();
+        issue(cur, kt + 3);
+        load(slot, 0, kt + 3);
+        fragments(next, 0);
+        products(slot, 1);
+        load(slot, 1, kt + 3);
+    };
+    constexpr std::integral_constant<int, 4 * RB> in_loop{};
+    constexpr std::integral_constant<int, 0> behind{};
+    if constexpr (gated(MODE)) {
+        const Buf tb = buffer_of(reinterpret_cast<const int8_t*>(p.tab), TAB);
+#pragma unroll
+        for (int i = 0; i < TAB / 1024 / WR; i++) lds_copy16(tb, l16, (wave * (TAB / 1024 / WR) + i) * 1024, tab + (wave * (TAB / 1024 / WR) + i) * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    auto first = [&](int8_t* sm, int slot) {
+        issue(sm, slot);
+        load(slot, 0, slot);
+        load(slot, 1, slot);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    first(sm0, 0);
+    first(sm1, 1);
+    first(sm2, 2);
+    wait_copies<2 * NC>();                           // x's first loads may have moved behind the copies
+    __builtin_amdgcn_s_barrier();
+    fragments(sm0, 0);
+    uint32_t kt = 0;
+    for (; kt + 3 <= p.steps; kt += 3) {
+        step(sm0, sm1, 0, kt, in_loop);
+        step(sm1, sm2, 1, kt + 1, in_loop);
+        step(sm2, sm0, 2, kt + 2, in_loop);
+    }
+    if (kt < p.steps) step(sm0, sm1, 0, kt, behind);
+    if (kt + 1 < p.steps) step(sm1, sm2, 1, kt + 1, behind);
+    wait_copies<0>();                                // no copy may land after the workgroup ends
+
+    epilogue<MODE, RB, CB>(p, acc, rb0, cb0, l32, lh, (const uint8_t*)tab);
+}
+
+// ---------------------------------------------------------------- a few tiles
+// Products of too few rows to fill the chip with the tiles above: a workgroup computes 32 RB x 32 CB outputs, its wavefronts
+// taking the 64-k steps in turn with operands straight from memory (nothing waits on another wavefront, two steps in flight), and
+// adds their sums in LDS (integer adds: any order).  Bound by the latency of the few steps a wavefront has.
+constexpr uint32_t kMidWaves = 4;
+
+template <uint32_t MODE, int RB, int CB>
+__global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
+    constexpr uint32_t R = 32 * RB, COLS = 32 * CB, OUT = gated(MODE) ? COLS / 2 : COLS;
+    constexpr uint32_t LD = COLS + 8;                // rows four apart 32 banks apart
+    static_assert(!gated(MODE) || CB % 2 == 0, "gate beside up");
+    __shared__ int32_t red[R * LD];
+    const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
+    const uint32_t W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t l32 = lane & 31, lh = lane >> 5, l16 = lane * 16, rb0 = t.r * RB, cb0 = t.c * CB;
+    const uint32_t line = pitch_of(p.steps);
+    Buf xa[RB], wb[CB];                              // blocks past the last: any, never stored
+#pragma unroll
+    for (int i = 0; i < RB; i++) xa[i] = buffer_of(p.a + (uint64_t)min(rb0 + i, p.rblocks - 1) * line, line);
+#pragma unroll
+    for (int j = 0; j < CB; j++) wb[j] = buffer_of(p.w + (uint64_t)min(cb0 + j, p.cblocks - 1) * line, line);
+    v4i a[2][2][RB], b[2][2][CB];
+    auto load = [&](int slot, uint32_t step) {
+        const uint32_t at = min(step, p.steps - 1) * kPiece;       // past the last step: any, never used
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int i = 0; i < RB; i++) a[slot][s][i] = load16(xa[i], l16, at + s * 1024);
+#pragma unroll
+            for (int j = 0; j < CB; j++) b[slot][s][j] = load16(wb[j], l16, at + s * 1024);
+        }
+    };
+    v16i acc[RB][CB];
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) acc[i][j] = v16i{};
+    auto products = [&](int slot) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < RB; i++)
+#pragma unroll
+                for (int j = 0; j < CB; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[slot][s][i], b[slot][s][j], acc[i][j], 0, 0, 0);
+    };
+    load(0, wave);
+    load(1, wave + W);
+    for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
+    for (uint32_t st = wave; st < p.steps; st += 2 * W) {
+        products(0);
+        load(0, st + 2 * W);
+        if (st + W < p.steps) products(1);
+        load(1, st + 3 * W);
+    }
+    lds_barrier();                                   // red is zeros
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                __hip_atomic_fetch_add(&red[(32 * i + 8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[i][j][r],
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    lds_barrier();
+    for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
+        const uint32_t rl = e / OUT, cl = e % OUT, row = rb0 * kLine + rl;
+        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl, col = (gated(MODE) ? cb0 / 2 : cb0) * kLine + cl;
+        if (row >= p.n || col >= p.m) continue;
+        const int32_t s0 = red[rl * LD + at], s1 = gated(MODE) ? red[rl * LD + at + 32] : 0;
+        const double2* c = p.cols + cb0 * kLine + at;
+        store<MODE>(p, row, col, s0, s1, (double)p.amax[row], c[0], gated(MODE) ? c[32] : double2{});
     }
 }
 
 // ---------------------------------------------------------------- few rows
 // At most 16 RF rows: the weight is read once and the time is the latency of a launch, of x and of a
-// weight's bytes.  A workgroup of W wavefronts takes NF fragments of 16 columns (kGated: half gate, half up) at
+// weight's bytes.  A workgroup of W wavefronts takes NF fragments of 16 columns (a gate: half gate, half up) at
 // all of k, the wavefronts its 64-k steps in turn; their sums meet in LDS (integer adds: any order).  With
 // x (DIRECT) a wavefront loads its own steps' pieces of the rows in the operand's layout, keeps them
 // in registers while the rows' maxima meet in LDS, and turns them into codes there: x is read once, no launch
@@ -220,22 +539,22 @@ __device__ __forceinline__ void load_weights(v4i (&b)[NF], const int8_t* const (
 
 template <uint32_t MODE, uint32_t RF, uint32_t NF, uint32_t S, bool DIRECT>
 __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k) {
-    constexpr uint32_t R = 16 * RF, COLS = 16 * NF, OUT = MODE == kGated ? COLS / 2 : COLS;
+    constexpr uint32_t R = 16 * RF, COLS = 16 * NF, OUT = gated(MODE) ? COLS / 2 : COLS;
     constexpr uint32_t LD = COLS + 4;                // the four k groups' rows in different banks
     __shared__ int32_t red[R * LD];                  // the unit's sums, zeros between units
     __shared__ int32_t part[R * kFewWaves], top[R];  // the rows' maxima: of a wavefront's pieces, and all
     const uint32_t W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const uint32_t units = (p.m + OUT - 1) / OUT;
     const int8_t* w[NF];
-    // fragment f of unit u: its column block and half (kGated: gate and up blocks alternate)
+    // fragment f of unit u: its column block and half (a gate's blocks alternate)
     auto weights_of = [&](uint32_t u) {
 #pragma unroll
         for (uint32_t f = 0; f < NF; f++) {
-            constexpr uint32_t per = MODE == kGated ? NF / 2 : NF;
+            constexpr uint32_t per = gated(MODE) ? NF / 2 : NF;
             const uint32_t q = u * per + f % per;
-            const uint32_t blk = MODE == kGated ? 2 * (q >> 1) + f / per : q >> 1;
+            const uint32_t blk = gated(MODE) ? 2 * (q >> 1) + f / per : q >> 1;
             // columns past the last block: any, never stored
-            w[f] = p.w + (uint64_t)min(blk, p.cblocks - 1) * p.steps * kPiece + g * 512 + (q & 1) * 256 + c * 16;
+            w[f] = p.w + (uint64_t)min(blk, p.cblocks - 1) * pitch_of(p.steps) + g * 512 + (q & 1) * 256 + c * 16;
         }
     };
     uint32_t u = blockIdx.x;
@@ -243,39 +562,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
     v4i a[S][RF], b[S][NF];
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     if constexpr (DIRECT) {
-        int4 xv[S][RF][2];
+        Piece xv[S][RF];
         const int16_t* xr[RF];
 #pragma unroll
         for (uint32_t f = 0; f < RF; f++) xr[f] = x + (uint64_t)min(16 * f + c, p.n - 1) * ld;
 #pragma unroll
-        for (uint32_t i = 0; i < S; i++) {
-            const uint32_t k0 = (wave + i * W) * kStep + 16 * g;
+        for (uint32_t i = 0; i < S; i++)
 #pragma unroll
-            for (uint32_t f = 0; f < RF; f++) {
-                if (k0 + 16 <= k) {
-                    xv[i][f][0] = load8(xr[f] + k0);
-                    xv[i][f][1] = load8(xr[f] + k0 + 8);
-                } else {
-                    int16_t e[16];
-#pragma unroll
-                    for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? xr[f][k0 + q] : (int16_t)0;
-                    __builtin_memcpy(&xv[i][f][0], e, 32);
-                }
-            }
-        }
+            for (uint32_t f = 0; f < RF; f++) xv[i][f] = load_piece(xr[f], (wave + i * W) * kStep + 16 * g, k);
 #pragma unroll
         for (uint32_t i = 0; i < S; i++)
             if (wave + i * W < p.steps) load_weights<NF>(b[i], w, wave + i * W);
         // the rows' maxima: this wavefront's pieces, its four k groups, then the wavefronts
 #pragma unroll
         for (uint32_t f = 0; f < RF; f++) {
-            int32_t t = 0;
+            Range range;
 #pragma unroll
-            for (uint32_t i = 0; i < S; i++) {
-                const int16_t* e = reinterpret_cast<const int16_t*>(&xv[i][f][0]);
-#pragma unroll
-                for (int q = 0; q < 16; q++) t = max(t, abs((int32_t)e[q]));
-            }
+            for (uint32_t i = 0; i < S; i++) range.add(xv[i][f]);
+            int32_t t = range.top();
             t = max(t, __shfl_xor(t, 16, 64));
             t = max(t, __shfl_xor(t, 32, 64));
             if (g == 0) part[(16 * f + c) * kFewWaves + wave] = t;
@@ -287,17 +591,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
             for (uint32_t i = 0; i < W; i++) am = max(am, part[(16 * f + c) * kFewWaves + i]);
             if (wave == 0 && g == 0) top[16 * f + c] = am;
             const int32_t rc = (int32_t)recip((uint32_t)am);
+            const bool small = __all(rc < 1 << 23);
 #pragma unroll
-            for (uint32_t i = 0; i < S; i++) {
-                const int16_t* e = reinterpret_cast<const int16_t*>(&xv[i][f][0]);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t word = 0;               // four codes: the top bytes of four sums
-#pragma unroll
-                    for (int h = 0; h < 4; h++) word |= ((uint32_t)(e[4 * q + h] * rc + (1 << 23)) >> 24) << (8 * h);
-                    a[i][f][q] = (int)word;
-                }
-            }
+            for (uint32_t i = 0; i < S; i++) a[i][f] = codes_of(xv[i][f], rc, small);
         }
     } else {
         lds_barrier();                               // red is zeros
@@ -350,13 +646,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
         lds_barrier();
         for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
             const uint32_t row = e / OUT, cl = e % OUT, col = u * OUT + cl;
-            const int32_t s0 = red[row * LD + cl], s1 = MODE == kGated ? red[row * LD + OUT + cl] : 0;
+            const int32_t s0 = red[row * LD + cl], s1 = gated(MODE) ? red[row * LD + OUT + cl] : 0;
             red[row * LD + cl] = 0;
-            if (MODE == kGated) red[row * LD + OUT + cl] = 0;
+            if (gated(MODE)) red[row * LD + OUT + cl] = 0;
             if (row >= p.n || col >= p.m) continue;
             const double am = (double)(DIRECT ? top[row] : p.amax[row]);
-            const uint32_t at = MODE == kGated ? (col >> 5) * 64 + (col & 31) : col;
-            store<MODE>(p, row, col, s0, s1, am, p.cols[at], MODE == kGated ? p.cols[at + 32] : double2{});
+            const uint32_t at = gated(MODE) ? (col >> 5) * 64 + (col & 31) : col;
+            store<MODE>(p, row, col, s0, s1, am, p.cols[at], gated(MODE) ? p.cols[at + 32] : double2{});
         }
         if (next >= units) return;
         u = next;
@@ -379,8 +675,14 @@ int check_weight(const char* what, const cm_linear8_weight* w, bool gated) {
 int quantise(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, hipStream_t s) {
     int8_t* codes = static_cast<int8_t*>(rows);
     int32_t* amax = reinterpret_cast<int32_t*>(codes + codes_bytes(blocks_of(n), k));
-    CM_LAUNCH("linear8_rows_kernel", linear8_rows_kernel, dim3(ceil_div(n, 4)), dim3(256), 0, s, x, x_ld, n, k, codes, amax,
-              steps_of(k));
+#define CM_ROWS(U) \
+    CM_LAUNCH("linear8_rows_kernel", linear8_rows_kernel<U>, dim3(ceil_div(n, 16)), dim3(1024), 0, s, x, x_ld, n, k, codes, amax, steps_of(k))
+    if (k <= 1024) { CM_ROWS(1); }
+    else if (k <= 2048) { CM_ROWS(2); }
+    else if (k <= 4096) { CM_ROWS(4); }
+    else if (k <= 8192) { CM_ROWS(8); }
+    else { CM_ROWS(0); }
+#undef CM_ROWS
     return CM_OK;
 }
 
@@ -410,11 +712,59 @@ int few_rows_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, uint32
 
 template <uint32_t MODE>
 int few_rows(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipStream_t s) {
-    constexpr uint32_t P = MODE == kGated ? 2 : 1;
+    constexpr uint32_t P = gated(MODE) ? 2 : 1;
     const uint32_t cap = 2 * (uint32_t)st->cus;
     if (p.n > 16) return few_rows_at<MODE, 2, P>(p, x, ld, k, std::min(ceil_div(p.m, 16), cap), s);
     if (p.m <= 16 * cap) return few_rows_at<MODE, 1, P>(p, x, ld, k, ceil_div(p.m, 16), s);
     return few_rows_at<MODE, 1, 2 * P>(p, x, ld, k, std::min(ceil_div(p.m, 32), cap), s);
+}
+
+// Tile columns of a strip of an XCD's run (tile_of).
+uint32_t strip_of(uint64_t tiles, uint32_t tc) {
+    const uint64_t run = (tiles + 7) / 8;
+    uint32_t xw = 1;
+    while ((uint64_t)xw * xw < run && xw < tc) xw++;
+    return xw;
+}
+
+template <uint32_t MODE, int RB, int CB>
+int mid_at(const Prod& p, hipStream_t s) {
+    const uint32_t tr = ceil_div(p.rblocks, RB), tc = ceil_div(p.cblocks, CB);
+    CM_LAUNCH("linear8_mid_kernel", (linear8_mid_kernel<MODE, RB, CB>), dim3(tr * tc), dim3(64 * std::min(kMidWaves, p.steps)), 0,
+              s, p, tr, tc, strip_of((uint64_t)tr * tc, tc));
+    return CM_OK;
+}
+
+template <uint32_t MODE, int CB>
+int ring_at(const Prod& p, hipStream_t s) {
+    const uint32_t tr = ceil_div(p.rblocks, 8), tc = ceil_div(p.cblocks, CB);
+    CM_LAUNCH("linear8_ring_kernel", (linear8_ring_kernel<MODE, CB>), dim3(tr * tc), dim3(256), 0, s, p, tr, tc,
+              strip_of((uint64_t)tr * tc, tc));
+    return CM_OK;
+}
+
+// The tile with the least of four estimates in ns, fitted to measured products (rows x k x columns: us of 256 x 128, 256 x 64,
+// 64 x 64 and 32 x 32 tiles): 64 x 960 x 960 9.6 / 6.3 / 6.7 / 3.3; 200 x 4096 x 4096 24.6 / 15.1 / 11.0 / 14.0; 512 x 960 x 2560
+// 10.4 / 6.9 / 8.8 / 7.9; 1024 x 2560 x 960 17.8 / 11.6 / 9.2 / 9.9; 1024 x 4096 x 4096 27.4 / 21.0 / 31.7 / 45.4; 2048 x 4096 x 4096
+// 34.3 / 36.3 / 62.4 / 98.0; 4096 x 960 x 2560 19.1 / 17.9 / 40.4 / 41.5.  A gate's output takes about four times a product's:
+// 300 x 960 x 2560 13.0 / 8.5 / 8.6 / 8.6 (its smallest tile 32 x (32 + 32)), 777 x 768 x 2049 12.6 / 11.7 / 16.0 / 14.7, 2048 x 960
+// x 2560 22.3 / 19.4 / 38.9 / 37.6; 64 x 64 tiles are never its best by more than a few per cent, and are not there for it.
+// Two workgroups of 256 x 128 tiles fit a compute unit, three of 256 x 64.
+template <uint32_t MODE>
+int many_rows(const DeviceState* st, const Prod& p, hipStream_t s) {
+    constexpr bool G = gated(MODE);
+    auto tiles = [&](uint32_t r, uint32_t c) { return (uint64_t)ceil_div(p.rblocks, r) * ceil_div(p.cblocks, c); };
+    const uint64_t cus = (uint64_t)st->cus, steps = p.steps;
+    if (tiles(1, 1) > 0x7FFFFFFFu) return fail(CM_EINVAL, "linear8: %u rows of %u columns", p.n, p.m);
+    const uint64_t r4 = (tiles(8, 4) + cus - 1) / cus * ((G ? 10000 : 6000) + 295 * steps);
+    const uint64_t r2 = std::max(tiles(8, 2), cus) * ((G ? 6000 : 4000) + 200 * steps) / cus;
+    const uint64_t small = 2800 + (G ? tiles(1, 2) * (4000 + 200 * steps) : tiles(1, 1) * (1300 + 145 * steps)) / 1000;
+    if constexpr (!G) {
+        const uint64_t mid = 4500 + std::max(tiles(2, 2) * (7000 + 330 * steps) / 1000, 100 * steps);
+        if (mid <= small && mid <= r2 && mid <= r4) return mid_at<MODE, 2, 2>(p, s);
+    }
+    if (small <= r2 && small <= r4) return mid_at<MODE, 1, G ? 2 : 1>(p, s);
+    return r2 <= r4 ? ring_at<MODE, 2>(p, s) : ring_at<MODE, 4>(p, s);
 }
 
 // The product behind its checks: the rows' codes (the caller's, or made in the workspace), then the kernel.
@@ -433,16 +783,16 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.m = w->m;
     p.steps = steps_of(w->k);
     p.rblocks = blocks_of(p.n);
-    p.cblocks = blocks_of(w->m) * (MODE == kGated ? 2 : 1);
+    p.cblocks = blocks_of(w->m) * (gated(MODE) ? 2 : 1);
     if (!direct) {
         p.a = static_cast<const int8_t*>(rows);
         p.amax = reinterpret_cast<const int32_t*>(p.a + codes_bytes(p.rblocks, w->k));
     }
     p.w = static_cast<const int8_t*>(w->image);
     p.cols = reinterpret_cast<const double2*>(p.w + codes_bytes(p.cblocks, w->k));
-    if (MODE == kGated) {
-        p.act = w->act;
+    if (gated(MODE)) {
         p.sa = w->gate_shift;
+        p.gscale = __builtin_ldexp(1.0, (int)w->gate_shift - 18);
         p.scale = __builtin_ldexp(1.0, -(int)w->out_shift);
         p.tab = w->act == kSilu ? st->ro_tables : st->act_tab + w->act * kActTabBytes;
         p.len = w->act == kSilu ? 0 : st->act_len[w->act];
@@ -451,16 +801,14 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
         const int16_t* src = direct ? x : nullptr;
         return few_rows<MODE>(st, p, src, x_ld, w->k, s);
     }
-    const dim3 grid(ceil_div(p.cblocks, 4), ceil_div(p.rblocks, 2));
-    if (grid.y > 65535u) return fail(CM_EINVAL, "linear8: %u rows", p.n);
-    CM_LAUNCH("linear8_tile_kernel", linear8_tile_kernel<MODE>, grid, dim3(256), 0, s, p);
-    return CM_OK;
+    return many_rows<MODE>(st, p, s);
 }
 
 int check_out(const char* what, const void* out, uint64_t ld, uint32_t n, uint32_t m, uint32_t bytes) {
     if (out == nullptr) return fail(CM_EINVAL, "%s: a null output", what);
     if (reinterpret_cast<uintptr_t>(out) & (bytes - 1)) return fail(CM_EALIGN, "%s: an operand is not aligned to its elements", what);
     if (n > 1 && ld < m) return fail(CM_EINVAL, "%s: rows of %u columns overlap at a stride of %llu", what, m, (unsigned long long)ld);
+    if (n > 1 && ld >= 1u << 23) return fail(CM_EINVAL, "%s: a row stride of %llu (below 2^23)", what, (unsigned long long)ld);
     return CM_OK;
 }
 
@@ -530,5 +878,6 @@ extern "C" int cm_linear8_gated(const cm_linear8_weight* weight, const int16_t* 
     p.n = n;
     p.out = out;
     p.out_ld = out_ld;
-    return product<kGated>(weight, x, x_ld, rows, p, as_stream(stream));
+    return weight->act == kSilu ? product<kSiluGate>(weight, x, x_ld, rows, p, as_stream(stream))
+                                : product<kTableGate>(weight, x, x_ld, rows, p, as_stream(stream));
 }

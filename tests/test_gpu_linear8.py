@@ -51,7 +51,10 @@ def host(t):
 
 SIZES = [(1, 1, 1), (1, 64, 32), (2, 63, 31), (1, 960, 960), (3, 65, 33), (15, 128, 70), (16, 1000, 100), (17, 129, 513),
          (31, 320, 64), (32, 64, 257), (33, 2560, 96), (47, 200, 129), (64, 1024, 64), (65, 77, 300), (100, 640, 1000), (129, 192, 257),
-         (200, 2049, 65), (256, 256, 256), (257, 96, 640), (300, 960, 1600), (513, 128, 384), (777, 65, 129)]
+         (200, 2049, 65), (256, 256, 256), (257, 96, 640), (300, 960, 1600), (513, 128, 384), (777, 65, 129),
+         # 64 x 64 tiles, then 256 x 64 and 256 x 128 ones of 1 to 7 steps, their last rows, columns and tiles part empty
+         (200, 4096, 1100), (1001, 2601, 999), (1025, 64, 4000), (2047, 100, 1601), (1500, 190, 2500), (800, 256, 2049),
+         (2049, 257, 4097), (2049, 64, 4096), (2300, 350, 4100), (4097, 448, 2049)]
 
 
 @pytest.mark.parametrize("n,k,m", SIZES, ids=str)
@@ -108,13 +111,13 @@ def test_rows(L, n, k):
     x = rng.integers(-32768, 32768, (n, k)).astype(np.int16) >> rng.integers(0, 16, (n, 1)).astype(np.int16)
     xv, _ = strided(dev(x), 3, 77)
     r = L.quant_rows(xv)
-    steps, blocks = -(-k // 64), -(-n // 32)
+    steps, pitch, blocks = -(-k // 64), -(-k // 64) | 1, -(-n // 32)
     data = host(r.data)
-    codes = data[:blocks * steps * 2048].view(np.int8).reshape(blocks, steps, 4, 32, 16).transpose(0, 3, 1, 2, 4).reshape(blocks * 32, -1)
+    codes = data[:blocks * pitch * 2048].view(np.int8).reshape(blocks, pitch, 4, 32, 16)[:, :steps].transpose(0, 3, 1, 2, 4).reshape(blocks * 32, -1)
     want, a = O.quant(x)
     np.testing.assert_array_equal(codes[:n, :k], want)
     assert (codes[:n, k:] == 0).all()
-    np.testing.assert_array_equal(data[blocks * steps * 2048:].view(np.int32)[:n], a)
+    np.testing.assert_array_equal(data[blocks * pitch * 2048:].view(np.int32)[:n], a)
 
 
 def extreme(n, k, m, rng):

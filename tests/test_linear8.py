@@ -93,11 +93,12 @@ def test_no_rows(lib):
 
 
 def test_sizes(lib):
-    """Whole 32-line blocks of whole 64-k steps, 16 bytes a channel, 4 a row."""
-    assert lib.cm_linear8_image_bytes(65, 33, 0) == 2 * 2 * 2048 + 64 * 16
+    """Whole 32-line blocks of an odd number of 64-k steps, 16 bytes a channel, 4 a row."""
+    assert lib.cm_linear8_image_bytes(65, 33, 0) == 2 * 3 * 2048 + 64 * 16
+    assert lib.cm_linear8_image_bytes(129, 33, 0) == 2 * 3 * 2048 + 64 * 16
     assert lib.cm_linear8_image_bytes(65, 33, 1) == 2 * lib.cm_linear8_image_bytes(65, 33, 0)
     assert lib.cm_linear8_rows_bytes(1, 64) == 2048 + 128
-    assert lib.cm_linear8_rows_bytes(33, 32768) == 64 * 32768 + 256
+    assert lib.cm_linear8_rows_bytes(33, 32768) == 64 * (32768 + 64) + 256
 
 
 def test_python_refusals():
