@@ -143,11 +143,13 @@ __device__ __forceinline__ Piece load_piece(const int16_t* row, uint32_t k0, uin
     if (k0 + 16 <= k) {
         p.v[0] = load8(row + k0);
         p.v[1] = load8(row + k0 + 8);
-    } else {
+    } else if (k0 < k) {
         int16_t e[16];
 #pragma unroll
         for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? row[k0 + q] : (int16_t)0;
         __builtin_memcpy(&p, e, 32);
+    } else {
+        p.v[0] = p.v[1] = int4{0, 0, 0, 0};
     }
     return p;
 }
@@ -188,15 +190,16 @@ __device__ __forceinline__ v4i codes_of(const Piece& p, int32_t r, bool small) {
     return out;
 }
 
-// 16 rows a workgroup, a wavefront a row: its maximum, then its codes, 16 elements a lane and pass of 1024; rows of up to 1024 U
-// elements stay in registers, U = 0: longer ones are read twice.  A pass's codes go through LDS, so that 16 lanes
-// write 256 consecutive bytes of a block.  Bound by memory for many rows.
-template <int U>
-__global__ __launch_bounds__(1024) void linear8_rows_kernel(const int16_t* __restrict__ x, uint64_t ld, uint32_t n, uint32_t k,
+// RW rows a workgroup, a wavefront a row: its maximum, then its codes, 16 elements a lane and pass of 1024; rows of up to 1024 U
+// elements stay in registers, U = 0: longer ones are read twice.  A pass's codes go through LDS, so that RW lanes
+// write 16 RW consecutive bytes of a block.  Bound by memory for many rows (16 a workgroup: 8192 x 4096 19.0 us; a wavefront's
+// own stores of 16 bytes a line 27), by latency for few (4 a workgroup: 512 x 2560 4.7 us, 16: 6.8).
+template <int U, uint32_t RW>
+__global__ __launch_bounds__(64 * RW) void linear8_rows_kernel(const int16_t* __restrict__ x, uint64_t ld, uint32_t n, uint32_t k,
                                                            int8_t* __restrict__ codes, int32_t* __restrict__ amax, uint32_t steps) {
-    constexpr uint32_t PL = 16 * 16 + 16;                  // bytes of a piece of 16 rows in LDS: pieces in different banks
+    constexpr uint32_t PL = 16 * RW + 16;                  // bytes of a piece of RW rows in LDS: pieces in different banks
     __shared__ __attribute__((aligned(16))) int8_t sm[2][64 * PL];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row0 = blockIdx.x * 16, row = row0 + wave;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row0 = blockIdx.x * RW, row = row0 + wave;
     const int16_t* r = x + (uint64_t)min(row, n - 1) * ld;
     Range range;
     Piece e[U ? U : 1];
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(1024) void linear8_rows_kernel(const int16_t* __res
     if (lane == 0 && row < n) amax[row] = top;
     const int32_t rc = (int32_t)recip((uint32_t)top);
     int8_t* to = codes + (uint64_t)(row0 >> 5) * pitch_of(steps) + (row0 & 31) * 16;
-    const uint32_t piece = threadIdx.x >> 4, line = threadIdx.x & 15;
+    const uint32_t piece = threadIdx.x / RW, line = threadIdx.x % RW;
     auto pass = [&](int i, const Piece& p) {
         *reinterpret_cast<v4i*>(&sm[i & 1][lane * PL + wave * 16]) = codes_of(p, rc, rc < 1 << 23);
         lds_barrier();                                     // two buffers: one barrier a pass
@@ -521,6 +524,85 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
     }
 }
 
+// The same from x: 32 rows by 32 CB columns, S steps a wavefront; the rows' pieces stay in registers while their maxima meet in
+// LDS and become codes there, as in the kernel of few rows: one launch instead of two.
+constexpr uint32_t kDirectWaves = 8, kDirectSteps = 2;
+
+template <uint32_t MODE, int CB, int S>
+__global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k,
+                                                                      uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
+    constexpr uint32_t R = 32, COLS = 32 * CB, OUT = gated(MODE) ? COLS / 2 : COLS, MW = kDirectWaves;
+    constexpr uint32_t LD = COLS + 8;                // rows four apart 32 banks apart
+    static_assert(!gated(MODE) || CB % 2 == 0, "gate beside up");
+    __shared__ int32_t red[R * LD];
+    __shared__ int32_t part[R * MW], top[R];
+    const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
+    const uint32_t W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t l32 = lane & 31, lh = lane >> 5, l16 = lane * 16, row0 = t.r * R, cb0 = t.c * CB;
+    const uint32_t line = pitch_of(p.steps);
+    Buf wb[CB];                                      // blocks past the last: any, never stored
+#pragma unroll
+    for (int j = 0; j < CB; j++) wb[j] = buffer_of(p.w + (uint64_t)min(cb0 + j, p.cblocks - 1) * line, line);
+    v4i a[S][2], b[S][2][CB];
+    auto load = [&](int slot, uint32_t step) {
+        const uint32_t at = min(step, p.steps - 1) * kPiece;       // past the last step: any, its codes are zeros
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int j = 0; j < CB; j++) b[slot][s][j] = load16(wb[j], l16, at + s * 1024);
+    };
+    const int16_t* xr = x + (uint64_t)min(row0 + l32, p.n - 1) * ld;
+    Piece xv[S][2];
+#pragma unroll
+    for (int i = 0; i < S; i++)
+#pragma unroll
+        for (int s = 0; s < 2; s++) xv[i][s] = load_piece(xr, (wave + i * W) * kStep + 32 * s + 16 * lh, k);
+#pragma unroll
+    for (int i = 0; i < S; i++) load(i, wave + i * W);
+    for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
+    Range range;
+#pragma unroll
+    for (int i = 0; i < S; i++)
+#pragma unroll
+        for (int s = 0; s < 2; s++) range.add(xv[i][s]);
+    int32_t am = range.top();
+    am = max(am, __shfl_xor(am, 32, 64));
+    if (lh == 0) part[l32 * MW + wave] = am;
+    lds_barrier();
+    for (uint32_t i = 0; i < W; i++) am = max(am, part[l32 * MW + i]);
+    if (wave == 0 && lh == 0) top[l32] = am;
+    const int32_t rc = (int32_t)recip((uint32_t)am);
+    const bool small = __all(rc < 1 << 23);
+#pragma unroll
+    for (int i = 0; i < S; i++)
+#pragma unroll
+        for (int s = 0; s < 2; s++) a[i][s] = codes_of(xv[i][s], rc, small);
+    v16i acc[CB];
+#pragma unroll
+    for (int j = 0; j < CB; j++) acc[j] = v16i{};
+#pragma unroll
+    for (int i = 0; i < S; i++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int j = 0; j < CB; j++) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i][s], b[i][s][j], acc[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < CB; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            __hip_atomic_fetch_add(&red[(8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[j][r], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+    lds_barrier();
+    for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
+        const uint32_t rl = e / OUT, cl = e % OUT, row = row0 + rl;
+        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl, col = (gated(MODE) ? cb0 / 2 : cb0) * kLine + cl;
+        if (row >= p.n || col >= p.m) continue;
+        const int32_t s0 = red[rl * LD + at], s1 = gated(MODE) ? red[rl * LD + at + 32] : 0;
+        const double2* c = p.cols + cb0 * kLine + at;
+        store<MODE>(p, row, col, s0, s1, (double)top[rl], c[0], gated(MODE) ? c[32] : double2{});
+    }
+}
+
 // ---------------------------------------------------------------- few rows
 // At most 16 RF rows: the weight is read once and the time is the latency of a launch, of x and of a
 // weight's bytes.  A workgroup of W wavefronts takes NF fragments of 16 columns (a gate: half gate, half up) at
@@ -672,11 +754,10 @@ int check_weight(const char* what, const cm_linear8_weight* w, bool gated) {
     return CM_OK;
 }
 
-int quantise(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, hipStream_t s) {
-    int8_t* codes = static_cast<int8_t*>(rows);
-    int32_t* amax = reinterpret_cast<int32_t*>(codes + codes_bytes(blocks_of(n), k));
+template <uint32_t RW>
+int quantise_at(const int16_t* x, uint64_t x_ld, int8_t* codes, int32_t* amax, uint32_t n, uint32_t k, hipStream_t s) {
 #define CM_ROWS(U) \
-    CM_LAUNCH("linear8_rows_kernel", linear8_rows_kernel<U>, dim3(ceil_div(n, 16)), dim3(1024), 0, s, x, x_ld, n, k, codes, amax, steps_of(k))
+    CM_LAUNCH("linear8_rows_kernel", (linear8_rows_kernel<U, RW>), dim3(ceil_div(n, RW)), dim3(64 * RW), 0, s, x, x_ld, n, k, codes, amax, steps_of(k))
     if (k <= 1024) { CM_ROWS(1); }
     else if (k <= 2048) { CM_ROWS(2); }
     else if (k <= 4096) { CM_ROWS(4); }
@@ -684,6 +765,12 @@ int quantise(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k
     else { CM_ROWS(0); }
 #undef CM_ROWS
     return CM_OK;
+}
+
+int quantise(const DeviceState* st, const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, hipStream_t s) {
+    int8_t* codes = static_cast<int8_t*>(rows);
+    int32_t* amax = reinterpret_cast<int32_t*>(codes + codes_bytes(blocks_of(n), k));
+    return n <= 16 * (uint32_t)st->cus ? quantise_at<4>(x, x_ld, codes, amax, n, k, s) : quantise_at<16>(x, x_ld, codes, amax, n, k, s);
 }
 
 int check_rows(const char* what, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n, uint32_t k) {
@@ -735,6 +822,28 @@ int mid_at(const Prod& p, hipStream_t s) {
     return CM_OK;
 }
 
+// Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers), at most a tile a compute
+// unit (each quantises its rows again) and rows in whole 16-byte words.  One launch / two (us; 32 x 32 tiles): 64 x 256 x 1024
+// 3.8 / 5.7, 128 x 960 x 960 5.4 / 6.2, 333 x 960 x 960 7.5 / 7.1; rows of 1001 64 x 1001 x 1537 8.1 / 6.6.
+template <uint32_t MODE>
+bool mid_direct(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld, uint32_t k) {
+    return p.steps <= kDirectWaves * kDirectSteps && aligned16(x) && ld % 8 == 0 && k % 8 == 0 &&
+           (uint64_t)p.rblocks * (p.cblocks / (gated(MODE) ? 2 : 1)) <= (uint64_t)st->cus;
+}
+
+template <uint32_t MODE>
+int mid_direct_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipStream_t s) {
+    constexpr int CB = gated(MODE) ? 2 : 1;
+    const uint32_t tc = p.cblocks / CB, tiles = p.rblocks * tc, xw = strip_of(tiles, tc);
+    const dim3 block(64 * std::min(kDirectWaves, p.steps));
+    if (p.steps <= kDirectWaves) {
+        CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, 1>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw);
+    } else {
+        CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, 2>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw);
+    }
+    return CM_OK;
+}
+
 template <uint32_t MODE, int CB>
 int ring_at(const Prod& p, hipStream_t s) {
     const uint32_t tr = ceil_div(p.rblocks, 8), tc = ceil_div(p.cblocks, CB);
@@ -773,17 +882,18 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     DeviceState* st;
     int rc = state(&st);
     if (rc) return rc;
-    const bool few = p.n <= 32, direct = few && rows == nullptr && steps_of(w->k) <= kFewSteps * kFewWaves;
-    if (rows == nullptr && !direct) {
-        void* ws;
-        if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;
-        if ((rc = quantise(x, x_ld, ws, p.n, w->k, s))) return rc;
-        rows = ws;
-    }
     p.m = w->m;
     p.steps = steps_of(w->k);
     p.rblocks = blocks_of(p.n);
     p.cblocks = blocks_of(w->m) * (gated(MODE) ? 2 : 1);
+    const bool few = p.n <= 32;
+    const bool direct = rows == nullptr && (few ? p.steps <= kFewSteps * kFewWaves : mid_direct<MODE>(st, p, x, x_ld, w->k));
+    if (rows == nullptr && !direct) {
+        void* ws;
+        if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;
+        if ((rc = quantise(st, x, x_ld, ws, p.n, w->k, s))) return rc;
+        rows = ws;
+    }
     if (!direct) {
         p.a = static_cast<const int8_t*>(rows);
         p.amax = reinterpret_cast<const int32_t*>(p.a + codes_bytes(p.rblocks, w->k));
@@ -801,6 +911,7 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
         const int16_t* src = direct ? x : nullptr;
         return few_rows<MODE>(st, p, src, x_ld, w->k, s);
     }
+    if (direct) return mid_direct_at<MODE>(p, x, x_ld, w->k, s);
     return many_rows<MODE>(st, p, s);
 }
 
@@ -844,7 +955,9 @@ extern "C" int cm_linear8_rows(const int16_t* x, uint64_t x_ld, void* rows, uint
     if (rc || n == 0) return rc;
     if (rows == nullptr) return fail(CM_EINVAL, "linear8 rows: a null output");
     if (reinterpret_cast<uintptr_t>(rows) & 255u) return fail(CM_EALIGN, "linear8 rows: the codes must be 256-byte aligned");
-    return quantise(x, x_ld, rows, n, k, as_stream(stream));
+    DeviceState* st;
+    if ((rc = state(&st))) return rc;
+    return quantise(st, x, x_ld, rows, n, k, as_stream(stream));
 }
 
 extern "C" int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n,

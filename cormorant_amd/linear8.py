@@ -120,29 +120,29 @@ class Rows8:
             raise ValueError(f"Rows8: {n} rows of {k} (up to {MAX_N} of {MAX_K})")
         self.cap, self.k, self.n = n, k, 0
         self.data = _buffer(_lib.lib().cm_linear8_rows_bytes(n, k), device)
-        self.device, self.index = self.data.device, self.data.get_device()
+        self.device, self.index, self.at = self.data.device, self.data.get_device(), self.data.data_ptr()
 
 
 def _stride(t: torch.Tensor, name: str, dtype, n: int, width: int) -> int:
-    """The row stride of an operand [n][width] of contiguous columns."""
-    if t.dtype is not dtype or not t.is_cuda:
-        raise ValueError(f"{name} must be a GPU {dtype} tensor")
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] != n or shape[1] != width or stride[1] != 1 and width > 1:
-        raise ValueError(f"{name} must be [{n}][{width}] rows of contiguous columns, got {list(shape)} at strides {list(stride)}")
-    if n > 1:
-        if stride[0] < width:
-            raise ValueError(f"{name}: rows of {width} columns overlap at a stride of {stride[0]}")
-        return stride[0]
-    return width
+    """The row stride of an operand [n][width] of contiguous columns (a call's checks are a third of its time on the host)."""
+    if t.dtype is not dtype or t.shape != (n, width):
+        raise ValueError(f"{name} must be a GPU {dtype} tensor [{n}][{width}], got {t.dtype} {list(t.shape)}")
+    rows, cols = t.stride()
+    if cols != 1 and width > 1:
+        raise ValueError(f"{name} must be rows of contiguous columns, got strides {[rows, cols]}")
+    if n <= 1:
+        return width
+    if rows < width:
+        raise ValueError(f"{name}: rows of {width} columns overlap at a stride of {rows}")
+    return rows
 
 
 def _on(index: int, *on) -> int:
     """The current stream of device ``index``, which every operand must be on and which must be current."""
     for t in on:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"the operands are on cuda:{index} and {t.device}")
-    if index != torch.cuda.current_device():
+        if t.get_device() != index:
+            raise ValueError(f"the weight is on cuda:{index}, an operand on {t.device}")
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"the weight is on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(index)         # torch.cuda.current_stream() takes 2.8 us of a 10 us call
 
@@ -168,12 +168,11 @@ def _x(x: Union[torch.Tensor, Rows8], k: int, what: str):
     if isinstance(x, Rows8):
         if x.k != k:
             raise ValueError(f"{what}: rows of {x.k} against a weight of {k}")
-        return x.n, None, 0, x.data.data_ptr(), x.data
-    if x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"{what}: x must be [n][{k}], got {list(x.shape)}")
-    n = x.shape[0]
-    if n > MAX_N:
-        raise ValueError(f"{what}: {n} rows (up to {MAX_N})")
+        return x.n, None, 0, x.at, x.data
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k or shape[0] > MAX_N:
+        raise ValueError(f"{what}: x must be [n][{k}] of up to {MAX_N} rows, got {list(shape)}")
+    n = shape[0]
     return n, x.data_ptr(), _stride(x, "x", torch.int16, n, k), None, x
 
 
@@ -185,18 +184,22 @@ def linear8(x: Union[torch.Tensor, Rows8], weight: Weight8, out: torch.Tensor, r
     if type(weight) is not Weight8:
         raise ValueError("linear8: a Weight8")
     n, at, ld, codes, t = _x(x, weight.k, "linear8")
-    out_ld = _stride(out, "out", torch.int16 if residual is None else torch.int32, n, weight.m)
-    res_at, res_ld = None, 0
-    if residual is not None:
-        res_at, res_ld = residual.data_ptr(), _stride(residual, "residual", torch.int32, n, weight.m)
-        if not 0 <= shift <= 16:
-            raise ValueError(f"linear8: a residual shift of {shift} (0 .. 16)")
     out_at = out.data_ptr()
     if at == out_at and n:
         raise ValueError("linear8: out is x")
-    stream = _on(weight.index, t, out, residual)
-    _lib.check(_lib.lib().cm_linear8(weight._ref, at, ld, codes, n, out_at, out_ld, res_at, res_ld,
-                                     shift if res_at else 0, stream), "cm_linear8")
+    if residual is None:
+        out_ld = _stride(out, "out", torch.int16, n, weight.m)
+        stream = _on(weight.index, t, out)
+        rc = _lib.lib().cm_linear8(weight._ref, at, ld, codes, n, out_at, out_ld, None, 0, 0, stream)
+    else:
+        if not 0 <= shift <= 16:
+            raise ValueError(f"linear8: a residual shift of {shift} (0 .. 16)")
+        out_ld = _stride(out, "out", torch.int32, n, weight.m)
+        res_ld = _stride(residual, "residual", torch.int32, n, weight.m)
+        stream = _on(weight.index, t, out, residual)
+        rc = _lib.lib().cm_linear8(weight._ref, at, ld, codes, n, out_at, out_ld, residual.data_ptr(), res_ld, shift, stream)
+    if rc:
+        _lib.check(rc, "cm_linear8")
     return out
 
 
@@ -205,11 +208,14 @@ def gated8(x: Union[torch.Tensor, Rows8], weight: GatedWeight8, out: torch.Tenso
     if type(weight) is not GatedWeight8:
         raise ValueError("gated8: a GatedWeight8")
     n, at, ld, codes, t = _x(x, weight.k, "gated8")
-    out_ld, out_at = _stride(out, "out", torch.int16, n, weight.m), out.data_ptr()
+    out_at = out.data_ptr()
     if at == out_at and n:
         raise ValueError("gated8: out is x")
+    out_ld = _stride(out, "out", torch.int16, n, weight.m)
     stream = _on(weight.index, t, out)
-    _lib.check(_lib.lib().cm_linear8_gated(weight._ref, at, ld, codes, n, out_at, out_ld, stream), "cm_linear8_gated")
+    rc = _lib.lib().cm_linear8_gated(weight._ref, at, ld, codes, n, out_at, out_ld, stream)
+    if rc:
+        _lib.check(rc, "cm_linear8_gated")
     return out
 
 
