@@ -35,7 +35,8 @@ LlmAttnScores, VitAttnSoftmax on the unit, LlmAttnPV, LlmAttnMerge: vit.py:19-32
 and ``LlmDecodeAttention`` (LlmAttnPrep's RoPE and cache-row writes, the scores, LlmAttnSoftmax,
 P.V: llm_nodes.py:1012-1030, rowops_nodes.py:893-1236 -> DecodePrepNode + DecodeAttentionNode).
 ``LlmPagedAttention`` (no reference op) is the same over a paged cache and packed tokens:
-PagedPrepNode + PagedAttentionNode.
+PagedPrepNode + PagedAttentionNode.  ``LlmLinear8``, ``LlmGatedLinear8`` and ``LlmColumns`` (no reference ops) are a
+decoder's linear layers with 8-bit weights: Linear8Node, GatedLinear8Node, ColumnsNode.
 """
 from __future__ import annotations
 
@@ -46,8 +47,8 @@ from typing import Any, Callable, Dict, List, Optional, Sequence
 import numpy as np
 
 from . import units
-from .graph import (KEY_QUANTUM, AttentionNode, AttnMergeNode, AttnSoftmaxNode, ConvNode, DecodeAttentionNode, Graph,
-                    LlmAttnConvNode, MatmulNode, PagedAttentionNode, PoolNode, ReshapeNode, ScheduledNode,
+from .graph import (KEY_QUANTUM, AttentionNode, AttnMergeNode, AttnSoftmaxNode, ColumnsNode, ConvNode,
+                    DecodeAttentionNode, GatedLinear8Node, Graph, Linear8Node, LlmAttnConvNode, MatmulNode, PagedAttentionNode, PoolNode, ReshapeNode, ScheduledNode,
                     SchedulerError, SelectRowNode, SoftmaxVopNode, TensorInfo, conv_out, fuse_activations, softmax_regs)
 from .host_ops import (GeluNode, LayerNormNode, LlmAttentionNode, LlmDequantNode, LlmEmbedNode, LlmResAddNode,
                        LlmRMSNormNode, LlmSiluMulNode, LlmToHostNode, SoftmaxNode, TransposeNode)
@@ -494,6 +495,23 @@ def _llm_paged_attention(op, ctx):
     return [prep, att]
 
 
+def _llm_linear8(op, ctx):
+    """inputs [x, w] or [x, w, residual] -> Linear8Node; attributes ``bias``, ``delta_exp`` (with a residual)."""
+    d = op.attrs.get("delta_exp")
+    return Linear8Node(ctx.ins(op), ctx.out(op), bias=op.attrs.get("bias"), delta_exp=None if d is None else int(d))
+
+
+def _llm_gated_linear8(op, ctx):
+    """inputs [x, wg, wu] -> GatedLinear8Node; attributes ``act``, ``gate_exp``, ``up_exp``."""
+    a = op.attrs
+    return GatedLinear8Node(ctx.ins(op), ctx.out(op), act=a.get("act", "silu"), gate_exp=int(a["gate_exp"]),
+                            up_exp=int(a["up_exp"]))
+
+
+def _llm_columns(op, ctx):
+    return ColumnsNode(ctx.ins(op), ctx.out(op), first=int(op.attrs["first"]))
+
+
 def _heads(op):
     a = op.attrs
     H, KV, HD = int(a["num_heads"]), int(a["num_kv_heads"]), int(a["head_dim"])
@@ -595,6 +613,7 @@ LLM_FACTORIES: Dict[str, Callable] = {
     "LlmDequant": _llm_dequant, "LlmToHost": _llm_dequant, "LlmAttention": _llm_attention,
     "VitLayerNorm": _vit_layernorm, "VitResAdd": _llm_resadd, "VitGelu": _vit_gelu, "VitAttention": _vit_attention,
     "LlmDecodeAttention": _llm_decode_attention, "LlmPagedAttention": _llm_paged_attention,
+    "LlmLinear8": _llm_linear8, "LlmGatedLinear8": _llm_gated_linear8, "LlmColumns": _llm_columns,
     "LlmAttnPrep": _llm_attn_prep, "LlmAttnScores": _llm_attn_conv,
     "LlmAttnPV": _llm_attn_conv, "LlmAttnSoftmax": _llm_attn_softmax, "LlmAttnMerge": _llm_attn_merge,
     "LlmSelectRow": _llm_select_row, "VitAttnPrep": _vit_attn_prep, "VitAttnSoftmax": _vit_attn_softmax,

@@ -343,6 +343,122 @@ class PagedAttentionNode(KernelNode):
             raise SchedulerError(f"{what}: window {self.window} (0, or below 2^30)")
 
 
+def _linear8_rows(what: str, x: TensorInfo, outs: int, y: TensorInfo, F: int) -> int:
+    """The exponent of an 8-bit layer's int16 input rows [.., k] whose output is [.., outs]."""
+    k = int(x.shape[-1])
+    if x.kind != "i16" or int(y.shape[-1]) != outs or x.numel * outs != y.numel * k:
+        raise SchedulerError(f"{what}: rows {list(x.shape)} ({x.kind}) -> {list(y.shape)} of {outs} columns")
+    return int(one_exponent(x.exp_full(F), what))
+
+
+def _linear8_weight(what: str, x: TensorInfo, w: TensorInfo) -> np.ndarray:
+    if w.data is None or np.ndim(w.data) != 2 or np.shape(w.data)[0] != int(x.shape[-1]):
+        raise SchedulerError(f"{what}: a constant weight [{int(x.shape[-1])}][m], got {list(w.shape)}")
+    return np.asarray(w.data)
+
+
+def _exponents(what: str, t: TensorInfo, n: int, F: int) -> np.ndarray:
+    e = t.exp_full(F).reshape(-1)
+    if e.size not in (1, n):
+        raise SchedulerError(f"{what}: '{t.onnx_name}' has {e.size} exponents for {n} columns")
+    return np.broadcast_to(e, (n,))
+
+
+def _quantised(what: str, w: np.ndarray, f_in: int, f_out):
+    from .linear8 import quantise_weight
+    try:
+        return quantise_weight(w, f_in, f_out)
+    except ValueError as e:
+        raise SchedulerError(f"{what}: {e}") from None
+
+
+@dataclass
+class Linear8Node(KernelNode):
+    """A decoder's linear layer in 8 bits (linear8.linear8): inputs [x, w] -> int16 rows at the output's
+    exponent (one, or one a column), or [x, w, residual] -> the int32 residual plus the product, whose own
+    exponent ``delta_exp`` is at most 16 coarser (a ResAddRoNode over it, in one call).  ``w`` is float data
+    [k][m], held as ``codes`` int8 and ``mult`` (linear8.quantise_weight); ``bias`` float [m] or None."""
+    inputs: List[TensorInfo]
+    output: TensorInfo
+    bias: Optional[np.ndarray] = None
+    delta_exp: Optional[int] = None
+    F: int = 8
+
+    def __post_init__(self):
+        what, x, y = f"linear8 '{self.output.onnx_name}'", self.inputs[0], self.output
+        w = _linear8_weight(what, x, self.inputs[1])
+        m = w.shape[1]
+        f_x = _linear8_rows(what, x, m, y, self.F)
+        self.shift = 0
+        f_y = _exponents(what, y, m, self.F)
+        if len(self.inputs) == 3:
+            r = self.inputs[2]
+            f_r = int(one_exponent(r.exp_full(self.F), what))
+            if self.delta_exp is None or r.kind != "i32" or y.kind != "i32" or r.numel != y.numel or (f_y != f_r).any():
+                raise SchedulerError(f"{what}: an int32 residual of the output's shape and exponent, and the product's")
+            self.shift = f_r - int(self.delta_exp)
+            if not 0 <= self.shift <= 16:
+                raise SchedulerError(f"{what}: a product at 2^-{self.delta_exp} onto a residual at 2^-{f_r}")
+            f_y = np.full(m, int(self.delta_exp))
+        elif y.kind != "i16":
+            raise SchedulerError(f"{what}: an int16 output")
+        self.codes, self.mult = _quantised(what, w, f_x, f_y)
+        self.bias_raw = None
+        if self.bias is not None:
+            b = np.asarray(self.bias, np.float64).reshape(-1)
+            b = np.rint(b * 2.0 ** f_y) if b.shape == (m,) else np.full(1, np.inf)
+            if not (np.abs(b) < 2.0 ** 31).all():
+                raise SchedulerError(f"{what}: a bias of {m} values within 32 bits")
+            self.bias_raw = b.astype(np.int32)
+
+
+@dataclass
+class GatedLinear8Node(KernelNode):
+    """A feed-forward block's gate in 8 bits (linear8.gated8): act(x Wg) (x Wu) of inputs [x, wg, wu]; the products
+    at 2^-gate_exp and 2^-up_exp, ``act`` "silu", "gelu" or "gelu_tanh" (LlmSiluMul's arithmetic, or the
+    activation unit's)."""
+    inputs: List[TensorInfo]
+    output: TensorInfo
+    act: str = "silu"
+    gate_exp: int = 8
+    up_exp: int = 8
+    F: int = 8
+
+    def __post_init__(self):
+        from .linear8 import gate_shifts
+        what, x, y = f"gated8 '{self.output.onnx_name}'", self.inputs[0], self.output
+        wg, wu = (_linear8_weight(what, x, w) for w in self.inputs[1:])
+        if wg.shape != wu.shape or y.kind != "i16":
+            raise SchedulerError(f"{what}: gate {list(wg.shape)} and up {list(wu.shape)} into int16 rows")
+        f_x = _linear8_rows(what, x, wg.shape[1], y, self.F)
+        self.out_exp = int(one_exponent(y.exp_full(self.F), what))
+        try:
+            self.gate_shift, self.out_shift = gate_shifts(self.act, self.gate_exp, self.up_exp, self.out_exp)
+        except ValueError as e:
+            raise SchedulerError(f"{what}: {e}") from None
+        self.gate_codes, self.gate_mult = _quantised(what, wg, f_x, self.gate_exp)
+        self.up_codes, self.up_mult = _quantised(what, wu, f_x, self.up_exp)
+
+
+@dataclass
+class ColumnsNode(KernelNode):
+    """Columns ``first`` .. of a row tensor (the q, k or v of a fused projection) as a tensor: a view, no copy.  Whole
+    16-byte words, the exponents of the columns it shows."""
+    inputs: List[TensorInfo]
+    output: TensorInfo
+    first: int = 0
+    F: int = 8
+
+    def __post_init__(self):
+        what, x, y = f"columns '{self.output.onnx_name}'", self.inputs[0], self.output
+        m, w = int(x.shape[-1]), int(y.shape[-1])
+        if x.kind != "i16" or y.kind != "i16" or x.numel * w != y.numel * m or not 0 <= self.first <= m - w or \
+                m % 8 or w % 8 or self.first % 8:
+            raise SchedulerError(f"{what}: columns {self.first} .. {self.first + w} of int16 rows {list(x.shape)} (whole words of 8)")
+        if (_exponents(what, x, m, self.F)[self.first:self.first + w] != _exponents(what, y, w, self.F)).any():
+            raise SchedulerError(f"{what}: exponents other than the columns'")
+
+
 def paged_pool(name: str, pages: int, page: int, kv_heads: int, head_dim: int, int8: bool = False) -> TensorInfo:
     """The state tensor of a paged cache's pool: its bytes as int32 words [pages][kv_heads][block / 4]
     (paged.block_bytes; zeros are valid rows of zeros)."""
@@ -716,7 +832,8 @@ def conv_out(size: int, k: int, stride: int, pad_lo: int, pad_hi: int, dil: int 
 
 
 __all__ = ["SchedulerError", "KernelNode", "TensorInfo", "HeadView", "ScheduledNode", "MatmulNode", "MatmulConvNode", "ConvNode", "PoolNode",
-           "ReshapeNode", "SoftmaxVopNode", "DecodeAttentionNode", "PagedAttentionNode", "paged_pool", "RowOpsNode",
+           "ReshapeNode", "SoftmaxVopNode", "DecodeAttentionNode", "PagedAttentionNode", "paged_pool",
+           "Linear8Node", "GatedLinear8Node", "ColumnsNode", "RowOpsNode",
            "LlmAttnConvNode", "KvWriteNode", "AttentionNode", "attn_keys",
            "AttnSoftmaxNode", "AttnMergeNode", "SelectRowNode", "KEY_QUANTUM", "SMX_MAX_KEYS",
            "Graph", "conv_out", "OP_ADD", "OP_SUB",

@@ -24,7 +24,7 @@ from . import _lib
 
 ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 MAX_K, MAX_M, MAX_N, MAX_MULT = 32768, 1 << 20, 1 << 22, 64.0
-SILU_BITS, G_BITS, ACT_BITS = 20, 14, 8
+SILU_BITS, G_BITS, ACT_BITS, MULT_BITS = 20, 14, 8, 18
 
 
 def _buffer(nbytes: int, device) -> torch.Tensor:
@@ -222,7 +222,7 @@ def gated8(x: Union[torch.Tensor, Rows8], weight: GatedWeight8, out: torch.Tenso
 def quantise_weight(w, f_in: int, f_out) -> tuple:
     """(codes int8 [k][m], mult float64 [m]) of a float weight [k][m] (numpy) between rows at 2^-f_in and
     2^-f_out (one exponent, or one a channel): each channel in 127 steps of its largest value, the
-    multiplier in 24 bits."""
+    multiplier in 18 bits (2^-18 of a result of 16: acc a_t M stays below 2^62, 64-bit integers restate it)."""
     import numpy as np
     w = np.asarray(w, np.float64)
     top = np.abs(w).max(axis=0)
@@ -232,7 +232,7 @@ def quantise_weight(w, f_in: int, f_out) -> tuple:
     codes = np.rint(w / step).clip(-127, 127).astype(np.int8)
     mu = np.where(top > 0, step, 0.0) * 2.0 ** (np.asarray(f_out, np.float64) - f_in) / 127.0
     man, exp = np.frexp(mu)
-    mult = np.ldexp(np.rint(man * 2.0 ** 24), exp - 24)
+    mult = np.ldexp(np.rint(man * 2.0 ** MULT_BITS), exp - MULT_BITS)
     if (mult > MAX_MULT).any() or math.isnan(float(mult.sum())):
         raise ValueError(f"quantise_weight: multipliers above {MAX_MULT:g} (exponents {f_in} -> {f_out})")
     return codes, mult

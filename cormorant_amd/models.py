@@ -774,6 +774,24 @@ def smollm2_decode(shape: LlamaShape = LlamaShape(), seed: int = 0, calib_seqs: 
     return g, inputs, exps
 
 
+def _llama_mlp8(add, p, L, e, S, T, om, hcur):
+    """_llama_mlp with 8-bit weights: o and down onto the residual, gate / up and the SiLU gate, one call each."""
+    from .graph import GatedLinear8Node, Linear8Node
+    from .rowops_nodes import RMSNormRoNode
+    T_ = TensorInfo
+    w = lambda nm, k, m: T_(p + nm, [k, m], data=L[nm])                  # noqa: E731
+    h1 = T_(p + "h1", [T, S.d], exp=RES_BITS, kind="i32")
+    add(Linear8Node([om, w("wo", S.heads * S.hd, S.d), hcur], h1, delta_exp=e["a"]), "LlmLinear8", delta_exp=e["a"])
+    x2 = T_(p + "x2", [T, S.d], exp=e["x2"])
+    add(RMSNormRoNode([h1], x2, gamma=L["g2"], eps=S.eps), "LlmRMSNorm", gamma=L["g2"], eps=S.eps)
+    mm = T_(p + "m", [T, S.ff], exp=e["m"])
+    gate = dict(act="silu", gate_exp=int(e["g"]), up_exp=int(e["u"]))
+    add(GatedLinear8Node([x2, w("wg", S.d, S.ff), w("wu", S.d, S.ff)], mm, **gate), "LlmGatedLinear8", **gate)
+    hn = T_(p + "h", [T, S.d], exp=RES_BITS, kind="i32")
+    add(Linear8Node([mm, w("wd", S.ff, S.d), h1], hn, delta_exp=e["d"]), "LlmLinear8", delta_exp=e["d"])
+    return hn
+
+
 def _llama_mlp(add, p, L, e, S, T, om, hcur):
     """A layer behind its attention: the o MatMul, ResAdd, RMSNorm, gate / up, SiluMul, down, ResAdd."""
     from .rowops_nodes import RMSNormRoNode, ResAddRoNode, SiluMulRoNode
@@ -797,15 +815,19 @@ def _llama_mlp(add, p, L, e, S, T, om, hcur):
     return hn
 
 
-def _llama_head(add, S, rows, emb, gf, fin, h):
+def _llama_head(add, S, rows, emb, gf, fin, h, weights8=False):
     """The final RMSNorm, the tied head and the dequant of ``rows`` rows to float32 logits."""
+    from .graph import Linear8Node
     from .rowops_nodes import DequantRoNode, RMSNormRoNode
     T_ = TensorInfo
     xf = T_("xf", [rows, S.d], exp=fin["xf"])
     add(RMSNormRoNode([h], xf, gamma=gf, eps=S.eps), "LlmRMSNorm", gamma=gf, eps=S.eps)
     lq = T_("logits_q", [rows, S.vocab], exp=fin["logits"])
-    add(MatmulNode([xf, T_("w.lm_head", [S.d, S.vocab], data=np.ascontiguousarray(emb.T))], lq), "MatMul",
-        domain="")
+    head = [xf, T_("w.lm_head", [S.d, S.vocab], data=np.ascontiguousarray(emb.T))]
+    if weights8:
+        add(Linear8Node(head, lq), "LlmLinear8")
+    else:
+        add(MatmulNode(head, lq), "MatMul", domain="")
     chunk = next(c for c in range(4096, 0, -8) if S.vocab % c == 0)
     lr = T_("logits_rows", [rows * S.vocab // chunk, chunk], exp=fin["logits"])
     add(ReshapeNode([lq], lr), "Reshape", domain="")
@@ -917,7 +939,8 @@ def smollm2_prefill(shape: LlamaShape, T: int, exps, weights, with_head: bool = 
 
 
 def smollm2_paged(shape: LlamaShape, tokens: int, batch: int, pages: int, page: int, max_pages: int, exps, weights,
-                  int8: bool = False, window: int = 0, with_head: bool = False, as_ops: bool = False):
+                  int8: bool = False, window: int = 0, with_head: bool = False, as_ops: bool = False,
+                  weights8: bool = False):
     """The serving entry over paged caches: ``tokens`` packed rows of ``batch`` sequences -- whole
     prompts, chunks of prompts and single decode tokens in one step, each sequence at its own length.
     Inputs (int32): ids [tokens], q_start [batch + 1], kv_len [batch], table [batch][max_pages] (as
@@ -930,10 +953,13 @@ def smollm2_paged(shape: LlamaShape, tokens: int, batch: int, pages: int, page: 
     (head dim 64 or 128; the rope tables reach max_pages * page positions): RMSNorm; q / k / v; the
     prep and the attention over the pages (PagedPrepNode, PagedAttentionNode); o, ResAdd, RMSNorm,
     gate / up, SiluMul, down, ResAdd.  ``window``: the keys a row sees (0: all).  ``as_ops``: (ops,
-    tensors, inputs, outputs) in place of the graph, the attention as LlmPagedAttention."""
+    tensors, inputs, outputs) in place of the graph, the attention as LlmPagedAttention.
+
+    ``weights8``: the linear layers' weights in 8 bits (Linear8Node, GatedLinear8Node): q / k / v one projection
+    (ColumnsNode views of its rows), o and down straight onto the residual, the gate in one call, the head."""
     from .dtype import AP_FIXED_16_8
     from .frontend import LLM_DOMAIN, OpDesc
-    from .graph import PagedAttentionNode, paged_pool
+    from .graph import ColumnsNode, Linear8Node, PagedAttentionNode, paged_pool
     from .numeric import encode_matmul_weights
     from .rowops_nodes import PagedPrepNode, RMSNormRoNode
 
@@ -969,8 +995,16 @@ def smollm2_paged(shape: LlamaShape, tokens: int, batch: int, pages: int, page: 
         x = T_(p + "x", [tokens, D], exp=e["x"])
         add(RMSNormRoNode([hcur], x, gamma=L["g1"], eps=S.eps), "LlmRMSNorm", gamma=L["g1"], eps=S.eps)
         q, k, v = (T_(p + c, [tokens, n], exp=e[c]) for c, n in (("q", A), ("k", KD), ("v", KD)))
-        for t, w in ((q, "wq"), (k, "wk"), (v, "wv")):
-            add(MatmulNode([x, T_(p + w, [D, t.shape[1]], data=L[w])], t), "MatMul", domain="")
+        if weights8:
+            f_qkv = np.repeat([e["q"], e["k"], e["v"]], [A, KD, KD])
+            qkv = T_(p + "qkv", [tokens, A + 2 * KD], exp=f_qkv)
+            wqkv = T_(p + "wqkv", [D, A + 2 * KD], data=np.concatenate([L["wq"], L["wk"], L["wv"]], axis=1))
+            add(Linear8Node([x, wqkv], qkv), "LlmLinear8")
+            for t, first in ((q, 0), (k, A), (v, A + KD)):
+                add(ColumnsNode([qkv], t, first=first), "LlmColumns", first=first)
+        else:
+            for t, w in ((q, "wq"), (k, "wk"), (v, "wv")):
+                add(MatmulNode([x, T_(p + w, [D, t.shape[1]], data=L[w])], t), "MatMul", domain="")
         qr, om = T_(p + "qr", [tokens, A], exp=e["q"]), T_(p + "om", [tokens, A], exp=e["o"])
         cmr, cfg = softmax_regs(e["s"], 1.0 / math.sqrt(HD), e["p"])
         ins = [q, k, v, pool] + step
@@ -978,8 +1012,8 @@ def smollm2_paged(shape: LlamaShape, tokens: int, batch: int, pages: int, page: 
         add(PagedAttentionNode([qr] + ins[3:], om, window=window, cm=cmr, cfg=cfg, f_v=e["v"], **geo),
             "LlmPagedAttention", ins=ins, outs=[qr, om], f_k=e["k"], f_v=e["v"], cos=cos, sin=sin, window=window,
             cm=cmr, cfg=cfg, **geo)
-        hcur = _llama_mlp(add, p, L, e, S, tokens, om, hcur)
-    out = _llama_head(add, S, tokens, emb, gf, exps[-1], hcur) if with_head else hcur
+        hcur = (_llama_mlp8 if weights8 else _llama_mlp)(add, p, L, e, S, tokens, om, hcur)
+    out = _llama_head(add, S, tokens, emb, gf, exps[-1], hcur, weights8) if with_head else hcur
     graph_inputs = [ids_t] + step
     if as_ops:
         return ops, reg, [t.onnx_name for t in graph_inputs], [out.onnx_name]

@@ -155,12 +155,13 @@ def check(nodes: Iterable, dtype: ApFixed16) -> None:
     exponents only Convs; power-of-two exponents MatMuls (constant B), Convs (per-tensor
     exponents, constant weight and bias), copies that carry one exponent through (Transpose,
     Permute, Reshape with equal exponents), and the LLM-side nodes."""
-    from .graph import (AttentionNode, AttnContractNode, KvWriteNode, LlmAttnConvNode, PagedAttentionNode, PermuteNode,
-                        ReshapeNode, RowOpsNode, SoftmaxVopNode)
+    from .graph import (AttentionNode, AttnContractNode, ColumnsNode, GatedLinear8Node, KvWriteNode, Linear8Node,
+                        LlmAttnConvNode, PagedAttentionNode, PermuteNode, ReshapeNode, RowOpsNode, SoftmaxVopNode)
     from .host_ops import HostNode, LlmEmbedNode
     from .rowops_nodes import PagedPrepNode, RoCallNode, RowOpsAdapter, TransposeRoNode
     llm = (HostNode, LlmEmbedNode, RowOpsAdapter, RoCallNode, RowOpsNode, LlmAttnConvNode, AttnContractNode,
-           AttentionNode, KvWriteNode, PagedAttentionNode, PagedPrepNode, SoftmaxVopNode)
+           AttentionNode, KvWriteNode, PagedAttentionNode, PagedPrepNode, SoftmaxVopNode, Linear8Node, GatedLinear8Node,
+           ColumnsNode)
     F = dtype.frac_bits
     for sn in nodes:
         label = f"{type(sn).__name__} '{sn.output.onnx_name}'"

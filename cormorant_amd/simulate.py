@@ -15,10 +15,10 @@ from typing import Dict, Iterable, List, Optional
 import numpy as np
 import torch
 
-from . import paged, residuals, units
+from . import linear8, paged, residuals, units
 from .dtype import AP_FIXED_16_8, ApFixed16
-from .graph import (AttentionNode, AttnContractNode, AttnMergeNode, AttnSoftmaxNode, ConvNode, DecodeAttentionNode, Graph,
-                    KvWriteNode, LlmAttnConvNode, MatmulConvNode, PagedAttentionNode, SelectRowNode,
+from .graph import (AttentionNode, AttnContractNode, AttnMergeNode, AttnSoftmaxNode, ColumnsNode, ConvNode,
+                    DecodeAttentionNode, GatedLinear8Node, Graph, KvWriteNode, Linear8Node, LlmAttnConvNode, MatmulConvNode, PagedAttentionNode, SelectRowNode,
                     MatmulNode, PermuteNode, PoolNode, ReshapeNode, RowOpsNode, ScheduledNode, SchedulerError, SoftmaxVopNode,
                     SMX_MAX_KEYS, TensorInfo, attn_keys, one_exponent)
 from .packing import conv_bias_image, conv_lowered_b_image, conv_weight_image, pack_matmul_b
@@ -271,6 +271,11 @@ class Simulator:
             raw[sn.output.onnx_name] = self._paged_attention(sn, raw)
         elif isinstance(sn, AttentionNode):
             raw[sn.output.onnx_name] = self._attention(sn, raw)
+        elif isinstance(sn, (Linear8Node, GatedLinear8Node)):
+            raw[sn.output.onnx_name] = self._linear8(sn, raw)
+        elif isinstance(sn, ColumnsNode):
+            x, w = sn.inputs[0], int(sn.output.shape[-1])
+            raw[sn.output.onnx_name] = self._get(x, raw).reshape(-1, int(x.shape[-1]))[:, sn.first:sn.first + w]
         elif isinstance(sn, ScheduledNode):
             raw[sn.output.onnx_name] = self._vectorop(sn, raw)
         else:
@@ -1548,6 +1553,38 @@ class Simulator:
         q = self._get(qt, raw).reshape(qt.shape)
         cache, batch = self._paged(sn, raw)
         return paged.paged_attention(cache, batch, q, self._paged_rows(sn), sn.heads, sn.cm, sn.cfg, sn.window)
+
+    def _weight8(self, sn):
+        """The image of an 8-bit node's weights, found by what they hold (as _constant's): entries and layers of equal
+        weights share one."""
+        w = self._constants.get((id(sn), "weight8"))
+        if w is None:
+            parts = [sn.codes, sn.mult, sn.bias_raw] if isinstance(sn, Linear8Node) else \
+                [sn.gate_codes, sn.up_codes, sn.gate_mult, sn.up_mult]
+            h = hashlib.blake2b(digest_size=16)
+            for a in parts:
+                h.update(b"none" if a is None else np.ascontiguousarray(a).view(np.uint8).reshape(-1))
+            kind = "" if isinstance(sn, Linear8Node) else f" {sn.act} {sn.gate_exp} {sn.up_exp} {sn.out_exp}"
+            key = f"weight8 {parts[0].shape}{kind} {h.hexdigest()}"
+            w = self._images.get(key)
+            if w is None:
+                dev = [None if a is None else torch.from_numpy(np.ascontiguousarray(a)).to(self.device) for a in parts]
+                w = linear8.Weight8(*dev) if isinstance(sn, Linear8Node) else \
+                    linear8.GatedWeight8(*dev, act=sn.act, gate_exp=sn.gate_exp, up_exp=sn.up_exp, out_exp=sn.out_exp)
+                self._images[key] = w
+            self._constants[id(sn), "weight8"] = w
+        return w
+
+    def _linear8(self, sn, raw) -> torch.Tensor:
+        """An 8-bit linear layer or gate of the rows of its first input."""
+        xt, w = sn.inputs[0], self._weight8(sn)
+        x = self._get(xt, raw).reshape(-1, w.k)
+        out = self._new(sn.output).view(-1, w.m)
+        if isinstance(sn, GatedLinear8Node):
+            return linear8.gated8(x, w, out)
+        if len(sn.inputs) == 3:
+            return linear8.linear8(x, w, out, self._get(sn.inputs[2], raw).reshape(-1, w.m), sn.shift)
+        return linear8.linear8(x, w, out)
 
     def _kv_write(self, sn: KvWriteNode, raw) -> torch.Tensor:
         """Row ``pos`` of every sequence's group-major cache from the step's rows, in place."""

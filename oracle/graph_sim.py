@@ -16,6 +16,7 @@ import numpy as np
 
 from oracle import cm
 from oracle import host_ref
+from oracle import linear8 as oracle_linear8
 from oracle import paged as oracle_paged
 from oracle import residual_ref
 from oracle import rowops_adapt
@@ -563,6 +564,21 @@ def forward(graph, inputs, states=None, algo="port", errors_out=None):
                 r = _paged_prep(sn, pool, qs, kl, tb, [rows(t) for t in sn.inputs[:3]])
                 words[...] = pool.data.view(np.int32).astype(np.float64).reshape(words.shape)
             vals[out.onnx_name] = (r / 2.0 ** float(F if out.exp is None else out.exp)).reshape(out.shape)
+        elif kind in ("Linear8Node", "GatedLinear8Node"):
+            xt = sn.inputs[0]
+            x = _raw_of(xt, get(xt)).reshape(-1, int(xt.shape[-1]))
+            if kind == "GatedLinear8Node":
+                table = None if sn.act == "silu" else cm.act_table(5 if sn.act == "gelu" else 6)
+                r = oracle_linear8.gated(x, sn.gate_codes, sn.up_codes, sn.gate_mult, sn.up_mult, sn.act, sn.gate_shift,
+                                         sn.out_shift, table)
+            else:
+                res = None if len(sn.inputs) < 3 else _raw_of(sn.inputs[2], get(sn.inputs[2])).reshape(-1, int(out.shape[-1]))
+                r = oracle_linear8.linear(x, sn.codes, sn.mult, sn.bias_raw, res, sn.shift)
+            fo = np.asarray(F if out.exp is None else out.exp, np.float64)
+            vals[out.onnx_name] = (r.reshape(out.shape) / 2.0 ** fo).reshape(out.shape)
+        elif kind == "ColumnsNode":
+            v = get(sn.inputs[0])
+            vals[out.onnx_name] = v.reshape(-1, v.shape[-1])[:, sn.first:sn.first + int(out.shape[-1])].reshape(out.shape).copy()
         elif kind == "DecodeAttentionNode":
             # per KV group: s = q K^T (wrap rule), the row-mode softmax (VectorOP op 10), o = P V
             qt, kt, vt = sn.inputs[:3]
