@@ -170,6 +170,18 @@ struct Range {
     }
 };
 
+// The largest of N maxima (N a multiple of 4, 16-byte aligned).
+template <uint32_t N>
+__device__ __forceinline__ int32_t top_of(const int32_t* part) {
+    int32_t t = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < N / 4; i++) {
+        const int4 v = reinterpret_cast<const int4*>(part)[i];
+        t = max(max(max(t, v.x), max(v.y, v.z)), v.w);
+    }
+    return t;
+}
+
 // The 16 codes of a piece: the top bytes of x R + 2^23.  `small`: every R of the wavefront is below 2^23 (maxima from 255 on),
 // so that a 24-bit multiply-add does (full rate; a 32-bit product a quarter of it).
 __device__ __forceinline__ v4i codes_of(const Piece& p, int32_t r, bool small) {
@@ -234,16 +246,63 @@ __global__ __launch_bounds__(64 * RW) void linear8_rows_kernel(const int16_t* __
     }
 }
 
+// A row a workgroup, N pieces a lane: few rows, where the time is one row's latency.
+template <uint32_t N>
+__global__ __launch_bounds__(1024) void linear8_row_kernel(const int16_t* __restrict__ x, uint64_t ld, uint32_t k,
+                                                          int8_t* __restrict__ codes, int32_t* __restrict__ amax, uint32_t steps) {
+    __shared__ __attribute__((aligned(16))) int32_t part[16];
+    const uint32_t row = blockIdx.x, W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    Piece e[N];
+    Range range;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) e[i] = load_piece(x + (uint64_t)row * ld, 16 * (threadIdx.x + i * blockDim.x), k);
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) range.add(e[i]);
+    int32_t top = range.top();
+    for (int off = 32; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
+    if (W > 1) {
+        if (lane == 0)
+            for (uint32_t i = wave; i < 16; i += W) part[i] = top;         // absent wavefronts' places too
+        lds_barrier();
+        top = top_of<16>(part);
+    }
+    top = __builtin_amdgcn_readfirstlane(top);
+    if (threadIdx.x == 0) amax[row] = top;
+    const int32_t rc = (int32_t)recip((uint32_t)top);
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+        const uint32_t q = threadIdx.x + i * blockDim.x;
+        if (q < 4 * steps)
+            *reinterpret_cast<v4i*>(codes + (uint64_t)(row >> 5) * pitch_of(steps) + (row & 31) * 16 + q * 512) = codes_of(e[i], rc, rc < 1 << 23);
+    }
+}
+
 // ---------------------------------------------------------------- products
+// What an output element needs besides its sums, loaded before them: its column's parameters and its residual.
+struct Elem {
+    double2 c0{}, c1{};
+    int32_t h = 0;
+};
+template <uint32_t MODE>
+__device__ __forceinline__ Elem element(const Prod& p, uint32_t row, uint32_t col) {
+    Elem e;
+    if (row >= p.n || col >= p.m) return e;
+    const double2* c = p.cols + (gated(MODE) ? (col >> 5) * 64 + (col & 31) : col);
+    e.c0 = c[0];
+    if (gated(MODE)) e.c1 = c[32];
+    if (MODE == kOut32) e.h = p.res[row * p.res_ld + col];
+    return e;
+}
+
 // One output element from the sums of its column (a gate: of both).
 template <uint32_t MODE>
-__device__ __forceinline__ void store(const Prod& p, uint32_t row, uint32_t col, int32_t acc0, int32_t acc1, double a,
-                                      double2 c0, double2 c1) {
-    const double z = scaled(acc0, a, c0);
+__device__ __forceinline__ void store(const Prod& p, uint32_t row, uint32_t col, int32_t acc0, int32_t acc1, double a, const Elem& e) {
+    if (row >= p.n || col >= p.m) return;
+    const double z = scaled(acc0, a, e.c0);
     if (MODE == kOut32) {
-        static_cast<int32_t*>(p.out)[row * p.out_ld + col] = add_res(p.res[row * p.res_ld + col], __double2loint(z), p.shift);
+        static_cast<int32_t*>(p.out)[row * p.out_ld + col] = add_res(e.h, __double2loint(z), p.shift);
     } else {
-        const int32_t o = gated(MODE) ? gate16<MODE>(z, scaled(acc1, a, c1), p.tab, p) : __double2loint(z);
+        const int32_t o = gated(MODE) ? gate16<MODE>(z, scaled(acc1, a, e.c1), p.tab, p) : __double2loint(z);
         static_cast<int16_t*>(p.out)[row * p.out_ld + col] = (int16_t)o;
     }
 }
@@ -497,6 +556,8 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
     };
     load(0, wave);
     load(1, wave + W);
+    const uint32_t row0 = rb0 * kLine, col0 = (gated(MODE) ? cb0 / 2 : cb0) * kLine;
+    const Elem el = element<MODE>(p, row0 + threadIdx.x / OUT, col0 + threadIdx.x % OUT);
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     for (uint32_t st = wave; st < p.steps; st += 2 * W) {
         products(0);
@@ -514,14 +575,15 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
                 __hip_atomic_fetch_add(&red[(32 * i + 8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[i][j][r],
                                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     lds_barrier();
-    for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
-        const uint32_t rl = e / OUT, cl = e % OUT, row = rb0 * kLine + rl;
-        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl, col = (gated(MODE) ? cb0 / 2 : cb0) * kLine + cl;
-        if (row >= p.n || col >= p.m) continue;
+    auto put = [&](uint32_t e, const Elem& x) {
+        const uint32_t rl = e / OUT, cl = e % OUT, row = row0 + rl;
+        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl;
         const int32_t s0 = red[rl * LD + at], s1 = gated(MODE) ? red[rl * LD + at + 32] : 0;
-        const double2* c = p.cols + cb0 * kLine + at;
-        store<MODE>(p, row, col, s0, s1, (double)p.amax[row], c[0], gated(MODE) ? c[32] : double2{});
-    }
+        store<MODE>(p, row, col0 + cl, s0, s1, (double)p.amax[min(row, p.n - 1)], x);
+    };
+    put(threadIdx.x, el);
+    for (uint32_t e = threadIdx.x + blockDim.x; e < R * OUT; e += blockDim.x)
+        put(e, element<MODE>(p, row0 + e / OUT, col0 + e % OUT));
 }
 
 // The same from x: 32 rows by 32 CB columns, S steps a wavefront; the rows' pieces stay in registers while their maxima meet in
@@ -535,7 +597,8 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
     constexpr uint32_t LD = COLS + 8;                // rows four apart 32 banks apart
     static_assert(!gated(MODE) || CB % 2 == 0, "gate beside up");
     __shared__ int32_t red[R * LD];
-    __shared__ int32_t part[R * MW], top[R];
+    __shared__ __attribute__((aligned(16))) int32_t part[R * MW];
+    __shared__ int32_t top[R];
     const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
     const uint32_t W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t l32 = lane & 31, lh = lane >> 5, l16 = lane * 16, row0 = t.r * R, cb0 = t.c * CB;
@@ -559,6 +622,8 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
         for (int s = 0; s < 2; s++) xv[i][s] = load_piece(xr, (wave + i * W) * kStep + 32 * s + 16 * lh, k);
 #pragma unroll
     for (int i = 0; i < S; i++) load(i, wave + i * W);
+    const uint32_t col0 = (gated(MODE) ? cb0 / 2 : cb0) * kLine;
+    const Elem el = element<MODE>(p, row0 + threadIdx.x / OUT, col0 + threadIdx.x % OUT);
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     Range range;
 #pragma unroll
@@ -567,9 +632,10 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
         for (int s = 0; s < 2; s++) range.add(xv[i][s]);
     int32_t am = range.top();
     am = max(am, __shfl_xor(am, 32, 64));
-    if (lh == 0) part[l32 * MW + wave] = am;
+    if (lh == 0)
+        for (uint32_t i = wave; i < MW; i += W) part[l32 * MW + i] = am;       // the places of absent wavefronts too
     lds_barrier();
-    for (uint32_t i = 0; i < W; i++) am = max(am, part[l32 * MW + i]);
+    am = top_of<MW>(part + l32 * MW);
     if (wave == 0 && lh == 0) top[l32] = am;
     const int32_t rc = (int32_t)recip((uint32_t)am);
     const bool small = __all(rc < 1 << 23);
@@ -593,14 +659,15 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
             __hip_atomic_fetch_add(&red[(8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[j][r], __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_WORKGROUP);
     lds_barrier();
-    for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
-        const uint32_t rl = e / OUT, cl = e % OUT, row = row0 + rl;
-        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl, col = (gated(MODE) ? cb0 / 2 : cb0) * kLine + cl;
-        if (row >= p.n || col >= p.m) continue;
+    auto put = [&](uint32_t e, const Elem& x) {
+        const uint32_t rl = e / OUT, cl = e % OUT;
+        const uint32_t at = gated(MODE) ? (cl >> 5) * 64 + (cl & 31) : cl;
         const int32_t s0 = red[rl * LD + at], s1 = gated(MODE) ? red[rl * LD + at + 32] : 0;
-        const double2* c = p.cols + cb0 * kLine + at;
-        store<MODE>(p, row, col, s0, s1, (double)top[rl], c[0], gated(MODE) ? c[32] : double2{});
-    }
+        store<MODE>(p, row0 + rl, col0 + cl, s0, s1, (double)top[rl], x);
+    };
+    if (threadIdx.x < R * OUT) put(threadIdx.x, el);
+    for (uint32_t e = threadIdx.x + blockDim.x; e < R * OUT; e += blockDim.x)
+        put(e, element<MODE>(p, row0 + e / OUT, col0 + e % OUT));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -624,7 +691,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
     constexpr uint32_t R = 16 * RF, COLS = 16 * NF, OUT = gated(MODE) ? COLS / 2 : COLS;
     constexpr uint32_t LD = COLS + 4;                // the four k groups' rows in different banks
     __shared__ int32_t red[R * LD];                  // the unit's sums, zeros between units
-    __shared__ int32_t part[R * kFewWaves], top[R];  // the rows' maxima: of a wavefront's pieces, and all
+    __shared__ __attribute__((aligned(16))) int32_t part[R * kFewWaves];       // the rows' maxima: of a wavefront's pieces,
+    __shared__ int32_t top[R];                                                 // and all
     const uint32_t W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const uint32_t units = (p.m + OUT - 1) / OUT;
     const int8_t* w[NF];
@@ -642,6 +710,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
     uint32_t u = blockIdx.x;
     weights_of(u);
     v4i a[S][RF], b[S][NF];
+    Elem el = element<MODE>(p, threadIdx.x / OUT, u * OUT + threadIdx.x % OUT);
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     if constexpr (DIRECT) {
         Piece xv[S][RF];
@@ -664,13 +733,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
             int32_t t = range.top();
             t = max(t, __shfl_xor(t, 16, 64));
             t = max(t, __shfl_xor(t, 32, 64));
-            if (g == 0) part[(16 * f + c) * kFewWaves + wave] = t;
+            if (g == 0)
+                for (uint32_t i = wave; i < kFewWaves; i += W) part[(16 * f + c) * kFewWaves + i] = t;     // absent wavefronts' too
         }
         lds_barrier();
 #pragma unroll
         for (uint32_t f = 0; f < RF; f++) {
-            int32_t am = 0;
-            for (uint32_t i = 0; i < W; i++) am = max(am, part[(16 * f + c) * kFewWaves + i]);
+            const int32_t am = top_of<kFewWaves>(part + (16 * f + c) * kFewWaves);
             if (wave == 0 && g == 0) top[16 * f + c] = am;
             const int32_t rc = (int32_t)recip((uint32_t)am);
             const bool small = __all(rc < 1 << 23);
@@ -726,18 +795,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
                     __hip_atomic_fetch_add(&red[(16 * f + 4 * g + i) * LD + 16 * q + c], sum[f][q][i], __ATOMIC_RELAXED,
                                            __HIP_MEMORY_SCOPE_WORKGROUP);
         lds_barrier();
-        for (uint32_t e = threadIdx.x; e < R * OUT; e += blockDim.x) {
-            const uint32_t row = e / OUT, cl = e % OUT, col = u * OUT + cl;
+        auto put = [&](uint32_t e, const Elem& x) {
+            const uint32_t row = e / OUT, cl = e % OUT;
             const int32_t s0 = red[row * LD + cl], s1 = gated(MODE) ? red[row * LD + OUT + cl] : 0;
             red[row * LD + cl] = 0;
             if (gated(MODE)) red[row * LD + OUT + cl] = 0;
-            if (row >= p.n || col >= p.m) continue;
-            const double am = (double)(DIRECT ? top[row] : p.amax[row]);
-            const uint32_t at = gated(MODE) ? (col >> 5) * 64 + (col & 31) : col;
-            store<MODE>(p, row, col, s0, s1, am, p.cols[at], gated(MODE) ? p.cols[at + 32] : double2{});
-        }
+            store<MODE>(p, row, u * OUT + cl, s0, s1, (double)(DIRECT ? top[row] : p.amax[min(row, p.n - 1)]), x);
+        };
+        if (threadIdx.x < R * OUT) put(threadIdx.x, el);
+        for (uint32_t e = threadIdx.x + blockDim.x; e < R * OUT; e += blockDim.x)
+            put(e, element<MODE>(p, e / OUT, u * OUT + e % OUT));
         if (next >= units) return;
         u = next;
+        el = element<MODE>(p, threadIdx.x / OUT, u * OUT + threadIdx.x % OUT);
         lds_barrier();                               // red is zeros again
     }
 }
@@ -770,6 +840,17 @@ int quantise_at(const int16_t* x, uint64_t x_ld, int8_t* codes, int32_t* amax, u
 int quantise(const DeviceState* st, const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, hipStream_t s) {
     int8_t* codes = static_cast<int8_t*>(rows);
     int32_t* amax = reinterpret_cast<int32_t*>(codes + codes_bytes(blocks_of(n), k));
+    // A row a workgroup up to a row a compute unit, and up to 1024 rows of more than 8192, which no wavefront's registers hold
+    // (rows x k, us a row / four rows a workgroup): 16 x 2560 2.9 / 3.3, 256 x 2560 3.4 / 3.5, 512 x 2560 4.0 / 3.5; 16 x
+    // 16384 3.5 / 11.2, 512 x 16384 10.1 / 15.8, 2048 x 16384 33.9 / 26.4.
+    if (n <= (k > 8192 ? 1024u : (uint32_t)st->cus)) {
+        if (k <= 16384) {
+            CM_LAUNCH("linear8_rows_kernel", linear8_row_kernel<1>, dim3(n), dim3(64 * ceil_div(k, 1024)), 0, s, x, x_ld, k, codes, amax, steps_of(k));
+        } else {
+            CM_LAUNCH("linear8_rows_kernel", linear8_row_kernel<2>, dim3(n), dim3(1024), 0, s, x, x_ld, k, codes, amax, steps_of(k));
+        }
+        return CM_OK;
+    }
     return n <= 16 * (uint32_t)st->cus ? quantise_at<4>(x, x_ld, codes, amax, n, k, s) : quantise_at<16>(x, x_ld, codes, amax, n, k, s);
 }
 
@@ -783,27 +864,44 @@ int check_rows(const char* what, const int16_t* x, uint64_t x_ld, const void* ro
     return CM_OK;
 }
 
-// Few rows: fragments of columns a workgroup, and the grid.
-template <uint32_t MODE, uint32_t RF, uint32_t NF>
-int few_rows_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, uint32_t grid, hipStream_t s) {
-    const uint32_t W = std::min(kFewWaves, p.steps), per = (p.steps + W - 1) / W;
-#define CM_FEW(S, D) \
-    CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D>), dim3(grid), dim3(64 * W), 0, s, p, x, ld, k)
-    if (x == nullptr) { CM_FEW(kFewSteps, false); }
-    else if (per == 1) { CM_FEW(1, true); }
-    else if (per == 2) { CM_FEW(2, true); }
-    else { CM_FEW(kFewSteps, true); }
-#undef CM_FEW
-    return CM_OK;
+// Few rows.  A workgroup takes 16 columns (a gate 16 of each), 32 where two workgroups of 16 a compute unit do not reach.
+constexpr uint32_t kFewPerCu = 2;
+uint32_t few_cap(const DeviceState* st) { return kFewPerCu * (uint32_t)st->cus; }
+uint32_t few_steps(const Prod& p) { return ceil_div(p.steps, std::min(kFewWaves, p.steps)); }
+
+// From x in one launch, or codes first?  What the one launch repeats in every workgroup is the quantisation: a wavefront's
+// steps, twice for more than 16 rows, times the workgroups a compute unit runs.  Up to 3 of those cost less than the second
+// launch (us, one / two; columns x rows): 960 x 4096 of 1 row 3.8 / 5.2, of 16 4.4 / 5.4, of 32 6.4 / 5.9; 2048 x 4096 of 16 5.9 /
+// 6.2; 2560 x 960 of 16 7.1 / 6.6 (0.5 for a launch less on the host); 4096 x 4096 of 16 8.6 / 7.5, of 1 6.2 / 7.2; 2048 x 16384
+// of 1 8.8 / 7.8, of 16 10.6 / 8.1; 960 x 49152 of 16 10.2 / 12.9.
+bool few_direct(const DeviceState* st, const Prod& p) {
+    const uint32_t cus = (uint32_t)st->cus, wgs = std::min(ceil_div(p.m, 16), few_cap(st)), per = few_steps(p);
+    if (p.n > 16) return per == 1 && wgs <= cus;
+    return per * std::max(wgs, cus) <= 3 * cus || (p.n <= 4 && per <= 4 && wgs <= cus);
 }
 
 template <uint32_t MODE>
 int few_rows(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipStream_t s) {
     constexpr uint32_t P = gated(MODE) ? 2 : 1;
-    const uint32_t cap = 2 * (uint32_t)st->cus;
-    if (p.n > 16) return few_rows_at<MODE, 2, P>(p, x, ld, k, std::min(ceil_div(p.m, 16), cap), s);
-    if (p.m <= 16 * cap) return few_rows_at<MODE, 1, P>(p, x, ld, k, ceil_div(p.m, 16), s);
-    return few_rows_at<MODE, 1, 2 * P>(p, x, ld, k, std::min(ceil_div(p.m, 32), cap), s);
+    const uint32_t cap = few_cap(st), per = few_steps(p);
+    const dim3 block(64 * std::min(kFewWaves, p.steps)), narrow(std::min(ceil_div(p.m, 16), cap)), wide(std::min(ceil_div(p.m, 32), cap));
+#define CM_FEW(RF, NF, S, D, G) \
+    CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D>), G, block, 0, s, p, x, ld, k)
+    if (p.n > 16) {
+        if (x != nullptr) { CM_FEW(2, P, 1, true, narrow); }
+        else { CM_FEW(2, P, kFewSteps, false, narrow); }
+    } else if (p.m > 16 * cap) {                     // columns again and again for a workgroup: a step a wavefront if from x
+        if (x != nullptr) { CM_FEW(1, 2 * P, 1, true, wide); }
+        else { CM_FEW(1, 2 * P, kFewSteps, false, wide); }
+    } else {
+        if (x == nullptr) { CM_FEW(1, P, kFewSteps, false, narrow); }
+        else if (per == 1) { CM_FEW(1, P, 1, true, narrow); }
+        else if (per == 2) { CM_FEW(1, P, 2, true, narrow); }
+        else if (per == 3) { CM_FEW(1, P, 3, true, narrow); }
+        else { CM_FEW(1, P, 4, true, narrow); }
+    }
+#undef CM_FEW
+    return CM_OK;
 }
 
 // Tile columns of a strip of an XCD's run (tile_of).
@@ -887,7 +985,7 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.rblocks = blocks_of(p.n);
     p.cblocks = blocks_of(w->m) * (gated(MODE) ? 2 : 1);
     const bool few = p.n <= 32;
-    const bool direct = rows == nullptr && (few ? p.steps <= kFewSteps * kFewWaves : mid_direct<MODE>(st, p, x, x_ld, w->k));
+    const bool direct = rows == nullptr && (few ? few_direct(st, p) : mid_direct<MODE>(st, p, x, x_ld, w->k));
     if (rows == nullptr && !direct) {
         void* ws;
         if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;

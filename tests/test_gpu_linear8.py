@@ -49,7 +49,8 @@ def host(t):
     return t.cpu().numpy()
 
 
-SIZES = [(1, 1, 1), (1, 64, 32), (2, 63, 31), (1, 960, 960), (3, 65, 33), (15, 128, 70), (16, 1000, 100), (17, 129, 513),
+SIZES = [(1, 1700, 9000), (4, 4000, 300), (5, 4000, 300), (16, 2500, 170), (9, 500, 9001), (30, 2000, 100), (12, 9000, 65),
+         (1, 1, 1), (1, 64, 32), (2, 63, 31), (1, 960, 960), (3, 65, 33), (15, 128, 70), (16, 1000, 100), (17, 129, 513),
          (31, 320, 64), (32, 64, 257), (33, 2560, 96), (47, 200, 129), (64, 1024, 64), (65, 77, 300), (100, 640, 1000), (129, 192, 257),
          (200, 2049, 65), (256, 256, 256), (257, 96, 640), (300, 960, 1600), (513, 128, 384), (777, 65, 129),
          # 64 x 64 tiles, then 256 x 64 and 256 x 128 ones of 1 to 7 steps, their last rows, columns and tiles part empty
@@ -103,7 +104,8 @@ def test_gated(L, oracle_lib, n, k, m, act):
         assert (np.delete(host(wide), np.s_[1:1 + m], axis=1) == GUARD16).all()
 
 
-@pytest.mark.parametrize("n,k", [(1, 1), (1, 17), (5, 63), (16, 64), (17, 65), (33, 1000), (64, 4096), (7, 32768), (700, 129), (1, 8192)], ids=str)
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 17), (5, 63), (16, 64), (17, 65), (33, 1000), (64, 4096), (7, 32768), (700, 129), (1, 8192),
+                                 (300, 2100), (300, 4097), (300, 8000), (257, 16400), (40, 20001), (1030, 8200), (4100, 1100), (4111, 2050), (5000, 65)], ids=str)
 def test_rows(L, n, k):
     """The codes themselves, where the documented layout puts them, and the rows' maxima; k's padding is zeros."""
     from oracle import linear8 as O
