@@ -124,41 +124,78 @@ __global__ __launch_bounds__(256) void linear8_pack_kernel(const int8_t* __restr
 }
 
 // ---------------------------------------------------------------- a row's codes
+__device__ __forceinline__ uint32_t recip(uint32_t a) { return a ? (127u * (1u << 24) + (a >> 1)) / a : 0u; }
+
+typedef short v2s __attribute__((ext_vector_type(2)));
+
+// A row, or with ODD the element before one that starts between two 4-byte words: then loads are of the words it lies in, shifted
+// into place once they are there (16 bytes a lane between two words take 1.4 us more: 16 rows of 1001 x 960 5.6 us, 4.6 with
+// ODD; 4.2 at even strides, 4.4 with ODD).
+template <bool ODD>
+struct Row {
+    const int16_t* p;
+    uint32_t shift;                  // 0, or 16 bits for an element
+};
+template <bool ODD>
+__device__ __forceinline__ Row<ODD> row_of(const int16_t* row) {
+    const uint32_t m = ODD ? (uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1u : 0;
+    return Row<ODD>{row - m, 16 * m};
+}
+
+// 16 elements from k0 of a row of k (zeros past its end); with ODD as they come from memory, until `settle`.
+template <bool ODD>
+struct Piece {
+    int4 v[2];
+};
+template <>
+struct Piece<true> {
+    int4 v[2];
+    uint32_t last;
+};
 __device__ __forceinline__ int4 load8(const int16_t* p) {                   // 8 elements at any alignment
     int4 v;
     __builtin_memcpy(&v, p, 16);
     return v;
 }
-
-__device__ __forceinline__ uint32_t recip(uint32_t a) { return a ? (127u * (1u << 24) + (a >> 1)) / a : 0u; }
-
-typedef short v2s __attribute__((ext_vector_type(2)));
-
-// 16 elements from k0 of a row of k (zeros past its end), as they come from memory.
-struct Piece {
-    int4 v[2];
-};
-__device__ __forceinline__ Piece load_piece(const int16_t* row, uint32_t k0, uint32_t k) {
-    Piece p;
+template <bool ODD>
+__device__ __forceinline__ Piece<ODD> load_piece(const Row<ODD>& r, uint32_t k0, uint32_t k) {
+    constexpr uint32_t N = ODD ? 18 : 16;
+    Piece<ODD> p;
     if (k0 + 16 <= k) {
-        p.v[0] = load8(row + k0);
-        p.v[1] = load8(row + k0 + 8);
+        p.v[0] = load8(r.p + k0);
+        p.v[1] = load8(r.p + k0 + 8);
+        if constexpr (ODD) __builtin_memcpy(&p.last, r.p + k0 + (r.shift ? 16 : 14), 4);     // a word that holds one of them
     } else if (k0 < k) {
-        int16_t e[16];
+        int16_t e[N];                                      // the row's last elements, one by one
+        const uint32_t m = ODD ? r.shift >> 4 : 0;         // at 0 with m: the element before the row is not the call's
 #pragma unroll
-        for (uint32_t q = 0; q < 16; q++) e[q] = k0 + q < k ? row[k0 + q] : (int16_t)0;
-        __builtin_memcpy(&p, e, 32);
+        for (uint32_t q = 0; q < N; q++) e[q] = k0 + q < k + m && (!ODD || k0 + q >= m) ? r.p[k0 + q] : (int16_t)0;
+        __builtin_memcpy(p.v, e, 32);
+        if constexpr (ODD) __builtin_memcpy(&p.last, e + 16, 4);
     } else {
         p.v[0] = p.v[1] = int4{0, 0, 0, 0};
+        if constexpr (ODD) p.last = 0;
     }
     return p;
+}
+template <bool ODD>
+__device__ __forceinline__ void settle(Piece<ODD>& p, const Row<ODD>& r) {
+    if constexpr (ODD) {
+        uint32_t w[9];
+        __builtin_memcpy(w, p.v, 32);
+        w[8] = p.last;
+#pragma unroll
+        for (int q = 0; q < 8; q++) w[q] = __builtin_amdgcn_alignbit(w[q + 1], w[q], r.shift);
+        __builtin_memcpy(p.v, w, 32);
+    }
 }
 
 // The largest and the smallest elements so far, two lanes of 16 bits each: |-32768| has no int16.
 struct Range {
     v2s hi{0, 0}, lo{0, 0};
-    __device__ __forceinline__ void add(const Piece& p) {
-        const v2s* e = reinterpret_cast<const v2s*>(&p);
+    template <bool ODD>
+    __device__ __forceinline__ void add(const Piece<ODD>& p) {
+        const v2s* e = reinterpret_cast<const v2s*>(p.v);
 #pragma unroll
         for (int q = 0; q < 8; q++) {
             hi = __builtin_elementwise_max(hi, e[q]);
@@ -184,8 +221,9 @@ __device__ __forceinline__ int32_t top_of(const int32_t* part) {
 
 // The 16 codes of a piece: the top bytes of x R + 2^23.  `small`: every R of the wavefront is below 2^23 (maxima from 255 on),
 // so that a 24-bit multiply-add does (full rate; a 32-bit product a quarter of it).
-__device__ __forceinline__ v4i codes_of(const Piece& p, int32_t r, bool small) {
-    const v2s* e = reinterpret_cast<const v2s*>(&p);
+template <bool ODD>
+__device__ __forceinline__ v4i codes_of(const Piece<ODD>& p, int32_t r, bool small) {
+    const v2s* e = reinterpret_cast<const v2s*>(p.v);
     v4i out;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -212,9 +250,9 @@ __global__ __launch_bounds__(64 * RW) void linear8_rows_kernel(const int16_t* __
     constexpr uint32_t PL = 16 * RW + 16;                  // bytes of a piece of RW rows in LDS: pieces in different banks
     __shared__ __attribute__((aligned(16))) int8_t sm[2][64 * PL];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row0 = blockIdx.x * RW, row = row0 + wave;
-    const int16_t* r = x + (uint64_t)min(row, n - 1) * ld;
+    const Row<false> r = row_of<false>(x + (uint64_t)min(row, n - 1) * ld);
     Range range;
-    Piece e[U ? U : 1];
+    Piece<false> e[U ? U : 1];
     if constexpr (U != 0) {
 #pragma unroll
         for (int i = 0; i < U; i++) e[i] = load_piece(r, 16 * lane + 1024 * i, k);
@@ -230,7 +268,7 @@ __global__ __launch_bounds__(64 * RW) void linear8_rows_kernel(const int16_t* __
     const int32_t rc = (int32_t)recip((uint32_t)top);
     int8_t* to = codes + (uint64_t)(row0 >> 5) * pitch_of(steps) + (row0 & 31) * 16;
     const uint32_t piece = threadIdx.x / RW, line = threadIdx.x % RW;
-    auto pass = [&](int i, const Piece& p) {
+    auto pass = [&](int i, const Piece<false>& p) {
         *reinterpret_cast<v4i*>(&sm[i & 1][lane * PL + wave * 16]) = codes_of(p, rc, rc < 1 << 23);
         lds_barrier();                                     // two buffers: one barrier a pass
         const uint32_t q = 64 * i + piece;
@@ -252,10 +290,11 @@ __global__ __launch_bounds__(1024) void linear8_row_kernel(const int16_t* __rest
                                                           int8_t* __restrict__ codes, int32_t* __restrict__ amax, uint32_t steps) {
     __shared__ __attribute__((aligned(16))) int32_t part[16];
     const uint32_t row = blockIdx.x, W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    Piece e[N];
+    const Row<false> r = row_of<false>(x + (uint64_t)row * ld);
+    Piece<false> e[N];
     Range range;
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++) e[i] = load_piece(x + (uint64_t)row * ld, 16 * (threadIdx.x + i * blockDim.x), k);
+    for (uint32_t i = 0; i < N; i++) e[i] = load_piece(r, 16 * (threadIdx.x + i * blockDim.x), k);
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) range.add(e[i]);
     int32_t top = range.top();
@@ -590,7 +629,7 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
 // LDS and become codes there, as in the kernel of few rows: one launch instead of two.
 constexpr uint32_t kDirectWaves = 8, kDirectSteps = 2;
 
-template <uint32_t MODE, int CB, int S>
+template <uint32_t MODE, int CB, int S, bool ODD>
 __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k,
                                                                       uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
     constexpr uint32_t R = 32, COLS = 32 * CB, OUT = gated(MODE) ? COLS / 2 : COLS, MW = kDirectWaves;
@@ -614,8 +653,8 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
 #pragma unroll
             for (int j = 0; j < CB; j++) b[slot][s][j] = load16(wb[j], l16, at + s * 1024);
     };
-    const int16_t* xr = x + (uint64_t)min(row0 + l32, p.n - 1) * ld;
-    Piece xv[S][2];
+    const Row<ODD> xr = row_of<ODD>(x + (uint64_t)min(row0 + l32, p.n - 1) * ld);
+    Piece<ODD> xv[S][2];
 #pragma unroll
     for (int i = 0; i < S; i++)
 #pragma unroll
@@ -629,7 +668,10 @@ __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(P
 #pragma unroll
     for (int i = 0; i < S; i++)
 #pragma unroll
-        for (int s = 0; s < 2; s++) range.add(xv[i][s]);
+        for (int s = 0; s < 2; s++) {
+            settle(xv[i][s], xr);
+            range.add(xv[i][s]);
+        }
     int32_t am = range.top();
     am = max(am, __shfl_xor(am, 32, 64));
     if (lh == 0)
@@ -686,7 +728,7 @@ __device__ __forceinline__ void load_weights(v4i (&b)[NF], const int8_t* const (
     for (uint32_t f = 0; f < NF; f++) b[f] = *reinterpret_cast<const v4i*>(w[f] + (uint64_t)step * kPiece);
 }
 
-template <uint32_t MODE, uint32_t RF, uint32_t NF, uint32_t S, bool DIRECT>
+template <uint32_t MODE, uint32_t RF, uint32_t NF, uint32_t S, bool DIRECT, bool ODD>
 __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k) {
     constexpr uint32_t R = 16 * RF, COLS = 16 * NF, OUT = gated(MODE) ? COLS / 2 : COLS;
     constexpr uint32_t LD = COLS + 4;                // the four k groups' rows in different banks
@@ -713,10 +755,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
     Elem el = element<MODE>(p, threadIdx.x / OUT, u * OUT + threadIdx.x % OUT);
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     if constexpr (DIRECT) {
-        Piece xv[S][RF];
-        const int16_t* xr[RF];
+        Piece<ODD> xv[S][RF];
+        Row<ODD> xr[RF];
 #pragma unroll
-        for (uint32_t f = 0; f < RF; f++) xr[f] = x + (uint64_t)min(16 * f + c, p.n - 1) * ld;
+        for (uint32_t f = 0; f < RF; f++) xr[f] = row_of<ODD>(x + (uint64_t)min(16 * f + c, p.n - 1) * ld);
 #pragma unroll
         for (uint32_t i = 0; i < S; i++)
 #pragma unroll
@@ -729,7 +771,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear8_few_kernel(Prod p, con
         for (uint32_t f = 0; f < RF; f++) {
             Range range;
 #pragma unroll
-            for (uint32_t i = 0; i < S; i++) range.add(xv[i][f]);
+            for (uint32_t i = 0; i < S; i++) {
+                settle(xv[i][f], xr[f]);
+                range.add(xv[i][f]);
+            }
             int32_t t = range.top();
             t = max(t, __shfl_xor(t, 16, 64));
             t = max(t, __shfl_xor(t, 32, 64));
@@ -864,6 +909,9 @@ int check_rows(const char* what, const int16_t* x, uint64_t x_ld, const void* ro
     return CM_OK;
 }
 
+// May a row start between two 4-byte words?
+bool odd_rows(const int16_t* x, uint64_t ld) { return (reinterpret_cast<uintptr_t>(x) & 2u) != 0 || (ld & 1u) != 0; }
+
 // Few rows.  A workgroup takes 16 columns (a gate 16 of each), 32 where two workgroups of 16 a compute unit do not reach.
 constexpr uint32_t kFewPerCu = 2;
 uint32_t few_cap(const DeviceState* st) { return kFewPerCu * (uint32_t)st->cus; }
@@ -885,8 +933,13 @@ int few_rows(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld
     constexpr uint32_t P = gated(MODE) ? 2 : 1;
     const uint32_t cap = few_cap(st), per = few_steps(p);
     const dim3 block(64 * std::min(kFewWaves, p.steps)), narrow(std::min(ceil_div(p.m, 16), cap)), wide(std::min(ceil_div(p.m, 32), cap));
-#define CM_FEW(RF, NF, S, D, G) \
-    CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D>), G, block, 0, s, p, x, ld, k)
+    const bool odd = odd_rows(x, ld);
+#define CM_FEW(RF, NF, S, D, G)                                                                                                 \
+    if (D && odd) {                                                                                                             \
+        CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D, D>), G, block, 0, s, p, x, ld, k);              \
+    } else {                                                                                                                    \
+        CM_LAUNCH("linear8_few_kernel", (linear8_few_kernel<MODE, RF, NF, S, D, false>), G, block, 0, s, p, x, ld, k);          \
+    }
     if (p.n > 16) {
         if (x != nullptr) { CM_FEW(2, P, 1, true, narrow); }
         else { CM_FEW(2, P, kFewSteps, false, narrow); }
@@ -921,12 +974,11 @@ int mid_at(const Prod& p, hipStream_t s) {
 }
 
 // Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers), at most a tile a compute
-// unit (each quantises its rows again) and rows in whole 16-byte words.  One launch / two (us; 32 x 32 tiles): 64 x 256 x 1024
-// 3.8 / 5.7, 128 x 960 x 960 5.4 / 6.2, 333 x 960 x 960 7.5 / 7.1; rows of 1001 64 x 1001 x 1537 8.1 / 6.6.
+// unit (each quantises its rows again).  One launch / two (us; 32 x 32 tiles): 64 x 256 x 1024 3.8 / 5.7, 128 x 960 x 960 5.4 / 6.2,
+// 333 x 960 x 960 7.5 / 7.1.
 template <uint32_t MODE>
-bool mid_direct(const DeviceState* st, const Prod& p, const int16_t* x, uint64_t ld, uint32_t k) {
-    return p.steps <= kDirectWaves * kDirectSteps && aligned16(x) && ld % 8 == 0 && k % 8 == 0 &&
-           (uint64_t)p.rblocks * (p.cblocks / (gated(MODE) ? 2 : 1)) <= (uint64_t)st->cus;
+bool mid_direct(const DeviceState* st, const Prod& p) {
+    return p.steps <= kDirectWaves * kDirectSteps && (uint64_t)p.rblocks * (p.cblocks / (gated(MODE) ? 2 : 1)) <= (uint64_t)st->cus;
 }
 
 template <uint32_t MODE>
@@ -934,11 +986,15 @@ int mid_direct_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipS
     constexpr int CB = gated(MODE) ? 2 : 1;
     const uint32_t tc = p.cblocks / CB, tiles = p.rblocks * tc, xw = strip_of(tiles, tc);
     const dim3 block(64 * std::min(kDirectWaves, p.steps));
+    const bool odd = odd_rows(x, ld);
+#define CM_MID(S, O) \
+    CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, S, O>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw)
     if (p.steps <= kDirectWaves) {
-        CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, 1>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw);
+        if (odd) { CM_MID(1, true); } else { CM_MID(1, false); }
     } else {
-        CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, 2>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw);
+        if (odd) { CM_MID(2, true); } else { CM_MID(2, false); }
     }
+#undef CM_MID
     return CM_OK;
 }
 
@@ -985,7 +1041,7 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.rblocks = blocks_of(p.n);
     p.cblocks = blocks_of(w->m) * (gated(MODE) ? 2 : 1);
     const bool few = p.n <= 32;
-    const bool direct = rows == nullptr && (few ? few_direct(st, p) : mid_direct<MODE>(st, p, x, x_ld, w->k));
+    const bool direct = rows == nullptr && (few ? few_direct(st, p) : mid_direct<MODE>(st, p));
     if (rows == nullptr && !direct) {
         void* ws;
         if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;
