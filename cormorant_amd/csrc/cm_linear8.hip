@@ -973,18 +973,24 @@ int mid_at(const Prod& p, hipStream_t s) {
     return CM_OK;
 }
 
-// Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers), at most a tile a compute
-// unit (each quantises its rows again).  One launch / two (us; 32 x 32 tiles): 64 x 256 x 1024 3.8 / 5.7, 128 x 960 x 960 5.4 / 6.2,
-// 333 x 960 x 960 7.5 / 7.1.
+// Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers); each workgroup quantises
+// its rows again.  Tiles of 32 columns up to one a compute unit, of 64 up to two (a gate's 32 + 32 up to 5 / 4), else 0: codes first.
+// One launch of tiles of 32 / of 64 / two launches (us): 64 x 256 x 1024 3.8 / 4.4 / 5.7, 333 x 256 x 1024 4.7 / 4.5 / 6.7, 128 x 960
+// x 960 5.4 / 6.0 / 6.2, 333 x 960 x 960 7.5 / 6.1 / 7.1, 640 x 960 x 1600 12.0 / 8.6 / 9.6, 333 x 1000 x 4000 14.8 / 11.9 / 11.0;
+// gates of 960 x 2560, 128 rows 8.5 / 8.7, 333 15.7 / 12.3.
 template <uint32_t MODE>
-bool mid_direct(const DeviceState* st, const Prod& p) {
-    return p.steps <= kDirectWaves * kDirectSteps && (uint64_t)p.rblocks * (p.cblocks / (gated(MODE) ? 2 : 1)) <= (uint64_t)st->cus;
+uint32_t mid_direct(const DeviceState* st, const Prod& p) {
+    if (p.steps > kDirectWaves * kDirectSteps) return 0;
+    auto fit = [&](uint32_t columns, uint32_t quarters) {
+        return 4 * (uint64_t)p.rblocks * ceil_div(p.cblocks, columns) <= quarters * (uint64_t)st->cus;
+    };
+    if (gated(MODE)) return fit(2, 5) ? 2 : 0;
+    return fit(1, 4) ? 1 : fit(2, 8) ? 2 : 0;
 }
 
-template <uint32_t MODE>
+template <uint32_t MODE, int CB>
 int mid_direct_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipStream_t s) {
-    constexpr int CB = gated(MODE) ? 2 : 1;
-    const uint32_t tc = p.cblocks / CB, tiles = p.rblocks * tc, xw = strip_of(tiles, tc);
+    const uint32_t tc = ceil_div(p.cblocks, CB), tiles = p.rblocks * tc, xw = strip_of(tiles, tc);
     const dim3 block(64 * std::min(kDirectWaves, p.steps));
     const bool odd = odd_rows(x, ld);
 #define CM_MID(S, O) \
@@ -1041,7 +1047,8 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.rblocks = blocks_of(p.n);
     p.cblocks = blocks_of(w->m) * (gated(MODE) ? 2 : 1);
     const bool few = p.n <= 32;
-    const bool direct = rows == nullptr && (few ? few_direct(st, p) : mid_direct<MODE>(st, p));
+    const uint32_t columns = rows == nullptr && !few ? mid_direct<MODE>(st, p) : 0;
+    const bool direct = few ? rows == nullptr && few_direct(st, p) : columns != 0;
     if (rows == nullptr && !direct) {
         void* ws;
         if ((rc = workspace(st, rows_bytes(p.n, w->k), &ws, s))) return rc;
@@ -1065,7 +1072,9 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
         const int16_t* src = direct ? x : nullptr;
         return few_rows<MODE>(st, p, src, x_ld, w->k, s);
     }
-    if (direct) return mid_direct_at<MODE>(p, x, x_ld, w->k, s);
+    if constexpr (!gated(MODE))
+        if (columns == 1) return mid_direct_at<MODE, 1>(p, x, x_ld, w->k, s);
+    if (columns == 2) return mid_direct_at<MODE, 2>(p, x, x_ld, w->k, s);
     return many_rows<MODE>(st, p, s);
 }
 
