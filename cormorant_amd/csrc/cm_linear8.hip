@@ -349,11 +349,13 @@ __device__ __forceinline__ void store(const Prod& p, uint32_t row, uint32_t col,
 // ---------------------------------------------------------------- many rows
 // LDS reads, LDS copies and vector memory each move 64 bytes a cycle and compute unit (measured), an i8 MFMA of 32 x
 // 32 x 32 takes 32 cycles: what bounds a product is how often its operands pass through those two ports.  So a
-// wavefront takes 64 rows by 128 columns, WR of them side by side over the same columns: x's fragments, which no other wavefront
-// reads, go from memory straight into registers, three steps ahead; the weight's 128 columns go through a ring of
-// three LDS stages, copied three steps ahead.  A 64-k step of two such workgroups on a compute unit (WR = 4) is 1024 cycles of MFMA
+// wavefront takes 64 rows by 128 columns, four of them side by side over the same columns: x's fragments, which no other
+// wavefront reads, go from memory straight into registers, three steps ahead; the weight's columns go through a ring of
+// three LDS stages, copied three steps ahead.  A 64-k step of two such workgroups on a compute unit is 1024 cycles of MFMA
 // on each SIMD, 64 KiB of LDS reads, 16 KiB of copies and 32 KiB of loads.  Operand pieces lie in memory, in LDS and in the
-// registers in one order (a lane's 16 bytes at 16 lane): whole lines, no bank conflict.
+// registers in one order (a lane's 16 bytes at 16 lane): whole lines, no bank conflict.  Fewer rows take a wavefront of 32
+// rows by 128 or 64 columns (RB, CB: blocks of a wavefront): half or a quarter of a workgroup's work, for a chip with fewer
+// tiles than it holds.
 // Buffer accesses: a block's base in scalar registers, the lane's 16 bytes in one vector register, the step's offset
 // scalar.  Copies to LDS go this way and not as global_load_lds, which the compiler counts as a flat access: every wait
 // for a register load or an LDS read behind one becomes a wait for all (8192 x 4096 x 8192: 268 us, 260 this way).
@@ -442,9 +444,9 @@ __device__ __forceinline__ void epilogue(const Prod& p, const v16i (&acc)[RB][CB
     }
 }
 
-template <uint32_t MODE, int CB>
+template <uint32_t MODE, int RB, int CB>
 __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
-    constexpr int WR = 4, RB = 2, NC = 2 * CB / WR;        // wavefronts; blocks of one; copies a wavefront and step
+    constexpr int WR = 4, NC = 2 * CB / WR;                // wavefronts; copies a wavefront and step
     __shared__ __attribute__((aligned(1024))) int8_t sm0[2 * CB * 1024];
     __shared__ __attribute__((aligned(1024))) int8_t sm1[2 * CB * 1024];
     __shared__ __attribute__((aligned(1024))) int8_t sm2[2 * CB * 1024];
@@ -553,49 +555,42 @@ __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t t
 // adds their sums in LDS (integer adds: any order).  Bound by the latency of the few steps a wavefront has.
 constexpr uint32_t kMidWaves = 4;
 
-template <uint32_t MODE, int RB, int CB>
+template <uint32_t MODE, int CB>
 __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
-    constexpr uint32_t R = 32 * RB, COLS = 32 * CB, OUT = gated(MODE) ? COLS / 2 : COLS;
+    constexpr uint32_t R = 32, COLS = 32 * CB, OUT = gated(MODE) ? COLS / 2 : COLS;
     constexpr uint32_t LD = COLS + 8;                // rows four apart 32 banks apart
     static_assert(!gated(MODE) || CB % 2 == 0, "gate beside up");
     __shared__ int32_t red[R * LD];
     const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
     const uint32_t W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t l32 = lane & 31, lh = lane >> 5, l16 = lane * 16, rb0 = t.r * RB, cb0 = t.c * CB;
+    const uint32_t l32 = lane & 31, lh = lane >> 5, l16 = lane * 16, row0 = t.r * R, cb0 = t.c * CB;
     const uint32_t line = pitch_of(p.steps);
-    Buf xa[RB], wb[CB];                              // blocks past the last: any, never stored
-#pragma unroll
-    for (int i = 0; i < RB; i++) xa[i] = buffer_of(p.a + (uint64_t)min(rb0 + i, p.rblocks - 1) * line, line);
+    const Buf xa = buffer_of(p.a + (uint64_t)t.r * line, line);
+    Buf wb[CB];                                      // blocks past the last: any, never stored
 #pragma unroll
     for (int j = 0; j < CB; j++) wb[j] = buffer_of(p.w + (uint64_t)min(cb0 + j, p.cblocks - 1) * line, line);
-    v4i a[2][2][RB], b[2][2][CB];
+    v4i a[2][2], b[2][2][CB];
     auto load = [&](int slot, uint32_t step) {
         const uint32_t at = min(step, p.steps - 1) * kPiece;       // past the last step: any, never used
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-#pragma unroll
-            for (int i = 0; i < RB; i++) a[slot][s][i] = load16(xa[i], l16, at + s * 1024);
+            a[slot][s] = load16(xa, l16, at + s * 1024);
 #pragma unroll
             for (int j = 0; j < CB; j++) b[slot][s][j] = load16(wb[j], l16, at + s * 1024);
         }
     };
-    v16i acc[RB][CB];
+    v16i acc[CB];
 #pragma unroll
-    for (int i = 0; i < RB; i++)
-#pragma unroll
-        for (int j = 0; j < CB; j++) acc[i][j] = v16i{};
+    for (int j = 0; j < CB; j++) acc[j] = v16i{};
     auto products = [&](int slot) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int i = 0; i < RB; i++)
-#pragma unroll
-                for (int j = 0; j < CB; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[slot][s][i], b[slot][s][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < CB; j++) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[slot][s], b[slot][s][j], acc[j], 0, 0, 0);
     };
     load(0, wave);
     load(1, wave + W);
-    const uint32_t row0 = rb0 * kLine, col0 = (gated(MODE) ? cb0 / 2 : cb0) * kLine;
+    const uint32_t col0 = (gated(MODE) ? cb0 / 2 : cb0) * kLine;
     const Elem el = element<MODE>(p, row0 + threadIdx.x / OUT, col0 + threadIdx.x % OUT);
     for (uint32_t e = threadIdx.x; e < R * LD; e += blockDim.x) red[e] = 0;
     for (uint32_t st = wave; st < p.steps; st += 2 * W) {
@@ -606,13 +601,11 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
     }
     lds_barrier();                                   // red is zeros
 #pragma unroll
-    for (int i = 0; i < RB; i++)
+    for (int j = 0; j < CB; j++)
 #pragma unroll
-        for (int j = 0; j < CB; j++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                __hip_atomic_fetch_add(&red[(32 * i + 8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[i][j][r],
-                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        for (int r = 0; r < 16; r++)
+            __hip_atomic_fetch_add(&red[(8 * (r >> 2) + 4 * lh + (r & 3)) * LD + 32 * j + l32], acc[j][r], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_WORKGROUP);
     lds_barrier();
     auto put = [&](uint32_t e, const Elem& x) {
         const uint32_t rl = e / OUT, cl = e % OUT, row = row0 + rl;
@@ -965,27 +958,28 @@ uint32_t strip_of(uint64_t tiles, uint32_t tc) {
     return xw;
 }
 
-template <uint32_t MODE, int RB, int CB>
+template <uint32_t MODE, int CB>
 int mid_at(const Prod& p, hipStream_t s) {
-    const uint32_t tr = ceil_div(p.rblocks, RB), tc = ceil_div(p.cblocks, CB);
-    CM_LAUNCH("linear8_mid_kernel", (linear8_mid_kernel<MODE, RB, CB>), dim3(tr * tc), dim3(64 * std::min(kMidWaves, p.steps)), 0,
+    const uint32_t tr = p.rblocks, tc = ceil_div(p.cblocks, CB);
+    CM_LAUNCH("linear8_mid_kernel", (linear8_mid_kernel<MODE, CB>), dim3(tr * tc), dim3(64 * std::min(kMidWaves, p.steps)), 0,
               s, p, tr, tc, strip_of((uint64_t)tr * tc, tc));
     return CM_OK;
 }
 
 // Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers); each workgroup quantises
-// its rows again.  Tiles of 32 columns up to one a compute unit, of 64 up to two (a gate's 32 + 32 up to 5 / 4), else 0: codes first.
-// One launch of tiles of 32 / of 64 / two launches (us): 64 x 256 x 1024 3.8 / 4.4 / 5.7, 333 x 256 x 1024 4.7 / 4.5 / 6.7, 128 x 960
-// x 960 5.4 / 6.0 / 6.2, 333 x 960 x 960 7.5 / 6.1 / 7.1, 640 x 960 x 1600 12.0 / 8.6 / 9.6, 333 x 1000 x 4000 14.8 / 11.9 / 11.0;
-// gates of 960 x 2560, 128 rows 8.5 / 8.7, 333 15.7 / 12.3.
+// its rows again.  Tiles of 32 columns up to one a compute unit, of 64 up to two; a gate's, of 32 + 32, up to 5 / 2 steps of a
+// wavefront a compute unit; else 0: codes first.  One launch of tiles of 32 / of 64 / two launches (us, 0.5 to 1 more for the second
+// launch on the host): 64 x 256 x 1024 3.7 / 4.3 / 5.9, 512 x 256 x 1024 4.6 / 4.5 / 6.8, 2048 x 256 x 1024 8.8 / 7.7 / 7.4, 200 x 960 x
+// 960 5.6 / 6.1 / 6.6, 333 x 960 x 960 7.6 / 6.2 / 7.4, 512 x 960 x 1600 12.5 / 9.0 / 8.9, 1024 x 960 x 960 12.1 / 8.7 / 9.1, 333 x 1000
+// x 4000 15.8 / 12.5 / 9.5; gates of 576 x 1536, 128 rows 5.8 / 7.4, 200 8.3 / 8.2, 512 11.9 / 8.6, of 256 x 1024, 512 rows 5.7 / 7.5.
 template <uint32_t MODE>
 uint32_t mid_direct(const DeviceState* st, const Prod& p) {
-    if (p.steps > kDirectWaves * kDirectSteps) return 0;
-    auto fit = [&](uint32_t columns, uint32_t quarters) {
-        return 4 * (uint64_t)p.rblocks * ceil_div(p.cblocks, columns) <= quarters * (uint64_t)st->cus;
-    };
-    if (gated(MODE)) return fit(2, 5) ? 2 : 0;
-    return fit(1, 4) ? 1 : fit(2, 8) ? 2 : 0;
+    const uint32_t per = ceil_div(p.steps, kDirectWaves);
+    if (per > kDirectSteps) return 0;
+    auto tiles = [&](uint32_t columns) { return (uint64_t)p.rblocks * ceil_div(p.cblocks, columns); };
+    const uint64_t cus = (uint64_t)st->cus;
+    if (gated(MODE)) return 2 * per * tiles(2) <= 5 * cus ? 2 : 0;
+    return tiles(1) <= cus ? 1 : tiles(2) <= 2 * cus ? 2 : 0;
 }
 
 template <uint32_t MODE, int CB>
@@ -1004,36 +998,37 @@ int mid_direct_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipS
     return CM_OK;
 }
 
-template <uint32_t MODE, int CB>
+template <uint32_t MODE, int RB, int CB>
 int ring_at(const Prod& p, hipStream_t s) {
-    const uint32_t tr = ceil_div(p.rblocks, 8), tc = ceil_div(p.cblocks, CB);
-    CM_LAUNCH("linear8_ring_kernel", (linear8_ring_kernel<MODE, CB>), dim3(tr * tc), dim3(256), 0, s, p, tr, tc,
+    const uint32_t tr = ceil_div(p.rblocks, 4 * RB), tc = ceil_div(p.cblocks, CB);
+    CM_LAUNCH("linear8_ring_kernel", (linear8_ring_kernel<MODE, RB, CB>), dim3(tr * tc), dim3(256), 0, s, p, tr, tc,
               strip_of((uint64_t)tr * tc, tc));
     return CM_OK;
 }
 
-// The tile with the least of four estimates in ns, fitted to measured products (rows x k x columns: us of 256 x 128, 256 x 64,
-// 64 x 64 and 32 x 32 tiles): 64 x 960 x 960 9.6 / 6.3 / 6.7 / 3.3; 200 x 4096 x 4096 24.6 / 15.1 / 11.0 / 14.0; 512 x 960 x 2560
-// 10.4 / 6.9 / 8.8 / 7.9; 1024 x 2560 x 960 17.8 / 11.6 / 9.2 / 9.9; 1024 x 4096 x 4096 27.4 / 21.0 / 31.7 / 45.4; 2048 x 4096 x 4096
-// 34.3 / 36.3 / 62.4 / 98.0; 4096 x 960 x 2560 19.1 / 17.9 / 40.4 / 41.5.  A gate's output takes about four times a product's:
-// 300 x 960 x 2560 13.0 / 8.5 / 8.6 / 8.6 (its smallest tile 32 x (32 + 32)), 777 x 768 x 2049 12.6 / 11.7 / 16.0 / 14.7, 2048 x 960
-// x 2560 22.3 / 19.4 / 38.9 / 37.6; 64 x 64 tiles are never its best by more than a few per cent, and are not there for it.
-// Two workgroups of 256 x 128 tiles fit a compute unit, three of 256 x 64.
+// The tile with the least of four estimates in ns, fitted to measured products (rows x k x columns: us of 256 x 128, 128 x 128,
+// 128 x 64 and 32 x 32 tiles): 128 x 2560 x 960 17.2 / 10.5 / 6.9 / 4.4; 512 x 960 x 2560 10.3 / 6.8 / 5.0 / 7.9; 1000 x 1024 x 1024 10.4 /
+// 6.9 / 5.0 / 6.9; 1024 x 2560 x 960 17.5 / 10.9 / 7.5 / 9.9; 2048 x 960 x 1600 11.0 / 7.6 / 7.6 / 15.8; 2048 x 8192 x 2048 46.8 / 36.5 /
+// 39.9 / 105; 4096 x 960 x 2560 20.4 / 18.7 / 17.7 / 44.0; 2048 x 4096 x 4096 35.2 / 35.3 / 41.7 / 99.7.  Gates (the smallest tile 32 x
+// (32 + 32)): 300 x 960 x 2560 12.9 / 8.2 / 5.9 / 8.5; 777 x 768 x 2049 12.6 / 8.5 / 8.3 / 15.1; 2048 x 960 x 2560 22.3 / 20.7 / 19.3 /
+// 39.5.  A compute unit holds two workgroups of 256 x 128, four of 128 x 128 and more than its work of the others.
 template <uint32_t MODE>
 int many_rows(const DeviceState* st, const Prod& p, hipStream_t s) {
     constexpr bool G = gated(MODE);
+    constexpr int C0 = G ? 2 : 1;                          // the smallest tile's blocks of columns
     auto tiles = [&](uint32_t r, uint32_t c) { return (uint64_t)ceil_div(p.rblocks, r) * ceil_div(p.cblocks, c); };
+    if (tiles(1, C0) > 0x7FFFFFFFu) return fail(CM_EINVAL, "linear8: %u rows of %u columns", p.n, p.m);
     const uint64_t cus = (uint64_t)st->cus, steps = p.steps;
-    if (tiles(1, 1) > 0x7FFFFFFFu) return fail(CM_EINVAL, "linear8: %u rows of %u columns", p.n, p.m);
-    const uint64_t r4 = (tiles(8, 4) + cus - 1) / cus * ((G ? 10000 : 6000) + 295 * steps);
-    const uint64_t r2 = std::max(tiles(8, 2), cus) * ((G ? 6000 : 4000) + 200 * steps) / cus;
-    const uint64_t small = 2800 + (G ? tiles(1, 2) * (4000 + 200 * steps) : tiles(1, 1) * (1300 + 145 * steps)) / 1000;
-    if constexpr (!G) {
-        const uint64_t mid = 4500 + std::max(tiles(2, 2) * (7000 + 330 * steps) / 1000, 100 * steps);
-        if (mid <= small && mid <= r2 && mid <= r4) return mid_at<MODE, 2, 2>(p, s);
-    }
-    if (small <= r2 && small <= r4) return mid_at<MODE, 1, G ? 2 : 1>(p, s);
-    return r2 <= r4 ? ring_at<MODE, 2>(p, s) : ring_at<MODE, 4>(p, s);
+    // quarters of a round of tiles: at least so many; whole rounds behind the first where a compute unit has one or two tiles at a time
+    auto rounds = [&](uint64_t t) { return 4 * t <= 3 * cus ? 3 : (t + cus - 1) / cus * 4; };
+    const uint64_t big = 4000 + rounds(tiles(8, 4)) * ((G ? 5000 : 2800) + 430 * steps) / 4;
+    const uint64_t square = 2400 + rounds(tiles(4, 4)) * ((G ? 3000 : 1400) + 250 * steps) / 4;
+    const uint64_t tall = 2400 + std::max(4 * tiles(4, 2), 3 * cus) * ((G ? 1500 : 700) + 150 * steps) / (4 * cus);
+    const uint64_t small = 2500 + std::max(tiles(1, C0), cus) * (G ? 1100 + 60 * steps : 700 + 30 * steps) / cus;
+    const uint64_t best = std::min(std::min(big, square), std::min(tall, small));
+    if (best == small) return mid_at<MODE, C0>(p, s);
+    if (best == tall) return ring_at<MODE, 1, 2>(p, s);
+    return best == square ? ring_at<MODE, 1, 4>(p, s) : ring_at<MODE, 2, 4>(p, s);
 }
 
 // The product behind its checks: the rows' codes (the caller's, or made in the workspace), then the kernel.
