@@ -37,10 +37,9 @@ constexpr uint32_t kPieces = 4096;                                    // of the 
 inline uint32_t steps_of(uint32_t k) { return ceil_div(k, kStep); }
 inline uint32_t blocks_of(uint32_t lines) { return ceil_div(lines, kLine); }
 
-// Where a rows image's maxima and a weight image's channel parameters start (behind the blocks).
-// Blocks of lines start an odd number of 2 KiB pieces apart: at a power of two, all that the workgroups read at one time
-// would lie in the same few channels of the L2s and of the memory.
-__host__ __device__ inline uint32_t pitch_of(uint32_t steps) { return (steps | 1u) * kPiece; }
+// Bytes of a block of lines; where a rows image's maxima and a weight image's channel parameters start (behind the blocks).  An
+// odd number of pieces between blocks, for k of powers of two, measured the same (8192 x 4096 x 8192).
+__host__ __device__ inline uint32_t pitch_of(uint32_t steps) { return steps * kPiece; }
 inline size_t codes_bytes(uint32_t blocks, uint32_t k) { return (size_t)blocks * pitch_of(steps_of(k)); }
 inline size_t rows_bytes(uint32_t n, uint32_t k) { return codes_bytes(blocks_of(n), k) + (size_t)blocks_of(n) * kLine * 4; }
 inline size_t image_bytes(uint32_t k, uint32_t m, bool gated) {
@@ -1073,6 +1072,36 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     return many_rows<MODE>(st, p, s);
 }
 
+// n rows of some bytes, `pitch` bytes apart.
+struct Extent {
+    uintptr_t at;
+    uint64_t pitch, bytes;
+};
+
+// Have two operands a byte in common?  Exact for equal pitches (columns of one buffer); others that reach into each other count as
+// sharing one.
+bool share(const Extent& a, const Extent& b, uint32_t n) {
+    typedef unsigned __int128 Wide;
+    const Wide ae = (Wide)a.at + (Wide)(n - 1) * a.pitch + a.bytes, be = (Wide)b.at + (Wide)(n - 1) * b.pitch + b.bytes;
+    if (ae <= b.at || be <= a.at) return false;
+    if (n == 1 || a.pitch != b.pitch) return true;
+    const uint64_t d = a.at <= b.at ? (b.at - a.at) % a.pitch : a.pitch - 1 - (a.at - b.at - 1) % a.pitch;       // b's column behind a's
+    return d < a.bytes || d + b.bytes > a.pitch;
+}
+
+Extent extent(const void* t, uint64_t ld, uint64_t columns, uint32_t bytes) {
+    return Extent{reinterpret_cast<uintptr_t>(t), ld * bytes, columns * bytes};
+}
+
+// The output against x and the residual (another workgroup may still read what one has written), but for the residual's own rows.
+int check_apart(const char* what, const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, uint32_t n, const Extent& out,
+                const Extent* res) {
+    if (x != nullptr && share(extent(x, x_ld, w->k, 2), out, n)) return fail(CM_EINVAL, "%s: the output overlaps x", what);
+    if (res == nullptr || (res->at == out.at && (n == 1 || res->pitch == out.pitch))) return CM_OK;
+    if (share(*res, out, n)) return fail(CM_EINVAL, "%s: the output overlaps the residual at another place or stride", what);
+    return CM_OK;
+}
+
 int check_out(const char* what, const void* out, uint64_t ld, uint32_t n, uint32_t m, uint32_t bytes) {
     if (out == nullptr) return fail(CM_EINVAL, "%s: a null output", what);
     if (reinterpret_cast<uintptr_t>(out) & (bytes - 1)) return fail(CM_EALIGN, "%s: an operand is not aligned to its elements", what);
@@ -1124,15 +1153,17 @@ extern "C" int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uin
     using namespace cm;
     int rc = check_weight("linear8", weight, false);
     if (rc || (rc = check_rows("linear8", x, x_ld, rows, n, weight->k)) || n == 0) return rc;
-    if ((rc = check_out("linear8", out, out_ld, n, weight->m, residual ? 4 : 2))) return rc;
+    const uint32_t bytes = residual ? 4 : 2;
+    const Extent to = extent(out, out_ld, weight->m, bytes), from = extent(residual, residual_ld, weight->m, 4);
+    if ((rc = check_out("linear8", out, out_ld, n, weight->m, bytes))) return rc;
+    if (residual != nullptr && (rc = check_out("linear8", residual, residual_ld, n, weight->m, 4))) return rc;
+    if ((rc = check_apart("linear8", weight, x, x_ld, n, to, residual ? &from : nullptr))) return rc;
     if (shift > 16) return fail(CM_EINVAL, "linear8: a residual shift of %u (up to 16)", shift);
     Prod p{};
     p.n = n;
     p.out = out;
     p.out_ld = out_ld;
     if (residual == nullptr) return product<kOut16>(weight, x, x_ld, rows, p, as_stream(stream));
-    if ((rc = check_out("linear8", residual, residual_ld, n, weight->m, 4))) return rc;
-    if (residual == out && residual_ld != out_ld && n > 1) return fail(CM_EINVAL, "linear8: the output is the residual at another stride");
     p.res = residual;
     p.res_ld = residual_ld;
     p.shift = shift;
@@ -1145,6 +1176,7 @@ extern "C" int cm_linear8_gated(const cm_linear8_weight* weight, const int16_t* 
     int rc = check_weight("linear8 gated", weight, true);
     if (rc || (rc = check_rows("linear8 gated", x, x_ld, rows, n, weight->k)) || n == 0) return rc;
     if ((rc = check_out("linear8 gated", out, out_ld, n, weight->m, 2))) return rc;
+    if ((rc = check_apart("linear8 gated", weight, x, x_ld, n, extent(out, out_ld, weight->m, 2), nullptr))) return rc;
     Prod p{};
     p.n = n;
     p.out = out;

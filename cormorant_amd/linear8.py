@@ -8,9 +8,13 @@ and a quarter of the byte products.  The reference's MatmulKernel has no 8-bit w
 and the gate are its row-ops jobs (rowops_nodes.py:401-447, 540-563), GELU its activation unit's table.
 The framework trains nothing, so neither has a backward pass.
 
-A ``Weight8`` / ``GatedWeight8`` lays its codes out once.  ``Rows8`` holds the codes of rows that several
-products read (``quant_rows``); a call given int16 rows makes them itself.  Calls enqueue on the current
-torch stream of the weight's device.
+A ``Weight8`` / ``GatedWeight8`` lays its codes out once, on the stream that is current then.  ``Rows8`` holds the
+codes of rows that several products read (``quant_rows``); a call given int16 rows makes them itself.  Calls enqueue on
+the current torch stream of the weight's device, which must be the current device.  A call given int16 rows may hold
+their codes in the device's workspace, like the units' calls: one stream at a time, and once before a capture at the
+same sizes.  A call given a Rows8 takes no workspace, so that two streams, or graphs replayed beside each other, each
+with a Rows8 of its own, do not meet.  A replayed graph writes the rows it was captured with; ``Rows8.n`` is of the last
+call, not of a replay.
 """
 from __future__ import annotations
 
@@ -180,13 +184,12 @@ def linear8(x: Union[torch.Tensor, Rows8], weight: Weight8, out: torch.Tensor, r
             shift: int = 0) -> torch.Tensor:
     """cm_linear8: out [n][m] = x's rows (int16 [n][k], or their codes) times the weight, int16; with a
     ``residual`` (int32 [n][m]) out is int32, the residual plus the product << ``shift`` (0 .. 16), and may
-    be the residual.  Rows may be strided.  out is apart from x."""
+    be the residual.  Rows may be strided (out's and the residual's below 2^23 elements).  out shares no element
+    with x, nor with a residual that it is not."""
     if type(weight) is not Weight8:
         raise ValueError("linear8: a Weight8")
     n, at, ld, codes, t = _x(x, weight.k, "linear8")
     out_at = out.data_ptr()
-    if at == out_at and n:
-        raise ValueError("linear8: out is x")
     if residual is None:
         out_ld = _stride(out, "out", torch.int16, n, weight.m)
         stream = _on(weight.index, t, out)
@@ -204,13 +207,11 @@ def linear8(x: Union[torch.Tensor, Rows8], weight: Weight8, out: torch.Tensor, r
 
 
 def gated8(x: Union[torch.Tensor, Rows8], weight: GatedWeight8, out: torch.Tensor) -> torch.Tensor:
-    """cm_linear8_gated: out [n][m] int16 = act(x Wg) (x Wu), x as linear8's; out is apart from x."""
+    """cm_linear8_gated: out [n][m] int16 = act(x Wg) (x Wu), x and out as linear8's."""
     if type(weight) is not GatedWeight8:
         raise ValueError("gated8: a GatedWeight8")
     n, at, ld, codes, t = _x(x, weight.k, "gated8")
     out_at = out.data_ptr()
-    if at == out_at and n:
-        raise ValueError("gated8: out is x")
     out_ld = _stride(out, "out", torch.int16, n, weight.m)
     stream = _on(weight.index, t, out)
     rc = _lib.lib().cm_linear8_gated(weight._ref, at, ld, codes, n, out_at, out_ld, stream)

@@ -589,9 +589,11 @@ size_t cm_linear8_rows_bytes(uint32_t n, uint32_t k);
 int cm_linear8_rows(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, void* stream);
 
 /* o of n rows: x (rows x_ld elements apart, 2-byte aligned) or, x NULL, their codes.  out int16 rows out_ld apart; with a
- * residual (int32, shift 0 .. 16) int32 rows, which may be the residual's own.  out is apart from x otherwise.  Called
- * with x, the codes may stand in the device's workspace: a call of the same sizes before a stream captures it, and no
- * two on different streams at once; with codes the workspace may still hold partial sums. */
+ * residual (int32, shift 0 .. 16) int32 rows, which may be the residual's own (same address and stride).  The strides of
+ * out and the residual are below 2^23.  An output that otherwise shares a byte with x or the residual is refused
+ * (CM_EINVAL); one that reaches into them at another stride counts as sharing.  Called with x, the codes may stand
+ * in the device's workspace: a call of the same sizes before a stream captures it, and no two on different streams at
+ * once.  Called with codes it takes none. */
 int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n, void* out,
                uint64_t out_ld, const int32_t* residual, uint64_t residual_ld, uint32_t shift, void* stream);
 

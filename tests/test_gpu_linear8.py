@@ -54,7 +54,7 @@ SIZES = [(1, 1700, 9000), (4, 4000, 300), (5, 4000, 300), (16, 2500, 170), (9, 5
          (1, 1, 1), (1, 64, 32), (2, 63, 31), (1, 960, 960), (3, 65, 33), (15, 128, 70), (16, 1000, 100), (17, 129, 513),
          (31, 320, 64), (32, 64, 257), (33, 2560, 96), (47, 200, 129), (64, 1024, 64), (65, 77, 300), (100, 640, 1000), (129, 192, 257),
          (200, 2049, 65), (256, 256, 256), (257, 96, 640), (300, 960, 1600), (513, 128, 384), (777, 65, 129),
-         # 64 x 64 tiles, then 256 x 64 and 256 x 128 ones of 1 to 7 steps, their last rows, columns and tiles part empty
+         # 32 x 32 tiles and 128 x 64 ones of 1 to 7 steps and more, their last rows, columns and tiles part empty
          (200, 4096, 1100), (1001, 2601, 999), (1025, 64, 4000), (2047, 100, 1601), (1500, 190, 2500), (800, 256, 2049),
          (2049, 257, 4097), (2049, 64, 4096), (2300, 350, 4100), (4097, 448, 2049)]
 
@@ -105,6 +105,66 @@ def test_gated(L, oracle_lib, n, k, m, act):
         assert (np.delete(host(wide), np.s_[1:1 + m], axis=1) == GUARD16).all()
 
 
+# 128 x 128 and 256 x 128 tiles, steps of each residue of the ring's three stages
+@pytest.mark.parametrize("n,k,m", [(300, 64, 8190), (300, 128, 8190), (300, 150, 8190), (1793, 1270, 3001), (1793, 1344, 3001), (1793, 1401, 3000)], ids=str)
+@pytest.mark.parametrize("form", ["plain", "both"])
+def test_large_tiles(L, n, k, m, form):
+    test_linear(L, n, k, m, form)
+
+
+@pytest.mark.parametrize("n,k,m", [(800, 128, 2300), (1793, 190, 1025), (513, 445, 2300), (1300, 64, 8190), (1300, 121, 8190), (5000, 1150, 513)], ids=str)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_large_gate_tiles(L, oracle_lib, n, k, m, act):
+    test_gated(L, oracle_lib, n, k, m, act)
+
+
+@pytest.mark.parametrize("n", [1, 9, 33, 90, 600])
+def test_columns_of_one_buffer(L, n):
+    """x and out as columns of the same rows, the output behind x and before it; other columns stay."""
+    import torch
+    from oracle import linear8 as O
+    rng = np.random.default_rng(n)
+    k, m = 200, 72
+    x, (w, mult) = rows(rng, n, k), weights(rng, k, m)
+    weight = L.Weight8(dev(w), dev(mult))
+    for at_x, at_o in ((0, k), (m, 0), (m + 3, 1)):
+        wide = torch.full((n, k + m + 5), GUARD16, dtype=torch.int16, device="cuda")
+        xv, ov = wide[:, at_x:at_x + k], wide[:, at_o:at_o + m]
+        xv.copy_(dev(x))
+        L.linear8(xv, weight, ov)
+        want = np.full((n, k + m + 5), GUARD16, np.int16)
+        want[:, at_x:at_x + k], want[:, at_o:at_o + m] = x, O.linear(x, w, mult)
+        np.testing.assert_array_equal(host(wide), want)
+
+
+def test_two_streams(L):
+    """Products of their own Rows8 on two streams, replayed beside each other."""
+    import torch
+    from oracle import linear8 as O
+    rng = np.random.default_rng(5)
+    n, k, m = 600, 1500, 700
+    xs, (w, mult) = [rows(rng, n, k) for _ in range(2)], weights(rng, k, m)
+    weight = L.Weight8(dev(w), dev(mult))
+    torch.cuda.synchronize()
+    dx, codes = [dev(x) for x in xs], [L.Rows8(n, k) for _ in range(2)]
+    outs, graphs, streams = [torch.zeros(n, m, dtype=torch.int16, device="cuda") for _ in xs], [], [torch.cuda.Stream() for _ in xs]
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            L.linear8(L.quant_rows(dx[i], codes[i]), weight, outs[i])
+        graphs.append(g)
+    for turn in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, o in zip(xs, outs):
+            np.testing.assert_array_equal(host(o), O.linear(x, w, mult), err_msg=f"turn {turn}")
+
+
 @pytest.mark.parametrize("n,k", [(1, 1), (1, 17), (5, 63), (16, 64), (17, 65), (33, 1000), (64, 4096), (7, 32768), (700, 129), (1, 8192),
                                  (300, 2100), (300, 4097), (300, 8000), (257, 16400), (40, 20001), (1030, 8200), (4100, 1100), (4111, 2050), (5000, 65)], ids=str)
 def test_rows(L, n, k):
@@ -114,13 +174,13 @@ def test_rows(L, n, k):
     x = rng.integers(-32768, 32768, (n, k)).astype(np.int16) >> rng.integers(0, 16, (n, 1)).astype(np.int16)
     xv, _ = strided(dev(x), 3, 77)
     r = L.quant_rows(xv)
-    steps, pitch, blocks = -(-k // 64), -(-k // 64) | 1, -(-n // 32)
+    steps, blocks = -(-k // 64), -(-n // 32)
     data = host(r.data)
-    codes = data[:blocks * pitch * 2048].view(np.int8).reshape(blocks, pitch, 4, 32, 16)[:, :steps].transpose(0, 3, 1, 2, 4).reshape(blocks * 32, -1)
+    codes = data[:blocks * steps * 2048].view(np.int8).reshape(blocks, steps, 4, 32, 16).transpose(0, 3, 1, 2, 4).reshape(blocks * 32, -1)
     want, a = O.quant(x)
     np.testing.assert_array_equal(codes[:n, :k], want)
     assert (codes[:n, k:] == 0).all()
-    np.testing.assert_array_equal(data[blocks * pitch * 2048:].view(np.int32)[:n], a)
+    np.testing.assert_array_equal(data[blocks * steps * 2048:].view(np.int32)[:n], a)
 
 
 def extreme(n, k, m, rng):

@@ -80,6 +80,39 @@ def test_layer_forms(torch_gpu, n, act, fg):
     np.testing.assert_array_equal(nodes[2].reference([want["c"], None, None]), want["y"])
 
 
+@pytest.mark.parametrize("reader", ["out", "reshape", "add", "relu", "matmul", "transpose", "silumul"])
+def test_readers_of_columns(torch_gpu, reader):
+    """Columns of a projection into nodes that read whole tensors, or out of the graph: as if they were a copy."""
+    from cormorant_amd.graph import MatmulNode, OP_ADD, OP_RELU, ReshapeNode, ScheduledNode
+    from cormorant_amd.rowops_nodes import SiluMulRoNode, TransposeRoNode
+    from cormorant_amd.simulate import Simulator
+    rng = np.random.default_rng(len(reader))
+    n, d = 24, 32
+    x, p = T("x", [n, d], exp=8), T("p", [n, 3 * d], exp=8)
+    c, c2, y = T("c", [n, d], exp=8), T("c2", [n, d], exp=8), T("y", [n, d], exp=8)
+    nodes = [Linear8Node([x, T("w", [d, 3 * d], data=rng.standard_normal((d, 3 * d)) * 0.2)], p), ColumnsNode([p], c, first=d),
+             ColumnsNode([p], c2, first=2 * d)]
+    if reader == "out":
+        y = c
+    elif reader == "reshape":
+        y = T("y", [n // 2, 2 * d], exp=8)
+        nodes += [ReshapeNode([c], y)]
+    elif reader == "add":
+        nodes += [ScheduledNode([c, c2], y, OP_ADD)]
+    elif reader == "relu":
+        nodes += [ScheduledNode([c], y, OP_RELU)]
+    elif reader == "matmul":
+        nodes += [MatmulNode([c, T("v", [d, d], data=rng.standard_normal((d, d)) * 0.2)], y)]
+    elif reader == "transpose":
+        y = T("y", [d, n], exp=8)
+        nodes += [TransposeRoNode([c], y, perm=(1, 0))]
+    else:
+        nodes += [SiluMulRoNode([c, c2], y)]
+    g = Graph(nodes, input_tensors=[x], output_tensors=[y, c])
+    f = {"x": np.rint(rng.standard_normal((n, d)) * 300) / 256}
+    same(Simulator(g)._forward_pass(f), og.forward(g, f), reader)
+
+
 def test_captured_pass_replayed(torch_gpu, model):
     """forward_raw captured once, replayed as the lengths grow with eager passes between, every replay as the oracle."""
     from cormorant_amd.simulate import Simulator

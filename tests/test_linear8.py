@@ -7,7 +7,8 @@ from fractions import Fraction
 import numpy as np
 import pytest
 
-OK = 0x10000                       # an aligned address that no refused call reads
+OK = 0x10000                       # an aligned address that no refused call reads, TO another
+TO = 0x20000
 
 
 @pytest.fixture(scope="module")
@@ -30,12 +31,12 @@ def refused(lib, rc):
 
 
 def linear(lib, w, **kw):
-    a = {**dict(x=OK, x_ld=96, rows=None, n=5, out=OK, out_ld=40, res=None, res_ld=0, shift=0), **kw}
+    a = {**dict(x=OK, x_ld=96, rows=None, n=5, out=TO, out_ld=40, res=None, res_ld=0, shift=0), **kw}
     return lib.cm_linear8(None if w is None else ctypes.byref(w), *a.values(), None)
 
 
 def gated(lib, w, **kw):
-    a = {**dict(x=OK, x_ld=96, rows=None, n=5, out=OK, out_ld=40), **kw}
+    a = {**dict(x=OK, x_ld=96, rows=None, n=5, out=TO, out_ld=40), **kw}
     return lib.cm_linear8_gated(None if w is None else ctypes.byref(w), *a.values(), None)
 
 
@@ -58,16 +59,29 @@ def test_bad_gates(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(x=None), dict(rows=OK), dict(x=None, rows=OK + 16), dict(x=OK + 1), dict(x_ld=95),
-                                dict(n=(1 << 22) + 1), dict(out=None), dict(out=OK + 1), dict(out_ld=39)], ids=str)
+                                dict(n=(1 << 22) + 1), dict(out=None), dict(out=OK + 1), dict(out_ld=39), dict(out_ld=1 << 23)], ids=str)
 def test_bad_operands(lib, kw):
     refused(lib, linear(lib, weight(), **kw))
     refused(lib, gated(lib, weight(gated=1), **kw))
 
 
-@pytest.mark.parametrize("kw", [dict(res=OK + 2, res_ld=40), dict(res=2 * OK, res_ld=39), dict(res=OK, res_ld=48), dict(res=2 * OK, res_ld=40, shift=17),
-                                dict(res=2 * OK, res_ld=40, out=OK + 2), dict(shift=17)], ids=str)
+@pytest.mark.parametrize("kw", [dict(res=OK + 2, res_ld=40), dict(res=3 * OK, res_ld=39), dict(res=TO, res_ld=48), dict(res=3 * OK, res_ld=40, shift=17),
+                                dict(res=3 * OK, res_ld=40, out=TO + 2), dict(shift=17), dict(res=3 * OK, res_ld=1 << 23),
+                                dict(res=TO + 4, res_ld=40), dict(res=TO - 4 * 40, res_ld=40), dict(res=TO + 4 * 39, out_ld=80, res_ld=80),
+                                dict(res=OK + 64, res_ld=40, out=3 * OK, x=OK + 64, rows=TO)], ids=str)
 def test_bad_residuals(lib, kw):
     refused(lib, linear(lib, weight(), **kw))
+
+
+@pytest.mark.parametrize("kw", [dict(out=OK), dict(out=OK + 190), dict(out=OK + 2 * 4 * 96 + 190), dict(out=OK - 2 * (4 * 40 + 39)),
+                                dict(x_ld=136, out=OK + 2 * 95, out_ld=136), dict(x_ld=136, out=OK - 2 * 39, out_ld=136),
+                                dict(x_ld=136, out=OK + 2 * 97, out_ld=136), dict(x_ld=200, out=OK + 2 * 96, out_ld=204)], ids=str)
+def test_outputs_over_x(lib, kw):
+    """An output that shares an element with x, at its ends and as columns of x's buffer, or reaches into it at another stride."""
+    refused(lib, linear(lib, weight(), **kw))
+    assert b"overlaps x" in lib.cm_last_error()
+    refused(lib, gated(lib, weight(gated=1), **kw))
+    assert b"overlaps x" in lib.cm_last_error()
 
 
 @pytest.mark.parametrize("kw", [dict(w=None), dict(mult=None), dict(image=None), dict(image=OK + 128), dict(mult=OK + 4), dict(bias=OK + 2), dict(k=0),
@@ -93,12 +107,12 @@ def test_no_rows(lib):
 
 
 def test_sizes(lib):
-    """Whole 32-line blocks of an odd number of 64-k steps, 16 bytes a channel, 4 a row."""
-    assert lib.cm_linear8_image_bytes(65, 33, 0) == 2 * 3 * 2048 + 64 * 16
+    """Whole 32-line blocks of 64-k steps, 16 bytes a channel, 4 a row."""
+    assert lib.cm_linear8_image_bytes(65, 33, 0) == 2 * 2 * 2048 + 64 * 16
     assert lib.cm_linear8_image_bytes(129, 33, 0) == 2 * 3 * 2048 + 64 * 16
     assert lib.cm_linear8_image_bytes(65, 33, 1) == 2 * lib.cm_linear8_image_bytes(65, 33, 0)
     assert lib.cm_linear8_rows_bytes(1, 64) == 2048 + 128
-    assert lib.cm_linear8_rows_bytes(33, 32768) == 64 * (32768 + 64) + 256
+    assert lib.cm_linear8_rows_bytes(33, 32768) == 64 * 32768 + 256
 
 
 def test_python_refusals():
