@@ -349,12 +349,13 @@ __device__ __forceinline__ void store(const Prod& p, uint32_t row, uint32_t col,
 // LDS reads, LDS copies and vector memory each move 64 bytes a cycle and compute unit (measured), an i8 MFMA of 32 x
 // 32 x 32 takes 32 cycles: what bounds a product is how often its operands pass through those two ports.  So a
 // wavefront takes 64 rows by 128 columns, four of them side by side over the same columns: x's fragments, which no other
-// wavefront reads, go from memory straight into registers, three steps ahead; the weight's columns go through a ring of
-// three LDS stages, copied three steps ahead.  A 64-k step of two such workgroups on a compute unit is 1024 cycles of MFMA
+// wavefront reads, go from memory straight into registers, D steps ahead; the weight's columns go through a ring of
+// D LDS stages, copied D steps ahead.  A 64-k step of two such workgroups on a compute unit is 1024 cycles of MFMA
 // on each SIMD, 64 KiB of LDS reads, 16 KiB of copies and 32 KiB of loads.  Operand pieces lie in memory, in LDS and in the
 // registers in one order (a lane's 16 bytes at 16 lane): whole lines, no bank conflict.  Fewer rows take a wavefront of 32
 // rows by 128 or 64 columns (RB, CB: blocks of a wavefront): half or a quarter of a workgroup's work, for a chip with fewer
-// tiles than it holds.
+// tiles than it holds.  D is 3 where the registers hold no more (RB 2), else 4: operands past the L2 come too late for 3
+// (512 x 8192 x 1024 in 128 x 64 tiles 25.4 us, 4 stages 19.4, 6 19.3; 128 x 2560 x 960 6.8 / 6.8 / 7.0).
 // Buffer accesses: a block's base in scalar registers, the lane's 16 bytes in one vector register, the step's offset
 // scalar.  Copies to LDS go this way and not as global_load_lds, which the compiler counts as a flat access: every wait
 // for a register load or an LDS read behind one becomes a wait for all (8192 x 4096 x 8192: 268 us, 260 this way).
@@ -446,9 +447,11 @@ __device__ __forceinline__ void epilogue(const Prod& p, const v16i (&acc)[RB][CB
 template <uint32_t MODE, int RB, int CB>
 __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t tiles_r, uint32_t tiles_c, uint32_t xw) {
     constexpr int WR = 4, NC = 2 * CB / WR;                // wavefronts; copies a wavefront and step
+    constexpr int D = RB == 1 ? 4 : 3;                     // stages
     __shared__ __attribute__((aligned(1024))) int8_t sm0[2 * CB * 1024];
     __shared__ __attribute__((aligned(1024))) int8_t sm1[2 * CB * 1024];
     __shared__ __attribute__((aligned(1024))) int8_t sm2[2 * CB * 1024];
+    __shared__ __attribute__((aligned(1024))) int8_t sm3[D > 3 ? 2 * CB * 1024 : 16];
     // a gate's table, for gathers of 64 lanes; it lands before the ring's first copies
     constexpr int TAB = MODE == kSiluGate ? 8 * kPieces : MODE == kTableGate ? kActTabBytes : 16;
     __shared__ __attribute__((aligned(1024))) int8_t tab[TAB];
@@ -474,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t t
     for (int i = 0; i < RB; i++)
 #pragma unroll
         for (int j = 0; j < CB; j++) acc[i][j] = v16i{};
-    v4i a[3][2][RB], b[2][CB];
+    v4i a[D][2][RB], b[2][CB];
     auto at = [&](uint32_t step) { return min(step, p.steps - 1) * kPiece; };       // past the last step: any, never used
     auto issue = [&](int8_t* sm, uint32_t step) {
 #pragma unroll
@@ -498,24 +501,34 @@ __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t t
             for (int i = 0; i < RB; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[slot][s][i], b[s][j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Step kt (slot kt % 3), its first weight fragments read: the second ones are read under the first products, the next
-    // step's first ones under the second, behind the barrier that frees `cur` for step kt + 3 and says that step
-    // kt + 1 (`next`) has landed.  Behind that step's copies this wavefront has copied once more (NC) and, in the
-    // loop, loaded x twice (4 RB: the loads of a later step that feed no product may be left out by the compiler, so the
+    // Step kt + slot, its first weight fragments read: the second ones are read under the first products, the next step's
+    // first ones under the second, behind the barrier that frees its stage for D steps later and says that the next
+    // step has landed.  Behind that one's copies this wavefront has copied D - 2 times more (NC each) and, in the loop,
+    // loaded x 2 (D - 1) times (RB each: the loads of a later step that feed no product may be left out by the compiler, so the
     // steps behind the loop count none).  No copy is conditional: with a path that skips one the compiler waits for
     // every copy in flight before it reads a stage.
-    auto step = [&](int8_t* cur, const int8_t* next, int slot, uint32_t kt, auto loads) {
-        fragments(cur, 1);
-        products(slot, 0);
-        wait_copies<NC + loads.value>();
-        __builtin_amdgcn_s_barrier();
-        issue(cur, kt + 3);
-        load(slot, 0, kt + 3);
-        fragments(next, 0);
-        products(slot, 1);
-        load(slot, 1, kt + 3);
+    auto stage = [&](auto i) -> int8_t* {
+        if constexpr (i.value % D == 0) return sm0;
+        else if constexpr (i.value % D == 1) return sm1;
+        else if constexpr (i.value % D == 2) return sm2;
+        else return sm3;
     };
-    constexpr std::integral_constant<int, 4 * RB> in_loop{};
+    uint32_t kt = 0;
+    auto step = [&](auto slot, auto loads) {
+        int8_t* const cur = stage(slot);
+        const int8_t* const next = stage(std::integral_constant<int, slot.value + 1>{});
+        const uint32_t to = kt + slot.value + D;
+        fragments(cur, 1);
+        products(slot.value, 0);
+        wait_copies<(D - 2) * NC + loads.value>();
+        __builtin_amdgcn_s_barrier();
+        issue(cur, to);
+        load(slot.value, 0, to);
+        fragments(next, 0);
+        products(slot.value, 1);
+        load(slot.value, 1, to);
+    };
+    constexpr std::integral_constant<int, 2 * (D - 1) * RB> in_loop{};
     constexpr std::integral_constant<int, 0> behind{};
     if constexpr (gated(MODE)) {
         const Buf tb = buffer_of(reinterpret_cast<const int8_t*>(p.tab), TAB);
@@ -523,26 +536,25 @@ __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t t
         for (int i = 0; i < TAB / 1024 / WR; i++) lds_copy16(tb, l16, (wave * (TAB / 1024 / WR) + i) * 1024, tab + (wave * (TAB / 1024 / WR) + i) * 1024);
         __builtin_amdgcn_sched_barrier(0);
     }
-    auto first = [&](int8_t* sm, int slot) {
-        issue(sm, slot);
-        load(slot, 0, slot);
-        load(slot, 1, slot);
+    auto first = [&](auto slot) {
+        issue(stage(slot), slot.value);
+        load(slot.value, 0, slot.value);
+        load(slot.value, 1, slot.value);
         __builtin_amdgcn_sched_barrier(0);
     };
-    first(sm0, 0);
-    first(sm1, 1);
-    first(sm2, 2);
-    wait_copies<2 * NC>();                           // x's first loads may have moved behind the copies
+    auto each = [&](auto f) {                        // f of 0 .. D - 1
+        f(std::integral_constant<int, 0>{}), f(std::integral_constant<int, 1>{}), f(std::integral_constant<int, 2>{});
+        if constexpr (D > 3) f(std::integral_constant<int, 3>{});
+    };
+    each(first);
+    wait_copies<(D - 1) * NC>();                     // x's first loads may have moved behind the copies
     __builtin_amdgcn_s_barrier();
     fragments(sm0, 0);
-    uint32_t kt = 0;
-    for (; kt + 3 <= p.steps; kt += 3) {
-        step(sm0, sm1, 0, kt, in_loop);
-        step(sm1, sm2, 1, kt + 1, in_loop);
-        step(sm2, sm0, 2, kt + 2, in_loop);
-    }
-    if (kt < p.steps) step(sm0, sm1, 0, kt, behind);
-    if (kt + 1 < p.steps) step(sm1, sm2, 1, kt + 1, behind);
+    for (; kt + D <= p.steps; kt += D) each([&](auto i) { step(i, in_loop); });
+    each([&](auto i) {
+        if constexpr (i.value < D - 1)
+            if (kt + i.value < p.steps) step(i, behind);
+    });
     wait_copies<0>();                                // no copy may land after the workgroup ends
 
     epilogue<MODE, RB, CB>(p, acc, rb0, cb0, l32, lh, (const uint8_t*)tab);
