@@ -32,7 +32,9 @@ constexpr double kMagic = 6755399441055744.0;                           // 1.5 2
 enum : uint32_t { kOut16 = 0, kOut32 = 1, kSiluGate = 2, kTableGate = 3 };
 constexpr bool gated(uint32_t mode) { return mode >= kSiluGate; }
 enum : uint32_t { kSilu = 0, kGelu = 1, kGeluTanh = 2 };             // cm_linear8_weight's act
-constexpr uint32_t kPieces = 4096;                                    // of the sigmoid, 8 bytes each
+constexpr double kMagic70 = 0x1.8p70;
+constexpr uint32_t kPieces = 4096;                                    // of the sigmoid, 8 bytes each, and one behind them
+static_assert(kSigmoidBytes >= 8 * (kPieces + 1) && kSigmoidBytes % 4096 == 0, "whole copies of four wavefronts");
 
 inline uint32_t steps_of(uint32_t k) { return ceil_div(k, kStep); }
 inline uint32_t blocks_of(uint32_t lines) { return ceil_div(lines, kLine); }
@@ -60,8 +62,8 @@ struct Prod {
     uint64_t res_ld;
     uint32_t shift;
     const uint8_t* tab;              // a gate's: the sigmoid's pieces, or the activation's bytes (`len` of them)
-    uint32_t len, sa;
-    double gscale, scale;            // 2^(sa - 18), 2^-sc
+    uint32_t len;
+    double gscale, gneg, scale;      // SiLU: 2^sa, 2^(sa + 24), 2^(-18 - sc); a byte table: scale 2^-sc
 };
 
 // 1.5 2^52 + sat16(rne(acc a mu + b)): the low word is the result.
@@ -76,22 +78,20 @@ __device__ __forceinline__ int32_t add_res(int32_t h, int32_t o, uint32_t shift)
 }
 
 // act(g) u 2^-sc, rounded to even and saturated, of the two products zg, zu as `scaled` gives them.  SiLU by the row-ops
-// rule (MULACT): sigma at 2^-24 from the piece of |g| at 2^-14, silu at 2^-20.  gv sigma is exact in a double (below
-// 2^18 2^26, or a power of two times g), so is silu u (2^35 2^15), and each sum onto 1.5 2^52 is its one rounding.
+// rule (MULACT): s = sigma(|g|) at 2^-24 from the piece of m = |g| at 2^-14, silu(g) = rne(m s 2^-18) at 2^-20, for a negative
+// g of s - 2^24.  m s and m 2^24 are exact in a double (2^29 2^26), and one fused multiply-add of both onto 1.5 2^70, whose
+// last place is 2^18, is that rounding; so is the product with u (2^37 2^15) and its own rounding onto 1.5 2^52.
 template <uint32_t MODE, class Tab>
 __device__ __forceinline__ int32_t gate16(double zg, double zu, Tab tab, const Prod& p) {
-    const int32_t g = __double2loint(zg), a = max(g, -g);
     double f;
     if (MODE == kSiluGate) {
-        const uint32_t av = (uint32_t)a << p.sa, ai = min(av, (1u << 18) - 1), fr = ai & 63;
-        const uint2 e = *reinterpret_cast<const uint2*>(tab + 8 * (ai >> 6));        // {D << 25 | T}: 24 and 25 bits
-        const uint32_t T = e.x & 0x1FFFFFFu, D = (e.x >> 25 | e.y << 7) & 0xFFFFFFu;
-        int32_t sg = (int32_t)(T + ((D * fr) >> 6));
-        asm("" : "+v"(sg));                              // for every lane: a branch around it costs more
-        sg = av >= (1u << 18) ? 1 << 24 : sg;
-        if (g < 0) sg = (1 << 24) - sg;
-        f = __builtin_fma((zg - kMagic) * p.gscale, (double)sg, kMagic) - kMagic;
+        const double g = zg - kMagic, m = __builtin_fabs(g) * p.gscale;
+        const uint32_t av = (uint32_t)m, at = min(av, kPieces << 6);
+        const uint2 e = *reinterpret_cast<const uint2*>(tab + ((at >> 3) & ~7u));     // {64 value, step to the next} of 64 pieces
+        const uint32_t s = (e.x + __umul24(e.y, av & 63)) >> 6;
+        f = __builtin_fma(m, (double)s, __builtin_fma(__builtin_fmin(g, 0.0), p.gneg, kMagic70)) - kMagic70;
     } else {
+        const int32_t g = __double2loint(zg), a = max(g, -g);
         f = (double)(max(g, 0) - ((uint32_t)a < p.len ? (int32_t)tab[a] : 0));
     }
     const double z = __builtin_fma(f * (zu - kMagic), p.scale, kMagic);
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void linear8_ring_kernel(Prod p, uint32_t t
     __shared__ __attribute__((aligned(1024))) int8_t sm2[2 * CB * 1024];
     __shared__ __attribute__((aligned(1024))) int8_t sm3[D > 3 ? 2 * CB * 1024 : 16];
     // a gate's table, for gathers of 64 lanes; it lands before the ring's first copies
-    constexpr int TAB = MODE == kSiluGate ? 8 * kPieces : MODE == kTableGate ? kActTabBytes : 16;
+    constexpr int TAB = MODE == kSiluGate ? kSigmoidBytes : MODE == kTableGate ? kActTabBytes : 16;
     __shared__ __attribute__((aligned(1024))) int8_t tab[TAB];
     const Tile t = tile_of(blockIdx.x, tiles_r, tiles_c, xw);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1068,10 +1068,10 @@ int product(const cm_linear8_weight* w, const int16_t* x, uint64_t x_ld, const v
     p.w = static_cast<const int8_t*>(w->image);
     p.cols = reinterpret_cast<const double2*>(p.w + codes_bytes(p.cblocks, w->k));
     if (gated(MODE)) {
-        p.sa = w->gate_shift;
-        p.gscale = __builtin_ldexp(1.0, (int)w->gate_shift - 18);
-        p.scale = __builtin_ldexp(1.0, -(int)w->out_shift);
-        p.tab = w->act == kSilu ? st->ro_tables : st->act_tab + w->act * kActTabBytes;
+        p.gscale = __builtin_ldexp(1.0, (int)w->gate_shift);
+        p.gneg = __builtin_ldexp(1.0, (int)w->gate_shift + 24);
+        p.scale = __builtin_ldexp(1.0, -(int)w->out_shift - (w->act == kSilu ? 18 : 0));
+        p.tab = w->act == kSilu ? st->sigmoid : st->act_tab + w->act * kActTabBytes;
         p.len = w->act == kSilu ? 0 : st->act_len[w->act];
     }
     if (few) {

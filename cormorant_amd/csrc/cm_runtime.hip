@@ -104,6 +104,20 @@ static int compact_act_tables(const int16_t (*full)[65536], uint8_t* compact, ui
     return CM_OK;
 }
 
+// The sigmoid of a row-ops table image (pieces {step << 25 | value}, at 2^-24) as words {64 value, step}, 2^24 behind
+// the last piece: a product and a shift give the value, and what lies past the pieces needs no case.
+static std::vector<uint32_t> sigmoid_words(const void* img64k) {
+    std::vector<uint32_t> w(kSigmoidBytes / 4, 0);
+    for (uint32_t i = 0; i < 4096; i++) {
+        uint64_t e;
+        memcpy(&e, static_cast<const uint8_t*>(img64k) + 8 * i, 8);
+        w[2 * i] = (uint32_t)(e & 0x1FFFFFFu) << 6;
+        w[2 * i + 1] = (uint32_t)(e >> 25) & 0xFFFFFFu;
+    }
+    w[2 * 4096] = 1u << 30;
+    return w;
+}
+
 static int prepare(DeviceState* st, int dev) {
     static int16_t full[3][65536];
     build_act_tables_full(full);
@@ -118,10 +132,12 @@ static int prepare(DeviceState* st, int dev) {
     CM_HIP_CHECK(hipMalloc(&st->act_tab, 3 * kActTabBytes));
     CM_HIP_CHECK(hipMalloc(&st->smx_tab, sizeof(smx)));
     CM_HIP_CHECK(hipMalloc(&st->ro_tables, 65536));
+    CM_HIP_CHECK(hipMalloc(&st->sigmoid, kSigmoidBytes));
     CM_HIP_CHECK(hipMalloc(&st->ro_pram, 4096 * 16));
     CM_HIP_CHECK(hipMemcpy(st->act_tab, compact.data(), compact.size(), hipMemcpyHostToDevice));
     CM_HIP_CHECK(hipMemcpy(st->smx_tab, smx, sizeof(smx), hipMemcpyHostToDevice));
     CM_HIP_CHECK(hipMemcpy(st->ro_tables, img.data(), 65536, hipMemcpyHostToDevice));
+    CM_HIP_CHECK(hipMemcpy(st->sigmoid, sigmoid_words(img.data()).data(), kSigmoidBytes, hipMemcpyHostToDevice));
     CM_HIP_CHECK(hipMemset(st->ro_pram, 0, 4096 * 16));
     int cus = 0, lds_cu = 0, lds_blk = 0, lds_optin = 0;
     CM_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
@@ -399,5 +415,6 @@ extern "C" int cm_rowops_tables_init(const void* img64k) {
     if (rc) return rc;
     if (img64k == nullptr) return fail(CM_EINVAL, "row-ops tables: null");
     CM_HIP_CHECK(hipMemcpy(st->ro_tables, img64k, 65536, hipMemcpyHostToDevice));
+    CM_HIP_CHECK(hipMemcpy(st->sigmoid, sigmoid_words(img64k).data(), kSigmoidBytes, hipMemcpyHostToDevice));
     return CM_OK;
 }
