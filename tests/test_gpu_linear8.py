@@ -105,14 +105,16 @@ def test_gated(L, oracle_lib, n, k, m, act):
         assert (np.delete(host(wide), np.s_[1:1 + m], axis=1) == GUARD16).all()
 
 
-# 128 x 128 and 256 x 128 tiles, steps of each residue of the ring's three stages
-@pytest.mark.parametrize("n,k,m", [(300, 64, 8190), (300, 128, 8190), (300, 150, 8190), (1793, 1270, 3001), (1793, 1344, 3001), (1793, 1401, 3000)], ids=str)
+# 128 x 128 and 256 x 128 tiles, steps of each residue of the ring's four or three stages
+@pytest.mark.parametrize("n,k,m", [(300, 64, 8190), (300, 128, 8190), (300, 150, 8190), (300, 250, 8190), (1793, 1270, 3001), (1793, 1344, 3001),
+                                   (1793, 1401, 3000)], ids=str)
 @pytest.mark.parametrize("form", ["plain", "both"])
 def test_large_tiles(L, n, k, m, form):
     test_linear(L, n, k, m, form)
 
 
-@pytest.mark.parametrize("n,k,m", [(800, 128, 2300), (1793, 190, 1025), (513, 445, 2300), (1300, 64, 8190), (1300, 121, 8190), (5000, 1150, 513)], ids=str)
+@pytest.mark.parametrize("n,k,m", [(513, 512, 2300), (513, 570, 2300), (513, 640, 2300), (513, 700, 2300), (5000, 1280, 513), (5000, 1340, 513),
+                                   (800, 1400, 3001)], ids=str)
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_large_gate_tiles(L, oracle_lib, n, k, m, act):
     test_gated(L, oracle_lib, n, k, m, act)
