@@ -1018,7 +1018,7 @@ int ring_at(const Prod& p, hipStream_t s) {
 }
 
 // The tile with the least of four estimates in ns, fitted to 150 measured products of 33 to 8192 rows (0.7 % behind the best
-// tile of each, gates 0.4 %).  Among them (rows x k x columns: us of 256 x 128, 128 x 128, 128 x 64 and 32 x 32 tiles): 128 x 2560 x 960
+// tile of each, gates 0.5 %).  Among them (rows x k x columns: us of 256 x 128, 128 x 128, 128 x 64 and 32 x 32 tiles): 128 x 2560 x 960
 // 17.2 / 10.6 / 6.8 / 4.4; 512 x 960 x 2560 10.3 / 6.8 / 5.0 / 7.9; 1000 x 1024 x 1024 10.4 / 6.9 / 5.0 / 6.9; 1024 x 2560 x 960 17.5 /
 // 10.9 / 7.5 / 9.9; 512 x 8192 x 1024 - / 25.9 / 19.2 / 12.5; 2048 x 8192 x 2048 46.8 / 36.5 / 39.9 / 105; 4096 x 960 x 2560 20.4 /
 // 18.7 / 17.7 / 44.0; 2048 x 4096 x 4096 35.2 / 35.3 / 41.7 / 99.7.  Gates (the smallest tile 32 x (32 + 32)): 300 x 960 x 2560
@@ -1035,7 +1035,7 @@ int many_rows(const DeviceState* st, const Prod& p, hipStream_t s) {
     // quarters of a round of tiles: at least so many; whole rounds behind the first where a compute unit has one or two tiles at a time
     auto rounds = [&](uint64_t t) { return 4 * t <= 3 * cus ? 3 : (t + cus - 1) / cus * 4; };
     const uint64_t big = (G ? 6000 : 4000) + rounds(tiles(8, 4)) * (G ? 4800 + 310 * steps : 2800 + 430 * steps) / 4;
-    const uint64_t square = (G ? 2800 : 2400) + rounds(tiles(4, 4)) * (G ? 2700 + 200 * steps : 1400 + 250 * steps) / 4;
+    const uint64_t square = (G ? 2800 : 2400) + rounds(tiles(4, 4)) * (G ? 3000 + 200 * steps : 1400 + 250 * steps) / 4;
     const uint64_t tall = 2400 + std::max(4 * tiles(4, 2), 3 * cus) * (G ? 1300 + 160 * steps : 700 + 150 * steps) / (4 * cus);
     const uint64_t small = 2500 + std::max(tiles(1, C0), cus) * (G ? 1500 + 60 * steps : 700 + 30 * steps) / cus;
     const uint64_t best = std::min(std::min(big, square), std::min(tall, small));

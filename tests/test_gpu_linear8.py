@@ -113,7 +113,7 @@ def test_large_tiles(L, n, k, m, form):
     test_linear(L, n, k, m, form)
 
 
-@pytest.mark.parametrize("n,k,m", [(513, 512, 2300), (513, 570, 2300), (513, 640, 2300), (513, 700, 2300), (5000, 1280, 513), (5000, 1340, 513),
+@pytest.mark.parametrize("n,k,m", [(513, 700, 2300), (513, 768, 2300), (513, 822, 2300), (513, 886, 2300), (5000, 1280, 513), (5000, 1340, 513),
                                    (800, 1400, 3001)], ids=str)
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_large_gate_tiles(L, oracle_lib, n, k, m, act):
