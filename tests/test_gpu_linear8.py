@@ -261,14 +261,14 @@ def test_gate_ranges(L, oracle_lib, act, fg, fu, fy, n):
     np.testing.assert_array_equal(host(out), O.gated(x, w, wu, mg, mu, act, *L.gate_shifts(act, fg, fu, fy), table))
 
 
-def test_gate_is_the_row_ops_job(L):
-    """The gate of two linear8 outputs by the row-ops unit's MULACT job equals gated8."""
+def gate_and_job(L, n, m, fg):
+    """gated8's rows, and the gate of two linear8 outputs by the row-ops unit's MULACT job."""
     import torch
     from cormorant_amd import units as U
     from cormorant_amd.rowops_nodes import SiluMulRoNode
     from cormorant_amd.graph import TensorInfo
-    rng = np.random.default_rng(6)
-    n, k, m, fg, fu, fy = 24, 320, 128, 10, 9, 10
+    rng = np.random.default_rng([6, n])
+    k, fu, fy = 320, 9, 10
     x, (wg, mg), (wu, mu) = dev(rows(rng, n, k)), weights(rng, k, m, 3000), weights(rng, k, m, 2000)
     g, u, y, z = (torch.zeros(n, m, dtype=torch.int16, device="cuda") for _ in range(4))
     L.linear8(x, L.Weight8(dev(wg), dev(mg)), g)
@@ -279,7 +279,30 @@ def test_gate_is_the_row_ops_job(L):
     job = node.jobs()[0]
     b = lambda t: t.view(-1).view(torch.uint8)                       # noqa: E731
     U.rowops(b(g), b(u), b(z), dev(np.asarray(node._params).reshape(-1).view(np.uint8)), job.op, m, n, 1, 2 * m, 0, 2 * m, 0, 2 * m, 0)
-    np.testing.assert_array_equal(host(y), host(z))
+    return host(y), host(z)
+
+
+def test_gate_is_the_row_ops_job(L):
+    np.testing.assert_array_equal(*gate_and_job(L, 24, 128, 10))
+
+
+@pytest.mark.parametrize("n,m", [(24, 128), (100, 128), (400, 2048)], ids=str)
+def test_gate_of_an_installed_table(L, n, m):
+    """A caller's sigmoid (cm_rowops_tables_init) in the gate as in the MULACT job, and the library's own again."""
+    from cormorant_amd import units as U
+    img = U.host_rowops_table_image()
+    own = gate_and_job(L, n, m, 6)[0]
+    changed, rng = img.copy(), np.random.default_rng(n)
+    e = changed[:32768].view(np.uint64)
+    e[:] = rng.integers(0, 2 ** 24, 4096).astype(np.uint64) | rng.integers(0, 2 ** 24, 4096).astype(np.uint64) << np.uint64(25)
+    try:
+        U.rowops_tables_init(changed)
+        y, z = gate_and_job(L, n, m, 6)
+        np.testing.assert_array_equal(y, z)
+        assert (y != own).any()
+    finally:
+        U.rowops_tables_init(img)
+    np.testing.assert_array_equal(gate_and_job(L, n, m, 6)[0], own)
 
 
 @pytest.mark.parametrize("n", [1, 20, 300])
