@@ -139,6 +139,35 @@ def test_columns_of_one_buffer(L, n):
         np.testing.assert_array_equal(host(wide), want)
 
 
+@pytest.mark.parametrize("n,k,m,pad", [(1 << 20, 2048, 40, 0), (1 << 18, 64, 10000, 0), ((1 << 22) - 5, 33, 7, 3), (300, 70, 40, (1 << 23) - 41),
+                                       (40, 64, (1 << 20) - 9, 0), (7, 64, 1 << 20, 1), (50, 32768, 33, 0)], ids=str)
+@pytest.mark.parametrize("kind", ["linear", "residual", "gate"])
+def test_offsets_past_32_bits(L, kind, n, k, m, pad):
+    """Rows, codes and outputs of more than 2^32 bytes, the most rows, columns and k, the widest strides: the first, some middle and the
+    last rows and columns as of a call of their own."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(n + m)
+    rand = lambda lo, hi, shape, t: torch.randint(lo, hi, shape, generator=g, device="cuda", dtype=torch.int32).to(t)     # noqa: E731
+    x = torch.empty(n, k + pad, dtype=torch.int16, device="cuda")[:, :k]
+    for i in range(0, n, 1 << 18):
+        x[i:i + (1 << 18)] = rand(-400, 401, (min(1 << 18, n - i), k), torch.int16)
+    w = [rand(-127, 128, (k, m), torch.int8) for _ in range(2)]
+    mult = torch.exp2(rand(-34, -28, (m,), torch.float64))
+    cut = lambda c: L.GatedWeight8(w[0][:, c], w[1][:, c], mult[c], mult[c]) if kind == "gate" else L.Weight8(w[0][:, c], mult[c])     # noqa: E731
+    run = lambda x, weight, out: L.gated8(x, weight, out) if kind == "gate" else \
+        L.linear8(x, weight, out, residual=out if kind == "residual" else None, shift=3)                # noqa: E731
+    dtype = torch.int32 if kind == "residual" else torch.int16
+    out = torch.empty(n, m + pad, dtype=dtype, device="cuda")[:, :m]
+    for i in range(0, n, 1 << 18):
+        out[i:i + (1 << 18)] = 1000
+    run(x, cut(slice(0, m)), out)
+    for r in (slice(0, 33), slice(n // 2, n // 2 + 40), slice(max(0, n - 70), n)):
+        for c in (slice(0, min(m, 65)), slice(max(0, m - 70), m)):
+            want = torch.full((x[r].shape[0], w[0][:, c].shape[1]), 1000, dtype=dtype, device="cuda")
+            run(x[r].contiguous(), cut(c), want)
+            assert torch.equal(out[r, c], want), (r, c)
+
+
 def test_two_streams(L):
     """Products of their own Rows8 on two streams, replayed beside each other."""
     import torch
