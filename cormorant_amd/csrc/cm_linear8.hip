@@ -631,7 +631,7 @@ __global__ __launch_bounds__(64 * kMidWaves) void linear8_mid_kernel(Prod p, uin
 
 // The same from x: 32 rows by 32 CB columns, S steps a wavefront; the rows' pieces stay in registers while their maxima meet in
 // LDS and become codes there, as in the kernel of few rows: one launch instead of two.
-constexpr uint32_t kDirectWaves = 8, kDirectSteps = 2;
+constexpr uint32_t kDirectWaves = 8, kDirectSteps = 3;
 
 template <uint32_t MODE, int CB, int S, bool ODD>
 __global__ __launch_bounds__(64 * kDirectWaves) void linear8_mid_direct_kernel(Prod p, const int16_t* __restrict__ x, uint64_t ld, uint32_t k,
@@ -977,12 +977,14 @@ int mid_at(const Prod& p, hipStream_t s) {
     return CM_OK;
 }
 
-// Rows of a few tiles from x in one launch: up to 1024 columns (the pieces of 2 steps in registers); each workgroup quantises
-// its rows again.  Tiles of 32 columns up to one a compute unit, of 64 up to two; a gate's, of 32 + 32, up to 5 / 2 steps of a
-// wavefront a compute unit; else 0: codes first.  One launch of tiles of 32 / of 64 / two launches (us, 0.5 to 1 more for the second
-// launch on the host): 64 x 256 x 1024 3.7 / 4.3 / 5.9, 512 x 256 x 1024 4.6 / 4.5 / 6.8, 2048 x 256 x 1024 8.8 / 7.7 / 7.4, 200 x 960 x
-// 960 5.6 / 6.1 / 6.6, 333 x 960 x 960 7.6 / 6.2 / 7.4, 512 x 960 x 1600 12.5 / 9.0 / 8.9, 1024 x 960 x 960 12.1 / 8.7 / 9.1, 333 x 1000
-// x 4000 15.8 / 12.5 / 9.5; gates of 576 x 1536, 128 rows 5.8 / 7.4, 200 8.3 / 8.2, 512 11.9 / 8.6, of 256 x 1024, 512 rows 5.7 / 7.5.
+// Rows of a few tiles from x in one launch: up to 1536 columns (the pieces of 3 steps in registers); each workgroup quantises
+// its rows again.  Tiles of 32 columns up to one a compute unit, of 64 up to two (one of 3 steps); a gate's, of 32 + 32, up to 5 / 2
+// steps of a wavefront a compute unit; else 0: codes first.  One launch of tiles of 32 / of 64 / two launches (us, 0.5 to 1 more for
+// the second launch on the host): 64 x 256 x 1024 3.7 / 4.3 / 5.9, 512 x 256 x 1024 4.6 / 4.5 / 6.8, 2048 x 256 x 1024 8.8 / 7.7 / 7.4,
+// 200 x 960 x 960 5.6 / 6.1 / 6.6, 333 x 960 x 960 7.6 / 6.2 / 7.4, 512 x 960 x 1600 12.5 / 9.0 / 8.9, 1024 x 960 x 960 12.1 / 8.7 / 9.1,
+// 333 x 1000 x 4000 15.8 / 12.5 / 9.5, 128 x 1500 x 1600 6.6 / 7.3 / 7.6, 256 x 1500 x 1600 9.9 / 7.5 / 9.0, 512 x 1500 x 1600 17.3 /
+// 11.4 / 10.7; a fourth step 128 x 2048 x 512 8.0 / 8.9 / 7.5; gates of 576 x 1536, 128 rows 5.8 / 7.4, 200 8.3 / 8.2, 512 11.9 / 8.6,
+// of 256 x 1024, 512 rows 5.7 / 7.5, of 1500 x 1600, 128 rows 7.4 / 8.8, 256 11.2 / 10.5.
 template <uint32_t MODE>
 uint32_t mid_direct(const DeviceState* st, const Prod& p) {
     const uint32_t per = ceil_div(p.steps, kDirectWaves);
@@ -990,7 +992,7 @@ uint32_t mid_direct(const DeviceState* st, const Prod& p) {
     auto tiles = [&](uint32_t columns) { return (uint64_t)p.rblocks * ceil_div(p.cblocks, columns); };
     const uint64_t cus = (uint64_t)st->cus;
     if (gated(MODE)) return 2 * per * tiles(2) <= 5 * cus ? 2 : 0;
-    return tiles(1) <= cus ? 1 : tiles(2) <= 2 * cus ? 2 : 0;
+    return tiles(1) <= cus ? 1 : tiles(2) <= (per < 3 ? 2 : 1) * cus ? 2 : 0;
 }
 
 template <uint32_t MODE, int CB>
@@ -1002,8 +1004,10 @@ int mid_direct_at(const Prod& p, const int16_t* x, uint64_t ld, uint32_t k, hipS
     CM_LAUNCH("linear8_mid_kernel", (linear8_mid_direct_kernel<MODE, CB, S, O>), dim3(tiles), block, 0, s, p, x, ld, k, p.rblocks, tc, xw)
     if (p.steps <= kDirectWaves) {
         if (odd) { CM_MID(1, true); } else { CM_MID(1, false); }
-    } else {
+    } else if (p.steps <= 2 * kDirectWaves) {
         if (odd) { CM_MID(2, true); } else { CM_MID(2, false); }
+    } else {
+        if (odd) { CM_MID(3, true); } else { CM_MID(3, false); }
     }
 #undef CM_MID
     return CM_OK;

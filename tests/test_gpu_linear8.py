@@ -51,6 +51,7 @@ def host(t):
 
 SIZES = [(1, 1700, 9000), (4, 4000, 300), (5, 4000, 300), (16, 2500, 170), (9, 500, 9001), (30, 2000, 100), (12, 9000, 65),
          (333, 256, 1030), (400, 1000, 1100), (401, 999, 1090), (90, 500, 2000), (91, 501, 2001),
+         (128, 1500, 1600), (77, 1025, 900), (250, 1536, 1500), (131, 1301, 1601),
          (1, 1, 1), (1, 64, 32), (2, 63, 31), (1, 960, 960), (3, 65, 33), (15, 128, 70), (16, 1000, 100), (17, 129, 513),
          (31, 320, 64), (32, 64, 257), (33, 2560, 96), (47, 200, 129), (64, 1024, 64), (65, 77, 300), (100, 640, 1000), (129, 192, 257),
          (200, 2049, 65), (256, 256, 256), (257, 96, 640), (300, 960, 1600), (513, 128, 384), (777, 65, 129),
