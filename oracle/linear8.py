@@ -1,5 +1,5 @@
 """CPU restatements of the 8-bit linear layers in whole numbers (numpy int64, Python integers where
-they pass 64 bits).  TEST INFRASTRUCTURE ONLY (the checker, never the thing measured or shipped).
+they pass 64 bits).  TEST INFRASTRUCTURE ONLY (the oracle, never the thing measured or shipped).
 Nothing here imports the product."""
 from fractions import Fraction
 
