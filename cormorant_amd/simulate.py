@@ -1520,7 +1520,8 @@ class Simulator:
         return self._shared[key]
 
     def _step_private(self) -> set:
-        """The paged nodes' outputs that only the node behind them reads: overwritten safely by the next layer's."""
+        """The paged nodes' outputs that only the node behind them reads, and that node not as a view of its own (a reshape, columns):
+        overwritten safely by the next layer's."""
         if self._private is None:
             nodes, readers = self._graph.nodes, {}
             for i, sn in enumerate(nodes):
@@ -1529,7 +1530,7 @@ class Simulator:
                         readers.setdefault(u.onnx_name, []).append(i)
             self._private = {sn.output.onnx_name for i, sn in enumerate(nodes)
                              if isinstance(sn, (PagedPrepNode, PagedAttentionNode)) and readers.get(sn.output.onnx_name) == [i + 1]
-                             and not isinstance(nodes[i + 1], ReshapeNode)}
+                             and not isinstance(nodes[i + 1], (ReshapeNode, ColumnsNode))}
         return self._private
 
     def _paged_prep(self, sn: PagedPrepNode, raw) -> torch.Tensor:
