@@ -1564,8 +1564,10 @@ class Simulator:
                 [sn.gate_codes, sn.up_codes, sn.gate_mult, sn.up_mult]
             h = hashlib.blake2b(digest_size=16)
             for a in parts:
-                h.update(b"none" if a is None else np.ascontiguousarray(a).view(np.uint8).reshape(-1))
-            kind = "" if isinstance(sn, Linear8Node) else f" {sn.act} {sn.gate_exp} {sn.up_exp} {sn.out_exp}"
+                if a is not None:
+                    h.update(np.ascontiguousarray(a).view(np.uint8).reshape(-1))
+            kind = ("" if sn.bias_raw is None else " bias") if isinstance(sn, Linear8Node) else \
+                f" {sn.act} {sn.gate_exp} {sn.up_exp} {sn.out_exp}"
             key = f"weight8 {parts[0].shape}{kind} {h.hexdigest()}"
             w = self._images.get(key)
             if w is None:

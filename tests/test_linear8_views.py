@@ -1,8 +1,10 @@
-"""Columns of tensors that other nodes write again, on the CPU: which buffers a pass may reuse."""
+"""The 8-bit nodes in the Simulator, on the CPU: which buffers a pass may reuse, which weights share an image."""
+import numpy as np
 import pytest
+import torch
 
 from cormorant_amd import models
-from cormorant_amd.graph import ColumnsNode, PagedAttentionNode, ReshapeNode, TensorInfo
+from cormorant_amd.graph import ColumnsNode, Linear8Node, PagedAttentionNode, ReshapeNode, TensorInfo
 
 SHAPE = models.LlamaShape(layers=2, batch=2, d=128, heads=2, kv=1, hd=64, ff=128, vocab=256, ctx=64)
 
@@ -44,3 +46,19 @@ def test_viewed_rows_are_not_shared(small, kind):
     assert "l0.om" in names(plain) and "l0.qr" in names(plain)
     private = names(viewed(small, kind)[0])
     assert "l0.om" not in private and "l1.om" not in private and "l0.qr" in private
+
+
+def test_a_bias_of_any_bytes_is_its_own_weight(monkeypatch):
+    """A weight without a bias and the same weight with one are two images, whatever the bias holds."""
+    from cormorant_amd import linear8, simulate
+    monkeypatch.setattr(linear8, "Weight8", lambda *a: ("w", a[2] is None))
+    images, x = {}, TensorInfo("x", [3, 40], exp=9)
+    w = TensorInfo("w", [40, 1], data=np.linspace(-1, 1, 40)[:, None])
+    for raw in (int.from_bytes(b"none", "little"), 0, -1):
+        nodes = [Linear8Node([x, w], TensorInfo("y", [3, 1], exp=0), bias=b) for b in (None, [float(raw)])]
+        assert int(nodes[1].bias_raw[0]) == raw
+        for node, alone in zip(nodes, (True, False)):
+            sim = object.__new__(simulate.Simulator)
+            sim.device, sim._images, sim._constants = torch.device("cpu"), images, {}
+            assert sim._weight8(node) == ("w", alone)
+    assert len(images) == 4
