@@ -117,14 +117,19 @@ def gate_shifts(act: str, gate_exp: int, up_exp: int, out_exp: int):
 
 
 class Rows8:
-    """The codes of up to ``n`` rows of ``k`` (quant_rows writes them; the first ``self.n`` are valid)."""
+    """The codes of up to ``n`` rows of ``k`` (quant_rows writes them; ``self.n`` rows of its last call are valid).  The rows' maxima
+    lie behind the blocks of that many rows, so the products take all of them, never their first few."""
 
     def __init__(self, n: int, k: int, device="cuda"):
         if not (1 <= n <= MAX_N and 1 <= k <= MAX_K):
             raise ValueError(f"Rows8: {n} rows of {k} (up to {MAX_N} of {MAX_K})")
-        self.cap, self.k, self.n = n, k, 0
+        self.cap, self.k, self._n = n, k, 0
         self.data = _buffer(_lib.lib().cm_linear8_rows_bytes(n, k), device)
         self.device, self.index, self.at = self.data.device, self.data.get_device(), self.data.data_ptr()
+
+    @property
+    def n(self) -> int:
+        return self._n
 
 
 def _stride(t: torch.Tensor, name: str, dtype, n: int, width: int) -> int:
@@ -163,7 +168,7 @@ def quant_rows(x: torch.Tensor, rows: Optional[Rows8] = None) -> Rows8:
     ld = _stride(x, "x", torch.int16, n, k)
     stream = _on(rows.index, x)
     _lib.check(_lib.lib().cm_linear8_rows(x.data_ptr(), ld, rows.data.data_ptr(), n, k, stream), "cm_linear8_rows")
-    rows.n = n
+    rows._n = n
     return rows
 
 
@@ -172,7 +177,7 @@ def _x(x: Union[torch.Tensor, Rows8], k: int, what: str):
     if isinstance(x, Rows8):
         if x.k != k:
             raise ValueError(f"{what}: rows of {x.k} against a weight of {k}")
-        return x.n, None, 0, x.at, x.data
+        return x._n, None, 0, x.at, x.data
     shape = x.shape
     if len(shape) != 2 or shape[1] != k or shape[0] > MAX_N:
         raise ValueError(f"{what}: x must be [n][{k}] of up to {MAX_N} rows, got {list(shape)}")

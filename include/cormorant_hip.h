@@ -574,7 +574,9 @@ int cm_paged_read(const cm_paged_cache* cache, const cm_paged_batch* batch, int1
  * A weight's image (cm_linear8_image_bytes, 256-byte aligned): cm_linear8_pack lays out w [k][m], element
  * (kk, j) at w + kk k_stride + j m_stride, with its multipliers [m] and an int32 bias [m] or NULL; `part` 0
  * the weight, 1 / 2 the gate / up half of a gated image (gated 1, two calls).  Rows' codes
- * (cm_linear8_rows_bytes, 256-byte aligned): cm_linear8_rows, for rows that several products read. */
+ * (cm_linear8_rows_bytes, 256-byte aligned): cm_linear8_rows, for rows that several products read.  They are read with the
+ * n and k they were made with: the rows' maxima lie behind the blocks of all n rows, so a product of the first few of
+ * them, or of more, takes other bytes for maxima; the codes do not say how many there are, and no call can check it. */
 typedef struct cm_linear8_weight {
     const void* image;
     uint32_t k, m;
@@ -588,12 +590,12 @@ int cm_linear8_pack(const int8_t* w, uint64_t k_stride, uint64_t m_stride, const
 size_t cm_linear8_rows_bytes(uint32_t n, uint32_t k);
 int cm_linear8_rows(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uint32_t k, void* stream);
 
-/* o of n rows: x (rows x_ld elements apart, 2-byte aligned) or, x NULL, their codes.  out int16 rows out_ld apart; with a
- * residual (int32, shift 0 .. 16) int32 rows, which may be the residual's own (same address and stride).  The strides of
- * out and the residual are below 2^23.  An output that otherwise shares a byte with x or the residual is refused
- * (CM_EINVAL); one that reaches into them at another stride counts as sharing.  Called with x, the codes may stand
- * in the device's workspace: a call of the same sizes before a stream captures it, and no two on different streams at
- * once.  Called with codes it takes none. */
+/* o of n rows: x (rows x_ld elements apart, 2-byte aligned) or, x NULL, their codes (of cm_linear8_rows with this n).
+ * out int16 rows out_ld apart; with a residual (int32, shift 0 .. 16) int32 rows, which may be the residual's own (same
+ * address and stride).  The strides of out and the residual are below 2^23.  An output that otherwise shares a byte with x
+ * or the residual is refused (CM_EINVAL); one that reaches into them at another stride counts as sharing.  Called with x,
+ * the codes may stand in the device's workspace: a call of the same sizes before a stream captures it, and no two on
+ * different streams at once.  Called with codes it takes none. */
 int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n, void* out,
                uint64_t out_ld, const int32_t* residual, uint64_t residual_ld, uint32_t shift, void* stream);
 

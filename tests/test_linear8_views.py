@@ -1,4 +1,5 @@
-"""The 8-bit nodes in the Simulator, on the CPU: which buffers a pass may reuse, which weights share an image."""
+"""The 8-bit nodes in the Simulator, on the CPU: which buffers a pass may reuse, which weights share an image, what of their
+rows' codes a caller may change."""
 import numpy as np
 import pytest
 import torch
@@ -62,3 +63,13 @@ def test_a_bias_of_any_bytes_is_its_own_weight(monkeypatch):
             sim.device, sim._images, sim._constants = torch.device("cpu"), images, {}
             assert sim._weight8(node) == ("w", alone)
     assert len(images) == 4
+
+
+def test_the_count_of_quantised_rows_is_not_the_callers():
+    """Where the codes' maxima lie depends on how many rows were quantised: a Rows8's count is quant_rows' alone."""
+    from cormorant_amd import linear8
+    rows = linear8.Rows8(100, 64, "cpu")
+    assert (rows.n, rows.cap) == (0, 100)
+    with pytest.raises(AttributeError):
+        rows.n = 16
+    assert rows.n == 0
