@@ -442,8 +442,8 @@ class GatedLinear8Node(KernelNode):
 
 @dataclass
 class ColumnsNode(KernelNode):
-    """Columns ``first`` .. of a row tensor (the q, k or v of a fused projection) as a tensor: a view, no copy.  Whole
-    16-byte words, the exponents of the columns it shows."""
+    """Columns ``first`` .. of a row tensor (the q, k or v of a fused projection) as a tensor: a view of a
+    product's rows (Linear8Node, MatmulNode), a copy of other tensors.  Whole 16-byte words, the exponents of the columns it shows."""
     inputs: List[TensorInfo]
     output: TensorInfo
     first: int = 0

@@ -89,6 +89,7 @@ class Simulator:
         self._staging: Dict[tuple, torch.Tensor] = {}     # row-ops nodes' staging buffers
         self._constants: Dict[tuple, torch.Tensor] = {}   # nodes' constants, in _images by what they hold
         self._private = None                               # _step_private's set
+        self._products = None                              # _columns' set
         self._plan = None                                  # MatMuls fed byte planes by their A's producer
         self._keep = None                                  # forward_raw's keep (None: every tensor)
         self._batches: Dict[tuple, paged.PagedBatch] = {}  # a pass's, one for all the layers of a step
@@ -274,8 +275,7 @@ class Simulator:
         elif isinstance(sn, (Linear8Node, GatedLinear8Node)):
             raw[sn.output.onnx_name] = self._linear8(sn, raw)
         elif isinstance(sn, ColumnsNode):
-            x, w = sn.inputs[0], int(sn.output.shape[-1])
-            raw[sn.output.onnx_name] = self._get(x, raw).reshape(-1, int(x.shape[-1]))[:, sn.first:sn.first + w]
+            raw[sn.output.onnx_name] = self._columns(sn, raw)
         elif isinstance(sn, ScheduledNode):
             raw[sn.output.onnx_name] = self._vectorop(sn, raw)
         else:
@@ -1588,6 +1588,15 @@ class Simulator:
         if len(sn.inputs) == 3:
             return linear8.linear8(x, w, out, self._get(sn.inputs[2], raw).reshape(-1, w.m), sn.shift)
         return linear8.linear8(x, w, out)
+
+    def _columns(self, sn: ColumnsNode, raw) -> torch.Tensor:
+        """Columns of a row tensor: a view of a product's rows, which no node writes again; of any other tensor (a state, a caller's
+        input, a node's view of one) a copy, so that they keep the values they have here."""
+        xt, w = sn.inputs[0], int(sn.output.shape[-1])
+        x = self._get(xt, raw).reshape(-1, int(xt.shape[-1]))[:, sn.first:sn.first + w]
+        if self._products is None:
+            self._products = {p.output.onnx_name for p in self._graph.nodes if isinstance(p, (Linear8Node, MatmulNode)) and not p.output.state}
+        return x if xt.onnx_name in self._products else x.clone(memory_format=torch.contiguous_format)
 
     def _kv_write(self, sn: KvWriteNode, raw) -> torch.Tensor:
         """Row ``pos`` of every sequence's group-major cache from the step's rows, in place."""

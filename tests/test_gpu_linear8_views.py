@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from oracle import graph_sim as og
-from test_linear8_views import SHAPE, small, viewed  # noqa: F401
+from test_linear8_views import SHAPE, small, viewed, written_again  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,14 @@ def test_views_of_attention_rows_outlive_the_next_layer(small, kind, weights8): 
     want = og.forward(g, f, states={k: v.copy() for k, v in st.items()})
     assert (want[views[0].onnx_name] != want[views[1].onnx_name]).any()
     same(Simulator(g)._forward_pass(f, states=st, keep=[t.onnx_name for t in g.output_tensors]), want, kind)
+
+
+@pytest.mark.parametrize("kind", ["state", "reshape"])
+def test_columns_of_a_state_written_later(kind):
+    from cormorant_amd.simulate import Simulator
+    g, f, c = written_again(kind)
+    states = {"x": f.pop("x")}
+    want = og.forward(g, f, states={k: v.copy() for k, v in states.items()})[c.onnx_name]
+    for _ in range(2):
+        got = Simulator(g)._forward_pass(f, states={k: v.copy() for k, v in states.items()}, keep=[c.onnx_name])
+        np.testing.assert_array_equal(got[c.onnx_name], want)

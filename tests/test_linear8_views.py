@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cormorant_amd import models
-from cormorant_amd.graph import ColumnsNode, Linear8Node, PagedAttentionNode, ReshapeNode, TensorInfo
+from cormorant_amd.graph import ColumnsNode, Graph, Linear8Node, PagedAttentionNode, ReshapeNode, SelectRowNode, TensorInfo
 
 SHAPE = models.LlamaShape(layers=2, batch=2, d=128, heads=2, kv=1, hd=64, ff=128, vocab=256, ctx=64)
 
@@ -73,3 +73,44 @@ def test_the_count_of_quantised_rows_is_not_the_callers():
     with pytest.raises(AttributeError):
         rows.n = 16
     assert rows.n == 0
+
+
+def written_again(kind):
+    """Columns of rows that a later node of the pass writes: (graph, feeds, the columns)."""
+    n, d = 4, 16
+    h, x = TensorInfo("h", [n, d], exp=8), TensorInfo("x", [1, d], exp=8, state=True)
+    rows, rng = TensorInfo("n", [], kind="host"), np.random.default_rng(2)
+    c, y = TensorInfo("c", [1, 8], exp=8), TensorInfo("y", [1, d], exp=8, state=True)
+    r = x if kind == "state" else TensorInfo("r", [1, d], exp=8)
+    nodes = [ColumnsNode([r], c, first=8), SelectRowNode([h, rows], y)]
+    if kind == "reshape":
+        nodes.insert(0, ReshapeNode([x], r))
+    y.onnx_name = "x"                                # the state, written in place
+    f = {"h": rng.integers(-99, 99, (n, d)) / 256, "n": np.array(3.0), "x": rng.integers(-99, 99, (1, d)) / 256}
+    return Graph(nodes, input_tensors=[h, rows, x], output_tensors=[c]), f, c
+
+
+@pytest.mark.parametrize("kind", ["state", "reshape"])
+def test_columns_of_a_state_are_of_their_time(kind):
+    """The dispatch's columns of a state's buffer are a copy: a node that writes the state leaves them."""
+    from cormorant_amd import simulate
+    g, f, c = written_again(kind)
+    sim = object.__new__(simulate.Simulator)
+    sim._graph, sim._products, sim._weights = g, None, {}
+    raw = {"x": torch.arange(16, dtype=torch.int16).view(1, 16)}
+    for sn in g.nodes[:-1]:
+        sim._dispatch(sn, raw)
+    raw["x"].zero_()
+    np.testing.assert_array_equal(raw[c.onnx_name].numpy(), [list(range(8, 16))])
+
+
+def test_columns_of_a_product_are_a_view():
+    from cormorant_amd import simulate
+    x, p, c = TensorInfo("x", [3, 16], exp=8), TensorInfo("p", [3, 24], exp=8), TensorInfo("c", [3, 8], exp=8)
+    g = Graph([Linear8Node([x, TensorInfo("w", [16, 24], data=np.ones((16, 24)))], p), ColumnsNode([p], c, first=16)])
+    sim = object.__new__(simulate.Simulator)
+    sim._graph, sim._products = g, None
+    raw = {"p": torch.zeros(72, dtype=torch.int16)}
+    sim._dispatch(g.nodes[1], raw)
+    raw["p"][16] = 5
+    assert int(raw["c"][0, 0]) == 5
