@@ -343,6 +343,16 @@ class PagedAttentionNode(KernelNode):
             raise SchedulerError(f"{what}: window {self.window} (0, or below 2^30)")
 
 
+def _row_tensors(what: str, rows: Sequence[TensorInfo], y: TensorInfo):
+    """Refuses what the 8-bit nodes do not read or write as rows of contiguous columns: caches stored group-major, exponents of
+    axis 1, and a state as the output, whose buffer the caller holds and no such node writes."""
+    for t in [*rows, y]:
+        if t.group_layout is not None or t.chexp is not None:
+            raise SchedulerError(f"{what}: '{t.onnx_name}' is stored group-major, or at exponents of axis 1")
+    if y.state:
+        raise SchedulerError(f"{what}: the output '{y.onnx_name}' is a state")
+
+
 def _linear8_rows(what: str, x: TensorInfo, outs: int, y: TensorInfo, F: int) -> int:
     """The exponent of an 8-bit layer's int16 input rows [.., k] whose output is [.., outs]."""
     k = int(x.shape[-1])
@@ -388,6 +398,7 @@ class Linear8Node(KernelNode):
         what, x, y = f"linear8 '{self.output.onnx_name}'", self.inputs[0], self.output
         w = _linear8_weight(what, x, self.inputs[1])
         m = w.shape[1]
+        _row_tensors(what, [x, *self.inputs[2:]], y)
         f_x = _linear8_rows(what, x, m, y, self.F)
         self.shift = 0
         f_y = _exponents(what, y, m, self.F)
@@ -428,6 +439,7 @@ class GatedLinear8Node(KernelNode):
         from .linear8 import gate_shifts
         what, x, y = f"gated8 '{self.output.onnx_name}'", self.inputs[0], self.output
         wg, wu = (_linear8_weight(what, x, w) for w in self.inputs[1:])
+        _row_tensors(what, [x], y)
         if wg.shape != wu.shape or y.kind != "i16":
             raise SchedulerError(f"{what}: gate {list(wg.shape)} and up {list(wu.shape)} into int16 rows")
         f_x = _linear8_rows(what, x, wg.shape[1], y, self.F)
@@ -451,6 +463,7 @@ class ColumnsNode(KernelNode):
 
     def __post_init__(self):
         what, x, y = f"columns '{self.output.onnx_name}'", self.inputs[0], self.output
+        _row_tensors(what, [x], y)
         m, w = int(x.shape[-1]), int(y.shape[-1])
         if x.kind != "i16" or y.kind != "i16" or x.numel * w != y.numel * m or not 0 <= self.first <= m - w or \
                 m % 8 or w % 8 or self.first % 8:

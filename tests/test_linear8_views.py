@@ -1,11 +1,12 @@
 """The 8-bit nodes in the Simulator, on the CPU: which buffers a pass may reuse, which weights share an image, what of their
-rows' codes a caller may change."""
+rows' codes a caller may change, and which tensors they refuse."""
 import numpy as np
 import pytest
 import torch
 
 from cormorant_amd import models
-from cormorant_amd.graph import ColumnsNode, Graph, Linear8Node, PagedAttentionNode, ReshapeNode, SelectRowNode, TensorInfo
+from cormorant_amd.graph import (ColumnsNode, GatedLinear8Node, Graph, Linear8Node, PagedAttentionNode, ReshapeNode, SchedulerError,
+                                 SelectRowNode, TensorInfo)
 
 SHAPE = models.LlamaShape(layers=2, batch=2, d=128, heads=2, kv=1, hd=64, ff=128, vocab=256, ctx=64)
 
@@ -114,3 +115,27 @@ def test_columns_of_a_product_are_a_view():
     sim._dispatch(g.nodes[1], raw)
     raw["p"][16] = 5
     assert int(raw["c"][0, 0]) == 5
+
+
+NOT_ROWS = {"group-major": dict(group_layout=(3, 8)), "axis 1": dict(chexp=np.arange(24)), "state": dict(state=True)}
+
+
+@pytest.mark.parametrize("how", NOT_ROWS)
+@pytest.mark.parametrize("where", ["x", "y", "residual"])
+@pytest.mark.parametrize("node", ["linear", "gate", "columns"])
+def test_tensors_that_are_not_rows_are_refused(node, where, how):
+    """Group-major caches and exponents of axis 1 anywhere, states as outputs; a state may be read."""
+    kw = {at: NOT_ROWS[how] if at == where else {} for at in ("x", "y", "residual")}
+    if where == "residual" and node != "linear":
+        pytest.skip("no residual")
+    x, w = TensorInfo("x", [4, 24], exp=8, **kw["x"]), TensorInfo("w", [24, 24], data=np.eye(24))
+    wide = where == "residual"
+    y = TensorInfo("y", [4, 24], exp=8, kind="i32" if wide else "i16", **kw["y"])
+    h = [TensorInfo("h", [4, 24], exp=8, kind="i32", **kw["residual"])] if wide else []
+    make = {"linear": lambda: Linear8Node([x, w] + h, y, delta_exp=8 if wide else None), "gate": lambda: GatedLinear8Node([x, w, w], y),
+            "columns": lambda: ColumnsNode([x], y)}[node]
+    if how == "state" and where != "y":
+        make()
+    else:
+        with pytest.raises(SchedulerError):
+            make()
