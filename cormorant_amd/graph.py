@@ -361,10 +361,12 @@ def _linear8_rows(what: str, x: TensorInfo, outs: int, y: TensorInfo, F: int) ->
     return int(one_exponent(x.exp_full(F), what))
 
 
-def _linear8_weight(what: str, x: TensorInfo, w: TensorInfo) -> np.ndarray:
-    if w.data is None or np.ndim(w.data) != 2 or np.shape(w.data)[0] != int(x.shape[-1]):
-        raise SchedulerError(f"{what}: a constant weight [{int(x.shape[-1])}][m], got {list(w.shape)}")
-    return np.asarray(w.data)
+def _linear8_weight(what: str, x: TensorInfo, w: TensorInfo, F: int) -> np.ndarray:
+    """The values of a constant weight: its data, or where a MatMul has encoded it (raw / 2^F at wexp) those."""
+    if w.data is None or w.raw or np.ndim(w.data) != 2 or np.shape(w.data)[0] != int(x.shape[-1]):
+        raise SchedulerError(f"{what}: a constant weight's values [{int(x.shape[-1])}][m], got {list(w.shape)}{' (raw lanes)' if w.raw else ''}")
+    data = np.asarray(w.data)
+    return data if w.wexp is None else np.ldexp(data.astype(np.float64), F - np.asarray(w.wexp, np.int64))
 
 
 def _exponents(what: str, t: TensorInfo, n: int, F: int) -> np.ndarray:
@@ -396,7 +398,7 @@ class Linear8Node(KernelNode):
 
     def __post_init__(self):
         what, x, y = f"linear8 '{self.output.onnx_name}'", self.inputs[0], self.output
-        w = _linear8_weight(what, x, self.inputs[1])
+        w = _linear8_weight(what, x, self.inputs[1], self.F)
         m = w.shape[1]
         _row_tensors(what, [x, *self.inputs[2:]], y)
         f_x = _linear8_rows(what, x, m, y, self.F)
@@ -438,7 +440,7 @@ class GatedLinear8Node(KernelNode):
     def __post_init__(self):
         from .linear8 import gate_shifts
         what, x, y = f"gated8 '{self.output.onnx_name}'", self.inputs[0], self.output
-        wg, wu = (_linear8_weight(what, x, w) for w in self.inputs[1:])
+        wg, wu = (_linear8_weight(what, x, w, self.F) for w in self.inputs[1:])
         _row_tensors(what, [x], y)
         if wg.shape != wu.shape or y.kind != "i16":
             raise SchedulerError(f"{what}: gate {list(wg.shape)} and up {list(wu.shape)} into int16 rows")

@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from cormorant_amd import models
-from cormorant_amd.graph import (ColumnsNode, GatedLinear8Node, Graph, Linear8Node, PagedAttentionNode, ReshapeNode, SchedulerError,
-                                 SelectRowNode, TensorInfo)
+from cormorant_amd.graph import (ColumnsNode, GatedLinear8Node, Graph, Linear8Node, MatmulNode, PagedAttentionNode, ReshapeNode,
+                                 SchedulerError, SelectRowNode, TensorInfo)
+from cormorant_amd.numeric import encode_matmul_weights
 
 SHAPE = models.LlamaShape(layers=2, batch=2, d=128, heads=2, kv=1, hd=64, ff=128, vocab=256, ctx=64)
 
@@ -139,3 +140,25 @@ def test_tensors_that_are_not_rows_are_refused(node, where, how):
     else:
         with pytest.raises(SchedulerError):
             make()
+
+
+def test_a_weight_that_a_matmul_has_encoded():
+    """The values of a weight of both widths: its int16 lanes at their exponents, not the lanes over 2^8; raw lanes are refused."""
+    from cormorant_amd.dtype import AP_FIXED_16_8
+    from cormorant_amd.linear8 import quantise_weight
+    rng = np.random.default_rng(3)
+    x, y = TensorInfo("x", [2, 24], exp=rng.integers(8, 10, 24)), TensorInfo("y", [2, 16], exp=rng.integers(9, 12, 16))
+    values = rng.standard_normal((24, 16)) * 0.05
+    w = TensorInfo("w", [24, 16], data=values.copy())
+    encode_matmul_weights([MatmulNode([x, w], y)], AP_FIXED_16_8)
+    x8 = TensorInfo("x8", [2, 24], exp=9)
+    lanes = np.asarray(w.data, np.float64) * 2.0 ** 8 / 2.0 ** np.asarray(w.wexp, np.float64)
+    assert np.abs(lanes - values).max() <= 2.0 ** -(np.asarray(w.wexp).min() + 1.0) and (w.wexp != 8).any()
+    for node in (Linear8Node([x8, w], y), Linear8Node([x8, TensorInfo("v", [24, 16], data=lanes)], y)):
+        codes, mult = quantise_weight(lanes, 9, np.asarray(y.exp))
+        np.testing.assert_array_equal(node.codes, codes)
+        np.testing.assert_array_equal(node.mult, mult)
+    gate = GatedLinear8Node([x8, w, TensorInfo("u", [24, 16], data=values)], TensorInfo("m", [2, 16], exp=9))
+    np.testing.assert_array_equal(gate.gate_codes, quantise_weight(lanes, 9, 8)[0])
+    with pytest.raises(SchedulerError):
+        Linear8Node([x8, TensorInfo("r", [24, 16], data=np.ones((24, 16), np.int16), raw=True)], y)
