@@ -127,9 +127,10 @@ __device__ __forceinline__ uint32_t recip(uint32_t a) { return a ? (127u * (1u <
 
 typedef short v2s __attribute__((ext_vector_type(2)));
 
-// A row, or with ODD the element before one that starts between two 4-byte words: then loads are of the words it lies in, shifted
-// into place once they are there (16 bytes a lane between two words take 1.4 us more: 16 rows of 1001 x 960 5.6 us, 4.6 with
-// ODD; 4.2 at even strides, 4.4 with ODD).
+// A row, or with ODD the element before one that starts between two 4-byte words: then loads are of the words that hold the row's
+// elements, the first and the last of which may hold another's beside them (in the word of one of the row's, so no load leaves its
+// page; shifted out before it counts), and `settle` moves them into place once they are there.  16 bytes a lane between two
+// words take 1.4 us more: 16 rows of 1001 x 960 5.6 us, 4.6 with ODD; 4.2 at even strides, 4.4 with ODD.
 template <bool ODD>
 struct Row {
     const int16_t* p;
@@ -166,9 +167,9 @@ __device__ __forceinline__ Piece<ODD> load_piece(const Row<ODD>& r, uint32_t k0,
         if constexpr (ODD) __builtin_memcpy(&p.last, r.p + k0 + (r.shift ? 16 : 14), 4);     // a word that holds one of them
     } else if (k0 < k) {
         int16_t e[N];                                      // the row's last elements, one by one
-        const uint32_t m = ODD ? r.shift >> 4 : 0;         // at 0 with m: the element before the row is not the call's
+        const uint32_t m = ODD ? r.shift >> 4 : 0;
 #pragma unroll
-        for (uint32_t q = 0; q < N; q++) e[q] = k0 + q < k + m && (!ODD || k0 + q >= m) ? r.p[k0 + q] : (int16_t)0;
+        for (uint32_t q = 0; q < N; q++) e[q] = k0 + q < k + m ? r.p[k0 + q] : (int16_t)0;
         __builtin_memcpy(p.v, e, 32);
         if constexpr (ODD) __builtin_memcpy(&p.last, e + 16, 4);
     } else {

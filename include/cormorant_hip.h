@@ -595,7 +595,8 @@ int cm_linear8_rows(const int16_t* x, uint64_t x_ld, void* rows, uint32_t n, uin
  * address and stride).  The strides of out and the residual are below 2^23.  An output that otherwise shares a byte with x
  * or the residual is refused (CM_EINVAL); one that reaches into them at another stride counts as sharing.  Called with x,
  * the codes may stand in the device's workspace: a call of the same sizes before a stream captures it, and no two on
- * different streams at once.  Called with codes it takes none. */
+ * different streams at once.  Called with codes it takes none.  A row of x between two 4-byte words is read by the words
+ * that hold its elements: the 2 bytes before and behind it may be read, and are not used. */
 int cm_linear8(const cm_linear8_weight* weight, const int16_t* x, uint64_t x_ld, const void* rows, uint32_t n, void* out,
                uint64_t out_ld, const int32_t* residual, uint64_t residual_ld, uint32_t shift, void* stream);
 
