@@ -1,11 +1,29 @@
-"""The 8-bit linear layers on the GPU, more of their paths bit for bit against the oracle: rows whose neighbours hold the largest
-values."""
+"""The 8-bit linear layers on the GPU, more of their paths bit for bit against the oracle: 17 to 32 rows whose workgroups take
+several units of columns, and rows whose neighbours hold the largest values."""
 import numpy as np
 import pytest
 
+import test_gpu_linear8 as cases
 from test_gpu_linear8 import L, dev, host, rows, weights  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+WIDE = [(17, 200, 8300), (32, 700, 9001), (31, 1500, 16500), (20, 64, 49152)]
+
+
+@pytest.mark.parametrize("n,k,m", WIDE, ids=str)
+@pytest.mark.parametrize("form", ["plain", "bias", "residual", "both"])
+def test_columns_unit_by_unit(L, n, k, m, form):  # noqa: F811
+    """Two fragments of rows, more columns than the workgroups take at once: the sums cleared, the weights, the parameters and the
+    residual loaded for each unit."""
+    cases.test_linear(L, n, k, m, form)
+
+
+@pytest.mark.parametrize("n,k,m", [(17, 200, 8300), (32, 700, 9001)], ids=str)
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_gate_unit_by_unit(L, oracle_lib, n, k, m, act):  # noqa: F811
+    cases.test_gated(L, oracle_lib, n, k, m, act)
+
 
 @pytest.mark.parametrize("n,k,m", [(1, 1, 33), (1, 16, 33), (3, 17, 40), (16, 960, 96), (16, 961, 96), (9, 1023, 300), (30, 64, 40),
                                    (40, 63, 64), (64, 256, 64), (100, 960, 200), (77, 1001, 90), (200, 1536, 64), (300, 4096, 64)], ids=str)
