@@ -13,7 +13,6 @@
 // A 32 x 32 x 32 operand is then 1 KiB in lane order, a 16 x 16 x 64 operand four runs of 256 bytes.  A gated
 // weight alternates blocks of 32 gate columns and the same 32 up columns.
 #include "cm_common.h"
-#include "cm_rowops_math.h"
 
 #include <algorithm>
 #include <type_traits>
