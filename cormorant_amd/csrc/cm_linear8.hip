@@ -1021,8 +1021,8 @@ int ring_at(const Prod& p, hipStream_t s) {
     return CM_OK;
 }
 
-// The tile with the least of four estimates in ns, fitted to 150 measured products of 33 to 8192 rows (0.7 % behind the best
-// tile of each, gates 0.5 %).  Among them (rows x k x columns: us of 256 x 128, 128 x 128, 128 x 64 and 32 x 32 tiles): 128 x 2560 x 960
+// The tile with the least of four estimates in ns, fitted to 150 measured products of 33 to 8192 rows (0.9 % behind the best
+// tile of each, gates 0.6 %).  Among them (rows x k x columns: us of 256 x 128, 128 x 128, 128 x 64 and 32 x 32 tiles): 128 x 2560 x 960
 // 17.2 / 10.6 / 6.8 / 4.4; 512 x 960 x 2560 10.3 / 6.8 / 5.0 / 7.9; 1000 x 1024 x 1024 10.4 / 6.9 / 5.0 / 6.9; 1024 x 2560 x 960 17.5 /
 // 10.9 / 7.5 / 9.9; 512 x 8192 x 1024 - / 25.9 / 19.2 / 12.5; 2048 x 8192 x 2048 46.8 / 36.5 / 39.9 / 105; 4096 x 960 x 2560 20.4 /
 // 18.7 / 17.7 / 44.0; 2048 x 4096 x 4096 35.2 / 35.3 / 41.7 / 99.7.  Gates (the smallest tile 32 x (32 + 32)): 300 x 960 x 2560
